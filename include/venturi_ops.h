@@ -418,6 +418,53 @@ int venturi_rowcodec_project(const VRCPlan* plan, const void* x, const void* cod
                              const void* scales, void* out, void* workspace, uint64_t available, int tokens, int n,
                              int k, int padded, int packed, void* stream);
 
+/* ---- Between the projections and after the head (extensions). ----
+ * Cache planes, K and V each: codes uint8 [pages][kv_heads][page_tokens][dp], code + 128, dp = head_dim
+ * rounded up to 32; scales fp16 [pages][kv_heads][dp / 32][page_tokens]. Slot s is token s % page_tokens of
+ * page s / page_tokens. head_dim: a multiple of 8 up to 256; page_tokens: a multiple of 16 up to 4096;
+ * dtype 0 or 1; row operands (qkv, q, k, v, out, keys, values, logits) and planes 16-byte aligned. */
+
+/* Rotates q and K of qkv [tokens][(q_heads + 2 kv_heads) * head_dim] and caches K and V at slots [tokens]
+ * (a slot outside the cache: not cached). rates: turns per position of each pair, fp64 [2][rotary_dim / 2]: the
+ * rounded numbers, then what the rounding left; factor multiplies cos and sin; rotary_dim 0: no rotation, positions and rates unused. q [tokens][q_heads]
+ * [head_dim] (NULL iff q_heads = 0); k [tokens][kv_heads][head_dim], the rotated keys, or NULL. */
+int venturi_kv_write_run(const void* qkv, const int64_t* positions, const int64_t* slots, const double* rates,
+                         void* q, void* k, void* key_codes, void* key_scales, void* value_codes,
+                         void* value_scales, int tokens, int q_heads, int kv_heads, int head_dim, int rotary_dim,
+                         int interleaved, float factor, int pages, int page_tokens, int dtype, void* stream);
+/* The cached rows of slots [tokens] in `dtype` (NaN for a slot outside the cache); keys or values may be NULL. */
+int venturi_kv_read_run(const void* key_codes, const void* key_scales, const void* value_codes,
+                        const void* value_scales, const int64_t* slots, void* keys, void* values, int tokens,
+                        int kv_heads, int head_dim, int pages, int page_tokens, int dtype, void* stream);
+/* Attention of query_tokens new tokens per sequence over the cached keys: out = softmax(scale q k^T) v, query i
+ * of t over the first lengths[b] - (t - 1 - i) keys of pages page_table[b][0 .. max_pages). Queries that see no
+ * key get zeros; a length outside [0, max_pages * page_tokens] or a reached page outside the cache gives NaN.
+ * workspace: venturi_kv_attention_bytes (may be 0), 256-byte aligned. */
+uint64_t venturi_kv_attention_bytes(int sequences, int query_tokens, int q_heads, int kv_heads, int head_dim,
+                                    int max_pages, int page_tokens);
+int venturi_kv_attention_run(const void* q, const void* key_codes, const void* key_scales, const void* value_codes,
+                             const void* value_scales, const int32_t* page_table, const int32_t* lengths, void* out,
+                             void* workspace, uint64_t available, int sequences, int query_tokens, int q_heads,
+                             int kv_heads, int head_dim, int pages, int page_tokens, int max_pages, float scale,
+                             int dtype, void* stream);
+/* Causal attention over packed sequences: rows q_offsets[b] .. q_offsets[b + 1] of q and out [tokens][q_heads]
+ * [head_dim], rows k_offsets[b] .. of k and v [keys][kv_heads][head_dim]; query i of t sees the first
+ * n - (t - 1 - i) of n keys. workspace: venturi_packed_attention_bytes (may be 0), 256-byte aligned. */
+uint64_t venturi_packed_attention_bytes(int tokens, int keys, int sequences, int q_heads, int kv_heads,
+                                        int head_dim);
+int venturi_packed_attention_run(const void* q, const void* k, const void* v, const int32_t* q_offsets,
+                                 const int32_t* k_offsets, void* out, void* workspace, uint64_t available,
+                                 int tokens, int keys, int sequences, int q_heads, int kv_heads, int head_dim,
+                                 float scale, int dtype, void* stream);
+/* One token per row of logits [rows][vocab] from uniforms [rows] in [0, 1): order by (logit descending, index),
+ * top_k (0: all), top_p of the top-k mass, min_p against the largest weight. Settings [rows], each NULL for none
+ * (temperature 1). tokens int64 [rows] (-1 for a row of -inf and NaN alone); probabilities fp32 [rows] or NULL.
+ * workspace: venturi_sample_bytes (may be 0), 256-byte aligned. */
+uint64_t venturi_sample_bytes(int rows, int vocab);
+int venturi_sample_run(const void* logits, const float* uniforms, const float* temperature, const int32_t* top_k,
+                       const float* top_p, const float* min_p, int64_t* tokens, float* probabilities,
+                       void* workspace, uint64_t available, int rows, int vocab, int dtype, void* stream);
+
 /* ---- Reference exports outside the quantized-linear path. The reference's
  * Python backend binds each of these when it is constructed
  * (blocks.py:336-427), so they are exported with the reference's signatures;

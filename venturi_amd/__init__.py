@@ -28,6 +28,7 @@ __all__ = [
     "OperatorSupport",
     "Q4RowSplitWeight",
     "Q8RowSplitWeight",
+    "RotaryEmbedding",
     "UnsupportedOperationError",
     "create_backend",
     "prepare_q8_dp4a",
@@ -44,6 +45,10 @@ def __getattr__(name):
         from .blocks import HipBackend
 
         return HipBackend
+    if name == "RotaryEmbedding":
+        from .rotary import RotaryEmbedding
+
+        return RotaryEmbedding
     if name == "prepare_q8_dp4a":
         from .q8_dp4a import prepare_q8_dp4a
 

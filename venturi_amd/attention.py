@@ -1,0 +1,73 @@
+"""Causal attention over packed prompts: sequences of different lengths side by side in one call.
+
+Sequence b owns rows q_offsets[b] .. q_offsets[b + 1] of q and rows k_offsets[b] .. k_offsets[b + 1] of k and v. Its
+queries are its last tokens: with n keys and t queries, query i sees the first n - (t - 1 - i) keys, so keys before the
+queries' own (cached ones, read back) are seen by all of them. Head h of q reads KV head h * kv_heads // q_heads.
+The reference's runtime calls its own attention kernel for one sequence (ops_api.h:13-15); packing, the past and the
+prepared plan are this package's.
+"""
+
+from dataclasses import dataclass, field
+
+import torch
+
+from .kv_cache import head_geometry, softmax_scale, vector_aligned
+from .operands import DTYPE_CODES, admit, disjoint, extents
+
+
+@dataclass(frozen=True)
+class PackedAttentionPlan:
+    """``HipBackend.prepare_attention``. The plan owns its workspace (partial sums of calls with few rows, split over
+    their keys), so runs of one plan must be ordered: one stream at a time."""
+
+    _backend: object
+    tokens: int
+    keys: int
+    sequences: int
+    q_heads: int
+    kv_heads: int
+    head_dim: int
+    scale: float
+    dtype: torch.dtype
+    device: torch.device
+    _workspace: object = field(repr=False)
+    workspace_bytes = 0  # nothing for the caller to provide
+
+    @property
+    def storage_tensors(self):
+        return () if self._workspace is None else (self._workspace,)
+
+    @classmethod
+    def create(cls, backend, *, tokens, keys, sequences, q_heads, kv_heads, head_dim, dtype, device, scale=None):
+        extents(tokens, keys, sequences)
+        head_geometry(q_heads, kv_heads, head_dim)
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("Packed attention takes FP16/BF16")
+        factor = softmax_scale(scale, head_dim)
+        target = backend.validate_device(dtype, device)
+        lib = backend._native
+        nbytes = lib.venturi_packed_attention_bytes(tokens, keys, sequences, q_heads, kv_heads, head_dim)
+        if nbytes == 0 and lib.venturi_blocks_error():
+            raise ValueError(lib.error())
+        workspace = None
+        if nbytes:
+            with torch.cuda.device(target):
+                workspace = torch.empty(nbytes, dtype=torch.uint8, device=target)
+        return cls(backend, tokens, keys, sequences, q_heads, kv_heads, head_dim, factor, dtype, target, workspace)
+
+    def run(self, q, k, v, q_offsets, k_offsets, *, out):
+        """``q`` and ``out`` [tokens, q_heads, head_dim], ``k`` and ``v`` [keys, kv_heads, head_dim], offsets int32
+        [sequences + 1] on the device, ascending from 0. Queries that see no key, and rows past the last offset, get
+        zeros. Offsets are not checked on the host; the kernel reads no row outside q, k and v whatever they hold.
+        """
+        q_shape, k_shape = (self.tokens, self.q_heads, self.head_dim), (self.keys, self.kv_heads, self.head_dim)
+        for name, t, shape in (("q", q, q_shape), ("k", k, k_shape), ("v", v, k_shape), ("out", out, q_shape)):
+            admit(t, shape, self.dtype, self.device, name)
+        for name, t in (("q_offsets", q_offsets), ("k_offsets", k_offsets)):
+            admit(t, (self.sequences + 1,), torch.int32, self.device, name)
+        vector_aligned(q, k, v, out)
+        disjoint(out, (q, k, v, q_offsets, k_offsets) + self.storage_tensors)
+        self._backend._launch("venturi_packed_attention_run", self.device, q, k, v, q_offsets, k_offsets, out, self._workspace,
+                              0 if self._workspace is None else self._workspace.numel(), self.tokens, self.keys, self.sequences,
+                              self.q_heads, self.kv_heads, self.head_dim, self.scale, DTYPE_CODES[self.dtype])
+        return out

@@ -102,6 +102,9 @@ def _capabilities():
         OperatorSupport("linear", devices, quant, "q8_g32_fp16", "row_split_k128_v1"),
         OperatorSupport("embedding", devices, quant, "q8_g32_fp16", "row_split_k128_v1"),
         OperatorSupport("linear", devices, quant, "q4_g64_fp16", "row_split_k128_v1"),
+        OperatorSupport("kv_cache", devices, quant),
+        OperatorSupport("attention", devices, quant),
+        OperatorSupport("sampling", devices, quant),
     ]
     return BackendCapabilities("venturi-ops-gfx950", tuple(operators), reference=False, cuda_graphs=True)
 
@@ -314,6 +317,28 @@ class HipBackend(Backend):
         """Plan of out = cast(a + b) over [tokens, features] (blocks.py:574-581)."""
         shape = extents(tokens, features)
         return _Pointwise(self, shape, dtype, self.validate_device(dtype, device), "venturi_add_run")
+
+    # -- between the projections and after the head ------------------------
+    def create_kv_cache(self, *, pages, page_tokens, kv_heads, head_dim, dtype, device):
+        """Paged Q8 cache of one layer's keys and values, with plans that write (with rotary positions), read back
+        and attend to it (kv_cache.Q8KVCache)."""
+        from .kv_cache import Q8KVCache
+
+        return Q8KVCache.create(self, pages=pages, page_tokens=page_tokens, kv_heads=kv_heads, head_dim=head_dim, dtype=dtype,
+                                device=device)
+
+    def prepare_attention(self, *, tokens, keys, sequences, q_heads, kv_heads, head_dim, dtype, device, scale=None):
+        """Plan of causal attention over packed sequences (attention.PackedAttentionPlan)."""
+        from .attention import PackedAttentionPlan
+
+        return PackedAttentionPlan.create(self, tokens=tokens, keys=keys, sequences=sequences, q_heads=q_heads,
+                                          kv_heads=kv_heads, head_dim=head_dim, dtype=dtype, device=device, scale=scale)
+
+    def prepare_sampling(self, *, rows, vocab, dtype, device):
+        """Plan of sampling one token per row of logits (sampling.SamplingPlan)."""
+        from .sampling import SamplingPlan
+
+        return SamplingPlan.create(self, rows=rows, vocab=vocab, dtype=dtype, device=device)
 
 
 @dataclass(frozen=True)
