@@ -24,6 +24,14 @@ struct WriteArgs {
     float factor;
 };
 
+// position * (rate + rest) less its whole turns, in [-1/2, 1/2]. The product has to be the rounded one in both places.
+__device__ __forceinline__ float part_of_turn(double position, double rate, double rest) {
+#pragma clang fp contract(off)
+    const double turns = position * rate;
+    const double part = (turns - rint(turns)) + fma(position, rest, fma(position, rate, -turns));
+    return static_cast<float>(part - rint(part));
+}
+
 // Eight columns at `column` of a head, rotated. `head` is the head's first column.
 template <class T>
 __device__ __forceinline__ void rotated(const T* __restrict__ head, int column, int rotary, int interleaved,
@@ -102,10 +110,8 @@ __global__ __launch_bounds__(256) void kv_write(WriteArgs<T> a) {
     if (a.rotary_dim) {
         const int pairs = a.rotary_dim >> 1;
         if (static_cast<int>(threadIdx.x) < pairs) {
-            const double position = static_cast<double>(a.positions[token]);
-            const double rate = a.rates[threadIdx.x], rest = a.rates[pairs + threadIdx.x], turns = position * rate;
-            const double whole = (turns - rint(turns)) + fma(position, rest, fma(position, rate, -turns));
-            const float part = static_cast<float>(whole - rint(whole));
+            const float part = part_of_turn(static_cast<double>(a.positions[token]), a.rates[threadIdx.x],
+                                            a.rates[pairs + threadIdx.x]);
             float s, c;
             sincospif(2.0f * part, &s, &c);
             cosines[threadIdx.x] = a.factor * c;
