@@ -1,73 +1,649 @@
-// Attention over the paged Q8 cache, one wave per query row and head.
-#include "attention_rows.hpp"
+// Attention over the paged Q8 cache: out = softmax(scale q k^T) v for the few new tokens of many sequences.
+//
+// Bound by HBM: every code and scale of K and V is read once (272 bytes a token and head at head_dim 128). A wave takes
+// 32 keys at a time, holds the next 32 keys' codes and scales in registers while it computes, and keeps weights,
+// outputs and statistics in registers; nothing goes through LDS until the waves of a workgroup join.
+//
+// Rows. The query rows of one KV head (query_tokens x group) are the columns of 16-wide matrix tiles, so that a KV
+// head's codes are converted once for all heads that share them. With S^T = K Q^T a lane holds four keys of one query,
+// which is the operand layout of O^T = V^T P^T if the 32 keys are taken in the order (tile, lane group, register): the
+// weights never leave their lane.
+//
+// Codes. A code c is stored as the byte u = c + 128, and a byte in the low half of a 16-bit word is the fp16 number
+// u 2^-24 (subnormal; the matrix cores keep it), so that one v_perm makes two operands.
+//   K: S = sum_groups scale_k * (sum u q - 128 sum q), the second term as the accumulator's start: exact products, fp32.
+//   V: a lane holds 8 keys of a few columns, a pair of keys is one v_perm of two keys' bytes, and v = fma(u 2^-24,
+//      scale_v 2^15 k, -scale_v k / 4) = v * k 2^-9, rounded once to fp16 (2^-11). k is a power of two that brings the
+//      largest scale so far to at most 1, so neither end of the scales' range overflows or underflows.
+// Queries are scaled by a power of two per row into fp16's range: exact for fp16 and, but for numbers 2^28 below the
+// row's largest, for bf16. The weights are rounded to fp16 (2^-11), their sum is of the unrounded ones.
+//
+// Softmax. One pass: weights are 2^(s - m) for a reference m that follows the maximum only when a score passes it by
+// more than 4 (a factor of 16 fits fp16's range): the rescaling of the outputs is rare.
+//
+// Split. The keys of all sequences are cut into chunks of one length, chosen on the device from the sum of the
+// lengths, so that the grid is about `kTarget` workgroups whatever the lengths; a workgroup finds its sequence by a scan.
+// A sequence of one chunk is finished by its workgroup, others leave partial outputs, joined by a second launch.
+#include "kv_cache.hpp"
 
 namespace vt {
 namespace {
 
-struct CachedSource {
-    CachePlanes p;
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4, kBlock = 32;           // keys of a wave's step
+constexpr int kMinChunk = kWaves * kBlock;
+constexpr int kTarget = 512;                     // workgroups: two to a CU
+constexpr float kLazy = 4.0f, kShift = 8.0f;     // weights are 2^(s - m + kShift), at most 2^12
+
+struct Geometry {
+    int sequences, query_tokens, q_heads, kv_heads, group, rows;  // rows = query_tokens * group, of one KV head
+    int head_dim, row_blocks, max_pages, tiles_per_page;
+    std::uint64_t page_magic;                    // ceil(2^36 / tiles_per_page)
+    int target;                                  // chunks per KV head and row block
+    float scale;
+    std::int64_t longest;                        // max_pages * page_tokens
+};
+
+// Where workgroup `flat` of the chunks works.
+struct Work {
+    int sequence, split, splits, length;
+    std::int64_t chunk;
+    int first;  // flat index of the sequence's first chunk
+};
+
+__device__ __forceinline__ std::int64_t wave_sum(std::int64_t v) {
+#pragma unroll
+    for (int step = 32; step; step >>= 1) v += __shfl_xor(v, step, 64);
+    return v;
+}
+
+__device__ __forceinline__ int admitted(int length, const Geometry& g) {
+    return length < 0 || length > g.longest ? 0 : length;  // a bad length is one chunk, which marks its rows
+}
+
+__device__ __forceinline__ std::int64_t chunk_length(const std::int32_t* __restrict__ lengths, const Geometry& g) {
+    const int lane = threadIdx.x & 63;
+    std::int64_t total = 0;
+    for (int s = lane; s < g.sequences; s += 64) total += admitted(lengths[s], g);
+    total = wave_sum(total);
+    const std::int64_t least = (total + g.target - 1) / g.target;
+    return max((least + kMinChunk - 1) / kMinChunk, std::int64_t{1}) * kMinChunk;
+}
+
+// Chunks per sequence: at least one. Their sum is at most target + sequences.
+__device__ __forceinline__ int chunks_of(int length, std::int64_t chunk) {
+    return max(static_cast<int>((length + chunk - 1) / chunk), 1);
+}
+
+__device__ __forceinline__ bool find_work(const std::int32_t* __restrict__ lengths, const Geometry& g, int flat, Work& w) {
+    const int lane = threadIdx.x & 63;
+    w.chunk = chunk_length(lengths, g);
+    int before = 0;
+    for (int base = 0; base < g.sequences; base += 64) {
+        const int s = base + lane, length = s < g.sequences ? lengths[s] : 0;
+        const int n = s < g.sequences ? chunks_of(admitted(length, g), w.chunk) : 0;
+        int end = n;
+#pragma unroll
+        for (int step = 1; step < 64; step <<= 1) {
+            const int below = __shfl_up(end, step, 64);
+            if (lane >= step) end += below;
+        }
+        end += before;
+        const unsigned long long hit = __ballot(end > flat);
+        if (hit) {
+            const int at = __ffsll(hit) - 1;
+            w.sequence = base + at;
+            w.length = __shfl(length, at, 64);
+            w.splits = __shfl(n, at, 64);
+            w.first = __shfl(end, at, 64) - w.splits;
+            w.split = flat - w.first;
+            return true;
+        }
+        before = __shfl(end, 63, 64);
+    }
+    return false;
+}
+
+__device__ __forceinline__ std::uint32_t permute(std::uint32_t high, std::uint32_t low, std::uint32_t selector) {
+    return __builtin_amdgcn_perm(high, low, selector);
+}
+
+// Bytes b and b + 1 of a word as two fp16 u 2^-24 (selector 0x0c is a zero byte).
+template <int B>
+__device__ __forceinline__ std::uint32_t spread(std::uint32_t word) {
+    return permute(0, word, 0x0c000c00u | B | (B + 1) << 16);
+}
+
+__device__ __forceinline__ half8v spread8(std::uint32_t a, std::uint32_t b) {
+    const uint4 w = make_uint4(spread<0>(a), spread<2>(a), spread<0>(b), spread<2>(b));
+    return __builtin_bit_cast(half8v, w);
+}
+
+__device__ __forceinline__ std::uint32_t pack(float a, float b) {
+    half2v v;
+    v[0] = static_cast<_Float16>(a);
+    v[1] = static_cast<_Float16>(b);
+    return __builtin_bit_cast(std::uint32_t, v);
+}
+
+__device__ __forceinline__ float half_at(const uint2& w, int i) {
+    return i & 1 ? half_hi(i < 2 ? w.x : w.y) : half_lo(i < 2 ? w.x : w.y);
+}
+
+// The value columns of a lane. A row of D columns is cut into segments of 256, 128, 64 and 32; in a segment of width W
+// lane m holds the W / 16 columns from (W / 16) m on.
+template <int D>
+struct Segments {
+    static constexpr int count = (D >= 256 ? 1 : 0) + (D % 256 >= 128 ? 1 : 0) + (D % 128 >= 64 ? 1 : 0) + (D % 64 >= 32 ? 1 : 0);
+    static constexpr int width(int i) {
+        int left = D;
+        for (int w = 256; w >= 32; w >>= 1)
+            if (left >= w) {
+                if (i-- == 0) return w;
+                left -= w;
+            }
+        return 0;
+    }
+    static constexpr int offset(int i) {
+        int sum = 0;
+        for (int j = 0; j < i; ++j) sum += width(j);
+        return sum;
+    }
+    static constexpr int tile(int i) { return offset(i) / 16; }  // first of the segment's matrix tiles
+    static constexpr int word(int i) {                           // first of its words in a lane's register copy of a key
+        int sum = 0;
+        for (int j = 0; j < i; ++j) sum += (width(j) / 16 + 3) / 4;
+        return sum;
+    }
+    static constexpr int words = word(count);
+};
+
+// One step's codes and scales of a wave, as its lanes hold them.
+template <int D>
+struct Step {
+    std::uint32_t key[2][D / 32][2];           // tile, group: 8 codes of one key
+    uint2 key_scale[2][D / 32];                // four keys
+    std::uint32_t value[8][Segments<D>::words];  // keys 4g + 0..3 of both tiles
+    uint2 value_scale[2][Segments<D>::count];
+};
+
+struct Pages {
+    CachePlanes planes;
     const std::int32_t* table;
+    int tiles_per_page;
+    std::uint64_t magic;
     int head;
-    __device__ std::int64_t slot(std::int64_t j) const {
-        const std::int64_t at = j / p.page_tokens;
-        return static_cast<std::int64_t>(table[at]) * p.page_tokens + (j - at * p.page_tokens);
-    }
-    __device__ float key(std::int64_t j, int d) const {
-        const std::int64_t s = slot(j);
-        return static_cast<float>(p.key_codes[p.code_at(s, head) + d] - 128) * __half2float(p.key_scales[p.scale_at(s, head, d >> 5)]);
-    }
-    __device__ float value(std::int64_t j, int d) const {
-        const std::int64_t s = slot(j);
-        return static_cast<float>(p.value_codes[p.code_at(s, head) + d] - 128) *
-               __half2float(p.value_scales[p.scale_at(s, head, d >> 5)]);
+    __device__ __forceinline__ int page_of(int tile) const {
+        return static_cast<int>((static_cast<std::uint64_t>(tile) * magic) >> 36);
     }
 };
 
-template <class T>
-__global__ __launch_bounds__(256) void kv_attention(const T* __restrict__ q, CachePlanes planes,
-                                                    const std::int32_t* __restrict__ page_table,
-                                                    const std::int32_t* __restrict__ lengths, T* __restrict__ out,
-                                                    int sequences, int query_tokens, int q_heads, int head_dim, int max_pages,
-                                                    float scale) {
-    __shared__ float query[4][256];
+template <int D>
+__device__ __forceinline__ void load_step(const Pages& p, int first_tile, int last_tile, Step<D>& s, bool& bad) {
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const int page_tokens = p.tiles_per_page * 16;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int tile = __builtin_amdgcn_readfirstlane(min(first_tile + t, last_tile));
+        const int at = p.page_of(tile), inside = (tile - at * p.tiles_per_page) * 16;
+        int page = __builtin_amdgcn_readfirstlane(p.table[at]);
+        if (page < 0 || page >= p.planes.pages) {
+            bad = true;
+            page = 0;
+        }
+        const std::int64_t base = static_cast<std::int64_t>(page) * p.planes.kv_heads + p.head;
+        const std::uint8_t* keys = p.planes.key_codes + (base * page_tokens + inside) * D;
+        const std::uint8_t* values = p.planes.value_codes + (base * page_tokens + inside) * D;
+        const __half* key_scales = p.planes.key_scales + base * (D / 32) * page_tokens + inside;
+        const __half* value_scales = p.planes.value_scales + base * (D / 32) * page_tokens + inside;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+            const uint2 w = *reinterpret_cast<const uint2*>(keys + m * D + 32 * c + 8 * g);
+            s.key[t][c][0] = w.x;
+            s.key[t][c][1] = w.y;
+            s.key_scale[t][c] = *reinterpret_cast<const uint2*>(key_scales + c * page_tokens + 4 * g);
+        }
+#pragma unroll
+        for (int i = 0; i < Segments<D>::count; ++i) {
+            const int w = Segments<D>::width(i), columns = w / 16, word = Segments<D>::word(i), column = Segments<D>::offset(i) + columns * m;
+            s.value_scale[t][i] =
+                *reinterpret_cast<const uint2*>(value_scales + (column >> 5) * page_tokens + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const std::uint8_t* row = values + (4 * g + r) * D + column;
+                std::uint32_t* out = s.value[4 * t + r] + word;
+                if (w == 256) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(row);
+                    out[0] = v.x, out[1] = v.y, out[2] = v.z, out[3] = v.w;
+                } else if (w == 128) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(row);
+                    out[0] = v.x, out[1] = v.y;
+                } else if (w == 64) {
+                    out[0] = *reinterpret_cast<const std::uint32_t*>(row);
+                } else {
+                    out[0] = *reinterpret_cast<const unsigned short*>(row);
+                }
+            }
+        }
+    }
+}
+
+// A wave's running state over its 16 * QT query rows.
+template <int D, int QT>
+struct State {
+    half8v query[QT][D / 32];
+    float4v start[QT][D / 32];   // -128 * 2^-24 sum of the group's query numbers
+    float factor[QT];            // scale * log2 e * 2^24 * the row's power of two
+    int seen[QT];                // keys that the lane's row sees
+    float reference[QT], sum[QT];
+    float4v out[QT][D / 16];
+    float bring;                 // k: 2^(-ceil(log2 of the largest value scale so far))
+};
+
+__device__ __forceinline__ float power_above(float v) {  // the smallest power of two >= v, for v > 0
+    int e;
+    const float f = frexpf(v, &e);
+    return ldexpf(1.0f, f == 0.5f ? e - 1 : e);
+}
+
+template <int D, int QT>
+__device__ __forceinline__ void compute(const Step<D>& s, State<D, QT>& a, int first_key, int length, bool full) {
+    const int g = (threadIdx.x & 63) >> 4;
+    float score[QT][8];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int q = 0; q < QT; ++q)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) score[q][4 * t + r] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+            const half8v keys = spread8(s.key[t][c][0], s.key[t][c][1]);
+#pragma unroll
+            for (int q = 0; q < QT; ++q) {
+                const float4v raw = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, a.query[q][c], a.start[q][c], 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    score[q][4 * t + r] = fmaf(raw[r], half_at(s.key_scale[t][c], r), score[q][4 * t + r]);
+            }
+        }
+    }
+    float value_scale[Segments<D>::count][8], top_scale = 0.0f;
+#pragma unroll
+    for (int i = 0; i < Segments<D>::count; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            value_scale[i][j] = half_at(s.value_scale[j >> 2][i], j & 3);
+            // Slots past the length hold anything: their weights are 0, and so has to be what they multiply.
+            if (!full && first_key + 16 * (j >> 2) + 4 * g + (j & 3) >= length) value_scale[i][j] = 0.0f;
+            top_scale = fmaxf(top_scale, value_scale[i][j] <= 65504.0f ? value_scale[i][j] : 0.0f);
+        }
+    bool raise = top_scale * a.bring > 1.99f;
+#pragma unroll
+    for (int q = 0; q < QT; ++q)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            score[q][j] *= a.factor[q];
+            if (!full && first_key + 16 * (j >> 2) + 4 * g + (j & 3) >= a.seen[q]) score[q][j] = -__builtin_inff();
+            raise = raise || score[q][j] > a.reference[q] + kLazy;
+        }
+    if (__any(raise)) {
+#pragma unroll
+        for (int step = 1; step < 64; step <<= 1) top_scale = fmaxf(top_scale, __shfl_xor(top_scale, step, 64));
+        float shrink = 1.0f;
+        if (top_scale * a.bring > 1.0f) {
+            const float bring = 1.0f / power_above(top_scale);
+            shrink = bring / a.bring;
+            a.bring = bring;
+        }
+#pragma unroll
+        for (int q = 0; q < QT; ++q) {
+            float top = a.reference[q];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, score[q][j]);
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float keep = a.reference[q] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(a.reference[q] - top);
+            a.reference[q] = top;
+            a.sum[q] *= keep;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) a.out[q][d] *= keep * shrink;
+        }
+    }
+    half8v weights[QT];
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+        const float base = a.reference[q] == -__builtin_inff() ? 0.0f : a.reference[q] - kShift;
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            p[j] = __builtin_amdgcn_exp2f(score[q][j] - base);
+            a.sum[q] += p[j];
+        }
+        const uint4 w = make_uint4(pack(p[0], p[1]), pack(p[2], p[3]), pack(p[4], p[5]), pack(p[6], p[7]));
+        weights[q] = __builtin_bit_cast(half8v, w);
+    }
+#pragma unroll
+    for (int i = 0; i < Segments<D>::count; ++i) {
+        half2v steep[4], flat[4];
+        bool broken = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float x = value_scale[i][2 * j] * a.bring, y = value_scale[i][2 * j + 1] * a.bring;
+            // A row that does not see a key must not see its NaN: while rows differ, such scales are kept out of the
+            // product and marked below.
+            const bool mark = !full && !(x < 2.0f && y < 2.0f);
+            broken = broken || mark;
+            steep[j] = __builtin_bit_cast(half2v, pack(!full && !(x < 2.0f) ? 0.0f : x * 32768.0f, !full && !(y < 2.0f) ? 0.0f : y * 32768.0f));
+            flat[j] = __builtin_bit_cast(half2v, pack(!full && !(x < 2.0f) ? 0.0f : x * -0.25f, !full && !(y < 2.0f) ? 0.0f : y * -0.25f));
+        }
+        const int columns = Segments<D>::width(i) / 16, word = Segments<D>::word(i), tile = Segments<D>::tile(i);
+#pragma unroll
+        for (int d = 0; d < columns; ++d) {
+            std::uint32_t v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const std::uint32_t pair = permute(s.value[2 * j + 1][word + d / 4], s.value[2 * j][word + d / 4],
+                                                   0x0c000c00u | (d & 3) | (4 + (d & 3)) << 16);
+                const half2v x = __builtin_bit_cast(half2v, pair);
+                v[j] = __builtin_bit_cast(std::uint32_t, __builtin_elementwise_fma(x, steep[j], flat[j]));
+            }
+            const half8v values = __builtin_bit_cast(half8v, make_uint4(v[0], v[1], v[2], v[3]));
+#pragma unroll
+            for (int q = 0; q < QT; ++q)
+                a.out[q][tile + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values, weights[q], a.out[q][tile + d], 0, 0, 0);
+        }
+        if (!full && __any(broken)) {
+            half8v marks;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                marks[j] = value_scale[i][j] * a.bring < 2.0f ? static_cast<_Float16>(0.0f) : static_cast<_Float16>(1.0f);
+#pragma unroll
+            for (int q = 0; q < QT; ++q) {
+                half8v sees;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    sees[j] = first_key + 16 * (j >> 2) + 4 * g + (j & 3) < a.seen[q] ? static_cast<_Float16>(1.0f)
+                                                                                      : static_cast<_Float16>(0.0f);
+                const float4v none = {0.0f, 0.0f, 0.0f, 0.0f};
+                const float4v hits = __builtin_amdgcn_mfma_f32_16x16x32_f16(marks, sees, none, 0, 0, 0);
+#pragma unroll
+                for (int d = 0; d < columns; ++d)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (hits[r] > 0.0f) a.out[q][tile + d][r] = __builtin_nanf("");
+            }
+        }
+    }
+}
+
+template <class T, int D, int QT>
+__device__ __forceinline__ void load_queries(const T* __restrict__ q, const Geometry& g, const Work& w, int head, int block,
+                                             State<D, QT>& a) {
+    const int lane = threadIdx.x & 63, m = lane & 15, lg = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int row = (block * QT + t) * 16 + m;
+        const bool live = row < g.rows;
+        const int token = live ? row / g.group : 0;
+        const T* source = q + ((static_cast<std::int64_t>(w.sequence) * g.query_tokens + token) * g.q_heads +
+                               head * g.group + (live ? row - token * g.group : 0)) * g.head_dim;
+        a.seen[t] = live ? w.length - (g.query_tokens - 1 - token) : 0;
+        float x[D / 32][8], top = 0.0f;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+            const int column = 32 * c + 8 * lg;
+            if (live && column < g.head_dim) {
+                load8(source + column, x[c]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[c][j] = 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[c][j]));
+        }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        // The largest number comes to [2^14, 2^15).
+        const int e = top > 0.0f && top <= 3.402823466e38f ? ilogbf(top) - 14 : 0;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+            float total = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                a.query[t][c][j] = static_cast<_Float16>(ldexpf(x[c][j], -e));
+                total += static_cast<float>(a.query[t][c][j]);
+            }
+            total += __shfl_xor(total, 16, 64);
+            total += __shfl_xor(total, 32, 64);
+            total *= -128.0f * 0x1p-24f;
+            a.start[t][c] = float4v{total, total, total, total};
+        }
+        a.factor[t] = ldexpf(g.scale * 1.44269504088896340736f, e + 24);
+        a.reference[t] = -__builtin_inff();
+        a.sum[t] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) a.out[t][d] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    a.bring = 0x1p24f;
+}
+
+// Partial results of a chunk: per row D outputs, then the reference and the sum.
+template <int D>
+constexpr int partial_floats() { return D + 2; }
+
+template <class T, int D, int QT>
+__global__ __launch_bounds__(kWaves * 64, D * QT <= 128 ? 2 : 1) void kv_attention(const T* __restrict__ q, CachePlanes planes,
+                                                            const std::int32_t* __restrict__ page_table,
+                                                            const std::int32_t* __restrict__ lengths, T* __restrict__ out,
+                                                            float* __restrict__ partial, Geometry g) {
+    __shared__ __align__(16) float joined[kWaves][16][D];
+    __shared__ float references[kWaves][16], sums[kWaves][16];
+    __shared__ int broken;
+    Work w;
+    if (!find_work(lengths, g, blockIdx.x, w)) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, lg = lane >> 4;
+    const int head = blockIdx.y / g.row_blocks, block = blockIdx.y - head * g.row_blocks;
+    if (threadIdx.x == 0) broken = 0;
+    const bool bad_length = w.length < 0 || w.length > g.longest;
+    const int length = bad_length ? 0 : w.length;
+    const int begin = static_cast<int>(w.split * w.chunk), end = static_cast<int>(min<std::int64_t>(begin + w.chunk, length));
+    State<D, QT> a;
+    load_queries<T, D, QT>(q, g, w, head, block, a);
+    const Pages pages{planes, page_table + static_cast<std::int64_t>(w.sequence) * g.max_pages, g.tiles_per_page, g.page_magic, head};
+    const int last_tile = (length + 15) / 16 - 1;
+    const int all_see = length - (g.query_tokens - 1);  // keys below are seen by every row
+    bool bad = false;
+    int key = begin + wave * kBlock;
+    if (key < end) {
+        Step<D> now;
+        load_step<D>(pages, key >> 4, last_tile, now, bad);
+        for (; key < end; key += kWaves * kBlock) {
+            Step<D> next;
+            const int after = key + kWaves * kBlock;
+            if (after < end) load_step<D>(pages, after >> 4, last_tile, next, bad);
+            compute<D, QT>(now, a, key, length, key + kBlock <= all_see);
+            now = next;
+        }
+    }
+    __syncthreads();
+    if (bad && lane == 0) broken = 1;
+    const float nan = __builtin_nanf("");
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        float sum = a.sum[t];
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (lg == 0) references[wave][m] = a.reference[t], sums[wave][m] = sum;
+        __syncthreads();
+        float top = references[0][m];
+#pragma unroll
+        for (int i = 1; i < kWaves; ++i) top = fmaxf(top, references[i][m]);
+        // 512 / bring undoes the values' power of two.
+        const float keep = a.reference[t] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(a.reference[t] - top);
+        const float undo = keep * (512.0f / a.bring);
+#pragma unroll
+        for (int i = 0; i < Segments<D>::count; ++i) {
+            const int columns = Segments<D>::width(i) / 16;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int d = 0; d < columns; ++d)
+                    joined[wave][m][Segments<D>::offset(i) + columns * (4 * lg + r) + d] = a.out[t][Segments<D>::tile(i) + d][r] * undo;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 16 * D / 4; i += kWaves * 64) {
+            const int r = i / (D / 4), column = (i - r * (D / 4)) * 4, row = (block * QT + t) * 16 + r;
+            if (row >= g.rows) continue;
+            float best = references[0][r], total = 0.0f;
+#pragma unroll
+            for (int j = 1; j < kWaves; ++j) best = fmaxf(best, references[j][r]);
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int j = 0; j < kWaves; ++j) {
+                const float own = references[j][r];
+                if (own != -__builtin_inff()) total += sums[j][r] * __builtin_amdgcn_exp2f(own - best);
+                else if (sums[j][r] != 0.0f) total = nan;  // scores of NaN alone
+                const float4 x = *reinterpret_cast<const float4*>(&joined[j][r][column]);
+                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+            }
+            if (broken || bad_length) total = nan;
+            if (w.splits == 1) {
+                const int token = row / g.group;
+                T* target = out + ((static_cast<std::int64_t>(w.sequence) * g.query_tokens + token) * g.q_heads + head * g.group +
+                                   row - token * g.group) * g.head_dim + column;
+                const float scale = total == 0.0f ? 0.0f : 1.0f / total;
+                if (column < g.head_dim) {
+                    const std::uint32_t lo = __builtin_bit_cast(unsigned short, from_f32<T>(total == 0.0f ? 0.0f : v.x * scale)) |
+                                             static_cast<std::uint32_t>(__builtin_bit_cast(unsigned short, from_f32<T>(total == 0.0f ? 0.0f : v.y * scale))) << 16;
+                    const std::uint32_t hi = __builtin_bit_cast(unsigned short, from_f32<T>(total == 0.0f ? 0.0f : v.z * scale)) |
+                                             static_cast<std::uint32_t>(__builtin_bit_cast(unsigned short, from_f32<T>(total == 0.0f ? 0.0f : v.w * scale))) << 16;
+                    *reinterpret_cast<uint2*>(target) = make_uint2(lo, hi);
+                }
+            } else {
+                const std::int64_t slot = static_cast<std::int64_t>(blockIdx.x) * g.kv_heads + head;
+                float* target = partial + (slot * g.rows + row) * partial_floats<D>();
+                // Rows of D + 2 floats are 8-byte aligned.
+                *reinterpret_cast<float2*>(target + column) = make_float2(v.x, v.y);
+                *reinterpret_cast<float2*>(target + column + 2) = make_float2(v.z, v.w);
+                if (column == 0) *reinterpret_cast<float2*>(target + D) = make_float2(best, total);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Joins the partial results of a sequence of several chunks: a wave per query row.
+template <class T, int D>
+__global__ __launch_bounds__(256) void kv_attention_join(const std::int32_t* __restrict__ lengths, T* __restrict__ out,
+                                                         const float* __restrict__ partial, Geometry g) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * 4 + wave;
-    const std::int64_t token = row / q_heads;
-    const int head = static_cast<int>(row - token * q_heads);
-    if (token >= static_cast<std::int64_t>(sequences) * query_tokens) return;
-    const std::int64_t b = token / query_tokens;
-    const int length = lengths[b];
-    const std::int32_t* table = page_table + b * max_pages;
-    bool bad = length < 0 || length > static_cast<std::int64_t>(max_pages) * planes.page_tokens;
-    if (!bad)
-        for (int i = lane; i < (length + planes.page_tokens - 1) / planes.page_tokens; i += 64)
-            bad |= table[i] < 0 || table[i] >= planes.pages;
-    bad = __any(bad);
-    for (int d = lane; d < head_dim; d += 64) query[wave][d] = to_f32(q[row * head_dim + d]) * scale;
-    float acc[4], total;
-    const std::int64_t seen = bad ? 0 : length - (query_tokens - 1 - (token - b * query_tokens));
-    attend_row(CachedSource{planes, table, head / (q_heads / planes.kv_heads)}, query[wave], head_dim, seen, acc, total);
-    if (bad) total = __builtin_nanf("");
-    store_row(out + row * head_dim, acc, total, head_dim);
+    const int sequence = blockIdx.y;
+    const std::int64_t index = static_cast<std::int64_t>(blockIdx.x) * 4 + wave;  // token * q_heads + head
+    if (index >= static_cast<std::int64_t>(g.query_tokens) * g.q_heads) return;
+    const std::int64_t chunk = chunk_length(lengths, g);
+    const int splits = chunks_of(admitted(lengths[sequence], g), chunk);
+    if (splits == 1) return;
+    int first = 0;
+    for (int s = lane; s < sequence; s += 64) first += chunks_of(admitted(lengths[s], g), chunk);
+    first = static_cast<int>(wave_sum(static_cast<std::int64_t>(first)));
+    const int token = static_cast<int>(index / g.q_heads), q_head = static_cast<int>(index - static_cast<std::int64_t>(token) * g.q_heads);
+    const int head = q_head / g.group, row = token * g.group + q_head - head * g.group;
+    const auto at = [&](int split) {
+        return partial + ((static_cast<std::int64_t>(first + split) * g.kv_heads + head) * g.rows + row) * partial_floats<D>();
+    };
+    float best = -__builtin_inff();
+    for (int i = lane; i < splits; i += 64) best = fmaxf(best, at(i)[D]);
+#pragma unroll
+    for (int step = 32; step; step >>= 1) best = fmaxf(best, __shfl_xor(best, step, 64));
+    float total = 0.0f, v[D / 64 + 1] = {};
+    for (int i = 0; i < splits; ++i) {
+        const float* p = at(i);
+        const float own = p[D], sum = p[D + 1];
+        const float keep = own == -__builtin_inff() ? (sum == 0.0f ? 0.0f : __builtin_nanf("")) : __builtin_amdgcn_exp2f(own - best);
+        total += sum * keep;
+#pragma unroll
+        for (int d = 0; d <= D / 64; ++d)
+            if (lane + 64 * d < D) v[d] += p[lane + 64 * d] * keep;
+    }
+    T* target = out + ((static_cast<std::int64_t>(sequence) * g.query_tokens + token) * g.q_heads + q_head) * g.head_dim;
+#pragma unroll
+    for (int d = 0; d <= D / 64; ++d)
+        if (lane + 64 * d < g.head_dim) target[lane + 64 * d] = from_f32<T>(total == 0.0f ? 0.0f : v[d] / total);
 }
 
-template <class T>
-void launch(const void* q, const CachePlanes& planes, const std::int32_t* page_table, const std::int32_t* lengths, void* out,
-            int sequences, int query_tokens, int q_heads, int head_dim, int max_pages, float scale, hipStream_t stream) {
-    const std::int64_t rows = static_cast<std::int64_t>(sequences) * query_tokens * q_heads;
-    kv_attention<T><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(
-        static_cast<const T*>(q), planes, page_table, lengths, static_cast<T*>(out), sequences, query_tokens, q_heads, head_dim,
-        max_pages, scale);
-}
+// Row tiles of a wave: two where a KV head has more than 16 rows and the registers hold them.
+int row_tiles(int rows, int head_dim) { return rows > 16 && head_dim <= 128 ? 2 : 1; }
 
-void require_geometry(int sequences, int query_tokens, int q_heads, int kv_heads, int head_dim, int max_pages,
-                      int page_tokens) {
+// Chunks per KV head and row block that the grid aims at.
+int target_chunks(int kv_heads, int row_blocks) { return std::max(1, kTarget / (kv_heads * row_blocks)); }
+
+Geometry geometry(int sequences, int query_tokens, int q_heads, int kv_heads, int head_dim, int max_pages, int page_tokens,
+                  float scale) {
     require_head_dim(head_dim);
     require(sequences > 0 && query_tokens > 0 && q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0 && max_pages > 0 &&
-                page_tokens > 0 && page_tokens % 16 == 0,
+                page_tokens > 0 && page_tokens % 16 == 0 && page_tokens <= 4096,
             "invalid cached attention geometry");
-    require(static_cast<std::int64_t>(max_pages) * page_tokens < (1ll << 31), "a sequence's slots must fit int32");
+    Geometry g;
+    g.longest = static_cast<std::int64_t>(max_pages) * page_tokens;
+    require(g.longest < (1ll << 31) - 4096, "a sequence's slots must fit int32");
     require(static_cast<std::int64_t>(sequences) * query_tokens * q_heads < (1ll << 31), "cached attention rows must fit int32");
+    g.sequences = sequences, g.query_tokens = query_tokens, g.q_heads = q_heads, g.kv_heads = kv_heads;
+    g.group = q_heads / kv_heads, g.rows = query_tokens * g.group, g.head_dim = head_dim;
+    const int block = 16 * row_tiles(g.rows, head_dim);
+    g.row_blocks = (g.rows + block - 1) / block;
+    require(static_cast<std::int64_t>(kv_heads) * g.row_blocks <= 65535 && sequences <= 65535,
+            "cached attention takes at most 65535 sequences, and KV heads times row blocks");
+    g.max_pages = max_pages, g.tiles_per_page = page_tokens / 16;
+    g.page_magic = ((std::uint64_t{1} << 36) + g.tiles_per_page - 1) / g.tiles_per_page;
+    g.target = target_chunks(kv_heads, g.row_blocks);
+    g.scale = scale;
+    return g;
+}
+
+// Slots for every chunk that could be one of several; none where no sequence can pass one chunk.
+std::uint64_t partial_bytes(const Geometry& g) {
+    if (g.longest <= kMinChunk) return 0;
+    const std::uint64_t chunks = static_cast<std::uint64_t>(g.target) + g.sequences;
+    return chunks * g.kv_heads * g.rows * ((g.head_dim + 31) / 32 * 32 + 2) * sizeof(float);
+}
+
+template <class T, int D>
+void launch(const void* q, const CachePlanes& planes, const std::int32_t* page_table, const std::int32_t* lengths, void* out,
+            void* workspace, const Geometry& g, hipStream_t stream) {
+    const dim3 grid(g.target + g.sequences, g.kv_heads * g.row_blocks);
+    const auto* queries = static_cast<const T*>(q);
+    auto* target = static_cast<T*>(out);
+    auto* partial = static_cast<float*>(workspace);
+    if constexpr (D <= 128) {
+        if (row_tiles(g.rows, D) == 2)
+            kv_attention<T, D, 2><<<grid, kWaves * 64, 0, stream>>>(queries, planes, page_table, lengths, target, partial, g);
+    }
+    if (row_tiles(g.rows, D) == 1)
+        kv_attention<T, D, 1><<<grid, kWaves * 64, 0, stream>>>(queries, planes, page_table, lengths, target, partial, g);
+    check(hipGetLastError());
+    if (partial_bytes(g)) {
+        const auto rows = static_cast<unsigned>((static_cast<std::int64_t>(g.query_tokens) * g.q_heads + 3) / 4);
+        kv_attention_join<T, D><<<dim3(rows, g.sequences), 256, 0, stream>>>(lengths, target, partial, g);
+    }
+}
+
+template <class T>
+void launch_any(const void* q, const CachePlanes& planes, const std::int32_t* page_table, const std::int32_t* lengths, void* out,
+                void* workspace, const Geometry& g, hipStream_t stream) {
+    switch (planes.padded) {
+        case 32: return launch<T, 32>(q, planes, page_table, lengths, out, workspace, g, stream);
+        case 64: return launch<T, 64>(q, planes, page_table, lengths, out, workspace, g, stream);
+        case 96: return launch<T, 96>(q, planes, page_table, lengths, out, workspace, g, stream);
+        case 128: return launch<T, 128>(q, planes, page_table, lengths, out, workspace, g, stream);
+        case 160: return launch<T, 160>(q, planes, page_table, lengths, out, workspace, g, stream);
+        case 192: return launch<T, 192>(q, planes, page_table, lengths, out, workspace, g, stream);
+        case 224: return launch<T, 224>(q, planes, page_table, lengths, out, workspace, g, stream);
+        default: return launch<T, 256>(q, planes, page_table, lengths, out, workspace, g, stream);
+    }
 }
 
 }  // namespace
@@ -77,9 +653,12 @@ void require_geometry(int sequences, int query_tokens, int q_heads, int kv_heads
 
 VT_EXPORT std::uint64_t venturi_kv_attention_bytes(int sequences, int query_tokens, int q_heads, int kv_heads, int head_dim,
                                                    int max_pages, int page_tokens) {
-    vt::host_guarded(
-        [&] { vt::require_geometry(sequences, query_tokens, q_heads, kv_heads, head_dim, max_pages, page_tokens); });
-    return 0;
+    std::uint64_t bytes = 0;
+    vt::host_guarded([&] {
+        bytes = vt::partial_bytes(
+            vt::geometry(sequences, query_tokens, q_heads, kv_heads, head_dim, max_pages, page_tokens, 1.0f));
+    });
+    return bytes;
 }
 
 VT_EXPORT int venturi_kv_attention_run(const void* q, const void* key_codes, const void* key_scales, const void* value_codes,
@@ -90,15 +669,17 @@ VT_EXPORT int venturi_kv_attention_run(const void* q, const void* key_codes, con
     return vt::guarded([&] {
         const auto planes = vt::cache_planes(key_codes, key_scales, value_codes, value_scales, kv_heads, head_dim, pages,
                                              page_tokens);
-        vt::require_geometry(sequences, query_tokens, q_heads, kv_heads, head_dim, max_pages, page_tokens);
+        const auto g = vt::geometry(sequences, query_tokens, q_heads, kv_heads, head_dim, max_pages, page_tokens, scale);
         vt::require(q && page_table && lengths && out, "null cached attention operand");
         vt::require(vt::aligned(q, 16) && vt::aligned(out, 16), "cached attention rows must be 16-byte aligned");
+        const std::uint64_t bytes = vt::partial_bytes(g);
+        vt::require(!bytes || (workspace && available >= bytes && vt::aligned(workspace, 256)),
+                    "cached attention needs its workspace, 256-byte aligned");
         const auto s = static_cast<hipStream_t>(stream);
         if (dtype == vt::kF16)
-            vt::launch<__half>(q, planes, page_table, lengths, out, sequences, query_tokens, q_heads, head_dim, max_pages, scale, s);
+            vt::launch_any<__half>(q, planes, page_table, lengths, out, workspace, g, s);
         else if (dtype == vt::kBF16)
-            vt::launch<__hip_bfloat16>(q, planes, page_table, lengths, out, sequences, query_tokens, q_heads, head_dim, max_pages,
-                                       scale, s);
+            vt::launch_any<__hip_bfloat16>(q, planes, page_table, lengths, out, workspace, g, s);
         else
             throw vt::Invalid("cached attention takes fp16 or bf16");
     });
