@@ -1,59 +1,413 @@
-// Causal attention over packed sequences, one wave per query row and head.
-#include "attention_rows.hpp"
+// Causal attention over packed sequences: out = softmax(scale q k^T) v, every query over the keys up to its own.
+//
+// Bound by the matrix cores (4 rows keys head_dim operations) and, beside them, by the exponentials: at head_dim 128 a
+// score costs half a cycle of a SIMD in the matrix unit and as much in the vector unit. A wave takes 32 query rows and
+// works through the keys in tiles that its workgroup stages in LDS, double buffered: the next tile's global loads are
+// in flight while the present one is computed.
+//
+// Rows. The rows of a KV head are its (query, head of the group) pairs, query by query, cut into blocks of 128, so that
+// all heads of a group share the staged keys, short sequences fill their tiles, and the diagonal's waste is
+// small. S^T = K Q^T leaves a lane 16 keys of one query, which is the operand layout of O^T = V^T P^T with the keys in the
+// order (lane half, register): weights, maxima and sums stay in their lane, but for one exchange between the lane halves
+// when the reference moves. V^T comes out of row-major V through the transposing LDS reads.
+//
+// LDS. A row of keys or values takes a power of two of 16-byte units; a unit's place is XORed with the row (values: pairs
+// of units, which the transposing read takes together), so that both kinds of reads find their rows on different banks.
+//
+// Softmax. Weights are 2^(s - m + 8), rounded to the model's type (fp16 2^-11, bf16 2^-8 of each), for a reference m that
+// follows the maximum only when a score passes it by more than 4; sums are of the unrounded weights, in 32 bits.
+#include "kv_cache.hpp"
+
+#include <climits>
 
 namespace vt {
 namespace {
 
-template <class T>
-struct DenseSource {
-    const T* k;
-    const T* v;
-    std::int64_t stride;  // elements between keys
-    __device__ float key(std::int64_t j, int d) const { return to_f32(k[j * stride + d]); }
-    __device__ float value(std::int64_t j, int d) const { return to_f32(v[j * stride + d]); }
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef __bf16 bfloat8v __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bfloat2v __attribute__((ext_vector_type(2)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef float float16v __attribute__((ext_vector_type(16)));
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves, kWaveRows = 32, kRows = kWaves * kWaveRows;
+constexpr float kLazy = 4.0f, kShift = 8.0f;
+
+struct Geometry {
+    int tokens, keys, sequences, q_heads, kv_heads, group, head_dim;
+    float scale;
 };
 
-template <class T>
-__global__ __launch_bounds__(256) void packed_attention(const T* __restrict__ q, const T* __restrict__ k,
-                                                        const T* __restrict__ v, const std::int32_t* __restrict__ q_offsets,
-                                                        const std::int32_t* __restrict__ k_offsets, T* __restrict__ out,
-                                                        int tokens, int keys, int sequences, int q_heads, int kv_heads,
-                                                        int head_dim, float scale) {
-    __shared__ float query[4][256];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * 4 + wave;
-    if (row >= static_cast<std::int64_t>(tokens) * q_heads) return;
-    const int token = static_cast<int>(row / q_heads), head = static_cast<int>(row % q_heads);
-    std::int64_t first = 0, seen = 0;
-    for (int b = 0; b < sequences; ++b) {
-        if (token >= q_offsets[b] && token < q_offsets[b + 1]) {
-            first = min(max(k_offsets[b], 0), keys);
-            seen = min(max(k_offsets[b + 1], static_cast<int>(first)), keys) - first - (q_offsets[b + 1] - 1 - token);
-            break;
+template <class T> struct Matrix;
+template <> struct Matrix<__half> {
+    static constexpr std::uint32_t kExponent = 0x7c00;
+    static __device__ __forceinline__ float16v multiply(uint4 a, uint4 b, float16v c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8v, a), __builtin_bit_cast(half8v, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ std::uint32_t pack(float a, float b) {
+        half2v v;
+        v[0] = static_cast<_Float16>(a);
+        v[1] = static_cast<_Float16>(b);
+        return __builtin_bit_cast(std::uint32_t, v);
+    }
+};
+template <> struct Matrix<__hip_bfloat16> {
+    static constexpr std::uint32_t kExponent = 0x7f80;
+    static __device__ __forceinline__ float16v multiply(uint4 a, uint4 b, float16v c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bfloat8v, a), __builtin_bit_cast(bfloat8v, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ std::uint32_t pack(float a, float b) {
+        bfloat2v v;
+        v[0] = static_cast<__bf16>(a);
+        v[1] = static_cast<__bf16>(b);
+        return __builtin_bit_cast(std::uint32_t, v);
+    }
+};
+
+// Geometry of a staged tile of rows of D columns.
+template <int D>
+struct Tile {
+    static constexpr int keys = D <= 128 ? 64 : 32;
+    static constexpr int columns = D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256;  // of an LDS row
+    static constexpr int units = columns / 8;                                            // 16-byte units of an LDS row
+    static constexpr int bytes = keys * columns * 2;
+    static constexpr int loads = keys * units / kThreads;                                // per thread
+    // What a unit's place in its row is XORed with.
+    static __device__ __forceinline__ int key_swizzle(int row) {
+        if constexpr (units >= 16) return row & 15;
+        else return (row / (16 / units)) & (units - 1);
+    }
+    static __device__ __forceinline__ int value_swizzle(int row) {  // even: pairs of units keep their order
+        if constexpr (units >= 16) return 2 * (row & 7);
+        else return 2 * ((row / (16 / units)) & (units / 2 - 1));
+    }
+};
+
+// A sequence's part of the packed rows, clamped to the tensors.
+struct Span {
+    int q_first, queries, k_first, keys;
+};
+
+__device__ __forceinline__ Span span_of(const std::int32_t* __restrict__ q_offsets, const std::int32_t* __restrict__ k_offsets,
+                                        int sequence, const Geometry& g) {
+    Span s;
+    s.q_first = min(max(q_offsets[sequence], 0), g.tokens);
+    s.queries = min(max(q_offsets[sequence + 1], s.q_first), g.tokens) - s.q_first;
+    s.k_first = min(max(k_offsets[sequence], 0), g.keys);
+    s.keys = min(max(k_offsets[sequence + 1], s.k_first), g.keys) - s.k_first;
+    return s;
+}
+
+__device__ __forceinline__ int blocks_of(const std::int32_t* __restrict__ q_offsets, int sequence, const Geometry& g) {
+    const int first = min(max(q_offsets[sequence], 0), g.tokens), end = min(max(q_offsets[sequence + 1], first), g.tokens);
+    return static_cast<int>((static_cast<std::int64_t>(end - first) * g.group + kRows - 1) / kRows);
+}
+
+// The sequence and row block of flat block `flat`; blocks come sequence by sequence, each one's last block first.
+__device__ __forceinline__ bool find_block(const std::int32_t* __restrict__ q_offsets, const Geometry& g, int flat, int& sequence,
+                                           int& block) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int base = 0; base < g.sequences; base += 64) {
+        const int n = base + lane < g.sequences ? blocks_of(q_offsets, base + lane, g) : 0;
+        int end = n;
+#pragma unroll
+        for (int step = 1; step < 64; step <<= 1) {
+            const int below = __shfl_up(end, step, 64);
+            if (lane >= step) end += below;
+        }
+        end += before;
+        const unsigned long long hit = __ballot(end > flat);
+        if (hit) {
+            const int at = __ffsll(hit) - 1;
+            sequence = base + at;
+            block = __shfl(end, at, 64) - 1 - flat;
+            return true;
+        }
+        before = __shfl(end, 63, 64);
+    }
+    block = flat - before;  // workgroups past the last block, counted from 0
+    return false;
+}
+
+// Sixteen bytes of keys and of values per thread and load; rows past the sequence and columns past the head are zero.
+template <class T, int D>
+struct Stage {
+    uint4 key[Tile<D>::loads], value[Tile<D>::loads];
+
+    __device__ __forceinline__ void load(const T* __restrict__ k, const T* __restrict__ v, std::int64_t stride, int rows,
+                                         int head_dim) {
+#pragma unroll
+        for (int i = 0; i < Tile<D>::loads; ++i) {
+            const int u = threadIdx.x + i * kThreads, row = u / Tile<D>::units, column = u % Tile<D>::units * 8;
+            const bool inside = row < rows && column < head_dim;
+            const std::int64_t at = inside ? row * stride + column : 0;
+            key[i] = inside ? *reinterpret_cast<const uint4*>(k + at) : make_uint4(0, 0, 0, 0);
+            value[i] = inside ? *reinterpret_cast<const uint4*>(v + at) : make_uint4(0, 0, 0, 0);
         }
     }
-    for (int d = lane; d < head_dim; d += 64) query[wave][d] = to_f32(q[row * head_dim + d]) * scale;
-    const std::int64_t stride = static_cast<std::int64_t>(kv_heads) * head_dim;
-    const std::int64_t offset = first * stride + head / (q_heads / kv_heads) * head_dim;
-    float acc[4], total;
-    attend_row(DenseSource<T>{k + offset, v + offset, stride}, query[wave], head_dim, seen, acc, total);
-    store_row(out + row * head_dim, acc, total, head_dim);
+    __device__ __forceinline__ void store(unsigned char* keys, unsigned char* values) const {
+#pragma unroll
+        for (int i = 0; i < Tile<D>::loads; ++i) {
+            const int u = threadIdx.x + i * kThreads, row = u / Tile<D>::units, unit = u % Tile<D>::units;
+            *reinterpret_cast<uint4*>(keys + (row * Tile<D>::units + (unit ^ Tile<D>::key_swizzle(row))) * 16) = key[i];
+            *reinterpret_cast<uint4*>(values + (row * Tile<D>::units + (unit ^ Tile<D>::value_swizzle(row))) * 16) = value[i];
+        }
+    }
+};
+
+template <int D>
+struct State {
+    uint4 query[D / 16];
+    float16v out[D / 32];
+    float reference, sum;
+};
+
+__device__ __forceinline__ std::uint32_t finite_part(std::uint32_t w, std::uint32_t exponent) {
+    const std::uint32_t high = exponent << 16;
+    return ((w & exponent) == exponent ? 0 : w & 0xffffu) | ((w & high) == high ? 0 : w & 0xffff0000u);
 }
 
+// One tile of keys for a wave's 32 rows. MASKED: some row sees only a part of it (`seen` keys of the lane's row, counted
+// from the tile's first).
+template <class T, int D, bool MASKED>
+__device__ __forceinline__ void compute(const unsigned char* __restrict__ keys, const unsigned char* __restrict__ values,
+                                        State<D>& a, float factor, int seen) {
+    constexpr int kTiles = Tile<D>::keys / 32;
+    const int lane = threadIdx.x & 63, m = lane & 31, h = lane >> 5;
+    float16v score[kTiles];
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) score[t][r] = 0.0f;
+        const int row = 32 * t + m;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+            const uint4 k = *reinterpret_cast<const uint4*>(
+                keys + (row * Tile<D>::units + ((2 * s + h) ^ Tile<D>::key_swizzle(row))) * 16);
+            score[t] = Matrix<T>::multiply(k, a.query[s], score[t]);
+        }
+    }
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            if (MASKED && 32 * t + 8 * (r / 4) + 4 * h + r % 4 >= seen) score[t][r] = -__builtin_inff();
+            top = fmaxf(top, score[t][r]);
+        }
+    top *= factor;
+    if (__any(top > a.reference + kLazy)) {
+        const float next = fmaxf(a.reference, fmaxf(top, __shfl_xor(top, 32, 64)));
+        const float keep = a.reference == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(a.reference - next);
+        a.reference = next;
+        a.sum *= keep;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) a.out[d] *= keep;
+    }
+    const float base = a.reference == -__builtin_inff() ? 0.0f : kShift - a.reference;
+    uint4 weight[2 * kTiles];
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+        std::uint32_t w[8];
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(score[t][r], factor, base));
+            const float y = __builtin_amdgcn_exp2f(fmaf(score[t][r + 1], factor, base));
+            a.sum += x + y;
+            w[r / 2] = Matrix<T>::pack(x, y);
+        }
+        weight[2 * t] = make_uint4(w[0], w[1], w[2], w[3]);
+        weight[2 * t + 1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+    const int group = lane >> 4, i = lane & 15;
+    const int row0 = 4 * h + (i >> 2);
+    bool broken = false;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) {
+        const int unit = (4 * d + 2 * (group & 1) + ((i & 3) >> 1)) ^ Tile<D>::value_swizzle(row0);
+#pragma unroll
+        for (int t = 0; t < 2 * kTiles; ++t) {
+            // Rows 16 t + 8 p + row0: the swizzle repeats with period 8.
+            uint2 part[2];
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const int row = 16 * t + 8 * p + row0;
+                const int place = Tile<D>::units >= 16 ? unit
+                                                       : (4 * d + 2 * (group & 1) + ((i & 3) >> 1)) ^ Tile<D>::value_swizzle(row);
+                const unsigned char* at = values + (row * Tile<D>::units + place) * 16 + 8 * (i & 1);
+                typedef __attribute__((address_space(3))) short4v* Lds;
+                part[p] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at)));
+            }
+            uint4 v = make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
+            if (MASKED) {
+                // A weight of 0 would make a NaN of an infinity that its row does not see.
+                const uint4 clean = make_uint4(finite_part(v.x, Matrix<T>::kExponent), finite_part(v.y, Matrix<T>::kExponent),
+                                               finite_part(v.z, Matrix<T>::kExponent), finite_part(v.w, Matrix<T>::kExponent));
+                broken = broken || clean.x != v.x || clean.y != v.y || clean.z != v.z || clean.w != v.w;
+                v = clean;
+            }
+            a.out[d] = Matrix<T>::multiply(v, weight[t], a.out[d]);
+        }
+    }
+    if (MASKED && __any(broken)) {
+        // Rare: infinities and NaN go to the rows that see them, key by key.
+        for (int key = 0; key < Tile<D>::keys; ++key) {
+            if (!__any(key < seen)) break;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int column = 32 * d + 8 * (r / 4) + 4 * h + r % 4;
+                    const int place = (key * Tile<D>::units + ((column >> 3) ^ Tile<D>::value_swizzle(key))) * 16 + (column & 7) * 2;
+                    const std::uint32_t bits = *reinterpret_cast<const unsigned short*>(values + place);
+                    if (key < seen && (bits & Matrix<T>::kExponent) == Matrix<T>::kExponent)
+                        a.out[d][r] += to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(bits)));
+                }
+        }
+    }
+}
+
+// Rows past the last sequence get zeros, from the workgroups that found no block (one a head at least).
 template <class T>
-void launch(const void* q, const void* k, const void* v, const std::int32_t* q_offsets, const std::int32_t* k_offsets,
-            void* out, int tokens, int keys, int sequences, int q_heads, int kv_heads, int head_dim, float scale,
-            hipStream_t stream) {
-    const std::int64_t rows = static_cast<std::int64_t>(tokens) * q_heads;
-    packed_attention<T><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(
-        static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), q_offsets, k_offsets,
-        static_cast<T*>(out), tokens, keys, sequences, q_heads, kv_heads, head_dim, scale);
+__device__ void clear_rest(const std::int32_t* __restrict__ q_offsets, T* __restrict__ out, const Geometry& g, int head, int spare,
+                           int spares) {
+    int first = 0;
+    for (int i = threadIdx.x & 63; i <= g.sequences; i += 64) first = max(first, min(q_offsets[i], g.tokens));
+#pragma unroll
+    for (int step = 32; step; step >>= 1) first = max(first, __shfl_xor(first, step, 64));
+    const int units = g.group * g.head_dim / 8;
+    const std::int64_t count = static_cast<std::int64_t>(g.tokens - first) * units;
+    for (std::int64_t i = static_cast<std::int64_t>(spare) * kThreads + threadIdx.x; i < count; i += static_cast<std::int64_t>(spares) * kThreads) {
+        const std::int64_t token = i / units;
+        T* row = out + ((first + token) * g.q_heads + head * g.group) * g.head_dim;
+        reinterpret_cast<uint4*>(row)[i - token * units] = make_uint4(0, 0, 0, 0);
+    }
 }
 
-void require_geometry(int tokens, int keys, int sequences, int q_heads, int kv_heads, int head_dim) {
+template <class T, int D>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void packed_attention(
+    const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const std::int32_t* __restrict__ q_offsets,
+    const std::int32_t* __restrict__ k_offsets, T* __restrict__ out, Geometry g) {
+    __shared__ __align__(16) unsigned char memory[4 * Tile<D>::bytes];
+    // Neighbouring workgroups go to different XCDs, round robin: with the head as the fast index the workgroups of one head
+    // meet in few of the eight L2 caches.
+    const int head = blockIdx.x % g.kv_heads;
+    int sequence, block;
+    if (const int flat = blockIdx.x / g.kv_heads; !find_block(q_offsets, g, flat, sequence, block)) {
+        clear_rest(q_offsets, out, g, head, block, gridDim.x / g.kv_heads - (flat - block));
+        return;
+    }
+    const Span s = span_of(q_offsets, k_offsets, sequence, g);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 31, h = lane >> 5;
+    const int rows = s.queries * g.group;
+    const int first_row = block * kRows + wave * kWaveRows, row = first_row + m;
+    const bool live = row < rows;
+    const int token = live ? row / g.group : 0;
+    const std::int64_t place = (static_cast<std::int64_t>(s.q_first + token) * g.q_heads + head * g.group +
+                                (live ? row - token * g.group : 0)) * g.head_dim;
+    const int hidden = s.queries - s.keys;  // query i sees i + 1 - hidden keys
+    const int seen = live ? token + 1 - hidden : INT_MAX;
+    // The keys that the wave's first row sees, that its last one sees, and that the workgroup's last one sees.
+    const int least = first_row < rows ? first_row / g.group + 1 - hidden : 0;
+    const int most = first_row < rows ? min(first_row + kWaveRows - 1, rows - 1) / g.group + 1 - hidden : 0;
+    const int end = min(block * kRows + kRows - 1, rows - 1) / g.group + 1 - hidden;
+
+    State<D> a;
+    // A negative scale turns the queries' signs, so that the largest product is the largest score; 0 empties them.
+    const float factor = g.scale == 0.0f ? 1.0f : fabsf(g.scale) * 1.44269504088896340736f;
+    const std::uint32_t sign = g.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+        const int column = 16 * i + 8 * h;
+        a.query[i] = make_uint4(0, 0, 0, 0);
+        if (live && column < g.head_dim && g.scale != 0.0f) {
+            const uint4 x = *reinterpret_cast<const uint4*>(q + place + column);
+            a.query[i] = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) a.out[d][r] = 0.0f;
+    a.reference = -__builtin_inff();
+    a.sum = 0.0f;
+
+    constexpr int kKeys = Tile<D>::keys;
+    const std::int64_t stride = static_cast<std::int64_t>(g.kv_heads) * g.head_dim;
+    const T* key = k + s.k_first * stride + head * g.head_dim;
+    const T* value = v + s.k_first * stride + head * g.head_dim;
+    Stage<T, D> stage;
+    if (end > 0) {
+        stage.load(key, value, stride, s.keys, g.head_dim);
+        stage.store(memory, memory + Tile<D>::bytes);
+    }
+    __syncthreads();
+    for (int at = 0, turn = 0; at < end; at += kKeys, turn ^= 1) {
+        const unsigned char* now = memory + turn * (2 * Tile<D>::bytes);
+        unsigned char* next = memory + (turn ^ 1) * (2 * Tile<D>::bytes);
+        const bool more = at + kKeys < end;
+        if (more)
+            stage.load(key + (at + kKeys) * stride, value + (at + kKeys) * stride, stride, s.keys - at - kKeys, g.head_dim);
+        if (at < most) {
+            if (at + kKeys <= least)
+                compute<T, D, false>(now, now + Tile<D>::bytes, a, factor, 0);
+            else
+                compute<T, D, true>(now, now + Tile<D>::bytes, a, factor, seen - at);
+        }
+        if (more) stage.store(next, next + Tile<D>::bytes);
+        __syncthreads();
+    }
+    a.sum += __shfl_xor(a.sum, 32, 64);
+    const float scale = a.sum != 0.0f ? 1.0f / a.sum : 0.0f;
+    if (!live) return;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int column = 32 * d + 2 * r + 4 * h;
+            if (column >= g.head_dim) continue;
+            float x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = a.sum == 0.0f ? 0.0f : a.out[d][r + j] * scale;
+            *reinterpret_cast<uint2*>(out + place + column) = make_uint2(Matrix<T>::pack(x[0], x[1]), Matrix<T>::pack(x[2], x[3]));
+        }
+}
+
+Geometry geometry(int tokens, int keys, int sequences, int q_heads, int kv_heads, int head_dim, float scale) {
     require_head_dim(head_dim);
     require(tokens > 0 && keys > 0 && sequences > 0 && q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0,
             "invalid packed attention geometry");
+    const int group = q_heads / kv_heads;
+    require(static_cast<std::int64_t>(tokens) * group < (1ll << 31) - kRows, "packed attention rows of a KV head must fit int32");
+    const std::int64_t blocks = static_cast<std::int64_t>(tokens) * group / kRows + 1 + sequences;
+    require(blocks * kv_heads < (1ll << 31), "packed attention blocks must fit int32");
+    return {tokens, keys, sequences, q_heads, kv_heads, group, head_dim, scale};
+}
+
+template <class T, int D>
+void launch(const void* q, const void* k, const void* v, const std::int32_t* q_offsets, const std::int32_t* k_offsets, void* out,
+            const Geometry& g, hipStream_t stream) {
+    // Every sequence leaves at most one block that is not full; one more clears what no sequence covers.
+    const std::int64_t blocks = static_cast<std::int64_t>(g.tokens) * g.group / kRows + g.sequences + 1;
+    packed_attention<T, D><<<static_cast<unsigned>(blocks * g.kv_heads), kThreads, 0, stream>>>(
+        static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), q_offsets, k_offsets, static_cast<T*>(out), g);
+}
+
+template <class T>
+void launch_any(const void* q, const void* k, const void* v, const std::int32_t* q_offsets, const std::int32_t* k_offsets,
+                void* out, const Geometry& g, hipStream_t stream) {
+    const int padded = (g.head_dim + 31) / 32 * 32;
+    switch (padded) {
+        case 32: launch<T, 32>(q, k, v, q_offsets, k_offsets, out, g, stream); break;
+        case 64: launch<T, 64>(q, k, v, q_offsets, k_offsets, out, g, stream); break;
+        case 96: launch<T, 96>(q, k, v, q_offsets, k_offsets, out, g, stream); break;
+        case 128: launch<T, 128>(q, k, v, q_offsets, k_offsets, out, g, stream); break;
+        case 160: launch<T, 160>(q, k, v, q_offsets, k_offsets, out, g, stream); break;
+        case 192: launch<T, 192>(q, k, v, q_offsets, k_offsets, out, g, stream); break;
+        case 224: launch<T, 224>(q, k, v, q_offsets, k_offsets, out, g, stream); break;
+        default: launch<T, 256>(q, k, v, q_offsets, k_offsets, out, g, stream); break;
+    }
 }
 
 }  // namespace
@@ -63,7 +417,7 @@ void require_geometry(int tokens, int keys, int sequences, int q_heads, int kv_h
 
 VT_EXPORT std::uint64_t venturi_packed_attention_bytes(int tokens, int keys, int sequences, int q_heads, int kv_heads,
                                                        int head_dim) {
-    vt::host_guarded([&] { vt::require_geometry(tokens, keys, sequences, q_heads, kv_heads, head_dim); });
+    vt::host_guarded([&] { vt::geometry(tokens, keys, sequences, q_heads, kv_heads, head_dim, 1.0f); });
     return 0;
 }
 
@@ -72,16 +426,15 @@ VT_EXPORT int venturi_packed_attention_run(const void* q, const void* k, const v
                                            int tokens, int keys, int sequences, int q_heads, int kv_heads, int head_dim,
                                            float scale, int dtype, void* stream) {
     return vt::guarded([&] {
-        vt::require_geometry(tokens, keys, sequences, q_heads, kv_heads, head_dim);
+        const auto g = vt::geometry(tokens, keys, sequences, q_heads, kv_heads, head_dim, scale);
         vt::require(q && k && v && q_offsets && k_offsets && out, "null packed attention operand");
         vt::require(vt::aligned(q, 16) && vt::aligned(k, 16) && vt::aligned(v, 16) && vt::aligned(out, 16),
                     "packed attention rows must be 16-byte aligned");
         const auto s = static_cast<hipStream_t>(stream);
         if (dtype == vt::kF16)
-            vt::launch<__half>(q, k, v, q_offsets, k_offsets, out, tokens, keys, sequences, q_heads, kv_heads, head_dim, scale, s);
+            vt::launch_any<__half>(q, k, v, q_offsets, k_offsets, out, g, s);
         else if (dtype == vt::kBF16)
-            vt::launch<__hip_bfloat16>(q, k, v, q_offsets, k_offsets, out, tokens, keys, sequences, q_heads, kv_heads, head_dim,
-                                       scale, s);
+            vt::launch_any<__hip_bfloat16>(q, k, v, q_offsets, k_offsets, out, g, s);
         else
             throw vt::Invalid("packed attention takes fp16 or bf16");
     });
