@@ -65,8 +65,11 @@ class Recorder:
         self._native = native.load()
         self.launches = []
 
-    def _launch(self, entry, device, *operands):
-        self.launches.append(entry)
+    def _call(self, entry, device, arguments):
+        assert len(arguments) + 1 == len(entry.argtypes)
+        for value, kind in zip(arguments, entry.argtypes):
+            kind(value)
+        self.launches.append(entry.__name__)
 
     def resolve_device(self, device):
         return CPU

@@ -11,8 +11,8 @@ from dataclasses import dataclass, field
 
 import torch
 
-from .kv_cache import head_geometry, softmax_scale, vector_aligned
-from .operands import DTYPE_CODES, admit, disjoint, extents
+from .kv_cache import head_geometry, settle, softmax_scale
+from .operands import DTYPE_CODES, address, apart, device_index, extents, spans
 
 
 @dataclass(frozen=True)
@@ -32,6 +32,14 @@ class PackedAttentionPlan:
     device: torch.device
     _workspace: object = field(repr=False)
     workspace_bytes = 0  # nothing for the caller to provide
+
+    def __post_init__(self):
+        w = self._workspace
+        settle(self, _entry=self._backend._native.venturi_packed_attention_run, _index=device_index(self.device),
+               _q=(self.tokens, self.q_heads, self.head_dim), _k=(self.keys, self.kv_heads, self.head_dim),
+               _offsets=(self.sequences + 1,), _spans=spans(*self.storage_tensors),
+               _tail=(None if w is None else w.data_ptr(), 0 if w is None else w.numel(), self.tokens, self.keys, self.sequences,
+                      self.q_heads, self.kv_heads, self.head_dim, self.scale, DTYPE_CODES[self.dtype]))
 
     @property
     def storage_tensors(self):
@@ -60,14 +68,14 @@ class PackedAttentionPlan:
         [sequences + 1] on the device, ascending from 0. Queries that see no key, and rows past the last offset, get
         zeros. Offsets are not checked on the host; the kernel reads no row outside q, k and v whatever they hold.
         """
-        q_shape, k_shape = (self.tokens, self.q_heads, self.head_dim), (self.keys, self.kv_heads, self.head_dim)
-        for name, t, shape in (("q", q, q_shape), ("k", k, k_shape), ("v", v, k_shape), ("out", out, q_shape)):
-            admit(t, shape, self.dtype, self.device, name)
-        for name, t in (("q_offsets", q_offsets), ("k_offsets", k_offsets)):
-            admit(t, (self.sequences + 1,), torch.int32, self.device, name)
-        vector_aligned(q, k, v, out)
-        disjoint(out, (q, k, v, q_offsets, k_offsets) + self.storage_tensors)
-        self._backend._launch("venturi_packed_attention_run", self.device, q, k, v, q_offsets, k_offsets, out, self._workspace,
-                              0 if self._workspace is None else self._workspace.numel(), self.tokens, self.keys, self.sequences,
-                              self.q_heads, self.kv_heads, self.head_dim, self.scale, DTYPE_CODES[self.dtype])
+        dtype, device, index = self.dtype, self.device, self._index
+        x = address(q, self._q, dtype, device, index, "q")
+        a = address(k, self._k, dtype, device, index, "k")
+        b = address(v, self._k, dtype, device, index, "v")
+        m = address(q_offsets, self._offsets, torch.int32, device, index, "q_offsets", 4)
+        n = address(k_offsets, self._offsets, torch.int32, device, index, "k_offsets", 4)
+        y = address(out, self._q, dtype, device, index, "out")
+        size, rows, starts = 2 * self.tokens * self.q_heads * self.head_dim, 2 * self.keys * self.kv_heads * self.head_dim, 4 * self._offsets[0]
+        apart(y, size, (x, x + size), (a, a + rows), (b, b + rows), (m, m + starts), (n, n + starts), *self._spans)
+        self._backend._call(self._entry, device, (x, a, b, m, n, y, *self._tail))
         return out

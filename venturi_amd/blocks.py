@@ -171,6 +171,13 @@ class HipBackend(Backend):
         with on_device(device):
             self._check(getattr(self._native, entry)(*arguments, stream_of(device)))
 
+    def _call(self, entry, device, arguments):
+        """``_launch`` of an entry point's function with plain arguments."""
+        with on_device(device):
+            status = entry(*arguments, stream_of(device))
+        if status < 0:
+            self._check(status)
+
     def synchronize(self, device):
         torch.cuda.synchronize(self.resolve_device(device))
 

@@ -19,7 +19,7 @@ import math
 
 import torch
 
-from .operands import DTYPE_CODES, admit, disjoint, extents
+from .operands import DTYPE_CODES, address, apart, device_index, extents, spans
 from .rotary import RotaryEmbedding
 
 GROUP = 32
@@ -44,11 +44,10 @@ def softmax_scale(scale, head_dim):
     raise ValueError("attention scale must be a finite number")
 
 
-def vector_aligned(*tensors):
-    """The kernels move 16 bytes at a time."""
-    for t in tensors:
-        if t.data_ptr() % 16:
-            raise ValueError("attention operands require 16-byte alignment")
+def settle(plan, **values):
+    """Sets what a frozen plan computes once."""
+    for name, value in values.items():
+        object.__setattr__(plan, name, value)
 
 
 @dataclass(frozen=True)
@@ -151,6 +150,17 @@ class KVWritePlan:
     _rates: object
     workspace_bytes = 0
 
+    def __post_init__(self):
+        c, r = self.cache, self.rotary
+        settle(
+            self, _entry=c._backend._native.venturi_kv_write_run, _index=device_index(c.device),
+            _rows=(self.tokens, (self.q_heads + 2 * c.kv_heads) * c.head_dim), _at=(self.tokens,),
+            _q=(self.tokens, self.q_heads, c.head_dim), _k=(self.tokens, c.kv_heads, c.head_dim),
+            _spans=spans(*self.storage_tensors), _table=None if self._rates is None else self._rates.data_ptr(),
+            _tail=(*(t.data_ptr() for t in c.storage_tensors), self.tokens, self.q_heads, c.kv_heads, c.head_dim,
+                   0 if r is None else r.rotary_dim, int(r is not None and r.layout == "interleaved"),
+                   1.0 if r is None else r.factor, c.pages, c.page_tokens, DTYPE_CODES[c.dtype]))
+
     @property
     def storage_tensors(self):
         return self.cache.storage_tensors + (() if self._rates is None else (self._rates,))
@@ -163,29 +173,25 @@ class KVWritePlan:
         the device. A row whose slot lies outside the cache (-1: padding) is not cached. Rows that share a slot leave
         one of theirs there, unspecified which.
         """
-        c = self.cache
-        admit(rows, (self.tokens, (self.q_heads + 2 * c.kv_heads) * c.head_dim), c.dtype, c.device, "rows")
-        admit(slots, (self.tokens,), torch.int64, c.device, "slots")
-        inputs = (rows, slots) + self.storage_tensors
-        if self._rates is not None:
-            admit(positions, (self.tokens,), torch.int64, c.device, "positions")
-            inputs += (positions,)
+        c, index, tokens = self.cache, self._index, self.tokens
+        dtype, device = c.dtype, c.device
         if (q is None) != (self.q_heads == 0):
             raise ValueError("q is the output of the plan's q heads: required with them, refused without")
-        vector_aligned(rows)
-        if q is not None:
-            admit(q, (self.tokens, self.q_heads, c.head_dim), c.dtype, c.device, "q")
-            vector_aligned(q)
-            disjoint(q, inputs if k is None else inputs + (k,))
+        x = address(rows, self._rows, dtype, device, index, "rows")
+        s = address(slots, self._at, torch.int64, device, index, "slots", 8)
+        inputs = ((x, x + 2 * tokens * self._rows[1]), (s, s + 8 * tokens)) + self._spans
+        p = y = z = None
+        if self._table is not None:
+            p = address(positions, self._at, torch.int64, device, index, "positions", 8)
+            inputs += ((p, p + 8 * tokens),)
         if k is not None:
-            admit(k, (self.tokens, c.kv_heads, c.head_dim), c.dtype, c.device, "k")
-            vector_aligned(k)
-            disjoint(k, inputs)
-        r = self.rotary
-        c._backend._launch("venturi_kv_write_run", c.device, rows, None if r is None else positions, slots, self._rates, q, k,
-                           *c.storage_tensors, self.tokens, self.q_heads, c.kv_heads, c.head_dim,
-                           0 if r is None else r.rotary_dim, int(r is not None and r.layout == "interleaved"),
-                           1.0 if r is None else r.factor, c.pages, c.page_tokens, DTYPE_CODES[c.dtype])
+            z, size = address(k, self._k, dtype, device, index, "k"), 2 * tokens * c.kv_heads * c.head_dim
+            apart(z, size, *inputs)
+            inputs += ((z, z + size),)
+        if q is not None:
+            y = address(q, self._q, dtype, device, index, "q")
+            apart(y, 2 * tokens * self.q_heads * c.head_dim, *inputs)
+        c._backend._call(self._entry, device, (x, p, s, self._table, y, z, *self._tail))
         return q
 
 
@@ -195,6 +201,13 @@ class KVReadPlan:
     tokens: int
     workspace_bytes = 0
 
+    def __post_init__(self):
+        c = self.cache
+        settle(self, _entry=c._backend._native.venturi_kv_read_run, _index=device_index(c.device), _at=(self.tokens,),
+               _rows=(self.tokens, c.kv_heads, c.head_dim), _spans=spans(*c.storage_tensors),
+               _planes=tuple(t.data_ptr() for t in c.storage_tensors),
+               _tail=(self.tokens, c.kv_heads, c.head_dim, c.pages, c.page_tokens, DTYPE_CODES[c.dtype]))
+
     @property
     def storage_tensors(self):
         return self.cache.storage_tensors
@@ -202,20 +215,20 @@ class KVReadPlan:
     def run(self, slots, *, keys=None, values=None):
         """Writes the cached rows of ``slots`` (int64 [tokens]) to ``keys`` and ``values`` [tokens, kv_heads, head_dim]
         (either may be left out). A slot outside the cache reads as NaN."""
-        c = self.cache
-        admit(slots, (self.tokens,), torch.int64, c.device, "slots")
-        inputs = (slots,) + c.storage_tensors
         if keys is None and values is None:
             raise ValueError("reading needs keys, values or both")
-        for name, out in (("keys", keys), ("values", values)):
-            if out is not None:
-                admit(out, (self.tokens, c.kv_heads, c.head_dim), c.dtype, c.device, name)
-                vector_aligned(out)
-                disjoint(out, inputs)
-        if keys is not None and values is not None:
-            disjoint(keys, (values,))
-        c._backend._launch("venturi_kv_read_run", c.device, *c.storage_tensors, slots, keys, values, self.tokens, c.kv_heads,
-                           c.head_dim, c.pages, c.page_tokens, DTYPE_CODES[c.dtype])
+        c, index = self.cache, self._index
+        s = address(slots, self._at, torch.int64, c.device, index, "slots", 8)
+        inputs = ((s, s + 8 * self.tokens),) + self._spans
+        size, k, v = 2 * self.tokens * c.kv_heads * c.head_dim, None, None
+        if keys is not None:
+            k = address(keys, self._rows, c.dtype, c.device, index, "keys")
+            apart(k, size, *inputs)
+            inputs += ((k, k + size),)
+        if values is not None:
+            v = address(values, self._rows, c.dtype, c.device, index, "values")
+            apart(v, size, *inputs)
+        c._backend._call(self._entry, c.device, (*self._planes, s, k, v, *self._tail))
         return keys, values
 
 
@@ -229,6 +242,15 @@ class KVAttentionPlan:
     scale: float
     workspace_bytes: int
 
+    def __post_init__(self):
+        c = self.cache
+        settle(self, _entry=c._backend._native.venturi_kv_attention_run, _index=device_index(c.device),
+               _rows=(self.sequences * self.query_tokens, self.q_heads, c.head_dim), _table=(self.sequences, self.max_pages),
+               _lengths=(self.sequences,), _spans=spans(*c.storage_tensors),
+               _planes=tuple(t.data_ptr() for t in c.storage_tensors),
+               _tail=(self.workspace_bytes, self.sequences, self.query_tokens, self.q_heads, c.kv_heads, c.head_dim, c.pages,
+                      c.page_tokens, self.max_pages, self.scale, DTYPE_CODES[c.dtype]))
+
     @property
     def storage_tensors(self):
         return self.cache.storage_tensors
@@ -241,24 +263,19 @@ class KVAttentionPlan:
         key get zeros, and sequences whose length lies outside [0, max_pages * page_tokens], or that reach a page
         outside the cache, get NaN. Page table entries past a sequence's length are not read.
         """
-        c = self.cache
-        shape = (self.sequences * self.query_tokens, self.q_heads, c.head_dim)
-        admit(q, shape, c.dtype, c.device, "q")
-        admit(page_table, (self.sequences, self.max_pages), torch.int32, c.device, "page_table")
-        admit(lengths, (self.sequences,), torch.int32, c.device, "lengths")
-        admit(out, shape, c.dtype, c.device, "out")
-        vector_aligned(q, out)
-        inputs = (q, page_table, lengths) + c.storage_tensors
+        c, index = self.cache, self._index
+        device = c.device
+        x = address(q, self._rows, c.dtype, device, index, "q")
+        t = address(page_table, self._table, torch.int32, device, index, "page_table", 4)
+        n = address(lengths, self._lengths, torch.int32, device, index, "lengths", 4)
+        y = address(out, self._rows, c.dtype, device, index, "out")
+        size = 2 * self._rows[0] * self.q_heads * c.head_dim
+        inputs = ((x, x + size), (t, t + 4 * self.sequences * self.max_pages), (n, n + 4 * self.sequences)) + self._spans
+        w = None
         if self.workspace_bytes:
-            admit(workspace, (self.workspace_bytes,), torch.uint8, c.device, "workspace")
-            if workspace.data_ptr() % 256:
-                raise ValueError("attention workspace requires 256-byte alignment")
-            disjoint(workspace, inputs)
-            disjoint(out, inputs + (workspace,))
-        else:
-            disjoint(out, inputs)
-        c._backend._launch("venturi_kv_attention_run", c.device, q, *c.storage_tensors, page_table, lengths, out,
-                           workspace if self.workspace_bytes else None, self.workspace_bytes, self.sequences, self.query_tokens,
-                           self.q_heads, c.kv_heads, c.head_dim, c.pages, c.page_tokens, self.max_pages, self.scale,
-                           DTYPE_CODES[c.dtype])
+            w = address(workspace, (self.workspace_bytes,), torch.uint8, device, index, "workspace", 256)
+            apart(w, self.workspace_bytes, *inputs)
+            inputs += ((w, w + self.workspace_bytes),)
+        apart(y, size, *inputs)
+        c._backend._call(self._entry, device, (x, *self._planes, t, n, y, w, *self._tail))
         return out

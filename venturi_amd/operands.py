@@ -70,6 +70,38 @@ def disjoint(out, operands, *, allow_inplace=False):
                 raise ValueError("output/workspace must not alias operand storage")
 
 
+# Plans whose kernels take as long as their host checks hold what never changes (shapes, sizes, the spans of their own
+# storage, the constant arguments) and read each operand's address once.
+def address(tensor, shape, dtype, device, index, name, align=16):
+    """The data pointer of an operand that passes ``admit`` and is aligned. ``index`` is ``device_index(device)``: one
+    integer comparison in place of two device objects."""
+    if not (isinstance(tensor, torch.Tensor) and tensor.shape == shape and tensor.dtype is dtype
+            and tensor.get_device() == index and tensor.is_contiguous() and not tensor.requires_grad):
+        admit(tensor, shape, dtype, device, name)
+    pointer = tensor.data_ptr()
+    if pointer % align:
+        raise ValueError(f"{name} requires {align}-byte alignment")
+    return pointer
+
+
+def device_index(device):
+    """What ``Tensor.get_device`` returns on a device."""
+    return -1 if device.type == "cpu" else device.index
+
+
+def spans(*tensors):
+    """[first, end) of every tensor, as ``apart`` takes them."""
+    return tuple(byte_span(t) for t in tensors)
+
+
+def apart(first, size, *others):
+    """Rejects an output of ``size`` bytes at ``first`` that shares a byte with one of the (first, end) spans."""
+    end = first + size
+    for start, stop in others:
+        if start < end and first < stop:
+            raise ValueError("output/workspace must not alias operand storage")
+
+
 def epsilon(value):
     """RMSNorm epsilon as a float: finite and within [smallest normal, largest] fp32."""
     if type(value) in (int, float) and math.isfinite(value) and _F32.tiny <= value <= _F32.max:

@@ -19,7 +19,8 @@ from dataclasses import dataclass, field
 
 import torch
 
-from .operands import DTYPE_CODES, admit, disjoint, extents
+from .kv_cache import settle
+from .operands import DTYPE_CODES, address, apart, device_index, extents, spans
 
 _SETTINGS = (("temperature", torch.float32), ("top_k", torch.int32), ("top_p", torch.float32), ("min_p", torch.float32))
 
@@ -36,6 +37,13 @@ class SamplingPlan:
     device: torch.device
     _workspace: object = field(repr=False)
     workspace_bytes = 0  # nothing for the caller to provide
+
+    def __post_init__(self):
+        w = self._workspace
+        settle(self, _entry=self._backend._native.venturi_sample_run, _index=device_index(self.device), _logits=(self.rows, self.vocab),
+               _row=(self.rows,), _spans=spans(*self.storage_tensors),
+               _tail=(None if w is None else w.data_ptr(), 0 if w is None else w.numel(), self.rows, self.vocab,
+                      DTYPE_CODES[self.dtype]))
 
     @property
     def storage_tensors(self):
@@ -61,23 +69,21 @@ class SamplingPlan:
         """``logits`` [rows, vocab], ``uniforms`` fp32 [rows]; per-row settings ``temperature``, ``top_p``, ``min_p`` fp32
         and ``top_k`` int32 [rows], each None for 1, no limit, no limit and no limit. Writes ``tokens`` int64 [rows] and,
         where given, ``probabilities`` fp32 [rows]."""
-        rows = (self.rows,)
-        admit(logits, (self.rows, self.vocab), self.dtype, self.device, "logits")
-        admit(uniforms, rows, torch.float32, self.device, "uniforms")
-        if logits.data_ptr() % 16:
-            raise ValueError("logits require 16-byte alignment")
-        inputs = [logits, uniforms]
+        device, index, row, size = self.device, self._index, self._row, 4 * self.rows
+        x = address(logits, self._logits, self.dtype, device, index, "logits")
+        u = address(uniforms, row, torch.float32, device, index, "uniforms", 4)
+        inputs = [(x, x + 2 * self.rows * self.vocab), (u, u + size), *self._spans]
+        settings = []
         for (name, dtype), value in zip(_SETTINGS, (temperature, top_k, top_p, min_p)):
+            pointer = None
             if value is not None:
-                admit(value, rows, dtype, self.device, name)
-                inputs.append(value)
-        inputs.extend(self.storage_tensors)
-        admit(tokens, rows, torch.int64, self.device, "tokens")
-        disjoint(tokens, inputs)
+                pointer = address(value, row, dtype, device, index, name, 4)
+                inputs.append((pointer, pointer + size))
+            settings.append(pointer)
+        t, p = address(tokens, row, torch.int64, device, index, "tokens", 8), None
+        apart(t, 2 * size, *inputs)
         if probabilities is not None:
-            admit(probabilities, rows, torch.float32, self.device, "probabilities")
-            disjoint(probabilities, inputs + [tokens])
-        self._backend._launch("venturi_sample_run", self.device, logits, uniforms, temperature, top_k, top_p, min_p, tokens,
-                              probabilities, self._workspace, 0 if self._workspace is None else self._workspace.numel(),
-                              self.rows, self.vocab, DTYPE_CODES[self.dtype])
+            p = address(probabilities, row, torch.float32, device, index, "probabilities", 4)
+            apart(p, size, (t, t + 2 * size), *inputs)
+        self._backend._call(self._entry, device, (x, u, *settings, t, p, *self._tail))
         return tokens
