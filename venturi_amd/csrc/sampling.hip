@@ -1,13 +1,16 @@
 // Sampling one token per row of 16-bit logits from given random numbers.
 //
 // A 16-bit logit has 65536 values, so a row's order is its histogram: classes of equal logits from the largest down,
-// ties by index within a class. The workgroup of a row counts the classes in LDS (whole numbers: the order of the
-// atomics leaves no trace), sums count * exp((v - max) / T) over steps of 64 neighbouring classes in 64 bits, and finds
-// the borders of top-k, top-p and min-p and the place of u in the prefix sums. 64 bits, because a border of a large
-// vocabulary is a token of 1e-6 of the mass, and one token more or less there moves every later draw. Only a class that
-// occurs costs an exponential. The token is then the class's rank-th occurrence in the row.
+// ties by index within a class. The workgroup of a row counts the classes in LDS by their bits (whole numbers: the order
+// of the atomics leaves no trace), sums count * exp((v - max) / T) in 64 bits, and finds the borders of top-k, top-p and
+// min-p and the place of u in the prefix sums. 64 bits, because a border of a large vocabulary is a token of 1e-6 of the
+// mass, and one token more or less there moves every later draw. The token is then the class's rank-th occurrence.
 //
-// Counters are 16 bits wide (128 KB of the CU's 160 KB): a row of more than 65535 logits is counted in segments, and
+// Weights. A lane holds 16 neighbouring classes, which are evenly spaced: their weights are the first one's times powers
+// of exp(-spacing / T), two exponentials for 16 classes (at most 16 roundings of 2^-53 apart from the exact ones). A turn
+// is a wave's 1024 classes; the 64 turns' sums are one scan, and only turns that a border falls into are opened again.
+//
+// Counters are 16 bits wide (128 KB of the CU's 160 KB): a row of more than 57344 logits is counted in segments, and
 // between two segments every class that has reached 16384 moves to a list (at most one entry per 16384 logits).
 #include "common.hpp"
 
@@ -15,17 +18,15 @@ namespace vt {
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kSteps = 1024;               // of 64 classes
-constexpr int kTurns = kSteps / 16;        // of 16 steps
+constexpr int kTurns = 64;                 // of 1024 classes, 16 a lane
 constexpr int kMaxVocab = 1 << 20;
 constexpr std::uint32_t kHeavy = 16384;
 constexpr int kHeavyEntries = 2 * kMaxVocab / kHeavy;
-constexpr std::uint32_t kNone = 0;         // the sort key of logits that are never taken
+constexpr int kNone = -1;                  // no class
 // Vectors of 8 logits that a thread counts before the first sweep for heavy classes (57344 logits), and between two
 // sweeps (49152, on counters below 16384).
 constexpr int kFirst = 7, kNext = 6;
 
-// Ascending sort key of a logit's bits: 0 for -inf and NaN, equal for both zeros.
 template <class T> struct Bits;
 template <> struct Bits<__half> {
     static constexpr std::uint32_t kInf = 0x7c00;
@@ -36,42 +37,54 @@ template <> struct Bits<__hip_bfloat16> {
     static constexpr int kMantissa = 7;
 };
 
+// Classes by place: 0 .. 32767 are the positive numbers from bits 0x7fff down to 0, the rest the negative ones from 0x8000
+// up. -0 belongs to the class of 0; the places of NaN and -inf hold no class.
+__device__ __forceinline__ std::uint32_t place_bits(int place) { return place < 32768 ? 32767 - place : place; }
+
 template <class T>
-__device__ __forceinline__ std::uint32_t sort_key(std::uint32_t bits) {
-    const std::uint32_t size = bits & 0x7fff;
-    if (size > Bits<T>::kInf || bits == (0x8000 | Bits<T>::kInf)) return kNone;
-    return size == 0 || !(bits & 0x8000) ? size | 0x8000 : bits ^ 0xffff;
+__device__ __forceinline__ bool is_class(int place) {
+    const std::uint32_t bits = place_bits(place);
+    return (bits & 0x7fff) <= Bits<T>::kInf && bits != (0x8000 | Bits<T>::kInf) && bits != 0x8000;
 }
 
 template <class T>
-__device__ __forceinline__ double key_value(std::uint32_t key) {
-    const auto bits = static_cast<unsigned short>(key & 0x8000 ? key ^ 0x8000 : key ^ 0xffff);
-    return static_cast<double>(to_f32(__builtin_bit_cast(T, bits)));
+__device__ __forceinline__ double class_value(int place) {
+    return static_cast<double>(to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(place_bits(place)))));
 }
 
-// The step between neighbouring classes at a key.
+// The difference of neighbouring classes at a place.
 template <class T>
-__device__ __forceinline__ double key_step(std::uint32_t key) {
-    const std::uint32_t size = (key & 0x8000 ? key : key ^ 0xffff) & 0x7fff;
-    const std::uint32_t low = size & ~((1u << Bits<T>::kMantissa) - 1);  // the binade's first
-    return key_value<T>(0x8000 | (low + 1)) - key_value<T>(0x8000 | low);
+__device__ __forceinline__ double class_step(int place) {
+    const std::uint32_t low = place_bits(place) & 0x7fff & ~((1u << Bits<T>::kMantissa) - 1);  // the binade's first
+    const auto value = [](std::uint32_t bits) {
+        return static_cast<double>(to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(bits))));
+    };
+    return value(low + 1) - value(low);
 }
 
+constexpr std::uint32_t kNoLogits = 0x7fff7fff;  // two NaN
+
+// A row as aligned vectors of 8 logits, of which the first and the last may lie partly outside it: those two are read
+// element by element, once, so that the others need no check beside their load.
 template <class T>
 struct Row {
     const unsigned short* logits;  // the tensor, 16-byte aligned
     std::int64_t first, end;       // the row's elements
     std::int64_t vector0;          // the aligned vector of 8 that holds its first
-    int vectors;
+    int vectors, whole0, whole1;   // the vectors that lie inside: whole0 .. whole1 - 1
+    uint4 head, tail;
 
     __device__ __forceinline__ Row(const void* tensor, int index, int vocab)
         : logits(static_cast<const unsigned short*>(tensor)), first(static_cast<std::int64_t>(index) * vocab), end(first + vocab),
-          vector0(first >> 3), vectors(static_cast<int>(((end + 7) >> 3) - vector0)) {}
+          vector0(first >> 3), vectors(static_cast<int>(((end + 7) >> 3) - vector0)) {
+        whole0 = first & 7 ? 1 : 0;
+        whole1 = vectors - (end & 7 ? 1 : 0);
+        head = part(0);
+        tail = part(vectors - 1);
+    }
 
-    // Vector i's logits; NaN bits for elements outside the row.
-    __device__ __forceinline__ uint4 load(int i) const {
+    __device__ __forceinline__ uint4 part(int i) const {
         const std::int64_t at = (vector0 + i) * 8;
-        if (at >= first && at + 8 <= end) return *reinterpret_cast<const uint4*>(logits + at);
         std::uint32_t u[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -79,6 +92,19 @@ struct Row {
             u[j] = (e >= first && e < end ? logits[e] : 0x7fffu) | (e + 1 >= first && e + 1 < end ? logits[e + 1] : 0x7fffu) << 16;
         }
         return make_uint4(u[0], u[1], u[2], u[3]);
+    }
+
+    // Vector i, for 0 <= i; NaN outside the row.
+    __device__ __forceinline__ uint4 load(int i) const {
+        uint4 w = make_uint4(kNoLogits, kNoLogits, kNoLogits, kNoLogits);
+        if (whole0 < whole1) {  // the same for the whole grid row: no lane waits for another's load
+            const auto* at = reinterpret_cast<const uint4*>(logits) + vector0 + min(max(i, whole0), whole1 - 1);
+            w = *at;
+        }
+        if (i < whole0) w = head;
+        else if (i >= vectors) w = make_uint4(kNoLogits, kNoLogits, kNoLogits, kNoLogits);
+        else if (i >= whole1) w = tail;
+        return w;
     }
 };
 
@@ -128,36 +154,30 @@ struct Settings {
 };
 
 struct Shared {
-    std::uint32_t histogram[32768];  // classes k (low half) and k + 32768 (high half)
-    double mass_before[kSteps + 1];
-    int count_before[kSteps + 1];
-    std::uint32_t heavy_key[kHeavyEntries], heavy_count[kHeavyEntries];
-    double wave_mass[kWaves];
-    int wave_count[kWaves];
+    std::uint32_t histogram[32768];  // of bits b (low half) and b + 0x8000 (high half)
+    double turn_mass[kTurns];
+    int turn_count[kTurns];
+    std::uint32_t heavy_bits[kHeavyEntries], heavy_count[kHeavyEntries];
     double probability;
-    int heavy, top, above_min, positive, rank, count, last;
-    std::uint32_t key;
+    int heavy, top, above_min, positive, place, rank, count;
 };
 
-// A row's chosen class: its key (kNone: nothing to take), and which of its `count` occurrences.
+// A row's chosen class (kNone: nothing to take), and which of its `count` occurrences.
 struct Choice {
-    std::uint32_t key;
-    int rank, count;
+    int place, rank, count;
 };
 
 __device__ __forceinline__ void clear(Shared& s) {
     for (int i = threadIdx.x; i < 32768 / 4; i += kThreads) reinterpret_cast<uint4*>(s.histogram)[i] = make_uint4(0, 0, 0, 0);
-    if (threadIdx.x == 0) s.heavy = s.top = s.above_min = s.positive = 0;
+    if (threadIdx.x == 0) s.heavy = s.above_min = s.positive = 0, s.top = 65536;
     __syncthreads();
 }
 
-template <class T>
-__device__ __forceinline__ void count_vector(Shared& s, const uint4& w, std::uint32_t& top) {
+__device__ __forceinline__ void count_vector(Shared& s, const uint4& w) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const std::uint32_t key = sort_key<T>(element(w, j));
-        top = max(top, key);
-        if (key != kNone) atomicAdd(&s.histogram[key & 0x7fff], 1u << (16 * (key >> 15)));
+        const std::uint32_t bits = element(w, j);
+        atomicAdd(&s.histogram[bits & 0x7fff], bits & 0x8000 ? 0x10000u : 1u);
     }
 }
 
@@ -172,7 +192,7 @@ __device__ __forceinline__ void sweep(Shared& s) {
             const std::uint32_t n = (word >> (16 * half)) & 0xffff;
             if (n >= kHeavy) {
                 const int e = atomicAdd(&s.heavy, 1);
-                s.heavy_key[e] = i + 32768 * half;
+                s.heavy_bits[e] = i + 32768 * half;
                 s.heavy_count[e] = n;
                 word -= n << (16 * half);
             }
@@ -182,93 +202,118 @@ __device__ __forceinline__ void sweep(Shared& s) {
     __syncthreads();
 }
 
-__device__ __forceinline__ int class_count(const Shared& s, std::uint32_t key) {
-    std::uint32_t n = (s.histogram[key & 0x7fff] >> (16 * (key >> 15))) & 0xffff;
-    for (int e = 0; e < s.heavy; ++e) n += s.heavy_key[e] == key ? s.heavy_count[e] : 0;
-    return static_cast<int>(n);
-}
-
-// Keys of a step, one a lane, falling; the weight of a class is the step's first occurring class's times
-// exp(-distance * spacing / T): neighbouring classes are evenly spaced within a step, so 16 steps of one binade share the
-// second factor and compute their first ones side by side. Both exponents are at most 0.
-__device__ __forceinline__ std::uint32_t step_key(int step) { return 65535 - (step * 64 + (threadIdx.x & 63)); }
-
+// A lane's 16 classes of a turn: places 1024 turn + 16 lane + i.
 template <class T>
-__device__ __forceinline__ double first_weight(std::uint32_t key, std::uint32_t top, double max_value, double heat) {
-    return key == top ? 1.0 : exp((key_value<T>(key) - max_value) / heat);
-}
-template <class T>
-__device__ __forceinline__ double distance_weight(std::uint32_t key, double heat) {
-    const int lane = threadIdx.x & 63;
-    return lane == 0 ? 1.0 : exp(-(lane * key_step<T>(key)) / heat);
-}
-// distance[lane - first], or 0 below it.
-__device__ __forceinline__ double at_distance(double distance, int first) {
-    const int lane = threadIdx.x & 63;
-    const double w = __shfl(distance, max(lane - first, 0), 64);
-    return lane >= first ? w : 0.0;
-}
+struct Lane {
+    int n[16];       // occurrences; 0 where there is no class
+    int first;       // weights start at class `first` (classes above the row's largest do not occur)
+    double start, ratio;
 
-// The largest step that passes a test which holds up to some step; every lane gets it.
-template <class Test>
-__device__ __forceinline__ int last_step(Test&& test) {
-    int passed = 0;
+    // Whether any of the turn's classes (or of the places without one) occurs in the counters.
+    static __device__ __forceinline__ bool occurs(const Shared& s, int heavy, int turn) {
+        const int place = 1024 * turn + 16 * static_cast<int>(threadIdx.x & 63);
+        const bool negative = turn >= kTurns / 2;
+        const auto* words = reinterpret_cast<const uint4*>(s.histogram + (negative ? place - 32768 : 32767 - 15 - place));
+        std::uint32_t any = 0;
 #pragma unroll
-    for (int i = 0; i < kSteps; i += 64) passed += __popcll(__ballot(test(i + static_cast<int>(threadIdx.x & 63))));
-    return max(passed - 1, 0);
-}
+        for (int i = 0; i < 4; ++i) {
+            const uint4 w = words[i];
+            any |= w.x | w.y | w.z | w.w;
+        }
+        return heavy > 0 || turn == kTurns / 2 - 1 || (negative ? any >> 16 : any & 0xffff) != 0;
+    }
 
-// Chooses from the workgroup's complete histogram; s.top has to hold the largest key.
+    __device__ __forceinline__ bool count(const Shared& s, int heavy, int turn) {
+        const int place = 1024 * turn + 16 * static_cast<int>(threadIdx.x & 63);
+        const bool negative = turn >= kTurns / 2;
+        const auto* words = reinterpret_cast<const uint4*>(s.histogram + (negative ? place - 32768 : 32767 - 15 - place));
+        const uint4 w[4] = {words[0], words[1], words[2], words[3]};
+        std::uint32_t u[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[4 * i] = w[i].x, u[4 * i + 1] = w[i].y, u[4 * i + 2] = w[i].z, u[4 * i + 3] = w[i].w;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) n[i] = negative ? u[i] >> 16 : u[15 - i] & 0xffff;
+        if (turn == kTurns / 2 - 1 && place == 32767 - 15) n[15] += s.histogram[0] >> 16;  // -0
+        for (int e = 0; e < heavy; ++e) {
+            const std::uint32_t bits = s.heavy_bits[e] == 0x8000 ? 0 : s.heavy_bits[e];
+            const int at = (bits & 0x8000 ? static_cast<int>(bits) : 32767 - static_cast<int>(bits)) - place;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) n[i] += at == i ? s.heavy_count[e] : 0;
+        }
+        // Places without a class: NaN and -inf at both halves' ends, and -0.
+        if (turn == 0 || turn == kTurns / 2 || turn == kTurns - 1) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) n[i] = is_class<T>(place + i) ? n[i] : 0;
+        }
+        bool some = false;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) some = some || n[i];
+        return some;
+    }
+
+    // Every exponent is at most 0: nothing overflows, whatever the temperature.
+    __device__ __forceinline__ void weigh(int turn, int top, double max_value, double heat) {
+        const int place = 1024 * turn + 16 * static_cast<int>(threadIdx.x & 63);
+        first = top > place ? top - place : 0;  // 16 and more: the lane's classes all lie above
+        start = first == 0 && place != top ? exp((class_value<T>(place) - max_value) / heat) : 1.0;
+        ratio = exp(-class_step<T>(place) / heat);
+    }
+
+    // Visits the lane's classes in order: (index, occurrences, weight).
+    template <class Visit>
+    __device__ __forceinline__ void each(Visit&& visit) const {
+        double w = start;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            visit(i, n[i], n[i] ? w : 0.0);
+            if (i >= first) w *= ratio;
+        }
+    }
+};
+
+// Chooses from the workgroup's complete histogram.
 template <class T>
 __device__ Choice choose(Shared& s, const Settings& set) {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const std::uint32_t top = s.top;
-    if (top == kNone) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, heavy = s.heavy;
+    for (int turn = wave; turn < kTurns; turn += kWaves) {
+        if (!__any(Lane<T>::occurs(s, heavy, turn))) continue;
+        Lane<T> l;
+        const unsigned long long occurs = __ballot(l.count(s, heavy, turn));
+        if (!occurs) continue;
+        if (lane == __ffsll(occurs) - 1) {
+            int at = 16;
+#pragma unroll
+            for (int i = 15; i >= 0; --i) at = l.n[i] ? i : at;
+            atomicMin(&s.top, 1024 * turn + 16 * lane + at);
+        }
+        break;  // this wave's other turns lie below
+    }
+    __syncthreads();
+    const int top = s.top;
+    if (top >= 65536) {
         if (t == 0) s.probability = 0.0;
         __syncthreads();
         return {kNone, 0, 0};
     }
-    if (!(set.temperature > 0.0f)) {
-        if (t == 0) s.probability = 1.0;
-        __syncthreads();
-        return {top, 0, class_count(s, top)};
-    }
-    const double max_value = key_value<T>(top), heat = fminf(set.temperature, 3.402823466e38f), least = set.min_p;
+    const double max_value = class_value<T>(top), heat = fminf(set.temperature, 3.402823466e38f), least = set.min_p;
+    const bool greedy = !(set.temperature > 0.0f);
     int above_min = 0, positive = 0;
-    for (int turn = wave; turn < kTurns; turn += kWaves) {
-        int n[16], first = 0, some = 0;  // lane i < 16 keeps step i's first occurring class
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const std::uint32_t key = step_key(turn * 16 + i);
-            n[i] = key != kNone ? class_count(s, key) : 0;
-            const unsigned long long occurs = __ballot(n[i] != 0);
-            some |= occurs ? 1 << i : 0;
-            const int at = occurs ? __ffsll(occurs) - 1 : 0;
-            first = lane == i ? at : first;
-        }
-        double mass = 0.0;  // lane i < 16 keeps step i's mass and count
+    for (int turn = wave; turn < kTurns && !greedy; turn += kWaves) {
+        Lane<T> l;
+        double mass = 0.0;
         int count = 0;
-        if (some) {
-            const std::uint32_t own = 65535 - ((turn * 16 + (lane & 15)) * 64 + first);
-            const double start = first_weight<T>(own, top, max_value, heat);
-            double distance = 0.0;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                constexpr int kShared = (1 << Bits<T>::kMantissa) / 64;  // steps of a binade
-                if (i % (kShared < 16 ? kShared : 16) == 0 && (some >> i) & ((1 << (kShared < 16 ? kShared : 16)) - 1))
-                    distance = distance_weight<T>(step_key(turn * 16 + i), heat);
-                if (!((some >> i) & 1)) continue;
-                const double w = lane_double(start, i) * at_distance(distance, lane_int(first, i));
-                if (n[i]) {
-                    above_min += w >= least ? n[i] : 0;
-                    positive += w > 0.0 ? n[i] : 0;
-                }
-                const double step_mass = wave_sum(n[i] * w);
-                const int step_count = wave_sum(n[i]);
-                if (lane == i) mass = step_mass, count = step_count;
-            }
+        if (__any(Lane<T>::occurs(s, heavy, turn)) && __any(l.count(s, heavy, turn))) {
+            l.weigh(turn, top, max_value, heat);
+            l.each([&](int, int n, double w) {
+                mass += n * w;
+                count += n;
+                above_min += w >= least ? n : 0;
+                positive += w > 0.0 ? n : 0;
+            });
+            mass = wave_sum(mass);
+            count = wave_sum(count);
         }
-        if (lane < 16) s.mass_before[turn * 16 + lane] = mass, s.count_before[turn * 16 + lane] = count;
+        if (lane == 0) s.turn_mass[turn] = mass, s.turn_count[turn] = count;
     }
     above_min = wave_sum(above_min);
     positive = wave_sum(positive);
@@ -277,100 +322,119 @@ __device__ Choice choose(Shared& s, const Settings& set) {
         if (positive) atomicAdd(&s.positive, positive);
     }
     __syncthreads();
-    const double mass_scan = wave_scan(s.mass_before[t]);
-    const int count_scan = wave_scan(s.count_before[t]);
-    if (lane == 63) s.wave_mass[wave] = mass_scan, s.wave_count[wave] = count_scan;
-    __syncthreads();
-    double mass_base = 0.0;
-    int count_base = 0;
-    for (int i = 0; i < wave; ++i) mass_base += s.wave_mass[i], count_base += s.wave_count[i];
-    s.mass_before[t + 1] = mass_base + mass_scan;
-    s.count_before[t + 1] = count_base + count_scan;
-    if (t == 0) s.mass_before[0] = 0.0, s.count_before[0] = 0;
-    __syncthreads();
     if (wave == 0) {
-        const int all = s.count_before[kSteps];
-        // The lane's class of a step: its key, count, weight and what comes before it in the whole order.
-        std::uint32_t key;
-        int n, before;
-        double w, mass_at;
-        const auto open = [&](int step) {
-            key = step_key(step);
-            n = key != kNone ? class_count(s, key) : 0;
-            const unsigned long long occurs = __ballot(n != 0);
-            const int first = occurs ? __ffsll(occurs) - 1 : 0;
-            const double start = first_weight<T>(65535 - (step * 64 + first), top, max_value, heat);
-            w = start * at_distance(distance_weight<T>(key, heat), first);  // every lane takes part in the exchange
-            if (!n) w = 0.0;
-            before = s.count_before[step] + wave_scan(n) - n;
-            const double scan = wave_scan(n * w), below = __shfl_up(scan, 1, 64);
-            mass_at = s.mass_before[step] + (lane ? below : 0.0);
-        };
-        const auto prefix_mass = [&](int length) {  // of the first `length` tokens
-            if (length >= all) return s.mass_before[kSteps];
-            const int step = last_step([&](int i) { return s.count_before[i] <= length; });
-            open(step);
-            return s.mass_before[step] + wave_sum(min(max(length - before, 0), n) * w);
-        };
-        const int limit = set.top_k > 0 ? min(set.top_k, all) : all;
-        int length = min(limit, s.above_min);
-        const double share = set.top_p;
-        if (!(share >= 1.0)) {
-            const double border = share * prefix_mass(limit);
-            int below = 0;  // tokens with less mass than the border before them
-            if (border > 0.0) {
-                const int step = last_step([&](int i) { return s.mass_before[i] < border; });
-                open(step);
-                int in = 0;
-                if (mass_at < border) {
-                    in = n;
-                    if (w > 0.0) {
-                        in = static_cast<int>(fmin(ceil((border - mass_at) / w), static_cast<double>(n)));
-                        if (in > 0 && mass_at + (in - 1) * w >= border) --in;
-                        if (in < n && mass_at + in * w < border) ++in;
+        Lane<T> l;
+        if (greedy) {
+            l.count(s, heavy, top >> 10);
+            if (lane == (top >> 4 & 63)) {
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) n = i == (top & 15) ? l.n[i] : n;
+                s.place = top, s.rank = 0, s.count = n, s.probability = 1.0;
+            }
+        } else {
+            // What comes before turn `lane` in the whole order.
+            const double turn_mass = s.turn_mass[lane], mass_scan = wave_scan(turn_mass), mass_all = lane_double(mass_scan, 63);
+            const int turn_count = s.turn_count[lane], count_scan = wave_scan(turn_count), all = lane_int(count_scan, 63);
+            const int count_before = count_scan - turn_count;
+            const double mass_up = __shfl_up(mass_scan, 1, 64), mass_before = lane ? mass_up : 0.0;
+            // The last turn of which a test (true up to some turn) holds; the lane's classes there and what precedes them.
+            int turn = -1, before;
+            double mass_at;
+            const auto open = [&](bool test) {
+                const int wanted = max(__popcll(__ballot(test)) - 1, 0);
+                if (wanted == turn) return;
+                turn = wanted;
+                l.count(s, heavy, turn);
+                l.weigh(turn, top, max_value, heat);
+                int n = 0;
+                double mass = 0.0;
+                l.each([&](int, int c, double w) { n += c, mass += c * w; });
+                before = lane_int(count_before, turn) + wave_scan(n) - n;
+                const double up = __shfl_up(wave_scan(mass), 1, 64);
+                mass_at = lane_double(mass_before, turn) + (lane ? up : 0.0);
+            };
+            const auto prefix_mass = [&](int length) {  // of the first `length` tokens
+                if (length >= all) return mass_all;
+                open(count_before <= length);
+                double mass = 0.0;
+                int left = length - before;
+                l.each([&](int, int n, double w) {
+                    mass += min(max(left, 0), n) * w;
+                    left -= n;
+                });
+                return lane_double(mass_before, turn) + wave_sum(mass);
+            };
+            // Tokens in order up to a border of mass: those that start below it, or those that end at or below it.
+            const auto tokens_below = [&](double border, bool ends) {
+                open(ends ? mass_before <= border : mass_before < border);
+                int in = 0, part = 0;
+                double at = mass_at, part_at = 0.0, part_w = 1.0;
+                l.each([&](int, int n, double w) {
+                    const double last = ends ? at + n * w : at + (n - 1) * w;
+                    const bool whole = ends ? last <= border : last < border, some = ends ? at <= border : at < border;
+                    if (n && whole) in += n;
+                    if (n && !whole && some) part = n, part_at = at, part_w = w;
+                    at += n * w;
+                });
+                if (part) {
+                    const double quotient = (border - part_at) / part_w;
+                    int count = static_cast<int>(fmin(ends ? floor(quotient) : ceil(quotient), static_cast<double>(part)));
+                    if (ends) {
+                        if (count > 0 && part_at + count * part_w > border) --count;
+                        if (count < part && part_at + (count + 1) * part_w <= border) ++count;
+                    } else {
+                        if (count > 0 && part_at + (count - 1) * part_w >= border) --count;
+                        if (count < part && part_at + count * part_w < border) ++count;
                     }
+                    in += count;
                 }
-                below = s.count_before[step] + wave_sum(in);
+                return lane_int(count_before, turn) + wave_sum(in);
+            };
+            const int limit = set.top_k > 0 ? min(set.top_k, all) : all;
+            int length = min(limit, s.above_min);
+            const double share = set.top_p;
+            if (!(share >= 1.0)) {
+                const double border = share * prefix_mass(limit);
+                length = min(length, border > 0.0 ? tokens_below(border, false) : 0);
             }
-            length = min(length, below);
-        }
-        length = max(length, 1);
-        const double kept = prefix_mass(length);
-        const double target = static_cast<double>(set.uniform) * kept;
-        int place = 0;  // tokens whose share ends at or below the target
-        if (target >= 0.0) {
-            const int step = last_step([&](int i) { return s.mass_before[i] <= target; });
-            open(step);
-            int in = 0;
-            if (mass_at <= target) {
-                in = n;
-                if (w > 0.0) {
-                    in = static_cast<int>(fmin(floor((target - mass_at) / w), static_cast<double>(n)));
-                    if (in > 0 && mass_at + in * w > target) --in;
-                    if (in < n && mass_at + (in + 1) * w <= target) ++in;
+            length = max(length, 1);
+            const double kept = prefix_mass(length), target = static_cast<double>(set.uniform) * kept;
+            int place = target >= 0.0 ? tokens_below(target, true) : 0;
+            place = max(min(place, min(length, s.positive) - 1), 0);
+            open(count_before <= place);
+            int at = before;
+            l.each([&](int i, int n, double w) {
+                if (place >= at && place < at + n) {
+                    s.place = 1024 * turn + 16 * lane + i;
+                    s.rank = place - at;
+                    s.count = n;
+                    s.probability = w / kept;
                 }
-            }
-            place = s.count_before[step] + wave_sum(in);
-        }
-        place = max(min(place, min(length, s.positive) - 1), 0);
-        open(last_step([&](int i) { return s.count_before[i] <= place; }));
-        if (place >= before && place < before + n) {
-            s.key = key;
-            s.rank = place - before;
-            s.count = n;
-            s.probability = w / kept;
+                at += n;
+            });
         }
     }
     __syncthreads();
-    return {s.key, s.rank, s.count};
+    return {s.place, s.rank, s.count};
 }
 
-template <class T>
-__device__ __forceinline__ int occurrences(const uint4& w, std::uint32_t key) {
-    int n = 0;
+// A class's bits twice in a word, and the bits to compare (the class of 0 takes either sign).
+struct Pattern {
+    std::uint32_t bits, mask;
+    __device__ __forceinline__ explicit Pattern(int place)
+        : bits(place_bits(place) * 0x10001u), mask(bits ? 0xffffffffu : 0x7fff7fffu) {}
+};
+
+// Elements of a vector that match: 8 less the halves that differ.
+__device__ __forceinline__ int occurrences(const uint4& w, const Pattern& p) {
+    typedef unsigned short short2v __attribute__((ext_vector_type(2)));
+    const short2v one = {1, 1};
+    short2v differ = {0, 0};
+    const std::uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) n += sort_key<T>(element(w, j)) == key;
-    return n;
+    for (int i = 0; i < 4; ++i) differ += __builtin_elementwise_min(__builtin_bit_cast(short2v, (u[i] ^ p.bits) & p.mask), one);
+    return 8 - differ.x - differ.y;
 }
 
 // Which of the chunk counts (`count` of them, in order) holds occurrence `rank`; `before` becomes what precedes it there.
@@ -394,14 +458,15 @@ __device__ __forceinline__ int find_chunk(const int* counts, int chunks, int ran
 
 // The element (of the row) at which occurrence `rank` of 64 vectors lies, if it is the lane's; else -1.
 template <class T>
-__device__ __forceinline__ int find_element(const Row<T>& row, int vector, int vectors, std::uint32_t key, int before, int rank) {
+__device__ __forceinline__ int find_element(const Row<T>& row, int vector, const Pattern& p, int before, int rank) {
     int at = -1;
-    const uint4 w = vector < vectors ? row.load(vector) : make_uint4(0x7fff7fff, 0x7fff7fff, 0x7fff7fff, 0x7fff7fff);
-    const int n = occurrences<T>(w, key);
+    const uint4 w = row.load(vector);
+    const int n = occurrences(w, p);
     int next = before + wave_scan(n) - n;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-        if (sort_key<T>(element(w, j)) == key && next++ == rank) at = static_cast<int>((row.vector0 + vector) * 8 + j - row.first);
+        if (((element(w, j) ^ p.bits) & p.mask & 0xffff) == 0 && next++ == rank)
+            at = static_cast<int>((row.vector0 + vector) * 8 + j - row.first);
     return at;
 }
 
@@ -422,27 +487,26 @@ struct Operands {
     }
 };
 
-// Visits a workgroup's vectors begin + t, begin + t + kThreads, .. below end, kAhead loads at a time; `between` runs, for the
-// whole workgroup, after every kFirst and then every kNext of them.
-constexpr int kAhead = 6;
+// Visits a workgroup's vectors begin + t, begin + t + kThreads, .. below end. The loads run a batch ahead; `between` runs, for
+// the whole workgroup, after every kFirst and then every kNext vectors of a thread.
 template <class T, class Visit, class Between>
 __device__ __forceinline__ void each_vector(const Row<T>& row, int begin, int end, Visit&& visit, Between&& between) {
-    static_assert(kNext == kAhead && kFirst == kAhead + 1, "a sweep between two batches of loads");
     const int at = begin + threadIdx.x;
-    const auto batch = [&](int i, int count) {
-        uint4 w[kFirst];
-#pragma unroll
-        for (int j = 0; j < kFirst; ++j)
-            w[j] = j < count && at + (i + j) * kThreads < end ? row.load(at + (i + j) * kThreads)
-                                                              : make_uint4(0x7fff7fff, 0x7fff7fff, 0x7fff7fff, 0x7fff7fff);
-#pragma unroll
-        for (int j = 0; j < kFirst; ++j)
-            if (j < count && begin + (i + j) * kThreads < end) visit(w[j], i + j);
+    const auto load = [&](int i) {
+        return at + i * kThreads < end ? row.load(at + i * kThreads) : make_uint4(kNoLogits, kNoLogits, kNoLogits, kNoLogits);
     };
-    batch(0, kFirst);
-    for (int i = kFirst; begin + i * kThreads < end; i += kNext) {
-        between();
-        batch(i, kNext);
+    uint4 now[kFirst], next[kNext];
+#pragma unroll
+    for (int j = 0; j < kFirst; ++j) now[j] = load(j);
+    for (int i = 0, count = kFirst; begin + i * kThreads < end; i += count, count = kNext) {
+#pragma unroll
+        for (int j = 0; j < kNext; ++j) next[j] = load(i + count + j);
+#pragma unroll
+        for (int j = 0; j < kFirst; ++j)
+            if (j < count && begin + (i + j) * kThreads < end) visit(now[j], i + j);
+        if (begin + (i + count) * kThreads < end) between();
+#pragma unroll
+        for (int j = 0; j < kNext; ++j) now[j] = next[j];
     }
 }
 
@@ -455,27 +519,24 @@ __global__ __launch_bounds__(kThreads) void sample(Operands o) {
     const Row<T> row(o.logits, index, o.vocab);
     const Settings set = o.settings(index);
     clear(s);
-    std::uint32_t top = kNone;
-    each_vector(row, 0, row.vectors, [&](const uint4& w, int) { count_vector<T>(s, w, top); }, [&] { sweep(s); });
-#pragma unroll
-    for (int step = 32; step; step >>= 1) top = max(top, static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(top), step, 64)));
-    if (lane == 0) atomicMax(&s.top, static_cast<int>(top));
+    each_vector(row, 0, row.vectors, [&](const uint4& w, int) { count_vector(s, w); }, [&] { sweep(s); });
     __syncthreads();
     const Choice choice = choose<T>(s, set);
     if (t == 0 && o.probabilities) o.probabilities[index] = static_cast<float>(s.probability);
-    if (choice.key == kNone) {
+    if (choice.place == kNone) {
         if (t == 0) o.tokens[index] = -1;
         return;
     }
     // The rank-th occurrence of the class: occurrences per chunk of 64 vectors, then within the chunk. (choose() has ended
     // with a barrier: the histogram's memory is free.)
-    __syncthreads();
+    const Pattern pattern(choice.place);
     int* counts = reinterpret_cast<int*>(s.histogram);
     const int chunks = (row.vectors + 63) / 64;
     each_vector(
         row, 0, row.vectors,
         [&](const uint4& w, int i) {
-            const int n = wave_sum(occurrences<T>(w, choice.key));
+            int n = occurrences(w, pattern);
+            n = __any(n) ? wave_sum(n) : 0;
             if (lane == 0) counts[i * kWaves + wave] = n;
         },
         [] {});
@@ -484,7 +545,7 @@ __global__ __launch_bounds__(kThreads) void sample(Operands o) {
         int before;
         const int chunk = find_chunk(counts, chunks, choice.rank, before);
         if (chunk >= 0) {
-            const int at = find_element(row, chunk * 64 + lane, row.vectors, choice.key, before, choice.rank);
+            const int at = find_element(row, chunk * 64 + lane, pattern, before, choice.rank);
             if (at >= 0) o.tokens[index] = at;
         }
     }
