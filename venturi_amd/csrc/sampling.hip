@@ -62,50 +62,21 @@ __device__ __forceinline__ double class_step(int place) {
     return value(low + 1) - value(low);
 }
 
-constexpr std::uint32_t kNoLogits = 0x7fff7fff;  // two NaN
-
-// A row as aligned vectors of 8 logits, of which the first and the last may lie partly outside it: those two are read
-// element by element, once, so that the others need no check beside their load.
-template <class T>
+// A row as `head` elements before its first 16-byte boundary, `vectors` whole vectors of 8, and `tail` elements.
 struct Row {
-    const unsigned short* logits;  // the tensor, 16-byte aligned
-    std::int64_t first, end;       // the row's elements
-    std::int64_t vector0;          // the aligned vector of 8 that holds its first
-    int vectors, whole0, whole1;   // the vectors that lie inside: whole0 .. whole1 - 1
-    uint4 head, tail;
+    const unsigned short* start;
+    int head, vectors, tail;
 
-    __device__ __forceinline__ Row(const void* tensor, int index, int vocab)
-        : logits(static_cast<const unsigned short*>(tensor)), first(static_cast<std::int64_t>(index) * vocab), end(first + vocab),
-          vector0(first >> 3), vectors(static_cast<int>(((end + 7) >> 3) - vector0)) {
-        whole0 = first & 7 ? 1 : 0;
-        whole1 = vectors - (end & 7 ? 1 : 0);
-        head = part(0);
-        tail = part(vectors - 1);
+    __device__ __forceinline__ Row(const void* logits, int index, int vocab) {
+        const std::int64_t first = static_cast<std::int64_t>(index) * vocab;
+        start = static_cast<const unsigned short*>(logits) + first;  // the tensor is 16-byte aligned
+        head = min(static_cast<int>(-first & 7), vocab);
+        vectors = (vocab - head) >> 3;
+        tail = vocab - head - 8 * vectors;
     }
-
-    __device__ __forceinline__ uint4 part(int i) const {
-        const std::int64_t at = (vector0 + i) * 8;
-        std::uint32_t u[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const std::int64_t e = at + 2 * j;
-            u[j] = (e >= first && e < end ? logits[e] : 0x7fffu) | (e + 1 >= first && e + 1 < end ? logits[e + 1] : 0x7fffu) << 16;
-        }
-        return make_uint4(u[0], u[1], u[2], u[3]);
-    }
-
-    // Vector i, for 0 <= i; NaN outside the row.
-    __device__ __forceinline__ uint4 load(int i) const {
-        uint4 w = make_uint4(kNoLogits, kNoLogits, kNoLogits, kNoLogits);
-        if (whole0 < whole1) {  // the same for the whole grid row: no lane waits for another's load
-            const auto* at = reinterpret_cast<const uint4*>(logits) + vector0 + min(max(i, whole0), whole1 - 1);
-            w = *at;
-        }
-        if (i < whole0) w = head;
-        else if (i >= vectors) w = make_uint4(kNoLogits, kNoLogits, kNoLogits, kNoLogits);
-        else if (i >= whole1) w = tail;
-        return w;
-    }
+    __device__ __forceinline__ const uint4* whole() const { return reinterpret_cast<const uint4*>(start + head); }
+    // Element i of the head and tail together, and its index in the row.
+    __device__ __forceinline__ int edge(int i) const { return i < head ? i : 8 * vectors + i; }
 };
 
 __device__ __forceinline__ std::uint32_t element(const uint4& w, int j) {
@@ -456,17 +427,14 @@ __device__ __forceinline__ int find_chunk(const int* counts, int chunks, int ran
     return -1;
 }
 
-// The element (of the row) at which occurrence `rank` of 64 vectors lies, if it is the lane's; else -1.
-template <class T>
-__device__ __forceinline__ int find_element(const Row<T>& row, int vector, const Pattern& p, int before, int rank) {
+// The element of a vector at which occurrence `rank` of the wave's 64 vectors lies, if it is the lane's; else -1.
+__device__ __forceinline__ int find_element(const uint4& w, const Pattern& p, int before, int rank) {
     int at = -1;
-    const uint4 w = row.load(vector);
     const int n = occurrences(w, p);
     int next = before + wave_scan(n) - n;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-        if (((element(w, j) ^ p.bits) & p.mask & 0xffff) == 0 && next++ == rank)
-            at = static_cast<int>((row.vector0 + vector) * 8 + j - row.first);
+        if (((element(w, j) ^ p.bits) & p.mask & 0xffff) == 0 && next++ == rank) at = j;
     return at;
 }
 
@@ -487,24 +455,30 @@ struct Operands {
     }
 };
 
-// Visits a workgroup's vectors begin + t, begin + t + kThreads, .. below end. The loads run a batch ahead; `between` runs, for
-// the whole workgroup, after every kFirst and then every kNext vectors of a thread.
-template <class T, class Visit, class Between>
-__device__ __forceinline__ void each_vector(const Row<T>& row, int begin, int end, Visit&& visit, Between&& between) {
+// Visits the vectors begin + t, begin + t + kThreads, .. below end. The loads run a batch ahead of the visits, unconditional
+// (past the end they repeat the last vector): a load under a condition is waited for before the next one is issued.
+// `before` runs once, after the first loads are issued; `between`, for the whole workgroup, after every kFirst and then every
+// kNext vectors of a thread; it returns whether to go on.
+template <class Before, class Visit, class Between>
+__device__ __forceinline__ void each_vector(const uint4* __restrict__ whole, int begin, int end, Before&& before, Visit&& visit,
+                                            Between&& between) {
+    if (begin >= end) {
+        before();
+        return;
+    }
     const int at = begin + threadIdx.x;
-    const auto load = [&](int i) {
-        return at + i * kThreads < end ? row.load(at + i * kThreads) : make_uint4(kNoLogits, kNoLogits, kNoLogits, kNoLogits);
-    };
+    const auto load = [&](int i) { return whole[min(at + i * kThreads, end - 1)]; };
     uint4 now[kFirst], next[kNext];
 #pragma unroll
     for (int j = 0; j < kFirst; ++j) now[j] = load(j);
+    before();
     for (int i = 0, count = kFirst; begin + i * kThreads < end; i += count, count = kNext) {
 #pragma unroll
         for (int j = 0; j < kNext; ++j) next[j] = load(i + count + j);
 #pragma unroll
         for (int j = 0; j < kFirst; ++j)
-            if (j < count && begin + (i + j) * kThreads < end) visit(now[j], i + j);
-        if (begin + (i + count) * kThreads < end) between();
+            if (j < count && begin + (i + j) * kThreads < end) visit(now[j], i + j, at + (i + j) * kThreads < end);
+        if (begin + (i + count) * kThreads < end && !between(i + count)) break;
 #pragma unroll
         for (int j = 0; j < kNext; ++j) now[j] = next[j];
     }
@@ -516,10 +490,19 @@ __global__ __launch_bounds__(kThreads) void sample(Operands o) {
     extern __shared__ __align__(16) unsigned char memory[];
     Shared& s = *reinterpret_cast<Shared*>(memory);
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, index = blockIdx.x;
-    const Row<T> row(o.logits, index, o.vocab);
+    const Row row(o.logits, index, o.vocab);
     const Settings set = o.settings(index);
-    clear(s);
-    each_vector(row, 0, row.vectors, [&](const uint4& w, int) { count_vector(s, w); }, [&] { sweep(s); });
+    const std::uint32_t edge = t < row.head + row.tail ? row.start[row.edge(t)] : 0;
+    each_vector(
+        row.whole(), 0, row.vectors, [&] { clear(s); },
+        [&](const uint4& w, int, bool live) {
+            if (live) count_vector(s, w);
+        },
+        [&](int) {
+            sweep(s);
+            return true;
+        });
+    if (t < row.head + row.tail) atomicAdd(&s.histogram[edge & 0x7fff], edge & 0x8000 ? 0x10000u : 1u);
     __syncthreads();
     const Choice choice = choose<T>(s, set);
     if (t == 0 && o.probabilities) o.probabilities[index] = static_cast<float>(s.probability);
@@ -527,27 +510,51 @@ __global__ __launch_bounds__(kThreads) void sample(Operands o) {
         if (t == 0) o.tokens[index] = -1;
         return;
     }
-    // The rank-th occurrence of the class: occurrences per chunk of 64 vectors, then within the chunk. (choose() has ended
-    // with a barrier: the histogram's memory is free.)
+    // The rank-th occurrence of the class: in the head; else occurrences per chunk of 64 vectors, batch by batch until there
+    // are enough, then within the chunk; else in the tail. (choose() has ended with a barrier: the histogram's memory is free.)
     const Pattern pattern(choice.place);
+    const bool match = t < row.head + row.tail && ((edge ^ pattern.bits) & pattern.mask & 0xffff) == 0;
     int* counts = reinterpret_cast<int*>(s.histogram);
-    const int chunks = (row.vectors + 63) / 64;
-    each_vector(
-        row, 0, row.vectors,
-        [&](const uint4& w, int i) {
-            int n = occurrences(w, pattern);
-            n = __any(n) ? wave_sum(n) : 0;
-            if (lane == 0) counts[i * kWaves + wave] = n;
-        },
-        [] {});
-    __syncthreads();
+    int* found = counts + kMaxVocab / 512 + 16;  // vectors' occurrences so far
     if (wave == 0) {
+        const unsigned long long in_head = __ballot(match && lane < row.head);
+        const int before = __popcll(in_head & ((1ull << lane) - 1));
+        if (match && lane < row.head && before == choice.rank) o.tokens[index] = row.edge(lane);
+        if (lane == 0) found[0] = found[1] = __popcll(in_head);
+    }
+    __syncthreads();
+    const int first = found[1];
+    if (first > choice.rank) return;
+    each_vector(
+        row.whole(), 0, row.vectors, [] {},
+        [&](const uint4& w, int i, bool live) {
+            int n = live ? occurrences(w, pattern) : 0;
+            n = __any(n) ? wave_sum(n) : 0;
+            if (lane == 0) {
+                counts[i * kWaves + wave] = n;
+                if (n) atomicAdd(found, n);
+            }
+        },
+        [&](int) {
+            __syncthreads();
+            const bool enough = found[0] > choice.rank;
+            __syncthreads();
+            return !enough;
+        });
+    __syncthreads();
+    if (wave != 0) return;
+    if (found[0] > choice.rank) {
         int before;
-        const int chunk = find_chunk(counts, chunks, choice.rank, before);
-        if (chunk >= 0) {
-            const int at = find_element(row, chunk * 64 + lane, pattern, before, choice.rank);
-            if (at >= 0) o.tokens[index] = at;
-        }
+        const int chunk = find_chunk(counts, (row.vectors + 63) / 64, choice.rank - first, before);
+        const int vector = chunk * 64 + lane;
+        const bool live = chunk >= 0 && vector < row.vectors;
+        const uint4 w = live ? row.whole()[vector] : make_uint4(~pattern.bits, ~pattern.bits, ~pattern.bits, ~pattern.bits);
+        const int at = find_element(w, pattern, before, choice.rank - first);
+        if (at >= 0) o.tokens[index] = row.head + 8ll * vector + at;
+    } else {
+        const unsigned long long in_tail = __ballot(match && lane >= row.head);
+        if (match && lane >= row.head && found[0] + __popcll(in_tail & ((1ull << lane) - 1)) == choice.rank)
+            o.tokens[index] = row.edge(lane);
     }
 }
 
