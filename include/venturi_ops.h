@@ -459,7 +459,8 @@ int venturi_packed_attention_run(const void* q, const void* k, const void* v, co
 /* One token per row of logits [rows][vocab] from uniforms [rows] in [0, 1): order by (logit descending, index),
  * top_k (0: all), top_p of the top-k mass, min_p against the largest weight. Settings [rows], each NULL for none
  * (temperature 1). tokens int64 [rows] (-1 for a row of -inf and NaN alone); probabilities fp32 [rows] or NULL.
- * workspace: venturi_sample_bytes (may be 0), 256-byte aligned. */
+ * workspace: venturi_sample_bytes (0 but for few rows), 256-byte aligned, zeroed once before its first call; every
+ * call leaves it ready for the next, and calls that share it run on one stream. */
 uint64_t venturi_sample_bytes(int rows, int vocab);
 int venturi_sample_run(const void* logits, const float* uniforms, const float* temperature, const int32_t* top_k,
                        const float* top_p, const float* min_p, int64_t* tokens, float* probabilities,

@@ -125,12 +125,12 @@ struct Settings {
 };
 
 struct Shared {
-    std::uint32_t histogram[32768];  // of bits b (low half) and b + 0x8000 (high half)
+    std::uint32_t histogram[32768];  // of bits 2 i (low half) and 2 i + 1 (high half)
     double turn_mass[kTurns];
     int turn_count[kTurns];
     std::uint32_t heavy_bits[kHeavyEntries], heavy_count[kHeavyEntries];
     double probability;
-    int heavy, top, above_min, positive, place, rank, count;
+    int heavy, top, above_min, place, rank, count;
 };
 
 // A row's chosen class (kNone: nothing to take), and which of its `count` occurrences.
@@ -140,21 +140,31 @@ struct Choice {
 
 __device__ __forceinline__ void clear(Shared& s) {
     for (int i = threadIdx.x; i < 32768 / 4; i += kThreads) reinterpret_cast<uint4*>(s.histogram)[i] = make_uint4(0, 0, 0, 0);
-    if (threadIdx.x == 0) s.heavy = s.above_min = s.positive = 0, s.top = 65536;
+    if (threadIdx.x == 0) s.heavy = s.above_min = 0, s.top = 65536;
     __syncthreads();
+}
+
+__device__ __forceinline__ void count_element(Shared& s, std::uint32_t bits) {
+    atomicAdd(&s.histogram[bits >> 1], 1u << (16 * (bits & 1)));
 }
 
 __device__ __forceinline__ void count_vector(Shared& s, const uint4& w) {
+    const std::uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    auto* bytes = reinterpret_cast<unsigned char*>(s.histogram);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const std::uint32_t bits = element(w, j);
-        atomicAdd(&s.histogram[bits & 0x7fff], bits & 0x8000 ? 0x10000u : 1u);
+    for (int j = 0; j < 4; ++j) {
+        // A shift takes the low five bits of its amount.
+        atomicAdd(reinterpret_cast<std::uint32_t*>(bytes + ((u[j] & 0xfffe) << 1)), 1u << ((u[j] << 4) & 31));
+        atomicAdd(reinterpret_cast<std::uint32_t*>(bytes + ((u[j] >> 15) & 0x1fffc)), 1u << ((u[j] >> 12) & 16));
     }
 }
 
+// A barrier of the workgroup's LDS accesses alone: __syncthreads() would also wait for the loads in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // Moves the classes that have reached kHeavy to the list.
 __device__ __forceinline__ void sweep(Shared& s) {
-    __syncthreads();
+    lds_barrier();
     for (int i = threadIdx.x; i < 32768; i += kThreads) {
         std::uint32_t word = s.histogram[i];
         if (!(word & 0xc000c000u)) continue;
@@ -163,14 +173,35 @@ __device__ __forceinline__ void sweep(Shared& s) {
             const std::uint32_t n = (word >> (16 * half)) & 0xffff;
             if (n >= kHeavy) {
                 const int e = atomicAdd(&s.heavy, 1);
-                s.heavy_bits[e] = i + 32768 * half;
+                s.heavy_bits[e] = 2 * i + half;
                 s.heavy_count[e] = n;
                 word -= n << (16 * half);
             }
         }
         s.histogram[i] = word;
     }
-    __syncthreads();
+    lds_barrier();
+}
+
+// 2^x for x <= 0, NaN as 0: the Taylor series of e^r for |r| <= ln 2 / 2, whose 13th power is below 2^-53, times 2^n.
+__device__ __forceinline__ double falling_power(double x) {
+    const double n = rint(x);
+    const double r = (x - n) * 0.693147180559945309417;
+    double p = 1.0 / 6227020800.0;
+    p = fma(p, r, 1.0 / 479001600.0);
+    p = fma(p, r, 1.0 / 39916800.0);
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return x > -1000.0 ? ldexp(p, static_cast<int>(n)) : 0.0;
 }
 
 // A lane's 16 classes of a turn: places 1024 turn + 16 lane + i.
@@ -180,31 +211,29 @@ struct Lane {
     int first;       // weights start at class `first` (classes above the row's largest do not occur)
     double start, ratio;
 
+    static __device__ __forceinline__ const uint4* words(const Shared& s, int place) {
+        return reinterpret_cast<const uint4*>(s.histogram + (place >= 32768 ? place : 32767 - 15 - place) / 2);
+    }
+
     // Whether any of the turn's classes (or of the places without one) occurs in the counters.
     static __device__ __forceinline__ bool occurs(const Shared& s, int heavy, int turn) {
-        const int place = 1024 * turn + 16 * static_cast<int>(threadIdx.x & 63);
-        const bool negative = turn >= kTurns / 2;
-        const auto* words = reinterpret_cast<const uint4*>(s.histogram + (negative ? place - 32768 : 32767 - 15 - place));
-        std::uint32_t any = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint4 w = words[i];
-            any |= w.x | w.y | w.z | w.w;
-        }
-        return heavy > 0 || turn == kTurns / 2 - 1 || (negative ? any >> 16 : any & 0xffff) != 0;
+        const auto* at = words(s, 1024 * turn + 16 * static_cast<int>(threadIdx.x & 63));
+        const uint4 a = at[0], b = at[1];
+        return heavy > 0 || turn == kTurns / 2 - 1 || ((a.x | a.y | a.z | a.w) | (b.x | b.y | b.z | b.w)) != 0;
     }
 
     __device__ __forceinline__ bool count(const Shared& s, int heavy, int turn) {
         const int place = 1024 * turn + 16 * static_cast<int>(threadIdx.x & 63);
         const bool negative = turn >= kTurns / 2;
-        const auto* words = reinterpret_cast<const uint4*>(s.histogram + (negative ? place - 32768 : 32767 - 15 - place));
-        const uint4 w[4] = {words[0], words[1], words[2], words[3]};
-        std::uint32_t u[16];
+        const auto* at = words(s, place);
+        const uint4 a = at[0], b = at[1];
+        const std::uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[4 * i] = w[i].x, u[4 * i + 1] = w[i].y, u[4 * i + 2] = w[i].z, u[4 * i + 3] = w[i].w;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) n[i] = negative ? u[i] >> 16 : u[15 - i] & 0xffff;
-        if (turn == kTurns / 2 - 1 && place == 32767 - 15) n[15] += s.histogram[0] >> 16;  // -0
+        for (int i = 0; i < 8; ++i) {
+            n[2 * i] = negative ? u[i] & 0xffff : u[7 - i] >> 16;
+            n[2 * i + 1] = negative ? u[i] >> 16 : u[7 - i] & 0xffff;
+        }
+        if (turn == kTurns / 2 - 1 && place == 32767 - 15) n[15] += s.histogram[16384] & 0xffff;  // -0
         for (int e = 0; e < heavy; ++e) {
             const std::uint32_t bits = s.heavy_bits[e] == 0x8000 ? 0 : s.heavy_bits[e];
             const int at = (bits & 0x8000 ? static_cast<int>(bits) : 32767 - static_cast<int>(bits)) - place;
@@ -226,8 +255,9 @@ struct Lane {
     __device__ __forceinline__ void weigh(int turn, int top, double max_value, double heat) {
         const int place = 1024 * turn + 16 * static_cast<int>(threadIdx.x & 63);
         first = top > place ? top - place : 0;  // 16 and more: the lane's classes all lie above
-        start = first == 0 && place != top ? exp((class_value<T>(place) - max_value) / heat) : 1.0;
-        ratio = exp(-class_step<T>(place) / heat);
+        start = falling_power((class_value<T>(first ? top : place) - max_value) * heat);
+        if (first || place == top) start = 1.0;  // also where the difference is of two infinities
+        ratio = falling_power(-class_step<T>(place) * heat);
     }
 
     // Visits the lane's classes in order: (index, occurrences, weight).
@@ -266,9 +296,12 @@ __device__ Choice choose(Shared& s, const Settings& set) {
         __syncthreads();
         return {kNone, 0, 0};
     }
-    const double max_value = class_value<T>(top), heat = fminf(set.temperature, 3.402823466e38f), least = set.min_p;
     const bool greedy = !(set.temperature > 0.0f);
-    int above_min = 0, positive = 0;
+    // log2 e / T, from 4e-39 to 2e45.
+    const double max_value = class_value<T>(top), least = set.min_p;
+    const double heat = 1.44269504088896340736 / (greedy ? 1.0 : static_cast<double>(fminf(set.temperature, 3.402823466e38f)));
+    const bool all_above = least <= 0.0;
+    int above_min = 0;
     for (int turn = wave; turn < kTurns && !greedy; turn += kWaves) {
         Lane<T> l;
         double mass = 0.0;
@@ -278,19 +311,16 @@ __device__ Choice choose(Shared& s, const Settings& set) {
             l.each([&](int, int n, double w) {
                 mass += n * w;
                 count += n;
-                above_min += w >= least ? n : 0;
-                positive += w > 0.0 ? n : 0;
             });
+            if (!all_above) l.each([&](int, int n, double w) { above_min += w >= least ? n : 0; });
             mass = wave_sum(mass);
             count = wave_sum(count);
         }
         if (lane == 0) s.turn_mass[turn] = mass, s.turn_count[turn] = count;
     }
-    above_min = wave_sum(above_min);
-    positive = wave_sum(positive);
-    if (lane == 0) {
-        if (above_min) atomicAdd(&s.above_min, above_min);
-        if (positive) atomicAdd(&s.positive, positive);
+    if (!all_above) {
+        above_min = wave_sum(above_min);
+        if (lane == 0 && above_min) atomicAdd(&s.above_min, above_min);
     }
     __syncthreads();
     if (wave == 0) {
@@ -363,16 +393,18 @@ __device__ Choice choose(Shared& s, const Settings& set) {
                 return lane_int(count_before, turn) + wave_sum(in);
             };
             const int limit = set.top_k > 0 ? min(set.top_k, all) : all;
-            int length = min(limit, s.above_min);
+            int length = all_above ? limit : min(limit, s.above_min);
             const double share = set.top_p;
             if (!(share >= 1.0)) {
                 const double border = share * prefix_mass(limit);
                 length = min(length, border > 0.0 ? tokens_below(border, false) : 0);
             }
             length = max(length, 1);
-            const double kept = prefix_mass(length), target = static_cast<double>(set.uniform) * kept;
-            int place = target >= 0.0 ? tokens_below(target, true) : 0;
-            place = max(min(place, min(length, s.positive) - 1), 0);
+            const double kept = prefix_mass(length);
+            // A uniform of 1 or more stays below the end of the mass: the last token that adds to it.
+            const double target = fmin(static_cast<double>(set.uniform) * kept, kept * (1.0 - 0x1p-52));
+            int place = target >= 0.0 && set.uniform >= 0.0f ? tokens_below(target, true) : 0;
+            place = max(min(place, length - 1), 0);
             open(count_before <= place);
             int at = before;
             l.each([&](int i, int n, double w) {
@@ -484,15 +516,74 @@ __device__ __forceinline__ void each_vector(const uint4* __restrict__ whole, int
     }
 }
 
+// A lane's element of the row's ragged ends (lanes below head + tail of the first wave).
+struct Edge {
+    std::uint32_t bits;
+    bool live;
+    __device__ __forceinline__ explicit Edge(const Row& row)
+        : live(static_cast<int>(threadIdx.x) < row.head + row.tail) {
+        bits = live ? row.start[row.edge(threadIdx.x)] : 0;
+    }
+    __device__ __forceinline__ bool match(const Pattern& p) const { return live && ((bits ^ p.bits) & p.mask & 0xffff) == 0; }
+};
+
+// Occurrences among the vectors [begin, end), batch by batch until more than `rank` are found; every thread gets their
+// number, and `counts` holds them by chunk of 64 vectors. `found` is a word of LDS apart from them.
+__device__ __forceinline__ int count_matches(const Row& row, int begin, int end, const Pattern& p, int rank, int* counts, int* found) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (threadIdx.x == 0) *found = 0;
+    __syncthreads();
+    each_vector(
+        row.whole(), begin, end, [] {},
+        [&](const uint4& w, int i, bool live) {
+            int n = live ? occurrences(w, p) : 0;
+            n = __any(n) ? wave_sum(n) : 0;
+            if (lane == 0) {
+                counts[i * kWaves + wave] = n;
+                if (n) atomicAdd(found, n);
+            }
+        },
+        [&](int) {
+            lds_barrier();
+            const bool enough = *found > rank;
+            lds_barrier();
+            return !enough;
+        });
+    __syncthreads();
+    return *found;
+}
+
+// Writes the token of occurrence `rank` of the vectors [begin, end) from their counts. One wave.
+__device__ __forceinline__ void write_match(const Row& row, int begin, int end, const Pattern& p, int rank, const int* counts,
+                                            std::int64_t* token) {
+    const int lane = threadIdx.x & 63;
+    int before;
+    const int chunk = find_chunk(counts, (end - begin + 63) / 64, rank, before);
+    const int vector = begin + chunk * 64 + lane;
+    const bool live = chunk >= 0 && vector < end;
+    const uint4 w = live ? row.whole()[vector] : make_uint4(~p.bits, ~p.bits, ~p.bits, ~p.bits);
+    const int at = find_element(w, p, before, rank);
+    if (at >= 0) *token = row.head + 8ll * vector + at;
+}
+
+// Occurrences in the row's head (tail: in its tail); the token, if rank is among them. One wave.
+__device__ __forceinline__ int edge_match(const Row& row, const Edge& edge, const Pattern& p, bool tail, int rank, std::int64_t* token) {
+    const int lane = threadIdx.x & 63;
+    const bool match = edge.match(p) && (lane < row.head) != tail;
+    const unsigned long long all = __ballot(match);
+    if (match && __popcll(all & ((1ull << lane) - 1)) == rank) *token = row.edge(lane);
+    return __popcll(all);
+}
+
 // A workgroup per row.
 template <class T>
 __global__ __launch_bounds__(kThreads) void sample(Operands o) {
     extern __shared__ __align__(16) unsigned char memory[];
     Shared& s = *reinterpret_cast<Shared*>(memory);
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, index = blockIdx.x;
+    const int t = threadIdx.x, wave = t >> 6, index = blockIdx.x;
     const Row row(o.logits, index, o.vocab);
     const Settings set = o.settings(index);
-    const std::uint32_t edge = t < row.head + row.tail ? row.start[row.edge(t)] : 0;
+    const Edge edge(row);
     each_vector(
         row.whole(), 0, row.vectors, [&] { clear(s); },
         [&](const uint4& w, int, bool live) {
@@ -502,7 +593,7 @@ __global__ __launch_bounds__(kThreads) void sample(Operands o) {
             sweep(s);
             return true;
         });
-    if (t < row.head + row.tail) atomicAdd(&s.histogram[edge & 0x7fff], edge & 0x8000 ? 0x10000u : 1u);
+    if (edge.live) count_element(s, edge.bits);
     __syncthreads();
     const Choice choice = choose<T>(s, set);
     if (t == 0 && o.probabilities) o.probabilities[index] = static_cast<float>(s.probability);
@@ -510,52 +601,23 @@ __global__ __launch_bounds__(kThreads) void sample(Operands o) {
         if (t == 0) o.tokens[index] = -1;
         return;
     }
-    // The rank-th occurrence of the class: in the head; else occurrences per chunk of 64 vectors, batch by batch until there
-    // are enough, then within the chunk; else in the tail. (choose() has ended with a barrier: the histogram's memory is free.)
+    // The rank-th occurrence of the class: in the head, in the vectors or in the tail. (choose() has ended with a barrier:
+    // the histogram's memory is free.)
     const Pattern pattern(choice.place);
-    const bool match = t < row.head + row.tail && ((edge ^ pattern.bits) & pattern.mask & 0xffff) == 0;
     int* counts = reinterpret_cast<int*>(s.histogram);
-    int* found = counts + kMaxVocab / 512 + 16;  // vectors' occurrences so far
     if (wave == 0) {
-        const unsigned long long in_head = __ballot(match && lane < row.head);
-        const int before = __popcll(in_head & ((1ull << lane) - 1));
-        if (match && lane < row.head && before == choice.rank) o.tokens[index] = row.edge(lane);
-        if (lane == 0) found[0] = found[1] = __popcll(in_head);
+        const int n = edge_match(row, edge, pattern, false, choice.rank, o.tokens + index);
+        if (t == 0) s.heavy = n;
     }
     __syncthreads();
-    const int first = found[1];
+    const int first = s.heavy;
     if (first > choice.rank) return;
-    each_vector(
-        row.whole(), 0, row.vectors, [] {},
-        [&](const uint4& w, int i, bool live) {
-            int n = live ? occurrences(w, pattern) : 0;
-            n = __any(n) ? wave_sum(n) : 0;
-            if (lane == 0) {
-                counts[i * kWaves + wave] = n;
-                if (n) atomicAdd(found, n);
-            }
-        },
-        [&](int) {
-            __syncthreads();
-            const bool enough = found[0] > choice.rank;
-            __syncthreads();
-            return !enough;
-        });
-    __syncthreads();
+    const int found = count_matches(row, 0, row.vectors, pattern, choice.rank - first, counts, &s.count);
     if (wave != 0) return;
-    if (found[0] > choice.rank) {
-        int before;
-        const int chunk = find_chunk(counts, (row.vectors + 63) / 64, choice.rank - first, before);
-        const int vector = chunk * 64 + lane;
-        const bool live = chunk >= 0 && vector < row.vectors;
-        const uint4 w = live ? row.whole()[vector] : make_uint4(~pattern.bits, ~pattern.bits, ~pattern.bits, ~pattern.bits);
-        const int at = find_element(w, pattern, before, choice.rank - first);
-        if (at >= 0) o.tokens[index] = row.head + 8ll * vector + at;
-    } else {
-        const unsigned long long in_tail = __ballot(match && lane >= row.head);
-        if (match && lane >= row.head && found[0] + __popcll(in_tail & ((1ull << lane) - 1)) == choice.rank)
-            o.tokens[index] = row.edge(lane);
-    }
+    if (found > choice.rank - first)
+        write_match(row, 0, row.vectors, pattern, choice.rank - first, counts, o.tokens + index);
+    else
+        edge_match(row, edge, pattern, true, choice.rank - first - found, o.tokens + index);
 }
 
 template <class T>

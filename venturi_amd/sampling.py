@@ -62,7 +62,8 @@ class SamplingPlan:
         workspace = None
         if nbytes:
             with torch.cuda.device(target):
-                workspace = torch.empty(nbytes, dtype=torch.uint8, device=target)
+                workspace = torch.zeros(nbytes, dtype=torch.uint8, device=target)  # counters: every run leaves them zero
+                torch.cuda.current_stream(target).synchronize()
         return cls(backend, rows, vocab, dtype, target, workspace)
 
     def run(self, logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=None, *, tokens, probabilities=None):
