@@ -71,10 +71,11 @@ struct Tile {
     static constexpr int columns = D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256;  // of an LDS row
     static constexpr int units = columns / 8;                                            // 16-byte units of an LDS row
     static constexpr int bytes = keys * columns * 2;
-    static constexpr int loads = keys * units / kThreads;                                // per thread
-    // What a unit's place in its row is XORed with.
+    static constexpr int loads = keys * units / kThreads;                                // per wave, of 64 units
+    static constexpr int load_rows = kThreads / units;                                   // rows that a load of all waves covers
+    // What a unit's place in its row is XORed with; the same for rows load_rows apart.
     static __device__ __forceinline__ int key_swizzle(int row) {
-        if constexpr (units >= 16) return row & 15;
+        if constexpr (units >= 16) return row & 7;
         else return (row / (16 / units)) & (units - 1);
     }
     static __device__ __forceinline__ int value_swizzle(int row) {  // even: pairs of units keep their order
@@ -130,31 +131,39 @@ __device__ __forceinline__ bool find_block(const std::int32_t* __restrict__ q_of
     return false;
 }
 
-// Sixteen bytes of keys and of values per thread and load; rows past the sequence and columns past the head are zero.
-template <class T, int D>
-struct Stage {
-    uint4 key[Tile<D>::loads], value[Tile<D>::loads];
+typedef int int4v __attribute__((ext_vector_type(4)));
 
-    __device__ __forceinline__ void load(const T* __restrict__ k, const T* __restrict__ v, std::int64_t stride, int rows,
-                                         int head_dim) {
-#pragma unroll
-        for (int i = 0; i < Tile<D>::loads; ++i) {
-            const int u = threadIdx.x + i * kThreads, row = u / Tile<D>::units, column = u % Tile<D>::units * 8;
-            const bool inside = row < rows && column < head_dim;
-            const std::int64_t at = inside ? row * stride + column : 0;
-            key[i] = inside ? *reinterpret_cast<const uint4*>(k + at) : make_uint4(0, 0, 0, 0);
-            value[i] = inside ? *reinterpret_cast<const uint4*>(v + at) : make_uint4(0, 0, 0, 0);
-        }
+// Copies tiles of rows from memory to LDS without a register: a load of a wave fills 64 consecutive units, so that the
+// swizzle is in the address that a lane reads. The buffer's range makes zeros of rows past the sequence; columns past the
+// head are sent past it.
+template <int D>
+struct Copy {
+    std::uint32_t key_at, value_at;  // bytes from the tile's first row to the lane's unit
+    std::uint32_t row_bytes;
+
+    __device__ __forceinline__ Copy(int stride, int head_dim) : row_bytes(2 * stride) {
+        const int row = threadIdx.x / Tile<D>::units, place = threadIdx.x % Tile<D>::units;
+        const int key_unit = place ^ Tile<D>::key_swizzle(row), value_unit = place ^ Tile<D>::value_swizzle(row);
+        key_at = 8 * key_unit < head_dim ? row * row_bytes + 16 * key_unit : 0x80000000u;
+        value_at = 8 * value_unit < head_dim ? row * row_bytes + 16 * value_unit : 0x80000000u;
     }
-    __device__ __forceinline__ void store(unsigned char* keys, unsigned char* values) const {
+    // The tile at `source`, of which `rows` rows exist, to `lds` (a byte address).
+    __device__ __forceinline__ void operator()(const void* source, int rows, std::uint32_t at, std::uint32_t lds) const {
+        const auto base = reinterpret_cast<std::uint64_t>(source);
+        const int4v buffer = {static_cast<int>(base), static_cast<int>(base >> 32) & 0xffff,
+                              static_cast<int>(min(rows, Tile<D>::keys) * row_bytes), 0x00020000};
+        const std::uint32_t first = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x >> 6) * 1024);
 #pragma unroll
-        for (int i = 0; i < Tile<D>::loads; ++i) {
-            const int u = threadIdx.x + i * kThreads, row = u / Tile<D>::units, unit = u % Tile<D>::units;
-            *reinterpret_cast<uint4*>(keys + (row * Tile<D>::units + (unit ^ Tile<D>::key_swizzle(row))) * 16) = key[i];
-            *reinterpret_cast<uint4*>(values + (row * Tile<D>::units + (unit ^ Tile<D>::value_swizzle(row))) * 16) = value[i];
-        }
+        for (int i = 0; i < Tile<D>::loads; ++i)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                         :
+                         : "s"(first + i * (kThreads * 16)), "v"(at + i * Tile<D>::load_rows * row_bytes), "s"(buffer)
+                         : "memory");
     }
 };
+
+// Waits for the wave's copies and then for the other waves.
+__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <int D>
 struct State {
@@ -286,7 +295,7 @@ __device__ void clear_rest(const std::int32_t* __restrict__ q_offsets, T* __rest
 }
 
 template <class T, int D>
-__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void packed_attention(
+__global__ __launch_bounds__(kThreads, 2) void packed_attention(
     const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const std::int32_t* __restrict__ q_offsets,
     const std::int32_t* __restrict__ k_offsets, T* __restrict__ out, Geometry g) {
     __shared__ __align__(16) unsigned char memory[4 * Tile<D>::bytes];
@@ -337,26 +346,25 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void packed_attention(
     const std::int64_t stride = static_cast<std::int64_t>(g.kv_heads) * g.head_dim;
     const T* key = k + s.k_first * stride + head * g.head_dim;
     const T* value = v + s.k_first * stride + head * g.head_dim;
-    Stage<T, D> stage;
-    if (end > 0) {
-        stage.load(key, value, stride, s.keys, g.head_dim);
-        stage.store(memory, memory + Tile<D>::bytes);
-    }
-    __syncthreads();
+    const Copy<D> copy(g.kv_heads * g.head_dim, g.head_dim);
+    typedef __attribute__((address_space(3))) unsigned char* Lds;
+    const auto lds = static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>((Lds)(memory)));
+    const auto fetch = [&](int at, int turn) {
+        copy(key + at * stride, s.keys - at, copy.key_at, lds + turn * (2 * Tile<D>::bytes));
+        copy(value + at * stride, s.keys - at, copy.value_at, lds + turn * (2 * Tile<D>::bytes) + Tile<D>::bytes);
+    };
+    if (end > 0) fetch(0, 0);
+    copies_done();
     for (int at = 0, turn = 0; at < end; at += kKeys, turn ^= 1) {
         const unsigned char* now = memory + turn * (2 * Tile<D>::bytes);
-        unsigned char* next = memory + (turn ^ 1) * (2 * Tile<D>::bytes);
-        const bool more = at + kKeys < end;
-        if (more)
-            stage.load(key + (at + kKeys) * stride, value + (at + kKeys) * stride, stride, s.keys - at - kKeys, g.head_dim);
+        if (at + kKeys < end) fetch(at + kKeys, turn ^ 1);
         if (at < most) {
             if (at + kKeys <= least)
                 compute<T, D, false>(now, now + Tile<D>::bytes, a, factor, 0);
             else
                 compute<T, D, true>(now, now + Tile<D>::bytes, a, factor, seen - at);
         }
-        if (more) stage.store(next, next + Tile<D>::bytes);
-        __syncthreads();
+        copies_done();
     }
     a.sum += __shfl_xor(a.sum, 32, 64);
     const float scale = a.sum != 0.0f ? 1.0f / a.sum : 0.0f;
@@ -382,6 +390,7 @@ Geometry geometry(int tokens, int keys, int sequences, int q_heads, int kv_heads
     require(static_cast<std::int64_t>(tokens) * group < (1ll << 31) - kRows, "packed attention rows of a KV head must fit int32");
     const std::int64_t blocks = static_cast<std::int64_t>(tokens) * group / kRows + 1 + sequences;
     require(blocks * kv_heads < (1ll << 31), "packed attention blocks must fit int32");
+    require(static_cast<std::int64_t>(kv_heads) * head_dim < (1 << 23), "packed attention takes key rows of at most 8388607 columns");
     return {tokens, keys, sequences, q_heads, kv_heads, group, head_dim, scale};
 }
 
