@@ -186,14 +186,18 @@ __device__ __forceinline__ void compute(const unsigned char* __restrict__ keys, 
     const int lane = threadIdx.x & 63, m = lane & 31, h = lane >> 5;
     float16v score[kTiles];
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
+    for (int t = 0; t < kTiles; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) score[t][r] = 0.0f;
-        const int row = 32 * t + m;
+    // The swizzle turns the low three bits of a unit; the rest of the address is a constant beside the row's.
+    const unsigned char* row = keys + m * (Tile<D>::units * 16);
+    const int turn = Tile<D>::key_swizzle(m);
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-            const uint4 k = *reinterpret_cast<const uint4*>(
-                keys + (row * Tile<D>::units + ((2 * s + h) ^ Tile<D>::key_swizzle(row))) * 16);
+    for (int s = 0; s < D / 16; ++s) {
+        const unsigned char* at = row + ((((2 * s) & 7) | h) ^ turn) * 16;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            const uint4 k = *reinterpret_cast<const uint4*>(at + 32 * t * (Tile<D>::units * 16) + ((2 * s) & ~7) * 16);
             score[t] = Matrix<T>::multiply(k, a.query[s], score[t]);
         }
     }
@@ -230,21 +234,20 @@ __device__ __forceinline__ void compute(const unsigned char* __restrict__ keys, 
         weight[2 * t + 1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
     const int group = lane >> 4, i = lane & 15;
-    const int row0 = 4 * h + (i >> 2);
+    const int row0 = 4 * h + (i >> 2);  // rows 16 t + 8 p + row0
     bool broken = false;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) {
-        const int unit = (4 * d + 2 * (group & 1) + ((i & 3) >> 1)) ^ Tile<D>::value_swizzle(row0);
 #pragma unroll
         for (int t = 0; t < 2 * kTiles; ++t) {
-            // Rows 16 t + 8 p + row0: the swizzle repeats with period 8.
             uint2 part[2];
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
-                const int row = 16 * t + 8 * p + row0;
-                const int place = Tile<D>::units >= 16 ? unit
-                                                       : (4 * d + 2 * (group & 1) + ((i & 3) >> 1)) ^ Tile<D>::value_swizzle(row);
-                const unsigned char* at = values + (row * Tile<D>::units + place) * 16 + 8 * (i & 1);
+                const int unit = ((4 * d) & 15) | 2 * (group & 1) | (i & 3) >> 1;
+                // From 16 units on the swizzle repeats every 8 rows.
+                const int place = unit ^ Tile<D>::value_swizzle(Tile<D>::units >= 16 ? row0 : 16 * t + 8 * p + row0);
+                const unsigned char* at = values + row0 * (Tile<D>::units * 16) + place * 16 + 8 * (i & 1) +
+                                          ((16 * t + 8 * p) * Tile<D>::units + ((4 * d) & ~15)) * 16;
                 typedef __attribute__((address_space(3))) short4v* Lds;
                 part[p] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at)));
             }
