@@ -50,6 +50,11 @@ template <> struct Matrix<__half> {
         v[1] = static_cast<_Float16>(b);
         return __builtin_bit_cast(std::uint32_t, v);
     }
+    // sum + both halves of w.
+    static __device__ __forceinline__ float add(std::uint32_t w, float sum) {
+        const half2v ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, w), ones, sum, false);
+    }
 };
 template <> struct Matrix<__hip_bfloat16> {
     static constexpr std::uint32_t kExponent = 0x7f80;
@@ -61,6 +66,10 @@ template <> struct Matrix<__hip_bfloat16> {
         v[0] = static_cast<__bf16>(a);
         v[1] = static_cast<__bf16>(b);
         return __builtin_bit_cast(std::uint32_t, v);
+    }
+    static __device__ __forceinline__ float add(std::uint32_t w, float sum) {
+        const bfloat2v ones = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bfloat2v, w), ones, sum, false);
     }
 };
 
@@ -227,8 +236,8 @@ __device__ __forceinline__ void compute(const unsigned char* __restrict__ keys, 
         for (int r = 0; r < 16; r += 2) {
             const float x = __builtin_amdgcn_exp2f(fmaf(score[t][r], factor, base));
             const float y = __builtin_amdgcn_exp2f(fmaf(score[t][r + 1], factor, base));
-            a.sum += x + y;
             w[r / 2] = Matrix<T>::pack(x, y);
+            a.sum = Matrix<T>::add(w[r / 2], a.sum);
         }
         weight[2 * t] = make_uint4(w[0], w[1], w[2], w[3]);
         weight[2 * t + 1] = make_uint4(w[4], w[5], w[6], w[7]);
