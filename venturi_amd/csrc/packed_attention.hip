@@ -210,6 +210,16 @@ __device__ __forceinline__ void compute(const unsigned char* __restrict__ keys, 
             score[t] = Matrix<T>::multiply(k, a.query[s], score[t]);
         }
     }
+    if constexpr (D <= 128) {
+        // The LDS reads run four ahead of the products.
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int i = 0; i < D / 16 * kTiles - 4; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
+    }
     float top = -__builtin_inff();
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
@@ -270,6 +280,15 @@ __device__ __forceinline__ void compute(const unsigned char* __restrict__ keys, 
             }
             a.out[d] = Matrix<T>::multiply(v, weight[t], a.out[d]);
         }
+    }
+    if constexpr (!MASKED && D <= 128) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 1);
+#pragma unroll
+        for (int i = 0; i < D / 32 * 2 * kTiles - 3; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 1);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 3, 1);
     }
     if (MASKED && __any(broken)) {
         // Rare: infinities and NaN go to the rows that see them, key by key.
