@@ -26,6 +26,8 @@
 // A sequence of one chunk is finished by its workgroup, others leave partial outputs, joined by a second launch.
 #include "kv_cache.hpp"
 
+#include <climits>
+
 namespace vt {
 namespace {
 
@@ -34,7 +36,7 @@ typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4, kBlock = 32;           // keys of a wave's step
-constexpr int kMinChunk = kWaves * kBlock;
+constexpr int kMinChunk = 128;
 constexpr int kTarget = 512;                     // workgroups: two to a CU
 constexpr float kLazy = 4.0f, kShift = 8.0f;     // weights are 2^(s - m + kShift), at most 2^12
 
@@ -69,8 +71,9 @@ __device__ __forceinline__ std::int64_t chunk_length(const std::int32_t* __restr
     std::int64_t total = 0;
     for (int s = lane; s < g.sequences; s += 64) total += admitted(lengths[s], g);
     total = wave_sum(total);
-    const std::int64_t least = (total + g.target - 1) / g.target;
-    return max((least + kMinChunk - 1) / kMinChunk, std::int64_t{1}) * kMinChunk;
+    // A chunk is no longer than a sequence need be: below 2^31 (uniform, so that the loops over it are).
+    const std::int64_t least = (total + g.target - 1) / g.target, blocks = max((least + kMinChunk - 1) / kMinChunk, std::int64_t{1});
+    return static_cast<std::int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(min(blocks, std::int64_t{INT_MAX / kMinChunk})))) * kMinChunk;
 }
 
 // Chunks per sequence: at least one. Their sum is at most target + sequences.
@@ -96,13 +99,13 @@ __device__ __forceinline__ bool find_work(const std::int32_t* __restrict__ lengt
         if (hit) {
             const int at = __ffsll(hit) - 1;
             w.sequence = base + at;
-            w.length = __shfl(length, at, 64);
-            w.splits = __shfl(n, at, 64);
-            w.first = __shfl(end, at, 64) - w.splits;
+            w.length = __builtin_amdgcn_readlane(length, at);
+            w.splits = __builtin_amdgcn_readlane(n, at);
+            w.first = __builtin_amdgcn_readlane(end, at) - w.splits;
             w.split = flat - w.first;
             return true;
         }
-        before = __shfl(end, 63, 64);
+        before = __builtin_amdgcn_readlane(end, 63);
     }
     return false;
 }
@@ -161,85 +164,100 @@ struct Segments {
     static constexpr int words = word(count);
 };
 
-// One step's codes and scales of a wave, as its lanes hold them.
+// One step of a wave in LDS: 16 keys' codes, twice, for K and for V, then their scales [group][16]. A row's 16-byte units are
+// turned by its number, so that the same columns of 16 rows lie on different banks.
 template <int D>
 struct Step {
-    std::uint32_t key[2][D / 32][2];           // tile, group: 8 codes of one key
-    uint2 key_scale[2][D / 32];                // four keys
-    std::uint32_t value[8][Segments<D>::words];  // keys 4g + 0..3 of both tiles
-    uint2 value_scale[2][Segments<D>::count];
+    static constexpr int units = D / 16;          // of a row
+    static constexpr int tile = 16 * D;           // bytes of a tile's codes
+    static constexpr int scales = D;              // bytes of a tile's scales
+    static constexpr int bytes = 4 * tile + 4 * scales;
+    static constexpr int loads = (D + 63) / 64 + 1;  // of a tile and side
+    static __device__ __forceinline__ int swizzle(int row) {
+        if constexpr (units == 16) return row & 15;
+        else if constexpr (units == 8) return (row >> 1) & 7;
+        else if constexpr (units == 4 || units == 12) return (row >> 2) & 3;
+        else return 0;  // the rows' own stride spreads them
+    }
 };
+
+// How a workgroup's waves divide a round: ROWS tiles of 16 rows by KEYS steps of 32 keys, and how many rounds are in flight.
+template <int D, int ROWS>
+struct Shape {
+    static constexpr int keys = kWaves / ROWS;
+    static constexpr int round_bytes = keys * Step<D>::bytes;
+    static constexpr int ring = 79872 / round_bytes < 2 ? 2 : 79872 / round_bytes > 4 ? 4 : 79872 / round_bytes;
+    static constexpr int bytes = ring * round_bytes;
+    static constexpr int loads = 4 * Step<D>::loads / ROWS;  // of a wave and round
+    static_assert(bytes <= 163840 - 1024 && 256 * D <= bytes, "the ring fits, and the joined rows fit the ring");
+};
+
+typedef const __attribute__((address_space(4))) std::int32_t* Constant;  // read through the scalar cache
 
 struct Pages {
     CachePlanes planes;
     const std::int32_t* table;
-    int tiles_per_page;
+    int tiles_per_page, head;
     std::uint64_t magic;
-    int head;
     __device__ __forceinline__ int page_of(int tile) const {
         return static_cast<int>((static_cast<std::uint64_t>(tile) * magic) >> 36);
     }
 };
 
-template <int D>
-__device__ __forceinline__ void load_step(const Pages& p, int first_tile, int last_tile, Step<D>& s, bool& bad) {
-    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+__device__ __forceinline__ void copy16(std::uint32_t lds, const void* base, std::uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void copy4(std::uint32_t lds, const void* base, std::uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory");
+}
+
+// Starts the copies of a wave's share of a step into LDS: parts (side, tile), every ROWS-th of the four.
+template <int D, int ROWS>
+__device__ __forceinline__ void fetch(const Pages& p, int first_tile, int last_tile, int share, std::uint32_t lds, bool& bad) {
+    const int lane = threadIdx.x & 63;
     const int page_tokens = p.tiles_per_page * 16;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const int tile = __builtin_amdgcn_readfirstlane(min(first_tile + t, last_tile));
         const int at = p.page_of(tile), inside = (tile - at * p.tiles_per_page) * 16;
-        int page = __builtin_amdgcn_readfirstlane(p.table[at]);
+        int page = reinterpret_cast<Constant>(reinterpret_cast<std::uintptr_t>(p.table))[at];
         if (page < 0 || page >= p.planes.pages) {
             bad = true;
             page = 0;
         }
         const std::int64_t base = static_cast<std::int64_t>(page) * p.planes.kv_heads + p.head;
-        const std::uint8_t* keys = p.planes.key_codes + (base * page_tokens + inside) * D;
-        const std::uint8_t* values = p.planes.value_codes + (base * page_tokens + inside) * D;
-        const __half* key_scales = p.planes.key_scales + base * (D / 32) * page_tokens + inside;
-        const __half* value_scales = p.planes.value_scales + base * (D / 32) * page_tokens + inside;
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-            const uint2 w = *reinterpret_cast<const uint2*>(keys + m * D + 32 * c + 8 * g);
-            s.key[t][c][0] = w.x;
-            s.key[t][c][1] = w.y;
-            s.key_scale[t][c] = *reinterpret_cast<const uint2*>(key_scales + c * page_tokens + 4 * g);
-        }
+        for (int side = 0; side < 2; ++side) {
+            if ((2 * side + t) % ROWS != share) continue;
+            const std::uint8_t* codes = (side ? p.planes.value_codes : p.planes.key_codes) + (base * page_tokens + inside) * D;
+            const __half* scales = (side ? p.planes.value_scales : p.planes.key_scales) + base * (D / 32) * page_tokens + inside;
+            const std::uint32_t to = __builtin_amdgcn_readfirstlane(lds + (2 * side + t) * Step<D>::tile);
 #pragma unroll
-        for (int i = 0; i < Segments<D>::count; ++i) {
-            const int w = Segments<D>::width(i), columns = w / 16, word = Segments<D>::word(i), column = Segments<D>::offset(i) + columns * m;
-            s.value_scale[t][i] =
-                *reinterpret_cast<const uint2*>(value_scales + (column >> 5) * page_tokens + 4 * g);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const std::uint8_t* row = values + (4 * g + r) * D + column;
-                std::uint32_t* out = s.value[4 * t + r] + word;
-                if (w == 256) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(row);
-                    out[0] = v.x, out[1] = v.y, out[2] = v.z, out[3] = v.w;
-                } else if (w == 128) {
-                    const uint2 v = *reinterpret_cast<const uint2*>(row);
-                    out[0] = v.x, out[1] = v.y;
-                } else if (w == 64) {
-                    out[0] = *reinterpret_cast<const std::uint32_t*>(row);
-                } else {
-                    out[0] = *reinterpret_cast<const unsigned short*>(row);
-                }
+            for (int i = 0; i < Step<D>::loads - 1; ++i) {
+                const int unit = 64 * i + lane, row = unit / Step<D>::units, place = unit % Step<D>::units;
+                if (64 * i + 64 <= D || unit < D)
+                    copy16(to + 1024 * i, codes, row * D + 16 * (place ^ Step<D>::swizzle(row)));
             }
+            const std::uint32_t to_scales = __builtin_amdgcn_readfirstlane(lds + 4 * Step<D>::tile + (2 * side + t) * Step<D>::scales);
+            if (D == 256 || lane < D / 4) copy4(to_scales, scales, (lane >> 3) * page_tokens * 2 + (lane & 7) * 4);
         }
     }
 }
 
-// A wave's running state over its 16 * QT query rows.
-template <int D, int QT>
+// Where the registers hold it the codes' offset is taken off by the accumulator's start; at large heads by an fma each, which
+// leaves two waves on a SIMD.
+template <int D>
+constexpr bool kOffsetInStart = D <= 128;
+
+// A wave's running state over its 16 query rows.
+template <int D>
 struct State {
-    half8v query[QT][D / 32];
-    float4v start[QT][D / 32];   // -128 * 2^-24 sum of the group's query numbers
-    float factor[QT];            // scale * log2 e * 2^24 * the row's power of two
-    int seen[QT];                // keys that the lane's row sees
-    float reference[QT], sum[QT];
-    float4v out[QT][D / 16];
+    half8v query[D / 32];
+    float4v start[kOffsetInStart<D> ? D / 32 : 1];  // -128 * 2^-24 sum of the group's query numbers
+    float factor;                // scale * log2 e * the row's and the codes' powers of two
+    int seen;                    // keys that the lane's row sees
+    float reference, sum;
+    float4v out[D / 16];
     float bring;                 // k: 2^(-ceil(log2 of the largest value scale so far))
 };
 
@@ -249,47 +267,55 @@ __device__ __forceinline__ float power_above(float v) {  // the smallest power o
     return ldexpf(1.0f, f == 0.5f ? e - 1 : e);
 }
 
-template <int D, int QT>
-__device__ __forceinline__ void compute(const Step<D>& s, State<D, QT>& a, int first_key, int length, bool full) {
-    const int g = (threadIdx.x & 63) >> 4;
-    float score[QT][8];
+// One step of 32 keys for the wave's rows, from LDS. FULL: every row sees all of them.
+template <int D, bool FULL>
+__device__ __forceinline__ void compute(const unsigned char* __restrict__ step, State<D>& a, int first_key, int length) {
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const unsigned char* key_rows = step + m * D + 8 * (g & 1);
+    const unsigned char* key_scales = step + 4 * Step<D>::tile + 8 * g;
+    float score[8];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
-        for (int q = 0; q < QT; ++q)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) score[q][4 * t + r] = 0.0f;
+        for (int r = 0; r < 4; ++r) score[4 * t + r] = 0.0f;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
-            const half8v keys = spread8(s.key[t][c][0], s.key[t][c][1]);
-#pragma unroll
-            for (int q = 0; q < QT; ++q) {
-                const float4v raw = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, a.query[q][c], a.start[q][c], 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    score[q][4 * t + r] = fmaf(raw[r], half_at(s.key_scale[t][c], r), score[q][4 * t + r]);
+            const uint2 codes = *reinterpret_cast<const uint2*>(key_rows + t * Step<D>::tile + 16 * ((2 * c + (g >> 1)) ^ Step<D>::swizzle(m)));
+            const uint2 scale = *reinterpret_cast<const uint2*>(key_scales + t * Step<D>::scales + 32 * c);
+            half8v keys = spread8(codes.x, codes.y);
+            if constexpr (!kOffsetInStart<D>) {
+                const half8v up = static_cast<_Float16>(32768.0f), down = static_cast<_Float16>(-0.25f);
+                keys = __builtin_elementwise_fma(keys, up, down);  // (u - 128) 2^-9
             }
+            const float4v raw = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, a.query[c], a.start[kOffsetInStart<D> ? c : 0], 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) score[4 * t + r] = fmaf(raw[r], half_at(scale, r), score[4 * t + r]);
         }
     }
     float value_scale[Segments<D>::count][8], top_scale = 0.0f;
 #pragma unroll
-    for (int i = 0; i < Segments<D>::count; ++i)
+    for (int i = 0; i < Segments<D>::count; ++i) {
+        const int group = (Segments<D>::offset(i) + Segments<D>::width(i) / 16 * m) >> 5;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            value_scale[i][j] = half_at(s.value_scale[j >> 2][i], j & 3);
-            // Slots past the length hold anything: their weights are 0, and so has to be what they multiply.
-            if (!full && first_key + 16 * (j >> 2) + 4 * g + (j & 3) >= length) value_scale[i][j] = 0.0f;
-            top_scale = fmaxf(top_scale, value_scale[i][j] <= 65504.0f ? value_scale[i][j] : 0.0f);
+        for (int t = 0; t < 2; ++t) {
+            const uint2 scale = *reinterpret_cast<const uint2*>(step + 4 * Step<D>::tile + (2 + t) * Step<D>::scales + 32 * group + 8 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float& v = value_scale[i][4 * t + r];
+                v = half_at(scale, r);
+                // Slots past the length hold anything: their weights are 0, and so has to be what they multiply.
+                if (!FULL && first_key + 16 * t + 4 * g + r >= length) v = 0.0f;
+                top_scale = fmaxf(top_scale, v <= 65504.0f ? v : 0.0f);
+            }
         }
+    }
     bool raise = top_scale * a.bring > 1.99f;
 #pragma unroll
-    for (int q = 0; q < QT; ++q)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            score[q][j] *= a.factor[q];
-            if (!full && first_key + 16 * (j >> 2) + 4 * g + (j & 3) >= a.seen[q]) score[q][j] = -__builtin_inff();
-            raise = raise || score[q][j] > a.reference[q] + kLazy;
-        }
+    for (int j = 0; j < 8; ++j) {
+        score[j] *= a.factor;
+        if (!FULL && first_key + 16 * (j >> 2) + 4 * g + (j & 3) >= a.seen) score[j] = -__builtin_inff();
+        raise = raise || score[j] > a.reference + kLazy;
+    }
     if (__any(raise)) {
 #pragma unroll
         for (int step = 1; step < 64; step <<= 1) top_scale = fmaxf(top_scale, __shfl_xor(top_scale, step, 64));
@@ -299,33 +325,25 @@ __device__ __forceinline__ void compute(const Step<D>& s, State<D, QT>& a, int f
             shrink = bring / a.bring;
             a.bring = bring;
         }
+        float top = a.reference;
 #pragma unroll
-        for (int q = 0; q < QT; ++q) {
-            float top = a.reference[q];
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, score[j]);
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float keep = a.reference == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(a.reference - top);
+        a.reference = top;
+        a.sum *= keep;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, score[q][j]);
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float keep = a.reference[q] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(a.reference[q] - top);
-            a.reference[q] = top;
-            a.sum[q] *= keep;
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d) a.out[q][d] *= keep * shrink;
-        }
+        for (int d = 0; d < D / 16; ++d) a.out[d] *= keep * shrink;
     }
-    half8v weights[QT];
+    const float base = a.reference == -__builtin_inff() ? 0.0f : a.reference - kShift;
+    float p[8];
 #pragma unroll
-    for (int q = 0; q < QT; ++q) {
-        const float base = a.reference[q] == -__builtin_inff() ? 0.0f : a.reference[q] - kShift;
-        float p[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            p[j] = __builtin_amdgcn_exp2f(score[q][j] - base);
-            a.sum[q] += p[j];
-        }
-        const uint4 w = make_uint4(pack(p[0], p[1]), pack(p[2], p[3]), pack(p[4], p[5]), pack(p[6], p[7]));
-        weights[q] = __builtin_bit_cast(half8v, w);
+    for (int j = 0; j < 8; ++j) {
+        p[j] = __builtin_amdgcn_exp2f(score[j] - base);
+        a.sum += p[j];
     }
+    const half8v weights = __builtin_bit_cast(half8v, make_uint4(pack(p[0], p[1]), pack(p[2], p[3]), pack(p[4], p[5]), pack(p[6], p[7])));
 #pragma unroll
     for (int i = 0; i < Segments<D>::count; ++i) {
         half2v steep[4], flat[4];
@@ -335,76 +353,91 @@ __device__ __forceinline__ void compute(const Step<D>& s, State<D, QT>& a, int f
             const float x = value_scale[i][2 * j] * a.bring, y = value_scale[i][2 * j + 1] * a.bring;
             // A row that does not see a key must not see its NaN: while rows differ, such scales are kept out of the
             // product and marked below.
-            const bool mark = !full && !(x < 2.0f && y < 2.0f);
+            const bool mark = !FULL && !(x < 2.0f && y < 2.0f);
             broken = broken || mark;
-            steep[j] = __builtin_bit_cast(half2v, pack(!full && !(x < 2.0f) ? 0.0f : x * 32768.0f, !full && !(y < 2.0f) ? 0.0f : y * 32768.0f));
-            flat[j] = __builtin_bit_cast(half2v, pack(!full && !(x < 2.0f) ? 0.0f : x * -0.25f, !full && !(y < 2.0f) ? 0.0f : y * -0.25f));
+            steep[j] = __builtin_bit_cast(half2v, pack(!FULL && !(x < 2.0f) ? 0.0f : x * 32768.0f, !FULL && !(y < 2.0f) ? 0.0f : y * 32768.0f));
+            flat[j] = __builtin_bit_cast(half2v, pack(!FULL && !(x < 2.0f) ? 0.0f : x * -0.25f, !FULL && !(y < 2.0f) ? 0.0f : y * -0.25f));
         }
-        const int columns = Segments<D>::width(i) / 16, word = Segments<D>::word(i), tile = Segments<D>::tile(i);
+        constexpr int kWords = 4;
+        const int columns = Segments<D>::width(i) / 16, tile = Segments<D>::tile(i);
+        const int column = Segments<D>::offset(i) + columns * m;
+        std::uint32_t value[8][kWords];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int row = 4 * g + (j & 3);
+            const unsigned char* at = step + (2 + (j >> 2)) * Step<D>::tile + row * D + 16 * ((column >> 4) ^ Step<D>::swizzle(row)) + (column & 15);
+            if (columns == 16) {
+                const uint4 v = *reinterpret_cast<const uint4*>(at);
+                value[j][0] = v.x, value[j][1] = v.y, value[j][2] = v.z, value[j][3] = v.w;
+            } else if (columns == 8) {
+                const uint2 v = *reinterpret_cast<const uint2*>(at);
+                value[j][0] = v.x, value[j][1] = v.y;
+            } else if (columns == 4) {
+                value[j][0] = *reinterpret_cast<const std::uint32_t*>(at);
+            } else {
+                value[j][0] = *reinterpret_cast<const unsigned short*>(at);
+            }
+        }
 #pragma unroll
         for (int d = 0; d < columns; ++d) {
             std::uint32_t v[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const std::uint32_t pair = permute(s.value[2 * j + 1][word + d / 4], s.value[2 * j][word + d / 4],
-                                                   0x0c000c00u | (d & 3) | (4 + (d & 3)) << 16);
+                const std::uint32_t pair = permute(value[2 * j + 1][d / 4], value[2 * j][d / 4], 0x0c000c00u | (d & 3) | (4 + (d & 3)) << 16);
                 const half2v x = __builtin_bit_cast(half2v, pair);
                 v[j] = __builtin_bit_cast(std::uint32_t, __builtin_elementwise_fma(x, steep[j], flat[j]));
             }
             const half8v values = __builtin_bit_cast(half8v, make_uint4(v[0], v[1], v[2], v[3]));
-#pragma unroll
-            for (int q = 0; q < QT; ++q)
-                a.out[q][tile + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values, weights[q], a.out[q][tile + d], 0, 0, 0);
+            a.out[tile + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values, weights, a.out[tile + d], 0, 0, 0);
         }
-        if (!full && __any(broken)) {
-            half8v marks;
+        if (!FULL && __any(broken)) {
+            half8v marks, sees;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 8; ++j) {
                 marks[j] = value_scale[i][j] * a.bring < 2.0f ? static_cast<_Float16>(0.0f) : static_cast<_Float16>(1.0f);
-#pragma unroll
-            for (int q = 0; q < QT; ++q) {
-                half8v sees;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    sees[j] = first_key + 16 * (j >> 2) + 4 * g + (j & 3) < a.seen[q] ? static_cast<_Float16>(1.0f)
-                                                                                      : static_cast<_Float16>(0.0f);
-                const float4v none = {0.0f, 0.0f, 0.0f, 0.0f};
-                const float4v hits = __builtin_amdgcn_mfma_f32_16x16x32_f16(marks, sees, none, 0, 0, 0);
-#pragma unroll
-                for (int d = 0; d < columns; ++d)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (hits[r] > 0.0f) a.out[q][tile + d][r] = __builtin_nanf("");
+                sees[j] = first_key + 16 * (j >> 2) + 4 * g + (j & 3) < a.seen ? static_cast<_Float16>(1.0f) : static_cast<_Float16>(0.0f);
             }
+            const float4v none = {0.0f, 0.0f, 0.0f, 0.0f};
+            const float4v hits = __builtin_amdgcn_mfma_f32_16x16x32_f16(marks, sees, none, 0, 0, 0);
+#pragma unroll
+            for (int d = 0; d < columns; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (hits[r] > 0.0f) a.out[tile + d][r] = __builtin_nanf("");
         }
     }
 }
 
-template <class T, int D, int QT>
-__device__ __forceinline__ void load_queries(const T* __restrict__ q, const Geometry& g, const Work& w, int head, int block,
-                                             State<D, QT>& a) {
-    const int lane = threadIdx.x & 63, m = lane & 15, lg = lane >> 4;
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        const int row = (block * QT + t) * 16 + m;
-        const bool live = row < g.rows;
+// The wave's 16 query rows from row `first` of the KV head's on: the loads, and what becomes of them.
+template <class T, int D>
+struct Queries {
+    T raw[D / 32][8];
+    bool live;
+
+    __device__ __forceinline__ Queries(const T* __restrict__ q, const Geometry& g, const Work& w, int head, int first, State<D>& a) {
+        const int lane = threadIdx.x & 63, m = lane & 15, lg = lane >> 4;
+        const int row = first + m;
+        live = row < g.rows;
         const int token = live ? row / g.group : 0;
-        const T* source = q + ((static_cast<std::int64_t>(w.sequence) * g.query_tokens + token) * g.q_heads +
-                               head * g.group + (live ? row - token * g.group : 0)) * g.head_dim;
-        a.seen[t] = live ? w.length - (g.query_tokens - 1 - token) : 0;
+        const T* source = q + ((static_cast<std::int64_t>(w.sequence) * g.query_tokens + token) * g.q_heads + head * g.group +
+                               (live ? row - token * g.group : 0)) * g.head_dim;
+        a.seen = live ? w.length - (g.query_tokens - 1 - token) : 0;
+        // Unconditional: a load under a condition is waited for at once.
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+            *reinterpret_cast<uint4*>(raw[c]) = *reinterpret_cast<const uint4*>(source + min(32 * c + 8 * lg, g.head_dim - 8));
+    }
+
+    __device__ __forceinline__ void settle(const Geometry& g, State<D>& a) const {
+        const int lg = (threadIdx.x & 63) >> 4;
         float x[D / 32][8], top = 0.0f;
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-            const int column = 32 * c + 8 * lg;
-            if (live && column < g.head_dim) {
-                load8(source + column, x[c]);
-            } else {
+        for (int c = 0; c < D / 32; ++c)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[c][j] = 0.0f;
+            for (int j = 0; j < 8; ++j) {
+                x[c][j] = live && 32 * c + 8 * lg < g.head_dim ? to_f32(raw[c][j]) : 0.0f;
+                top = fmaxf(top, fabsf(x[c][j]));
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[c][j]));
-        }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         // The largest number comes to [2^14, 2^15).
@@ -414,125 +447,143 @@ __device__ __forceinline__ void load_queries(const T* __restrict__ q, const Geom
             float total = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                a.query[t][c][j] = static_cast<_Float16>(ldexpf(x[c][j], -e));
-                total += static_cast<float>(a.query[t][c][j]);
+                a.query[c][j] = static_cast<_Float16>(ldexpf(x[c][j], -e));
+                total += static_cast<float>(a.query[c][j]);
             }
-            total += __shfl_xor(total, 16, 64);
-            total += __shfl_xor(total, 32, 64);
-            total *= -128.0f * 0x1p-24f;
-            a.start[t][c] = float4v{total, total, total, total};
+            if constexpr (kOffsetInStart<D>) {
+                total += __shfl_xor(total, 16, 64);
+                total += __shfl_xor(total, 32, 64);
+                total *= -128.0f * 0x1p-24f;
+                a.start[c] = float4v{total, total, total, total};
+            }
         }
-        a.factor[t] = ldexpf(g.scale * 1.44269504088896340736f, e + 24);
-        a.reference[t] = -__builtin_inff();
-        a.sum[t] = 0.0f;
+        if constexpr (!kOffsetInStart<D>) a.start[0] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        a.factor = ldexpf(g.scale * 1.44269504088896340736f, e + (kOffsetInStart<D> ? 24 : 9));
+        a.reference = -__builtin_inff();
+        a.sum = 0.0f;
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) a.out[t][d] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int d = 0; d < D / 16; ++d) a.out[d] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        a.bring = 0x1p24f;
     }
-    a.bring = 0x1p24f;
-}
+};
 
 // Partial results of a chunk: per row D outputs, then the reference and the sum.
 template <int D>
 constexpr int partial_floats() { return D + 2; }
 
-template <class T, int D, int QT>
-__global__ __launch_bounds__(kWaves * 64, D * QT <= 128 ? 2 : 1) void kv_attention(const T* __restrict__ q, CachePlanes planes,
+template <class T, int D, int ROWS>
+__global__ __launch_bounds__(kWaves * 64, 2) void kv_attention(const T* __restrict__ q, CachePlanes planes,
                                                             const std::int32_t* __restrict__ page_table,
                                                             const std::int32_t* __restrict__ lengths, T* __restrict__ out,
                                                             float* __restrict__ partial, Geometry g) {
-    __shared__ __align__(16) float joined[kWaves][16][D];
+    using S = Shape<D, ROWS>;
+    extern __shared__ __align__(16) unsigned char memory[];
     __shared__ float references[kWaves][16], sums[kWaves][16];
     __shared__ int broken;
     Work w;
     if (!find_work(lengths, g, blockIdx.x, w)) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, lg = lane >> 4;
+    const int lane = threadIdx.x & 63, m = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row_wave = wave % ROWS, key_wave = wave / ROWS;
     const int head = blockIdx.y / g.row_blocks, block = blockIdx.y - head * g.row_blocks;
     if (threadIdx.x == 0) broken = 0;
     const bool bad_length = w.length < 0 || w.length > g.longest;
     const int length = bad_length ? 0 : w.length;
     const int begin = static_cast<int>(w.split * w.chunk), end = static_cast<int>(min<std::int64_t>(begin + w.chunk, length));
-    State<D, QT> a;
-    load_queries<T, D, QT>(q, g, w, head, block, a);
-    const Pages pages{planes, page_table + static_cast<std::int64_t>(w.sequence) * g.max_pages, g.tiles_per_page, g.page_magic, head};
+    const Pages pages{planes, page_table + static_cast<std::int64_t>(w.sequence) * g.max_pages, g.tiles_per_page, head, g.page_magic};
     const int last_tile = (length + 15) / 16 - 1;
     const int all_see = length - (g.query_tokens - 1);  // keys below are seen by every row
+    typedef __attribute__((address_space(3))) unsigned char* Lds;
+    const auto lds = static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>((Lds)(memory)));
     bool bad = false;
-    int key = begin + wave * kBlock;
-    if (key < end) {
-        Step<D> now;
-        load_step<D>(pages, key >> 4, last_tile, now, bad);
-        for (; key < end; key += kWaves * kBlock) {
-            Step<D> next;
-            const int after = key + kWaves * kBlock;
-            if (after < end) load_step<D>(pages, after >> 4, last_tile, next, bad);
-            compute<D, QT>(now, a, key, length, key + kBlock <= all_see);
-            now = next;
-        }
+    const int rounds = end > begin ? (end - begin + S::keys * kBlock - 1) / (S::keys * kBlock) : 0;
+    const auto key_of = [&](int round) { return begin + (round * S::keys + key_wave) * kBlock; };
+    const auto place_of = [&](int round) { return (round % S::ring) * S::round_bytes + key_wave * Step<D>::bytes; };
+    const auto start = [&](int round) {
+        fetch<D, ROWS>(pages, key_of(round) >> 4, last_tile, row_wave, lds + place_of(round), bad);
+    };
+    State<D> a;
+    const Queries<T, D> queries(q, g, w, head, (block * ROWS + row_wave) * 16, a);
+#pragma unroll
+    for (int i = 0; i < S::ring - 1; ++i)
+        if (i < rounds) start(i);
+    queries.settle(g, a);
+    for (int i = 0; i < rounds; ++i) {
+        // The wave's copies of round i are done when those of the ring - 2 rounds after it are all that is in flight.
+        if (i + S::ring - 2 < rounds)
+            asm volatile("s_waitcnt vmcnt(%0)" : : "i"((S::ring - 2) * S::loads) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+        // Then everybody's are, and everybody has read round i - 1, whose place the next copies take.
+        if constexpr (ROWS > 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
+        if (i + S::ring - 1 < rounds) start(i + S::ring - 1);
+        const int key = key_of(i);
+        if (key + kBlock <= min(all_see, end))
+            compute<D, true>(memory + place_of(i), a, key, length);
+        else if (key < end)
+            compute<D, false>(memory + place_of(i), a, key, length);
     }
     __syncthreads();
     if (bad && lane == 0) broken = 1;
     const float nan = __builtin_nanf("");
+    auto* joined = reinterpret_cast<float*>(memory);  // [wave][16][D]
+    float sum = a.sum;
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (lg == 0) references[wave][m] = a.reference, sums[wave][m] = sum;
+    __syncthreads();
+    float top = references[row_wave][m];
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        float sum = a.sum[t];
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        if (lg == 0) references[wave][m] = a.reference[t], sums[wave][m] = sum;
-        __syncthreads();
-        float top = references[0][m];
+    for (int i = 1; i < S::keys; ++i) top = fmaxf(top, references[row_wave + i * ROWS][m]);
+    // 512 / bring undoes the values' power of two.
+    const float keep = a.reference == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(a.reference - top);
+    const float undo = keep * (512.0f / a.bring);
 #pragma unroll
-        for (int i = 1; i < kWaves; ++i) top = fmaxf(top, references[i][m]);
-        // 512 / bring undoes the values' power of two.
-        const float keep = a.reference[t] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(a.reference[t] - top);
-        const float undo = keep * (512.0f / a.bring);
+    for (int i = 0; i < Segments<D>::count; ++i) {
+        const int columns = Segments<D>::width(i) / 16;
 #pragma unroll
-        for (int i = 0; i < Segments<D>::count; ++i) {
-            const int columns = Segments<D>::width(i) / 16;
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int d = 0; d < columns; ++d)
+                joined[(wave * 16 + m) * D + Segments<D>::offset(i) + columns * (4 * lg + r) + d] = a.out[Segments<D>::tile(i) + d][r] * undo;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < ROWS * 16 * D / 4; i += kWaves * 64) {
+        const int r = i / (D / 4), column = (i - r * (D / 4)) * 4, row = block * ROWS * 16 + r;
+        if (row >= g.rows) continue;
+        const int first = r / 16, in = r % 16;
+        float best = references[first][in], total = 0.0f;
 #pragma unroll
-                for (int d = 0; d < columns; ++d)
-                    joined[wave][m][Segments<D>::offset(i) + columns * (4 * lg + r) + d] = a.out[t][Segments<D>::tile(i) + d][r] * undo;
+        for (int j = 1; j < S::keys; ++j) best = fmaxf(best, references[first + j * ROWS][in]);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < S::keys; ++j) {
+            const int from = first + j * ROWS;
+            const float own = references[from][in];
+            if (own != -__builtin_inff()) total += sums[from][in] * __builtin_amdgcn_exp2f(own - best);
+            else if (sums[from][in] != 0.0f) total = nan;  // scores of NaN alone
+            const float4 x = *reinterpret_cast<const float4*>(joined + (from * 16 + in) * D + column);
+            v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
         }
-        __syncthreads();
-        for (int i = threadIdx.x; i < 16 * D / 4; i += kWaves * 64) {
-            const int r = i / (D / 4), column = (i - r * (D / 4)) * 4, row = (block * QT + t) * 16 + r;
-            if (row >= g.rows) continue;
-            float best = references[0][r], total = 0.0f;
-#pragma unroll
-            for (int j = 1; j < kWaves; ++j) best = fmaxf(best, references[j][r]);
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int j = 0; j < kWaves; ++j) {
-                const float own = references[j][r];
-                if (own != -__builtin_inff()) total += sums[j][r] * __builtin_amdgcn_exp2f(own - best);
-                else if (sums[j][r] != 0.0f) total = nan;  // scores of NaN alone
-                const float4 x = *reinterpret_cast<const float4*>(&joined[j][r][column]);
-                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-            }
-            if (broken || bad_length) total = nan;
-            if (w.splits == 1) {
-                const int token = row / g.group;
-                T* target = out + ((static_cast<std::int64_t>(w.sequence) * g.query_tokens + token) * g.q_heads + head * g.group +
-                                   row - token * g.group) * g.head_dim + column;
-                const float scale = total == 0.0f ? 0.0f : 1.0f / total;
-                if (column < g.head_dim) {
-                    const std::uint32_t lo = __builtin_bit_cast(unsigned short, from_f32<T>(total == 0.0f ? 0.0f : v.x * scale)) |
-                                             static_cast<std::uint32_t>(__builtin_bit_cast(unsigned short, from_f32<T>(total == 0.0f ? 0.0f : v.y * scale))) << 16;
-                    const std::uint32_t hi = __builtin_bit_cast(unsigned short, from_f32<T>(total == 0.0f ? 0.0f : v.z * scale)) |
-                                             static_cast<std::uint32_t>(__builtin_bit_cast(unsigned short, from_f32<T>(total == 0.0f ? 0.0f : v.w * scale))) << 16;
-                    *reinterpret_cast<uint2*>(target) = make_uint2(lo, hi);
-                }
-            } else {
-                const std::int64_t slot = static_cast<std::int64_t>(blockIdx.x) * g.kv_heads + head;
-                float* target = partial + (slot * g.rows + row) * partial_floats<D>();
-                // Rows of D + 2 floats are 8-byte aligned.
-                *reinterpret_cast<float2*>(target + column) = make_float2(v.x, v.y);
-                *reinterpret_cast<float2*>(target + column + 2) = make_float2(v.z, v.w);
-                if (column == 0) *reinterpret_cast<float2*>(target + D) = make_float2(best, total);
-            }
+        if (broken || bad_length) total = nan;
+        if (w.splits == 1) {
+            const int token = row / g.group;
+            T* target = out + ((static_cast<std::int64_t>(w.sequence) * g.query_tokens + token) * g.q_heads + head * g.group +
+                               row - token * g.group) * g.head_dim + column;
+            const float scale = 1.0f / total;
+            const auto bits = [&](float x) {
+                return static_cast<std::uint32_t>(__builtin_bit_cast(unsigned short, from_f32<T>(total == 0.0f ? 0.0f : x * scale)));
+            };
+            if (column < g.head_dim)
+                *reinterpret_cast<uint2*>(target) = make_uint2(bits(v.x) | bits(v.y) << 16, bits(v.z) | bits(v.w) << 16);
+        } else {
+            const std::int64_t slot = static_cast<std::int64_t>(blockIdx.x) * g.kv_heads + head;
+            float* target = partial + (slot * g.rows + row) * partial_floats<D>();
+            // Rows of D + 2 floats are 8-byte aligned.
+            *reinterpret_cast<float2*>(target + column) = make_float2(v.x, v.y);
+            *reinterpret_cast<float2*>(target + column + 2) = make_float2(v.z, v.w);
+            if (column == 0) *reinterpret_cast<float2*>(target + D) = make_float2(best, total);
         }
-        __syncthreads();
     }
 }
 
@@ -575,8 +626,8 @@ __global__ __launch_bounds__(256) void kv_attention_join(const std::int32_t* __r
         if (lane + 64 * d < g.head_dim) target[lane + 64 * d] = from_f32<T>(total == 0.0f ? 0.0f : v[d] / total);
 }
 
-// Row tiles of a wave: two where a KV head has more than 16 rows and the registers hold them.
-int row_tiles(int rows, int head_dim) { return rows > 16 && head_dim <= 128 ? 2 : 1; }
+// Row tiles of a workgroup: one wave each, the rest of its four waves take other keys.
+int row_tiles(int rows) { return rows > 32 ? 4 : rows > 16 ? 2 : 1; }
 
 // Chunks per KV head and row block that the grid aims at.
 int target_chunks(int kv_heads, int row_blocks) { return std::max(1, kTarget / (kv_heads * row_blocks)); }
@@ -593,7 +644,7 @@ Geometry geometry(int sequences, int query_tokens, int q_heads, int kv_heads, in
     require(static_cast<std::int64_t>(sequences) * query_tokens * q_heads < (1ll << 31), "cached attention rows must fit int32");
     g.sequences = sequences, g.query_tokens = query_tokens, g.q_heads = q_heads, g.kv_heads = kv_heads;
     g.group = q_heads / kv_heads, g.rows = query_tokens * g.group, g.head_dim = head_dim;
-    const int block = 16 * row_tiles(g.rows, head_dim);
+    const int block = 16 * row_tiles(g.rows);
     g.row_blocks = (g.rows + block - 1) / block;
     require(static_cast<std::int64_t>(kv_heads) * g.row_blocks <= 65535 && sequences <= 65535,
             "cached attention takes at most 65535 sequences, and KV heads times row blocks");
@@ -611,19 +662,26 @@ std::uint64_t partial_bytes(const Geometry& g) {
     return chunks * g.kv_heads * g.rows * ((g.head_dim + 31) / 32 * 32 + 2) * sizeof(float);
 }
 
+template <class T, int D, int ROWS>
+void launch_rows(const T* q, const CachePlanes& planes, const std::int32_t* page_table, const std::int32_t* lengths, T* out,
+                 float* partial, const Geometry& g, hipStream_t stream) {
+    static LdsLimit limit;
+    limit.raise(kv_attention<T, D, ROWS>, Shape<D, ROWS>::bytes);
+    const dim3 grid(g.target + g.sequences, g.kv_heads * g.row_blocks);
+    kv_attention<T, D, ROWS><<<grid, kWaves * 64, Shape<D, ROWS>::bytes, stream>>>(q, planes, page_table, lengths, out, partial, g);
+}
+
 template <class T, int D>
 void launch(const void* q, const CachePlanes& planes, const std::int32_t* page_table, const std::int32_t* lengths, void* out,
             void* workspace, const Geometry& g, hipStream_t stream) {
-    const dim3 grid(g.target + g.sequences, g.kv_heads * g.row_blocks);
     const auto* queries = static_cast<const T*>(q);
     auto* target = static_cast<T*>(out);
     auto* partial = static_cast<float*>(workspace);
-    if constexpr (D <= 128) {
-        if (row_tiles(g.rows, D) == 2)
-            kv_attention<T, D, 2><<<grid, kWaves * 64, 0, stream>>>(queries, planes, page_table, lengths, target, partial, g);
+    switch (row_tiles(g.rows)) {
+        case 1: launch_rows<T, D, 1>(queries, planes, page_table, lengths, target, partial, g, stream); break;
+        case 2: launch_rows<T, D, 2>(queries, planes, page_table, lengths, target, partial, g, stream); break;
+        default: launch_rows<T, D, 4>(queries, planes, page_table, lengths, target, partial, g, stream); break;
     }
-    if (row_tiles(g.rows, D) == 1)
-        kv_attention<T, D, 1><<<grid, kWaves * 64, 0, stream>>>(queries, planes, page_table, lengths, target, partial, g);
     check(hipGetLastError());
     if (partial_bytes(g)) {
         const auto rows = static_cast<unsigned>((static_cast<std::int64_t>(g.query_tokens) * g.q_heads + 3) / 4);
