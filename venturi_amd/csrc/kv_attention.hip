@@ -187,9 +187,9 @@ struct Shape {
     static constexpr int keys = kWaves / ROWS;
     static constexpr int round_bytes = keys * Step<D>::bytes;
     static constexpr int ring = 79872 / round_bytes < 2 ? 2 : 79872 / round_bytes > 4 ? 4 : 79872 / round_bytes;
-    static constexpr int bytes = ring * round_bytes;
+    static constexpr int bytes = ring * round_bytes > 256 * (D + 4) ? ring * round_bytes : 256 * (D + 4);  // or the joined rows
     static constexpr int loads = 4 * Step<D>::loads / ROWS;  // of a wave and round
-    static_assert(bytes <= 163840 - 1024 && 256 * D <= bytes, "the ring fits, and the joined rows fit the ring");
+    static_assert(bytes <= 163840 - 1024, "the ring fits the LDS");
 };
 
 typedef const __attribute__((address_space(4))) std::int32_t* Constant;  // read through the scalar cache
@@ -211,26 +211,37 @@ __device__ __forceinline__ void copy4(std::uint32_t lds, const void* base, std::
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory");
 }
 
+// Where the two tiles of a step lie: their pages, and their first keys' places there.
+struct Places {
+    int page[2], inside[2];
+};
+
+__device__ __forceinline__ Places places_of(const Pages& p, int first_tile, int last_tile) {
+    Places at;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int tile = min(first_tile + t, last_tile), entry = p.page_of(tile);
+        at.inside[t] = (tile - entry * p.tiles_per_page) * 16;
+        at.page[t] = reinterpret_cast<Constant>(reinterpret_cast<std::uintptr_t>(p.table))[entry];
+    }
+    return at;
+}
+
 // Starts the copies of a wave's share of a step into LDS: parts (side, tile), every ROWS-th of the four.
 template <int D, int ROWS>
-__device__ __forceinline__ void fetch(const Pages& p, int first_tile, int last_tile, int share, std::uint32_t lds, bool& bad) {
+__device__ __forceinline__ void fetch(const Pages& p, const Places& at, int share, std::uint32_t lds, bool& bad) {
     const int lane = threadIdx.x & 63;
     const int page_tokens = p.tiles_per_page * 16;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        const int tile = __builtin_amdgcn_readfirstlane(min(first_tile + t, last_tile));
-        const int at = p.page_of(tile), inside = (tile - at * p.tiles_per_page) * 16;
-        int page = reinterpret_cast<Constant>(reinterpret_cast<std::uintptr_t>(p.table))[at];
-        if (page < 0 || page >= p.planes.pages) {
-            bad = true;
-            page = 0;
-        }
-        const std::int64_t base = static_cast<std::int64_t>(page) * p.planes.kv_heads + p.head;
+        const bool outside = at.page[t] < 0 || at.page[t] >= p.planes.pages;
+        bad = bad || outside;
+        const std::int64_t base = static_cast<std::int64_t>(outside ? 0 : at.page[t]) * p.planes.kv_heads + p.head;
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
             if ((2 * side + t) % ROWS != share) continue;
-            const std::uint8_t* codes = (side ? p.planes.value_codes : p.planes.key_codes) + (base * page_tokens + inside) * D;
-            const __half* scales = (side ? p.planes.value_scales : p.planes.key_scales) + base * (D / 32) * page_tokens + inside;
+            const std::uint8_t* codes = (side ? p.planes.value_codes : p.planes.key_codes) + (base * page_tokens + at.inside[t]) * D;
+            const __half* scales = (side ? p.planes.value_scales : p.planes.key_scales) + base * (D / 32) * page_tokens + at.inside[t];
             const std::uint32_t to = __builtin_amdgcn_readfirstlane(lds + (2 * side + t) * Step<D>::tile);
 #pragma unroll
             for (int i = 0; i < Step<D>::loads - 1; ++i) {
@@ -273,23 +284,64 @@ __device__ __forceinline__ void compute(const unsigned char* __restrict__ step, 
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const unsigned char* key_rows = step + m * D + 8 * (g & 1);
     const unsigned char* key_scales = step + 4 * Step<D>::tile + 8 * g;
+    // A tile's LDS reads before its products, and the values' before the softmax: a read costs its latency once.
     float score[8];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) score[4 * t + r] = 0.0f;
+    uint2 codes[2][D / 32], scales[2][D / 32];
+    const auto read = [&](int t) {
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
-            const uint2 codes = *reinterpret_cast<const uint2*>(key_rows + t * Step<D>::tile + 16 * ((2 * c + (g >> 1)) ^ Step<D>::swizzle(m)));
-            const uint2 scale = *reinterpret_cast<const uint2*>(key_scales + t * Step<D>::scales + 32 * c);
-            half8v keys = spread8(codes.x, codes.y);
+            codes[t][c] = *reinterpret_cast<const uint2*>(key_rows + t * Step<D>::tile + 16 * ((2 * c + (g >> 1)) ^ Step<D>::swizzle(m)));
+            scales[t][c] = *reinterpret_cast<const uint2*>(key_scales + t * Step<D>::scales + 32 * c);
+        }
+    };
+    read(0);
+    if constexpr (D <= 128) read(1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        if (D > 128 && t == 1) {  // the registers hold one tile
+            read(1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        float4v raw[D / 32];
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+            half8v keys = spread8(codes[t][c].x, codes[t][c].y);
             if constexpr (!kOffsetInStart<D>) {
                 const half8v up = static_cast<_Float16>(32768.0f), down = static_cast<_Float16>(-0.25f);
                 keys = __builtin_elementwise_fma(keys, up, down);  // (u - 128) 2^-9
             }
-            const float4v raw = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, a.query[c], a.start[kOffsetInStart<D> ? c : 0], 0, 0, 0);
+            float4v start = {0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (kOffsetInStart<D>) start = a.start[c];
+            raw[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, a.query[c], start, 0, 0, 0);
+        }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) score[4 * t + r] = fmaf(raw[r], half_at(scale, r), score[4 * t + r]);
+        for (int r = 0; r < 4; ++r) {
+            score[4 * t + r] = raw[0][r] * half_at(scales[t][0], r);
+#pragma unroll
+            for (int c = 1; c < D / 32; ++c) score[4 * t + r] = fmaf(raw[c][r], half_at(scales[t][c], r), score[4 * t + r]);
+        }
+    }
+    std::uint32_t value[8][Segments<D>::words];
+#pragma unroll
+    for (int i = 0; i < Segments<D>::count; ++i) {
+        const int columns = Segments<D>::width(i) / 16, column = Segments<D>::offset(i) + columns * m;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int row = 4 * g + (j & 3);
+            const unsigned char* at = step + (2 + (j >> 2)) * Step<D>::tile + row * D + 16 * ((column >> 4) ^ Step<D>::swizzle(row)) + (column & 15);
+            std::uint32_t* to = value[j] + Segments<D>::word(i);
+            if (columns == 16) {
+                const uint4 v = *reinterpret_cast<const uint4*>(at);
+                to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+            } else if (columns == 8) {
+                const uint2 v = *reinterpret_cast<const uint2*>(at);
+                to[0] = v.x, to[1] = v.y;
+            } else if (columns == 4) {
+                to[0] = *reinterpret_cast<const std::uint32_t*>(at);
+            } else {
+                to[0] = *reinterpret_cast<const unsigned short*>(at);
+            }
         }
     }
     float value_scale[Segments<D>::count][8], top_scale = 0.0f;
@@ -358,32 +410,13 @@ __device__ __forceinline__ void compute(const unsigned char* __restrict__ step, 
             steep[j] = __builtin_bit_cast(half2v, pack(!FULL && !(x < 2.0f) ? 0.0f : x * 32768.0f, !FULL && !(y < 2.0f) ? 0.0f : y * 32768.0f));
             flat[j] = __builtin_bit_cast(half2v, pack(!FULL && !(x < 2.0f) ? 0.0f : x * -0.25f, !FULL && !(y < 2.0f) ? 0.0f : y * -0.25f));
         }
-        constexpr int kWords = 4;
-        const int columns = Segments<D>::width(i) / 16, tile = Segments<D>::tile(i);
-        const int column = Segments<D>::offset(i) + columns * m;
-        std::uint32_t value[8][kWords];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int row = 4 * g + (j & 3);
-            const unsigned char* at = step + (2 + (j >> 2)) * Step<D>::tile + row * D + 16 * ((column >> 4) ^ Step<D>::swizzle(row)) + (column & 15);
-            if (columns == 16) {
-                const uint4 v = *reinterpret_cast<const uint4*>(at);
-                value[j][0] = v.x, value[j][1] = v.y, value[j][2] = v.z, value[j][3] = v.w;
-            } else if (columns == 8) {
-                const uint2 v = *reinterpret_cast<const uint2*>(at);
-                value[j][0] = v.x, value[j][1] = v.y;
-            } else if (columns == 4) {
-                value[j][0] = *reinterpret_cast<const std::uint32_t*>(at);
-            } else {
-                value[j][0] = *reinterpret_cast<const unsigned short*>(at);
-            }
-        }
+        const int columns = Segments<D>::width(i) / 16, tile = Segments<D>::tile(i), word = Segments<D>::word(i);
 #pragma unroll
         for (int d = 0; d < columns; ++d) {
             std::uint32_t v[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const std::uint32_t pair = permute(value[2 * j + 1][d / 4], value[2 * j][d / 4], 0x0c000c00u | (d & 3) | (4 + (d & 3)) << 16);
+                const std::uint32_t pair = permute(value[2 * j + 1][word + d / 4], value[2 * j][word + d / 4], 0x0c000c00u | (d & 3) | (4 + (d & 3)) << 16);
                 const half2v x = __builtin_bit_cast(half2v, pair);
                 v[j] = __builtin_bit_cast(std::uint32_t, __builtin_elementwise_fma(x, steep[j], flat[j]));
             }
@@ -457,7 +490,6 @@ struct Queries {
                 a.start[c] = float4v{total, total, total, total};
             }
         }
-        if constexpr (!kOffsetInStart<D>) a.start[0] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
         a.factor = ldexpf(g.scale * 1.44269504088896340736f, e + (kOffsetInStart<D> ? 24 : 9));
         a.reference = -__builtin_inff();
         a.sum = 0.0f;
@@ -499,14 +531,21 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv_attention(const T* __restri
     const int rounds = end > begin ? (end - begin + S::keys * kBlock - 1) / (S::keys * kBlock) : 0;
     const auto key_of = [&](int round) { return begin + (round * S::keys + key_wave) * kBlock; };
     const auto place_of = [&](int round) { return (round % S::ring) * S::round_bytes + key_wave * Step<D>::bytes; };
-    const auto start = [&](int round) {
-        fetch<D, ROWS>(pages, key_of(round) >> 4, last_tile, row_wave, lds + place_of(round), bad);
-    };
+    const auto places = [&](int round) { return places_of(pages, key_of(round) >> 4, last_tile); };
+    const auto start = [&](int round, const Places& at) { fetch<D, ROWS>(pages, at, row_wave, lds + place_of(round), bad); };
     State<D> a;
     const Queries<T, D> queries(q, g, w, head, (block * ROWS + row_wave) * 16, a);
+    // The page table is read a round before its pages are (past the last round, of the last tile again).
+    Places next = {};
+    if (rounds) {
+        Places first[S::ring];
 #pragma unroll
-    for (int i = 0; i < S::ring - 1; ++i)
-        if (i < rounds) start(i);
+        for (int i = 0; i < S::ring; ++i) first[i] = places(i);
+#pragma unroll
+        for (int i = 0; i < S::ring - 1; ++i)
+            if (i < rounds) start(i, first[i]);
+        next = first[S::ring - 1];
+    }
     queries.settle(g, a);
     for (int i = 0; i < rounds; ++i) {
         // The wave's copies of round i are done when those of the ring - 2 rounds after it are all that is in flight.
@@ -516,7 +555,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv_attention(const T* __restri
             asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
         // Then everybody's are, and everybody has read round i - 1, whose place the next copies take.
         if constexpr (ROWS > 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
-        if (i + S::ring - 1 < rounds) start(i + S::ring - 1);
+        if (i + S::ring - 1 < rounds) {
+            start(i + S::ring - 1, next);
+            next = places(i + S::ring);
+        }
         const int key = key_of(i);
         if (key + kBlock <= min(all_see, end))
             compute<D, true>(memory + place_of(i), a, key, length);
@@ -526,7 +568,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv_attention(const T* __restri
     __syncthreads();
     if (bad && lane == 0) broken = 1;
     const float nan = __builtin_nanf("");
-    auto* joined = reinterpret_cast<float*>(memory);  // [wave][16][D]
+    // [wave][16][D + 4]: rows on different banks.
+    auto* joined = reinterpret_cast<float*>(memory);
     float sum = a.sum;
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
@@ -545,7 +588,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv_attention(const T* __restri
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int d = 0; d < columns; ++d)
-                joined[(wave * 16 + m) * D + Segments<D>::offset(i) + columns * (4 * lg + r) + d] = a.out[Segments<D>::tile(i) + d][r] * undo;
+                joined[(wave * 16 + m) * (D + 4) + Segments<D>::offset(i) + columns * (4 * lg + r) + d] = a.out[Segments<D>::tile(i) + d][r] * undo;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < ROWS * 16 * D / 4; i += kWaves * 64) {
@@ -562,7 +605,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv_attention(const T* __restri
             const float own = references[from][in];
             if (own != -__builtin_inff()) total += sums[from][in] * __builtin_amdgcn_exp2f(own - best);
             else if (sums[from][in] != 0.0f) total = nan;  // scores of NaN alone
-            const float4 x = *reinterpret_cast<const float4*>(joined + (from * 16 + in) * D + column);
+            const float4 x = *reinterpret_cast<const float4*>(joined + (from * 16 + in) * (D + 4) + column);
             v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
         }
         if (broken || bad_length) total = nan;
