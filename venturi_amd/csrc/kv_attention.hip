@@ -66,10 +66,16 @@ __device__ __forceinline__ int admitted(int length, const Geometry& g) {
     return length < 0 || length > g.longest ? 0 : length;  // a bad length is one chunk, which marks its rows
 }
 
-__device__ __forceinline__ std::int64_t chunk_length(const std::int32_t* __restrict__ lengths, const Geometry& g) {
-    const int lane = threadIdx.x & 63;
-    std::int64_t total = 0;
-    for (int s = lane; s < g.sequences; s += 64) total += admitted(lengths[s], g);
+// The lane's share of the lengths: those of sequences base + lane, or 0 past the last.
+__device__ __forceinline__ int length_at(const std::int32_t* __restrict__ lengths, const Geometry& g, int base) {
+    const int s = base + static_cast<int>(threadIdx.x & 63), length = lengths[min(s, g.sequences - 1)];
+    return s < g.sequences ? length : 0;
+}
+
+// The chunk's length, from the lengths of the first 64 sequences (in hand) and of the others.
+__device__ __forceinline__ std::int64_t chunk_length(const std::int32_t* __restrict__ lengths, const Geometry& g, int first) {
+    std::int64_t total = admitted(first, g);
+    for (int base = 64; base < g.sequences; base += 64) total += admitted(length_at(lengths, g, base), g);
     total = wave_sum(total);
     // A chunk is no longer than a sequence need be: below 2^31 (uniform, so that the loops over it are).
     const std::int64_t least = (total + g.target - 1) / g.target, blocks = max((least + kMinChunk - 1) / kMinChunk, std::int64_t{1});
@@ -81,20 +87,27 @@ __device__ __forceinline__ int chunks_of(int length, std::int64_t chunk) {
     return max(static_cast<int>((length + chunk - 1) / chunk), 1);
 }
 
-__device__ __forceinline__ bool find_work(const std::int32_t* __restrict__ lengths, const Geometry& g, int flat, Work& w) {
+// Chunks of sequences base + lane (0 past the last), summed over lanes 0..lane.
+__device__ __forceinline__ int chunk_scan(int length, const Geometry& g, int base, std::int64_t chunk, int& own) {
     const int lane = threadIdx.x & 63;
-    w.chunk = chunk_length(lengths, g);
+    own = base + lane < g.sequences ? chunks_of(admitted(length, g), chunk) : 0;
+    int end = own;
+#pragma unroll
+    for (int step = 1; step < 64; step <<= 1) {
+        const int below = __shfl_up(end, step, 64);
+        if (lane >= step) end += below;
+    }
+    return end;
+}
+
+__device__ __forceinline__ bool find_work(const std::int32_t* __restrict__ lengths, const Geometry& g, int flat, Work& w) {
+    const int first = length_at(lengths, g, 0);
+    w.chunk = chunk_length(lengths, g, first);
     int before = 0;
     for (int base = 0; base < g.sequences; base += 64) {
-        const int s = base + lane, length = s < g.sequences ? lengths[s] : 0;
-        const int n = s < g.sequences ? chunks_of(admitted(length, g), w.chunk) : 0;
-        int end = n;
-#pragma unroll
-        for (int step = 1; step < 64; step <<= 1) {
-            const int below = __shfl_up(end, step, 64);
-            if (lane >= step) end += below;
-        }
-        end += before;
+        const int length = base ? length_at(lengths, g, base) : first;
+        int n;
+        const int end = before + chunk_scan(length, g, base, w.chunk, n);
         const unsigned long long hit = __ballot(end > flat);
         if (hit) {
             const int at = __ffsll(hit) - 1;
@@ -630,43 +643,71 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv_attention(const T* __restri
     }
 }
 
-// Joins the partial results of a sequence of several chunks: a wave per query row.
+// Joins the partial results of a sequence of several chunks: a wave per query row, whose lanes take four columns each of as
+// many chunks side by side as fit.
 template <class T, int D>
 __global__ __launch_bounds__(256) void kv_attention_join(const std::int32_t* __restrict__ lengths, T* __restrict__ out,
                                                          const float* __restrict__ partial, Geometry g) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int sequence = blockIdx.y;
-    const std::int64_t index = static_cast<std::int64_t>(blockIdx.x) * 4 + wave;  // token * q_heads + head
-    if (index >= static_cast<std::int64_t>(g.query_tokens) * g.q_heads) return;
-    const std::int64_t chunk = chunk_length(lengths, g);
-    const int splits = chunks_of(admitted(lengths[sequence], g), chunk);
+    const int index = blockIdx.x * 4 + wave;  // token * q_heads + head
+    if (index >= g.query_tokens * g.q_heads) return;
+    const int length = length_at(lengths, g, 0);
+    const std::int64_t chunk = chunk_length(lengths, g, length);
+    int first = 0, splits = 0;
+    for (int base = 0; base <= sequence; base += 64) {
+        int n;
+        const int end = chunk_scan(base ? length_at(lengths, g, base) : length, g, base, chunk, n);
+        const int at = min(sequence - base, 63);
+        splits = __builtin_amdgcn_readlane(n, at);
+        first += __builtin_amdgcn_readlane(end, at) - (sequence - base > 63 ? 0 : splits);
+    }
     if (splits == 1) return;
-    int first = 0;
-    for (int s = lane; s < sequence; s += 64) first += chunks_of(admitted(lengths[s], g), chunk);
-    first = static_cast<int>(wave_sum(static_cast<std::int64_t>(first)));
-    const int token = static_cast<int>(index / g.q_heads), q_head = static_cast<int>(index - static_cast<std::int64_t>(token) * g.q_heads);
+    const int token = index / g.q_heads, q_head = index - token * g.q_heads;
     const int head = q_head / g.group, row = token * g.group + q_head - head * g.group;
-    const auto at = [&](int split) {
-        return partial + ((static_cast<std::int64_t>(first + split) * g.kv_heads + head) * g.rows + row) * partial_floats<D>();
-    };
+    const std::int64_t stride = static_cast<std::int64_t>(g.kv_heads) * g.rows * partial_floats<D>();
+    const float* base = partial + ((static_cast<std::int64_t>(first) * g.kv_heads + head) * g.rows + row) * partial_floats<D>();
+    constexpr int kLanes = D / 4, kSide = 64 / kLanes;  // lanes of a row, and chunks side by side
+    const int side = lane / kLanes, column = (lane - side * kLanes) * 4;
     float best = -__builtin_inff();
-    for (int i = lane; i < splits; i += 64) best = fmaxf(best, at(i)[D]);
+    for (int i = lane; i < splits; i += 64) best = fmaxf(best, base[i * stride + D]);
 #pragma unroll
     for (int step = 32; step; step >>= 1) best = fmaxf(best, __shfl_xor(best, step, 64));
-    float total = 0.0f, v[D / 64 + 1] = {};
-    for (int i = 0; i < splits; ++i) {
-        const float* p = at(i);
-        const float own = p[D], sum = p[D + 1];
-        const float keep = own == -__builtin_inff() ? (sum == 0.0f ? 0.0f : __builtin_nanf("")) : __builtin_amdgcn_exp2f(own - best);
-        total += sum * keep;
+    float total = 0.0f, v[4] = {};
+    // Loads of four chunks a lane at once; past the last chunk they repeat it, at no weight.
+    for (int i = side; i < splits; i += 4 * kSide) {
+        float2 low[4], high[4], end[4];
 #pragma unroll
-        for (int d = 0; d <= D / 64; ++d)
-            if (lane + 64 * d < D) v[d] += p[lane + 64 * d] * keep;
+        for (int j = 0; j < 4; ++j) {
+            const float* p = base + min(i + j * kSide, splits - 1) * stride;
+            low[j] = *reinterpret_cast<const float2*>(p + column);
+            high[j] = *reinterpret_cast<const float2*>(p + column + 2);
+            end[j] = *reinterpret_cast<const float2*>(p + D);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (i + j * kSide >= splits || side >= kSide) continue;
+            const float keep = end[j].x == -__builtin_inff() ? (end[j].y == 0.0f ? 0.0f : __builtin_nanf(""))
+                                                             : __builtin_amdgcn_exp2f(end[j].x - best);
+            total += end[j].y * keep;
+            v[0] += low[j].x * keep, v[1] += low[j].y * keep, v[2] += high[j].x * keep, v[3] += high[j].y * keep;
+        }
     }
-    T* target = out + ((static_cast<std::int64_t>(sequence) * g.query_tokens + token) * g.q_heads + q_head) * g.head_dim;
+    if constexpr (kSide > 1) {  // the sides' sums, in order
+        const float own[5] = {total, v[0], v[1], v[2], v[3]};
+        float sum[5] = {};
 #pragma unroll
-    for (int d = 0; d <= D / 64; ++d)
-        if (lane + 64 * d < g.head_dim) target[lane + 64 * d] = from_f32<T>(total == 0.0f ? 0.0f : v[d] / total);
+        for (int i = 0; i < kSide; ++i)
+#pragma unroll
+            for (int j = 0; j < 5; ++j) sum[j] += __shfl(own[j], i * kLanes + lane % kLanes, 64);
+        total = sum[0], v[0] = sum[1], v[1] = sum[2], v[2] = sum[3], v[3] = sum[4];
+    }
+    if (lane >= kLanes || column >= g.head_dim) return;
+    const auto bits = [&](float x) {
+        return static_cast<std::uint32_t>(__builtin_bit_cast(unsigned short, from_f32<T>(total == 0.0f ? 0.0f : x / total)));
+    };
+    T* target = out + ((static_cast<std::int64_t>(sequence) * g.query_tokens + token) * g.q_heads + q_head) * g.head_dim + column;
+    *reinterpret_cast<uint2*>(target) = make_uint2(bits(v[0]) | bits(v[1]) << 16, bits(v[2]) | bits(v[3]) << 16);
 }
 
 // Row tiles of a workgroup: one wave each, the rest of its four waves take other keys.
