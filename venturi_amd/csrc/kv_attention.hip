@@ -643,15 +643,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv_attention(const T* __restri
     }
 }
 
-// Joins the partial results of a sequence of several chunks: a wave per query row, whose lanes take four columns each of as
-// many chunks side by side as fit.
+// Joins the partial results of a sequence of several chunks: a workgroup per query row, whose lanes take four columns each of
+// as many chunks side by side as fit.
 template <class T, int D>
 __global__ __launch_bounds__(256) void kv_attention_join(const std::int32_t* __restrict__ lengths, T* __restrict__ out,
                                                          const float* __restrict__ partial, Geometry g) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int sequence = blockIdx.y;
-    const int index = blockIdx.x * 4 + wave;  // token * q_heads + head
-    if (index >= g.query_tokens * g.q_heads) return;
+    const int index = blockIdx.x;  // token * q_heads + head
+    __shared__ float sums[4][5][64];
     const int length = length_at(lengths, g, 0);
     const std::int64_t chunk = chunk_length(lengths, g, length);
     int first = 0, splits = 0;
@@ -667,41 +667,44 @@ __global__ __launch_bounds__(256) void kv_attention_join(const std::int32_t* __r
     const int head = q_head / g.group, row = token * g.group + q_head - head * g.group;
     const std::int64_t stride = static_cast<std::int64_t>(g.kv_heads) * g.rows * partial_floats<D>();
     const float* base = partial + ((static_cast<std::int64_t>(first) * g.kv_heads + head) * g.rows + row) * partial_floats<D>();
-    constexpr int kLanes = D / 4, kSide = 64 / kLanes;  // lanes of a row, and chunks side by side
-    const int side = lane / kLanes, column = (lane - side * kLanes) * 4;
+    constexpr int kLanes = D / 4, kSide = 64 / kLanes, kSides = 4 * kSide;  // lanes of a row; chunks side by side
+    const int in_wave = lane / kLanes, side = wave * kSide + in_wave, column = (lane - in_wave * kLanes) * 4;
     float best = -__builtin_inff();
     for (int i = lane; i < splits; i += 64) best = fmaxf(best, base[i * stride + D]);
 #pragma unroll
     for (int step = 32; step; step >>= 1) best = fmaxf(best, __shfl_xor(best, step, 64));
     float total = 0.0f, v[4] = {};
     // Loads of four chunks a lane at once; past the last chunk they repeat it, at no weight.
-    for (int i = side; i < splits; i += 4 * kSide) {
+    for (int i = side; i < splits; i += 4 * kSides) {
         float2 low[4], high[4], end[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float* p = base + min(i + j * kSide, splits - 1) * stride;
+            const float* p = base + min(i + j * kSides, splits - 1) * stride;
             low[j] = *reinterpret_cast<const float2*>(p + column);
             high[j] = *reinterpret_cast<const float2*>(p + column + 2);
             end[j] = *reinterpret_cast<const float2*>(p + D);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (i + j * kSide >= splits || side >= kSide) continue;
+            if (i + j * kSides >= splits || in_wave >= kSide) continue;
             const float keep = end[j].x == -__builtin_inff() ? (end[j].y == 0.0f ? 0.0f : __builtin_nanf(""))
                                                              : __builtin_amdgcn_exp2f(end[j].x - best);
             total += end[j].y * keep;
             v[0] += low[j].x * keep, v[1] += low[j].y * keep, v[2] += high[j].x * keep, v[3] += high[j].y * keep;
         }
     }
-    if constexpr (kSide > 1) {  // the sides' sums, in order
-        const float own[5] = {total, v[0], v[1], v[2], v[3]};
-        float sum[5] = {};
+    // The sides' sums, in order.
+    const float own[5] = {total, v[0], v[1], v[2], v[3]};
 #pragma unroll
-        for (int i = 0; i < kSide; ++i)
+    for (int k = 0; k < 5; ++k) sums[wave][k][lane] = own[k];
+    __syncthreads();
+    if (wave) return;
+    float sum[5] = {};
 #pragma unroll
-            for (int j = 0; j < 5; ++j) sum[j] += __shfl(own[j], i * kLanes + lane % kLanes, 64);
-        total = sum[0], v[0] = sum[1], v[1] = sum[2], v[2] = sum[3], v[3] = sum[4];
-    }
+    for (int i = 0; i < kSides; ++i)
+#pragma unroll
+        for (int k = 0; k < 5; ++k) sum[k] += sums[i / kSide][k][i % kSide * kLanes + lane % kLanes];
+    total = sum[0], v[0] = sum[1], v[1] = sum[2], v[2] = sum[3], v[3] = sum[4];
     if (lane >= kLanes || column >= g.head_dim) return;
     const auto bits = [&](float x) {
         return static_cast<std::uint32_t>(__builtin_bit_cast(unsigned short, from_f32<T>(total == 0.0f ? 0.0f : x / total)));
@@ -768,8 +771,7 @@ void launch(const void* q, const CachePlanes& planes, const std::int32_t* page_t
     }
     check(hipGetLastError());
     if (partial_bytes(g)) {
-        const auto rows = static_cast<unsigned>((static_cast<std::int64_t>(g.query_tokens) * g.q_heads + 3) / 4);
-        kv_attention_join<T, D><<<dim3(rows, g.sequences), 256, 0, stream>>>(lengths, target, partial, g);
+        kv_attention_join<T, D><<<dim3(g.query_tokens * g.q_heads, g.sequences), 256, 0, stream>>>(lengths, target, partial, g);
     }
 }
 

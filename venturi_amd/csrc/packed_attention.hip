@@ -113,13 +113,27 @@ __device__ __forceinline__ int blocks_of(const std::int32_t* __restrict__ q_offs
     return static_cast<int>((static_cast<std::int64_t>(end - first) * g.group + kRows - 1) / kRows);
 }
 
-// The sequence and row block of flat block `flat`; blocks come sequence by sequence, each one's last block first.
-__device__ __forceinline__ bool find_block(const std::int32_t* __restrict__ q_offsets, const Geometry& g, int flat, int& sequence,
-                                           int& block) {
+// The sequence and row block of flat block `flat`. Up to 64 sequences come by falling number of keys, so that the longest
+// blocks start first; within a sequence its last block is the longest.
+__device__ __forceinline__ bool find_block(const std::int32_t* __restrict__ q_offsets, const std::int32_t* __restrict__ k_offsets,
+                                           const Geometry& g, int flat, int& sequence, int& block) {
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int base = 0; base < g.sequences; base += 64) {
-        const int n = base + lane < g.sequences ? blocks_of(q_offsets, base + lane, g) : 0;
+        const int s = min(base + lane, g.sequences - 1);
+        int n = blocks_of(q_offsets, s, g), own = s;
+        if (base + lane >= g.sequences) n = 0;
+        if (g.sequences > 1 && g.sequences <= 64) {
+            const Span span = span_of(q_offsets, k_offsets, s, g);
+            int rank = 0;
+            for (int i = 0; i < g.sequences; ++i) {
+                const int keys = __builtin_amdgcn_readlane(span.keys, i);
+                rank += keys > span.keys || (keys == span.keys && i < lane);
+            }
+            if (lane >= g.sequences) rank = lane;
+            n = __builtin_amdgcn_ds_permute(4 * rank, n);  // to the lane of its rank
+            own = __builtin_amdgcn_ds_permute(4 * rank, own);
+        }
         int end = n;
 #pragma unroll
         for (int step = 1; step < 64; step <<= 1) {
@@ -130,11 +144,11 @@ __device__ __forceinline__ bool find_block(const std::int32_t* __restrict__ q_of
         const unsigned long long hit = __ballot(end > flat);
         if (hit) {
             const int at = __ffsll(hit) - 1;
-            sequence = base + at;
-            block = __shfl(end, at, 64) - 1 - flat;
+            sequence = __builtin_amdgcn_readlane(own, at);
+            block = __builtin_amdgcn_readlane(end, at) - 1 - flat;
             return true;
         }
-        before = __shfl(end, 63, 64);
+        before = __builtin_amdgcn_readlane(end, 63);
     }
     block = flat - before;  // workgroups past the last block, counted from 0
     return false;
@@ -334,7 +348,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_attention(
     // meet in few of the eight L2 caches.
     const int head = blockIdx.x % g.kv_heads;
     int sequence, block;
-    if (const int flat = blockIdx.x / g.kv_heads; !find_block(q_offsets, g, flat, sequence, block)) {
+    if (const int flat = blockIdx.x / g.kv_heads; !find_block(q_offsets, k_offsets, g, flat, sequence, block)) {
         clear_rest(q_offsets, out, g, head, block, gridDim.x / g.kv_heads - (flat - block));
         return;
     }
