@@ -32,9 +32,11 @@ typedef float float16v __attribute__((ext_vector_type(16)));
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves, kWaveRows = 32, kRows = kWaves * kWaveRows;
 constexpr float kLazy = 4.0f, kShift = 8.0f;
+constexpr int kMaxParts = 8;
 
 struct Geometry {
     int tokens, keys, sequences, q_heads, kv_heads, group, head_dim;
+    int blocks, parts;  // row blocks of a KV head (at most), and workgroups that share a block's keys
     float scale;
 };
 
@@ -173,8 +175,9 @@ struct Copy {
     // The tile at `source`, of which `rows` rows exist, to `lds` (a byte address).
     __device__ __forceinline__ void operator()(const void* source, int rows, std::uint32_t at, std::uint32_t lds) const {
         const auto base = reinterpret_cast<std::uint64_t>(source);
-        const int4v buffer = {static_cast<int>(base), static_cast<int>(base >> 32) & 0xffff,
-                              static_cast<int>(min(rows, Tile<D>::keys) * row_bytes), 0x00020000};
+        const int4v buffer = {__builtin_amdgcn_readfirstlane(static_cast<int>(base)),
+                              __builtin_amdgcn_readfirstlane(static_cast<int>(base >> 32) & 0xffff),
+                              __builtin_amdgcn_readfirstlane(static_cast<int>(min(rows, Tile<D>::keys) * row_bytes)), 0x00020000};
         const std::uint32_t first = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x >> 6) * 1024);
 #pragma unroll
         for (int i = 0; i < Tile<D>::loads; ++i)
@@ -339,17 +342,24 @@ __device__ void clear_rest(const std::int32_t* __restrict__ q_offsets, T* __rest
     }
 }
 
+// Partial results: per workgroup and row D outputs, then the reference and the sum, 16-byte aligned.
+template <int D>
+constexpr int partial_floats() { return D + 4; }
+__host__ __device__ inline std::int64_t partial_row(const Geometry& g, int block_and_head, int part, int row) {
+    return (static_cast<std::int64_t>(part) * g.blocks * g.kv_heads + block_and_head) * kRows + row;
+}
+
 template <class T, int D>
 __global__ __launch_bounds__(kThreads, 2) void packed_attention(
     const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const std::int32_t* __restrict__ q_offsets,
-    const std::int32_t* __restrict__ k_offsets, T* __restrict__ out, Geometry g) {
+    const std::int32_t* __restrict__ k_offsets, T* __restrict__ out, float* __restrict__ partial, Geometry g) {
     __shared__ __align__(16) unsigned char memory[4 * Tile<D>::bytes];
     // Neighbouring workgroups go to different XCDs, round robin: with the head as the fast index the workgroups of one head
     // meet in few of the eight L2 caches.
-    const int head = blockIdx.x % g.kv_heads;
+    const int head = blockIdx.x % g.kv_heads, flat = blockIdx.x / g.kv_heads;
     int sequence, block;
-    if (const int flat = blockIdx.x / g.kv_heads; !find_block(q_offsets, k_offsets, g, flat, sequence, block)) {
-        clear_rest(q_offsets, out, g, head, block, gridDim.x / g.kv_heads - (flat - block));
+    if (!find_block(q_offsets, k_offsets, g, flat, sequence, block)) {
+        if (blockIdx.y == 0) clear_rest(q_offsets, out, g, head, block, g.blocks - (flat - block));
         return;
     }
     const Span s = span_of(q_offsets, k_offsets, sequence, g);
@@ -365,7 +375,14 @@ __global__ __launch_bounds__(kThreads, 2) void packed_attention(
     // The keys that the wave's first row sees, that its last one sees, and that the workgroup's last one sees.
     const int least = first_row < rows ? first_row / g.group + 1 - hidden : 0;
     const int most = first_row < rows ? min(first_row + kWaveRows - 1, rows - 1) / g.group + 1 - hidden : 0;
-    const int end = min(block * kRows + kRows - 1, rows - 1) / g.group + 1 - hidden;
+    int end = min(block * kRows + kRows - 1, rows - 1) / g.group + 1 - hidden, start = 0;
+    if (g.parts > 1) {
+        const int share = ((end + Tile<D>::keys - 1) / Tile<D>::keys + g.parts - 1) / g.parts * Tile<D>::keys;
+        start = static_cast<int>(blockIdx.y) * share;
+        end = min(end, start + share);
+    }
+    start = __builtin_amdgcn_readfirstlane(start);
+    end = __builtin_amdgcn_readfirstlane(end);
 
     State<D> a;
     // A negative scale turns the queries' signs, so that the largest product is the largest score; 0 empties them.
@@ -398,9 +415,9 @@ __global__ __launch_bounds__(kThreads, 2) void packed_attention(
         copy(key + at * stride, s.keys - at, copy.key_at, lds + turn * (2 * Tile<D>::bytes));
         copy(value + at * stride, s.keys - at, copy.value_at, lds + turn * (2 * Tile<D>::bytes) + Tile<D>::bytes);
     };
-    if (end > 0) fetch(0, 0);
+    if (start < end) fetch(start, 0);
     copies_done();
-    for (int at = 0, turn = 0; at < end; at += kKeys, turn ^= 1) {
+    for (int at = start, turn = 0; at < end; at += kKeys, turn ^= 1) {
         const unsigned char* now = memory + turn * (2 * Tile<D>::bytes);
         if (at + kKeys < end) fetch(at + kKeys, turn ^ 1);
         if (at < most) {
@@ -412,8 +429,21 @@ __global__ __launch_bounds__(kThreads, 2) void packed_attention(
         copies_done();
     }
     a.sum += __shfl_xor(a.sum, 32, 64);
-    const float scale = a.sum != 0.0f ? 1.0f / a.sum : 0.0f;
     if (!live) return;
+    if (g.parts > 1) {
+        float* target = partial + partial_row(g, blockIdx.x, blockIdx.y, wave * kWaveRows + m) * partial_floats<D>();
+        // A part whose rows see none of its keys leaves no outputs.
+        if (a.sum != 0.0f)
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4)
+                    *reinterpret_cast<float4*>(target + 32 * d + 2 * r + 4 * h) =
+                        make_float4(a.out[d][r], a.out[d][r + 1], a.out[d][r + 2], a.out[d][r + 3]);
+        if (h == 0) *reinterpret_cast<float2*>(target + D) = make_float2(a.reference, a.sum);
+        return;
+    }
+    const float scale = a.sum != 0.0f ? 1.0f / a.sum : 0.0f;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -427,40 +457,97 @@ __global__ __launch_bounds__(kThreads, 2) void packed_attention(
         }
 }
 
+// Joins the parts of a block's rows: a wave per row, four columns a lane.
+template <class T, int D>
+__global__ __launch_bounds__(kThreads) void packed_attention_join(const std::int32_t* __restrict__ q_offsets,
+                                                                  const std::int32_t* __restrict__ k_offsets, T* __restrict__ out,
+                                                                  const float* __restrict__ partial, Geometry g) {
+    const int head = blockIdx.x % g.kv_heads;
+    int sequence, block;
+    if (!find_block(q_offsets, k_offsets, g, blockIdx.x / g.kv_heads, sequence, block)) return;
+    const Span s = span_of(q_offsets, k_offsets, sequence, g);
+    const int lane = threadIdx.x & 63, in_block = blockIdx.y * kWaves + static_cast<int>(threadIdx.x >> 6);
+    const int row = block * kRows + in_block, column = 4 * lane;
+    if (row >= s.queries * g.group || column >= g.head_dim) return;
+    const std::int64_t stride = partial_row(g, 0, 1, 0) * partial_floats<D>();
+    const float* base = partial + partial_row(g, blockIdx.x, 0, in_block) * partial_floats<D>();
+    float best = -__builtin_inff(), total = 0.0f, v[4] = {};
+    float2 end[kMaxParts];
+    float4 x[kMaxParts];
+#pragma unroll
+    for (int i = 0; i < kMaxParts; ++i) {  // past the last part they repeat it, at no weight
+        const float* p = base + min(i, g.parts - 1) * stride;
+        end[i] = *reinterpret_cast<const float2*>(p + D);
+        x[i] = *reinterpret_cast<const float4*>(p + column);
+    }
+#pragma unroll
+    for (int i = 0; i < kMaxParts; ++i) best = fmaxf(best, end[i].x);
+#pragma unroll
+    for (int i = 0; i < kMaxParts; ++i) {
+        if (i >= g.parts || end[i].y == 0.0f) continue;  // without a weight the outputs were not written
+        const float keep = end[i].x == -__builtin_inff() ? __builtin_nanf("") : __builtin_amdgcn_exp2f(end[i].x - best);
+        total += end[i].y * keep;
+        v[0] += x[i].x * keep, v[1] += x[i].y * keep, v[2] += x[i].z * keep, v[3] += x[i].w * keep;
+    }
+    const int token = row / g.group;
+    const std::int64_t place = (static_cast<std::int64_t>(s.q_first + token) * g.q_heads + head * g.group + row - token * g.group) * g.head_dim;
+    const float scale = 1.0f / total;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = total == 0.0f ? 0.0f : v[j] * scale;
+    *reinterpret_cast<uint2*>(out + place + column) = make_uint2(Matrix<T>::pack(v[0], v[1]), Matrix<T>::pack(v[2], v[3]));
+}
+
 Geometry geometry(int tokens, int keys, int sequences, int q_heads, int kv_heads, int head_dim, float scale) {
     require_head_dim(head_dim);
     require(tokens > 0 && keys > 0 && sequences > 0 && q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0,
             "invalid packed attention geometry");
     const int group = q_heads / kv_heads;
     require(static_cast<std::int64_t>(tokens) * group < (1ll << 31) - kRows, "packed attention rows of a KV head must fit int32");
-    const std::int64_t blocks = static_cast<std::int64_t>(tokens) * group / kRows + 1 + sequences;
+    // Every sequence leaves at most one block that is not full; one more clears what no sequence covers.
+    const std::int64_t blocks = static_cast<std::int64_t>(tokens) * group / kRows + sequences + 1;
     require(blocks * kv_heads < (1ll << 31), "packed attention blocks must fit int32");
     require(static_cast<std::int64_t>(kv_heads) * head_dim < (1 << 23), "packed attention takes key rows of at most 8388607 columns");
-    return {tokens, keys, sequences, q_heads, kv_heads, group, head_dim, scale};
+    // Few rows over many keys: the blocks' keys are shared by as many workgroups as leave each about four tiles, while the
+    // card (two workgroups to a CU) has room. 5 queries over 1505 keys, 48 heads of 128: 32 -> 15 us; 40 over 1540: 36 -> 21;
+    // 300 over 1500, 32 heads (80 workgroups): 37 -> 32. Past 96 workgroups the join costs what the split saves (512
+    // queries, 196 workgroups: 19 us without, 35 with two parts).
+    const std::int64_t busy = (blocks - 1) * kv_heads, tiles = (keys / sequences + 63) / 64;
+    const int parts = busy > 96 ? 1 : static_cast<int>(std::max<std::int64_t>(std::min({512 / busy, tiles / 4, std::int64_t{kMaxParts}}), 1));
+    return {tokens, keys, sequences, q_heads, kv_heads, group, head_dim, static_cast<int>(blocks), parts, scale};
+}
+
+std::uint64_t partial_bytes(const Geometry& g) {
+    return g.parts > 1 ? static_cast<std::uint64_t>(partial_row(g, 0, g.parts, 0)) * ((g.head_dim + 31) / 32 * 32 + 4) * sizeof(float) : 0;
 }
 
 template <class T, int D>
 void launch(const void* q, const void* k, const void* v, const std::int32_t* q_offsets, const std::int32_t* k_offsets, void* out,
-            const Geometry& g, hipStream_t stream) {
-    // Every sequence leaves at most one block that is not full; one more clears what no sequence covers.
-    const std::int64_t blocks = static_cast<std::int64_t>(g.tokens) * g.group / kRows + g.sequences + 1;
-    packed_attention<T, D><<<static_cast<unsigned>(blocks * g.kv_heads), kThreads, 0, stream>>>(
-        static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), q_offsets, k_offsets, static_cast<T*>(out), g);
+            void* workspace, const Geometry& g, hipStream_t stream) {
+    const unsigned blocks = static_cast<unsigned>(g.blocks) * g.kv_heads;
+    auto* partial = static_cast<float*>(workspace);
+    packed_attention<T, D><<<dim3(blocks, g.parts), kThreads, 0, stream>>>(static_cast<const T*>(q), static_cast<const T*>(k),
+                                                                          static_cast<const T*>(v), q_offsets, k_offsets,
+                                                                          static_cast<T*>(out), partial, g);
+    if (g.parts > 1) {
+        check(hipGetLastError());
+        packed_attention_join<T, D><<<dim3(blocks, kRows / kWaves), kThreads, 0, stream>>>(q_offsets, k_offsets, static_cast<T*>(out),
+                                                                                          partial, g);
+    }
 }
 
 template <class T>
 void launch_any(const void* q, const void* k, const void* v, const std::int32_t* q_offsets, const std::int32_t* k_offsets,
-                void* out, const Geometry& g, hipStream_t stream) {
+                void* out, void* workspace, const Geometry& g, hipStream_t stream) {
     const int padded = (g.head_dim + 31) / 32 * 32;
     switch (padded) {
-        case 32: launch<T, 32>(q, k, v, q_offsets, k_offsets, out, g, stream); break;
-        case 64: launch<T, 64>(q, k, v, q_offsets, k_offsets, out, g, stream); break;
-        case 96: launch<T, 96>(q, k, v, q_offsets, k_offsets, out, g, stream); break;
-        case 128: launch<T, 128>(q, k, v, q_offsets, k_offsets, out, g, stream); break;
-        case 160: launch<T, 160>(q, k, v, q_offsets, k_offsets, out, g, stream); break;
-        case 192: launch<T, 192>(q, k, v, q_offsets, k_offsets, out, g, stream); break;
-        case 224: launch<T, 224>(q, k, v, q_offsets, k_offsets, out, g, stream); break;
-        default: launch<T, 256>(q, k, v, q_offsets, k_offsets, out, g, stream); break;
+        case 32: launch<T, 32>(q, k, v, q_offsets, k_offsets, out, workspace, g, stream); break;
+        case 64: launch<T, 64>(q, k, v, q_offsets, k_offsets, out, workspace, g, stream); break;
+        case 96: launch<T, 96>(q, k, v, q_offsets, k_offsets, out, workspace, g, stream); break;
+        case 128: launch<T, 128>(q, k, v, q_offsets, k_offsets, out, workspace, g, stream); break;
+        case 160: launch<T, 160>(q, k, v, q_offsets, k_offsets, out, workspace, g, stream); break;
+        case 192: launch<T, 192>(q, k, v, q_offsets, k_offsets, out, workspace, g, stream); break;
+        case 224: launch<T, 224>(q, k, v, q_offsets, k_offsets, out, workspace, g, stream); break;
+        default: launch<T, 256>(q, k, v, q_offsets, k_offsets, out, workspace, g, stream); break;
     }
 }
 
@@ -471,8 +558,9 @@ void launch_any(const void* q, const void* k, const void* v, const std::int32_t*
 
 VT_EXPORT std::uint64_t venturi_packed_attention_bytes(int tokens, int keys, int sequences, int q_heads, int kv_heads,
                                                        int head_dim) {
-    vt::host_guarded([&] { vt::geometry(tokens, keys, sequences, q_heads, kv_heads, head_dim, 1.0f); });
-    return 0;
+    std::uint64_t bytes = 0;
+    vt::host_guarded([&] { bytes = vt::partial_bytes(vt::geometry(tokens, keys, sequences, q_heads, kv_heads, head_dim, 1.0f)); });
+    return bytes;
 }
 
 VT_EXPORT int venturi_packed_attention_run(const void* q, const void* k, const void* v, const std::int32_t* q_offsets,
@@ -484,11 +572,14 @@ VT_EXPORT int venturi_packed_attention_run(const void* q, const void* k, const v
         vt::require(q && k && v && q_offsets && k_offsets && out, "null packed attention operand");
         vt::require(vt::aligned(q, 16) && vt::aligned(k, 16) && vt::aligned(v, 16) && vt::aligned(out, 16),
                     "packed attention rows must be 16-byte aligned");
+        const std::uint64_t bytes = vt::partial_bytes(g);
+        vt::require(!bytes || (workspace && available >= bytes && vt::aligned(workspace, 256)),
+                    "packed attention of few rows needs its workspace, 256-byte aligned");
         const auto s = static_cast<hipStream_t>(stream);
         if (dtype == vt::kF16)
-            vt::launch_any<__half>(q, k, v, q_offsets, k_offsets, out, g, s);
+            vt::launch_any<__half>(q, k, v, q_offsets, k_offsets, out, workspace, g, s);
         else if (dtype == vt::kBF16)
-            vt::launch_any<__hip_bfloat16>(q, k, v, q_offsets, k_offsets, out, g, s);
+            vt::launch_any<__hip_bfloat16>(q, k, v, q_offsets, k_offsets, out, workspace, g, s);
         else
             throw vt::Invalid("packed attention takes fp16 or bf16");
     });
