@@ -63,6 +63,14 @@ def test_lengths(backend, device, queries, past, hq, hk, d):
     check(backend, device, queries, past, hq, hk, d, FP16, seed=len(queries))
 
 
+@pytest.mark.parametrize("dtype", [FP16, BF16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("hk,d", [(1, 32), (1, 64), (1, 96), (1, 128), (1, 160), (1, 192), (1, 224), (1, 256), (2, 72)])
+def test_few_rows_over_many_keys(backend, device, dtype, hk, d):
+    """The keys of a block shared by several workgroups, some of which see none of a row's; sequences of other lengths."""
+    check(backend, device, [5], [1500], hk, hk, d, dtype, seed=d)
+    check(backend, device, [3, 1, 40], [1300, 0, 700], 3 * hk, hk, d, dtype, seed=d + 1)
+
+
 def test_many_sequences(backend, device):
     queries = [(5 * i * i + i) % 23 for i in range(301)]
     check(backend, device, queries, [i % 4 for i in range(301)], 4, 2, 64, BF16, seed=4)

@@ -81,6 +81,31 @@ def test_heads_and_lengths(backend, device, dtype, hq, hk, d, t):
     check(backend, device, [1, 0, 64, 17, 257, 3], hq, hk, d, dtype, 32, t, seed=hq + d)
 
 
+@pytest.mark.parametrize("dtype", [FP16, BF16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("hk,d", [(1, 32), (2, 64), (4, 96), (4, 128), (2, 160), (2, 192), (2, 224), (2, 256)])
+@pytest.mark.parametrize("t", [12, 33])
+def test_rows_of_two_and_four_tiles(backend, device, dtype, hk, d, t):
+    check(backend, device, [300, 20, 41], 2 * hk, hk, d, dtype, 32, t, seed=d + t)
+
+
+@pytest.mark.parametrize("hq,d", [(1, 64), (3, 128), (12, 256), (5, 96)])
+def test_numbers_that_are_none_in_the_new_tokens(backend, device, hq, d):
+    """The last new tokens' values and keys hold no number: the earlier ones do not see them. (Their bits may differ: the
+    rows of a wave move their references together.)"""
+    t, n = 4, 70
+    cache, q, table, sequences = make(backend, device, [n], hq, 1, d, FP16, 16, t, seed=14)
+    k, v = cached(cache, sequences[0])
+    want, mean, size = attend(q, k, v, [n - 3, n - 2, n - 1, n])
+    bound = attention_bound(want, mean, size, d, n, FP16, 2.0**-11, 2.0**-11)
+    value, key = (int(sequences[0][n - i]) for i in (2, 1))
+    cache.value_scales[value // 16, 0, 0, value % 16] = float("nan")
+    cache.key_scales[key // 16, 0, 0, key % 16] = float("inf")
+    out = run(cache, q, table, [n], t, hq, device)
+    assert ((out[:2].double() - want[:2]).abs() <= bound[:2]).all()
+    assert out[2, :, :32].isnan().all() and ((out[2, :, 32:].double() - want[2, :, 32:]).abs() <= bound[2, :, 32:]).all()
+    assert out[3].isnan().any(-1).all()
+
+
 @pytest.mark.parametrize("page", [16, 32, 48, 128, 1040])
 @pytest.mark.parametrize("t", [1, 2, 9])
 def test_pages(backend, device, page, t):
