@@ -1,11 +1,14 @@
 // Attention over the paged Q8 cache: out = softmax(scale q k^T) v for the few new tokens of many sequences.
 //
 // Bound by HBM: every code and scale of K and V is read once (272 bytes a token and head at head_dim 128). A wave takes
-// 32 keys at a time, holds the next 32 keys' codes and scales in registers while it computes, and keeps weights,
-// outputs and statistics in registers; nothing goes through LDS until the waves of a workgroup join.
+// 32 keys at a time out of LDS, into which the next ones' codes and scales are copied beside it without passing registers
+// (in registers they left one wave on a SIMD at head_dim 256: 16 x 5 drafted tokens 74 us, now 36), and keeps weights,
+// outputs and statistics in registers until the waves of a workgroup join. 4 sequences of 90000 to 131000 keys, 48 heads
+// on 4 of 128: 92 to 99 us, 4.8 to 5.2 TB/s, where a large copy reaches 4.9.
 //
 // Rows. The query rows of one KV head (query_tokens x group) are the columns of 16-wide matrix tiles, so that a KV
-// head's codes are converted once for all heads that share them. With S^T = K Q^T a lane holds four keys of one query,
+// head's codes are read once for all heads that share them: up to 16 rows the four waves of a workgroup take other keys, up
+// to 32 rows two waves share a step's codes, above that four. With S^T = K Q^T a lane holds four keys of one query,
 // which is the operand layout of O^T = V^T P^T if the 32 keys are taken in the order (tile, lane group, register): the
 // weights never leave their lane.
 //
@@ -16,15 +19,18 @@
 //      scale_v 2^15 k, -scale_v k / 4) = v * k 2^-9, rounded once to fp16 (2^-11). k is a power of two that brings the
 //      largest scale so far to at most 1, so neither end of the scales' range overflows or underflows.
 // Queries are scaled by a power of two per row into fp16's range: exact for fp16 and, but for numbers 2^28 below the
-// row's largest, for bf16. The weights are rounded to fp16 (2^-11) for bf16 rows, whose own rounding is eight times as
-// coarse; fp16 rows take a second term, what that rounding left, through the matrix cores too (1021 keys: the outputs'
-// error 1.6 times that of one rounding at the end without it, 1.3 times with it). Their sum is of the unrounded ones.
+// row's largest, for bf16. The weights are rounded to fp16 (2^-11); their sum is of the unrounded ones.
+// For bf16 rows, whose own rounding is eight times as coarse, that is that. For fp16 rows both factors of O = P V have a
+// second term, what the first one's rounding left: the outputs' error against 64 bits at 1021 keys is that of the one
+// rounding at the end (2.1e-4 of their norm) where single terms leave 3.3e-4, for 2 to 5% of the time (64 sequences of 1 to
+// 8190 keys: 45.8 -> 48.1 us).
 //
 // Softmax. One pass: weights are 2^(s - m) for a reference m that follows the maximum only when a score passes it by
 // more than 4 (a factor of 16 fits fp16's range): the rescaling of the outputs is rare.
 //
 // Split. The keys of all sequences are cut into chunks of one length, chosen on the device from the sum of the
 // lengths, so that the grid is about `kTarget` workgroups whatever the lengths; a workgroup finds its sequence by a scan.
+// Two workgroups to a CU, one round: 512 is faster than 768, 1024 and 2048 (long sequences: 104, 119, 120, 155 us).
 // A sequence of one chunk is finished by its workgroup, others leave partial outputs, joined by a second launch.
 #include "kv_cache.hpp"
 
@@ -294,7 +300,8 @@ __device__ __forceinline__ float power_above(float v) {  // the smallest power o
     return ldexpf(1.0f, f == 0.5f ? e - 1 : e);
 }
 
-// One step of 32 keys for the wave's rows, from LDS. FULL: every row sees all of them. FINE: weights in two fp16 terms.
+// One step of 32 keys for the wave's rows, from LDS. FULL: every row sees all of them. FINE: weights and values in two
+// fp16 terms.
 template <int D, bool FULL, bool FINE>
 __device__ __forceinline__ void compute(const unsigned char* __restrict__ step, State<D>& a, int first_key, int length) {
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
@@ -428,22 +435,35 @@ __device__ __forceinline__ void compute(const unsigned char* __restrict__ step, 
             // product and marked below.
             const bool mark = !FULL && !(x < 2.0f && y < 2.0f);
             broken = broken || mark;
-            steep[j] = __builtin_bit_cast(half2v, pack(!FULL && !(x < 2.0f) ? 0.0f : x * 32768.0f, !FULL && !(y < 2.0f) ? 0.0f : y * 32768.0f));
+            constexpr float kSteep = FINE ? 256.0f : 32768.0f;
+            steep[j] = __builtin_bit_cast(half2v, pack(!FULL && !(x < 2.0f) ? 0.0f : x * kSteep, !FULL && !(y < 2.0f) ? 0.0f : y * kSteep));
             flat[j] = __builtin_bit_cast(half2v, pack(!FULL && !(x < 2.0f) ? 0.0f : x * -0.25f, !FULL && !(y < 2.0f) ? 0.0f : y * -0.25f));
         }
         const int columns = Segments<D>::width(i) / 16, tile = Segments<D>::tile(i), word = Segments<D>::word(i);
 #pragma unroll
         for (int d = 0; d < columns; ++d) {
-            std::uint32_t v[4];
+            std::uint32_t v[4], left[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const std::uint32_t pair = permute(value[2 * j + 1][word + d / 4], value[2 * j][word + d / 4], 0x0c000c00u | (d & 3) | (4 + (d & 3)) << 16);
                 const half2v x = __builtin_bit_cast(half2v, pair);
-                v[j] = __builtin_bit_cast(std::uint32_t, __builtin_elementwise_fma(x, steep[j], flat[j]));
+                if constexpr (FINE) {
+                    const half2v up = static_cast<_Float16>(32768.0f), down = static_cast<_Float16>(-0.25f);
+                    const half2v code = __builtin_elementwise_fma(x, up, down);  // (u - 128) 2^-9, exact
+                    const half2v near = code * steep[j];
+                    v[j] = __builtin_bit_cast(std::uint32_t, near);
+                    left[j] = __builtin_bit_cast(std::uint32_t, __builtin_elementwise_fma(code, steep[j], -near));
+                } else {
+                    v[j] = __builtin_bit_cast(std::uint32_t, __builtin_elementwise_fma(x, steep[j], flat[j]));
+                }
             }
             const half8v values = __builtin_bit_cast(half8v, make_uint4(v[0], v[1], v[2], v[3]));
             a.out[tile + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values, weights, a.out[tile + d], 0, 0, 0);
-            if constexpr (FINE) a.out[tile + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values, rests, a.out[tile + d], 0, 0, 0);
+            if constexpr (FINE) {
+                const half8v lefts = __builtin_bit_cast(half8v, make_uint4(left[0], left[1], left[2], left[3]));
+                a.out[tile + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values, rests, a.out[tile + d], 0, 0, 0);
+                a.out[tile + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lefts, weights, a.out[tile + d], 0, 0, 0);
+            }
         }
         if (!FULL && __any(broken)) {
             half8v marks, sees;
@@ -600,9 +620,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv_attention(const T* __restri
     float top = references[row_wave][m];
 #pragma unroll
     for (int i = 1; i < S::keys; ++i) top = fmaxf(top, references[row_wave + i * ROWS][m]);
-    // 512 / bring undoes the values' power of two.
+    // 512 / bring (2 / bring with two terms) undoes the values' power of two.
     const float keep = a.reference == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(a.reference - top);
-    const float undo = keep * (512.0f / a.bring);
+    const float undo = keep * ((std::is_same<T, __half>::value ? 2.0f : 512.0f) / a.bring);
 #pragma unroll
     for (int i = 0; i < Segments<D>::count; ++i) {
         const int columns = Segments<D>::width(i) / 16;
