@@ -84,13 +84,17 @@ struct Tile {
     static constexpr int bytes = keys * columns * 2;
     static constexpr int loads = keys * units / kThreads;                                // per wave, of 64 units
     static constexpr int load_rows = kThreads / units;                                   // rows that a load of all waves covers
-    // What a unit's place in its row is XORed with; the same for rows load_rows apart.
+    // What a unit's place in its row is XORed with. Keys: the same unit of 16 rows lies in 16 places of the 256 bytes that the
+    // banks span; in 8 at the largest heads, whose registers do not hold the addresses (882 us against 961 at 8192 tokens and
+    // head_dim 256, with twice the LDS cycles). Values: of four rows' windows of four units (a transposing read of half a
+    // wave) no two share a place.
+    static constexpr int key_turn = units == 32 ? 7 : 15;
     static __device__ __forceinline__ int key_swizzle(int row) {
-        if constexpr (units >= 16) return row & 7;
+        if constexpr (units >= 16) return row & key_turn;
         else return (row / (16 / units)) & (units - 1);
     }
     static __device__ __forceinline__ int value_swizzle(int row) {  // even: pairs of units keep their order
-        if constexpr (units >= 16) return 2 * (row & 7);
+        if constexpr (units >= 16) return 4 * (row & 3);
         else return 2 * ((row / (16 / units)) & (units / 2 - 1));
     }
 };
@@ -163,17 +167,21 @@ typedef int int4v __attribute__((ext_vector_type(4)));
 // head are sent past it.
 template <int D>
 struct Copy {
-    std::uint32_t key_at, value_at;  // bytes from the tile's first row to the lane's unit
+    std::uint32_t key_at[2], value_at;  // bytes from the tile's first row to the lane's unit (of every other load, for keys)
     std::uint32_t row_bytes;
 
     __device__ __forceinline__ Copy(int stride, int head_dim) : row_bytes(2 * stride) {
         const int row = threadIdx.x / Tile<D>::units, place = threadIdx.x % Tile<D>::units;
-        const int key_unit = place ^ Tile<D>::key_swizzle(row), value_unit = place ^ Tile<D>::value_swizzle(row);
-        key_at = 8 * key_unit < head_dim ? row * row_bytes + 16 * key_unit : 0x80000000u;
+        const int value_unit = place ^ Tile<D>::value_swizzle(row);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {  // the swizzle repeats every 16 rows, one load or two
+            const int key_unit = place ^ Tile<D>::key_swizzle(row + i * Tile<D>::load_rows);
+            key_at[i] = 8 * key_unit < head_dim ? row * row_bytes + 16 * key_unit : 0x80000000u;
+        }
         value_at = 8 * value_unit < head_dim ? row * row_bytes + 16 * value_unit : 0x80000000u;
     }
     // The tile at `source`, of which `rows` rows exist, to `lds` (a byte address).
-    __device__ __forceinline__ void operator()(const void* source, int rows, std::uint32_t at, std::uint32_t lds) const {
+    __device__ __forceinline__ void operator()(const void* source, int rows, std::uint32_t even, std::uint32_t odd, std::uint32_t lds) const {
         const auto base = reinterpret_cast<std::uint64_t>(source);
         const int4v buffer = {__builtin_amdgcn_readfirstlane(static_cast<int>(base)),
                               __builtin_amdgcn_readfirstlane(static_cast<int>(base >> 32) & 0xffff),
@@ -183,7 +191,7 @@ struct Copy {
         for (int i = 0; i < Tile<D>::loads; ++i)
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                          :
-                         : "s"(first + i * (kThreads * 16)), "v"(at + i * Tile<D>::load_rows * row_bytes), "s"(buffer)
+                         : "s"(first + i * (kThreads * 16)), "v"((i & 1 ? odd : even) + i * Tile<D>::load_rows * row_bytes), "s"(buffer)
                          : "memory");
     }
 };
@@ -215,15 +223,16 @@ __device__ __forceinline__ void compute(const unsigned char* __restrict__ keys, 
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) score[t][r] = 0.0f;
-    // The swizzle turns the low three bits of a unit; the rest of the address is a constant beside the row's.
+    // The swizzle turns the low bits of a unit; the rest of the address is a constant beside the row's.
+    constexpr int kTurn = Tile<D>::units >= 16 ? Tile<D>::key_turn : 15;
     const unsigned char* row = keys + m * (Tile<D>::units * 16);
     const int turn = Tile<D>::key_swizzle(m);
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
-        const unsigned char* at = row + ((((2 * s) & 7) | h) ^ turn) * 16;
+        const unsigned char* at = row + ((((2 * s) & kTurn) | h) ^ turn) * 16;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
-            const uint4 k = *reinterpret_cast<const uint4*>(at + 32 * t * (Tile<D>::units * 16) + ((2 * s) & ~7) * 16);
+            const uint4 k = *reinterpret_cast<const uint4*>(at + 32 * t * (Tile<D>::units * 16) + ((2 * s) & ~kTurn) * 16);
             score[t] = Matrix<T>::multiply(k, a.query[s], score[t]);
         }
     }
@@ -280,7 +289,7 @@ __device__ __forceinline__ void compute(const unsigned char* __restrict__ keys, 
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const int unit = ((4 * d) & 15) | 2 * (group & 1) | (i & 3) >> 1;
-                // From 16 units on the swizzle repeats every 8 rows.
+                // From 16 units on the swizzle repeats every 4 rows.
                 const int place = unit ^ Tile<D>::value_swizzle(Tile<D>::units >= 16 ? row0 : 16 * t + 8 * p + row0);
                 const unsigned char* at = values + row0 * (Tile<D>::units * 16) + place * 16 + 8 * (i & 1) +
                                           ((16 * t + 8 * p) * Tile<D>::units + ((4 * d) & ~15)) * 16;
@@ -412,8 +421,8 @@ __global__ __launch_bounds__(kThreads, 2) void packed_attention(
     typedef __attribute__((address_space(3))) unsigned char* Lds;
     const auto lds = static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>((Lds)(memory)));
     const auto fetch = [&](int at, int turn) {
-        copy(key + at * stride, s.keys - at, copy.key_at, lds + turn * (2 * Tile<D>::bytes));
-        copy(value + at * stride, s.keys - at, copy.value_at, lds + turn * (2 * Tile<D>::bytes) + Tile<D>::bytes);
+        copy(key + at * stride, s.keys - at, copy.key_at[0], copy.key_at[1], lds + turn * (2 * Tile<D>::bytes));
+        copy(value + at * stride, s.keys - at, copy.value_at, copy.value_at, lds + turn * (2 * Tile<D>::bytes) + Tile<D>::bytes);
     };
     if (start < end) fetch(start, 0);
     copies_done();
