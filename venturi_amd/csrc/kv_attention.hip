@@ -29,7 +29,8 @@
 // more than 4 (a factor of 16 fits fp16's range): the rescaling of the outputs is rare.
 //
 // Split. The keys of all sequences are cut into chunks of one length, chosen on the device from the sum of the
-// lengths, so that the grid is about `kTarget` workgroups whatever the lengths; a workgroup finds its sequence by a scan.
+// lengths, so that the grid is about `kTarget` workgroups whatever the lengths; a workgroup finds its sequence by a scan,
+// whole chunks before the sequences' shorter ends.
 // Two workgroups to a CU, one round: 512 is faster than 768, 1024 and 2048 (long sequences: 104, 119, 120, 155 us).
 // A sequence of one chunk is finished by its workgroup, others leave partial outputs, joined by a second launch.
 #include "kv_cache.hpp"
@@ -58,11 +59,10 @@ struct Geometry {
     std::int64_t longest;                        // max_pages * page_tokens
 };
 
-// Where workgroup `flat` of the chunks works.
+// What a workgroup does: chunk `split` of a sequence's `splits`, whose partial results go to `slot`.
 struct Work {
-    int sequence, split, splits, length;
+    int sequence, split, splits, length, slot;
     std::int64_t chunk;
-    int first;  // flat index of the sequence's first chunk
 };
 
 __device__ __forceinline__ std::int64_t wave_sum(std::int64_t v) {
@@ -91,16 +91,18 @@ __device__ __forceinline__ std::int64_t chunk_length(const std::int32_t* __restr
     return static_cast<std::int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(min(blocks, std::int64_t{INT_MAX / kMinChunk})))) * kMinChunk;
 }
 
-// Chunks per sequence: at least one. Their sum is at most target + sequences.
-__device__ __forceinline__ int chunks_of(int length, std::int64_t chunk) {
-    return max(static_cast<int>((length + chunk - 1) / chunk), 1);
-}
+// A sequence's whole chunks, and whether a shorter one follows (also where the sequence is empty: it marks or clears its rows).
+struct Cut {
+    int whole, rest;
+    __device__ __forceinline__ Cut(int length, std::int64_t chunk)
+        : whole(static_cast<int>(length / chunk)), rest(length == 0 || length != whole * chunk) {}
+    __device__ __forceinline__ int chunks() const { return whole + rest; }
+};
 
-// Chunks of sequences base + lane (0 past the last), summed over lanes 0..lane.
-__device__ __forceinline__ int chunk_scan(int length, const Geometry& g, int base, std::int64_t chunk, int& own) {
+// Whole chunks of the sequences base + lane, summed over lanes 0..lane.
+__device__ __forceinline__ int whole_scan(int length, const Geometry& g, std::int64_t chunk) {
     const int lane = threadIdx.x & 63;
-    own = base + lane < g.sequences ? chunks_of(admitted(length, g), chunk) : 0;
-    int end = own;
+    int end = Cut(admitted(length, g), chunk).whole;
 #pragma unroll
     for (int step = 1; step < 64; step <<= 1) {
         const int below = __shfl_up(end, step, 64);
@@ -109,27 +111,36 @@ __device__ __forceinline__ int chunk_scan(int length, const Geometry& g, int bas
     return end;
 }
 
+// Workgroups take the whole chunks of all sequences first (at most `target`: one slot each, in order) and then the shorter
+// ends (slot target + sequence), which fill what the whole ones leave of the card.
 __device__ __forceinline__ bool find_work(const std::int32_t* __restrict__ lengths, const Geometry& g, int flat, Work& w) {
     const int first = length_at(lengths, g, 0);
     w.chunk = chunk_length(lengths, g, first);
     int before = 0;
     for (int base = 0; base < g.sequences; base += 64) {
         const int length = base ? length_at(lengths, g, base) : first;
-        int n;
-        const int end = before + chunk_scan(length, g, base, w.chunk, n);
+        const int end = before + whole_scan(length, g, w.chunk);
         const unsigned long long hit = __ballot(end > flat);
         if (hit) {
             const int at = __ffsll(hit) - 1;
             w.sequence = base + at;
             w.length = __builtin_amdgcn_readlane(length, at);
-            w.splits = __builtin_amdgcn_readlane(n, at);
-            w.first = __builtin_amdgcn_readlane(end, at) - w.splits;
-            w.split = flat - w.first;
+            const Cut cut(w.length, w.chunk);  // whole chunks: an admitted length
+            w.splits = cut.chunks();
+            w.split = flat - (__builtin_amdgcn_readlane(end, at) - cut.whole);
+            w.slot = flat;
             return true;
         }
         before = __builtin_amdgcn_readlane(end, 63);
     }
-    return false;
+    w.sequence = flat - before;
+    if (w.sequence >= g.sequences) return false;
+    w.length = __builtin_amdgcn_readfirstlane(lengths[w.sequence]);
+    const Cut cut(admitted(w.length, g), w.chunk);
+    w.splits = cut.chunks();
+    w.split = cut.whole;
+    w.slot = g.target + w.sequence;
+    return cut.rest;
 }
 
 __device__ __forceinline__ std::uint32_t permute(std::uint32_t high, std::uint32_t low, std::uint32_t selector) {
@@ -555,11 +566,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv_attention(const T* __restri
     __shared__ float references[kWaves][16], sums[kWaves][16];
     __shared__ int broken;
     Work w;
-    if (!find_work(lengths, g, blockIdx.x, w)) return;
+    // The head is the fast index: the same chunk of all heads, then the next.
+    const int heads = g.kv_heads * g.row_blocks, flat = blockIdx.x / heads, head_and_block = blockIdx.x - flat * heads;
+    if (!find_work(lengths, g, flat, w)) return;
     const int lane = threadIdx.x & 63, m = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row_wave = wave % ROWS, key_wave = wave / ROWS;
-    const int head = blockIdx.y / g.row_blocks, block = blockIdx.y - head * g.row_blocks;
+    const int head = head_and_block / g.row_blocks, block = head_and_block - head * g.row_blocks;
     if (threadIdx.x == 0) broken = 0;
     const bool bad_length = w.length < 0 || w.length > g.longest;
     const int length = bad_length ? 0 : w.length;
@@ -662,7 +675,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv_attention(const T* __restri
             if (column < g.head_dim)
                 *reinterpret_cast<uint2*>(target) = make_uint2(bits(v.x) | bits(v.y) << 16, bits(v.z) | bits(v.w) << 16);
         } else {
-            const std::int64_t slot = static_cast<std::int64_t>(blockIdx.x) * g.kv_heads + head;
+            const std::int64_t slot = static_cast<std::int64_t>(w.slot) * g.kv_heads + head;
             float* target = partial + (slot * g.rows + row) * partial_floats<D>();
             // Rows of D + 2 floats are 8-byte aligned.
             *reinterpret_cast<float2*>(target + column) = make_float2(v.x, v.y);
@@ -683,23 +696,24 @@ __global__ __launch_bounds__(256) void kv_attention_join(const std::int32_t* __r
     __shared__ float sums[4][5][64];
     const int length = length_at(lengths, g, 0);
     const std::int64_t chunk = chunk_length(lengths, g, length);
-    int first = 0, splits = 0;
+    const Cut cut(admitted(lengths[sequence], g), chunk);
+    const int splits = cut.chunks();
+    int first = 0;
     for (int base = 0; base <= sequence; base += 64) {
-        int n;
-        const int end = chunk_scan(base ? length_at(lengths, g, base) : length, g, base, chunk, n);
-        const int at = min(sequence - base, 63);
-        splits = __builtin_amdgcn_readlane(n, at);
-        first += __builtin_amdgcn_readlane(end, at) - (sequence - base > 63 ? 0 : splits);
+        const int end = whole_scan(base ? length_at(lengths, g, base) : length, g, chunk);
+        first += __builtin_amdgcn_readlane(end, min(sequence - base, 63));
     }
+    first -= cut.whole;
     if (splits == 1) return;
     const int token = index / g.q_heads, q_head = index - token * g.q_heads;
     const int head = q_head / g.group, row = token * g.group + q_head - head * g.group;
     const std::int64_t stride = static_cast<std::int64_t>(g.kv_heads) * g.rows * partial_floats<D>();
-    const float* base = partial + ((static_cast<std::int64_t>(first) * g.kv_heads + head) * g.rows + row) * partial_floats<D>();
+    const float* base = partial + (static_cast<std::int64_t>(head) * g.rows + row) * partial_floats<D>();
+    const auto part = [&](int i) { return base + (i < cut.whole ? first + i : g.target + sequence) * stride; };
     constexpr int kLanes = D / 4, kSide = 64 / kLanes, kSides = 4 * kSide;  // lanes of a row; chunks side by side
     const int in_wave = lane / kLanes, side = wave * kSide + in_wave, column = (lane - in_wave * kLanes) * 4;
     float best = -__builtin_inff();
-    for (int i = lane; i < splits; i += 64) best = fmaxf(best, base[i * stride + D]);
+    for (int i = lane; i < splits; i += 64) best = fmaxf(best, part(i)[D]);
 #pragma unroll
     for (int step = 32; step; step >>= 1) best = fmaxf(best, __shfl_xor(best, step, 64));
     float total = 0.0f, v[4] = {};
@@ -708,7 +722,7 @@ __global__ __launch_bounds__(256) void kv_attention_join(const std::int32_t* __r
         float2 low[4], high[4], end[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float* p = base + min(i + j * kSides, splits - 1) * stride;
+            const float* p = part(min(i + j * kSides, splits - 1));
             low[j] = *reinterpret_cast<const float2*>(p + column);
             high[j] = *reinterpret_cast<const float2*>(p + column + 2);
             end[j] = *reinterpret_cast<const float2*>(p + D);
@@ -762,8 +776,8 @@ Geometry geometry(int sequences, int query_tokens, int q_heads, int kv_heads, in
     g.group = q_heads / kv_heads, g.rows = query_tokens * g.group, g.head_dim = head_dim;
     const int block = 16 * row_tiles(g.rows);
     g.row_blocks = (g.rows + block - 1) / block;
-    require(static_cast<std::int64_t>(kv_heads) * g.row_blocks <= 65535 && sequences <= 65535,
-            "cached attention takes at most 65535 sequences, and KV heads times row blocks");
+    require(static_cast<std::int64_t>(kv_heads) * g.row_blocks * (sequences + kTarget) < (1ll << 31) && sequences <= 65535,
+            "cached attention takes at most 65535 sequences, and workgroups that fit int32");
     g.max_pages = max_pages, g.tiles_per_page = page_tokens / 16;
     g.page_magic = ((std::uint64_t{1} << 36) + g.tiles_per_page - 1) / g.tiles_per_page;
     g.target = target_chunks(kv_heads, g.row_blocks);
@@ -783,7 +797,7 @@ void launch_rows(const T* q, const CachePlanes& planes, const std::int32_t* page
                  float* partial, const Geometry& g, hipStream_t stream) {
     static LdsLimit limit;
     limit.raise(kv_attention<T, D, ROWS>, Shape<D, ROWS>::bytes);
-    const dim3 grid(g.target + g.sequences, g.kv_heads * g.row_blocks);
+    const unsigned grid = static_cast<unsigned>(g.target + g.sequences) * g.kv_heads * g.row_blocks;
     kv_attention<T, D, ROWS><<<grid, kWaves * 64, Shape<D, ROWS>::bytes, stream>>>(q, planes, page_table, lengths, out, partial, g);
 }
 
