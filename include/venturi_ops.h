@@ -426,8 +426,9 @@ int venturi_rowcodec_project(const VRCPlan* plan, const void* x, const void* cod
 
 /* Rotates q and K of qkv [tokens][(q_heads + 2 kv_heads) * head_dim] and caches K and V at slots [tokens]
  * (a slot outside the cache: not cached). rates: turns per position of each pair, fp64 [2][rotary_dim / 2]: the
- * rounded numbers, then what the rounding left; factor multiplies cos and sin; rotary_dim 0: no rotation, positions and rates unused. q [tokens][q_heads]
- * [head_dim] (NULL iff q_heads = 0); k [tokens][kv_heads][head_dim], the rotated keys, or NULL. */
+ * rounded numbers, then what the rounding left; factor multiplies cos and sin; rotary_dim 0: no rotation, positions
+ * and rates unused. q [tokens][q_heads][head_dim] (NULL iff q_heads = 0); k [tokens][kv_heads][head_dim], the
+ * rotated keys, or NULL. */
 int venturi_kv_write_run(const void* qkv, const int64_t* positions, const int64_t* slots, const double* rates,
                          void* q, void* k, void* key_codes, void* key_scales, void* value_codes,
                          void* value_scales, int tokens, int q_heads, int kv_heads, int head_dim, int rotary_dim,
@@ -459,12 +460,10 @@ int venturi_packed_attention_run(const void* q, const void* k, const void* v, co
 /* One token per row of logits [rows][vocab] from uniforms [rows] in [0, 1): order by (logit descending, index),
  * top_k (0: all), top_p of the top-k mass, min_p against the largest weight. Settings [rows], each NULL for none
  * (temperature 1). tokens int64 [rows] (-1 for a row of -inf and NaN alone); probabilities fp32 [rows] or NULL.
- * workspace: venturi_sample_bytes (0 but for few rows), 256-byte aligned, zeroed once before its first call; every
- * call leaves it ready for the next, and calls that share it run on one stream. */
-uint64_t venturi_sample_bytes(int rows, int vocab);
+ * vocab: at most 1048576. No workspace. */
 int venturi_sample_run(const void* logits, const float* uniforms, const float* temperature, const int32_t* top_k,
                        const float* top_p, const float* min_p, int64_t* tokens, float* probabilities,
-                       void* workspace, uint64_t available, int rows, int vocab, int dtype, void* stream);
+                       int rows, int vocab, int dtype, void* stream);
 
 /* ---- Reference exports outside the quantized-linear path. The reference's
  * Python backend binds each of these when it is constructed

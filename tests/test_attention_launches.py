@@ -22,7 +22,7 @@ def packed(tokens, keys, sequences, hq, hk, d, dtype):
 
 def sample(rows, vocab, dtype):
     logits, u, tokens = pointers(3)
-    return "venturi_sample_run", [logits, u, None, None, None, None, tokens, None, None, 0, rows, vocab, dtype, None]
+    return "venturi_sample_run", [logits, u, None, None, None, None, tokens, None, rows, vocab, dtype, None]
 
 
 def reached(calls):

@@ -2,8 +2,9 @@
 //
 // Bound by the matrix cores (4 rows keys head_dim operations) and, beside them, by the exponentials: at head_dim 128 a
 // score costs half a cycle of a SIMD in the matrix unit and as much in the vector unit. A wave takes 32 query rows and
-// works through the keys in tiles that its workgroup stages in LDS, double buffered: the next tile's global loads are
-// in flight while the present one is computed.
+// works through the keys in tiles that its workgroup stages in LDS, double buffered: the next tile is copied there, without
+// passing registers, while the present one is computed. 8192 tokens of one sequence, 48 heads on 4 of 128, bf16: 760 to 800
+// us, 1030 to 1080 TFLOP/s, matrix cores busy 58% of the time; a large matrix product reaches 1226 on this card.
 //
 // Rows. The rows of a KV head are its (query, head of the group) pairs, query by query, cut into blocks of 128, so that
 // all heads of a group share the staged keys, short sequences fill their tiles, and the diagonal's waste is
@@ -15,7 +16,12 @@
 // of units, which the transposing read takes together), so that both kinds of reads find their rows on different banks.
 //
 // Softmax. Weights are 2^(s - m + 8), rounded to the model's type (fp16 2^-11, bf16 2^-8 of each), for a reference m that
-// follows the maximum only when a score passes it by more than 4; sums are of the unrounded weights, in 32 bits.
+// follows the maximum only when a score passes it by more than 4. The sums, in 32 bits, are of the rounded weights, which
+// are what multiplies the values: a row's weights add to 1 whatever their rounding, and a dot product takes two at a time.
+//
+// Split. A workgroup per block of 128 rows and KV head; blocks with the most keys first, as far as a wave can rank the
+// sequences (11 prompts of 4096 tokens together: 196 -> 188 us). Few blocks over many keys are cut along the keys and joined
+// by a second launch.
 #include "kv_cache.hpp"
 
 #include <climits>

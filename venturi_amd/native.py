@@ -88,8 +88,7 @@ SIGNATURES = {
     "venturi_kv_attention_run": ([_P] * 9 + [_U64] + [_I] * 8 + [_F, _I, _P], _I),
     "venturi_packed_attention_bytes": ([_I] * 6, _U64),
     "venturi_packed_attention_run": ([_P] * 7 + [_U64] + [_I] * 6 + [_F, _I, _P], _I),
-    "venturi_sample_bytes": ([_I] * 2, _U64),
-    "venturi_sample_run": ([_P] * 9 + [_U64] + [_I] * 3 + [_P], _I),
+    "venturi_sample_run": ([_P] * 8 + [_I] * 3 + [_P], _I),
     # Reference exports outside the quantized-linear path: present so a binding
     # of the reference's whole table loads; each call returns -1 with a message.
     "venturi_greedy_run": ([_P] * 3 + [C.c_size_t] + [_I] * 3 + [_P], _I),

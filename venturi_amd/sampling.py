@@ -15,56 +15,41 @@ reference samples on the host apart from its greedy kernel (ops_api.h:46-47); th
 The result depends on the inputs alone: counts are whole numbers, masses 64-bit sums in a fixed order.
 """
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass
 
 import torch
 
 from .kv_cache import settle
-from .operands import DTYPE_CODES, address, apart, device_index, extents, spans
+from .operands import DTYPE_CODES, address, apart, device_index, extents
 
+_MAX_VOCAB = 1 << 20
 _SETTINGS = (("temperature", torch.float32), ("top_k", torch.int32), ("top_p", torch.float32), ("min_p", torch.float32))
 
 
 @dataclass(frozen=True)
 class SamplingPlan:
-    """``HipBackend.prepare_sampling``. The plan owns its workspace, so runs of one plan must be ordered: one stream at a
-    time."""
+    """``HipBackend.prepare_sampling``. It holds no memory: runs of one plan may overlap on several streams."""
 
     _backend: object
     rows: int
     vocab: int
     dtype: torch.dtype
     device: torch.device
-    _workspace: object = field(repr=False)
-    workspace_bytes = 0  # nothing for the caller to provide
+    workspace_bytes = 0
+    storage_tensors = ()
 
     def __post_init__(self):
-        w = self._workspace
         settle(self, _entry=self._backend._native.venturi_sample_run, _index=device_index(self.device), _logits=(self.rows, self.vocab),
-               _row=(self.rows,), _spans=spans(*self.storage_tensors),
-               _tail=(None if w is None else w.data_ptr(), 0 if w is None else w.numel(), self.rows, self.vocab,
-                      DTYPE_CODES[self.dtype]))
-
-    @property
-    def storage_tensors(self):
-        return () if self._workspace is None else (self._workspace,)
+               _row=(self.rows,), _tail=(self.rows, self.vocab, DTYPE_CODES[self.dtype]))
 
     @classmethod
     def create(cls, backend, *, rows, vocab, dtype, device):
         extents(rows, vocab)
         if dtype not in (torch.float16, torch.bfloat16):
             raise ValueError("Sampling takes FP16/BF16 logits")
-        target = backend.validate_device(dtype, device)
-        lib = backend._native
-        nbytes = lib.venturi_sample_bytes(rows, vocab)
-        if nbytes == 0 and lib.venturi_blocks_error():
-            raise ValueError(lib.error())
-        workspace = None
-        if nbytes:
-            with torch.cuda.device(target):
-                workspace = torch.zeros(nbytes, dtype=torch.uint8, device=target)  # counters: every run leaves them zero
-                torch.cuda.current_stream(target).synchronize()
-        return cls(backend, rows, vocab, dtype, target, workspace)
+        if vocab > _MAX_VOCAB:
+            raise ValueError(f"Sampling takes a vocabulary of at most {_MAX_VOCAB}")
+        return cls(backend, rows, vocab, dtype, backend.validate_device(dtype, device))
 
     def run(self, logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=None, *, tokens, probabilities=None):
         """``logits`` [rows, vocab], ``uniforms`` fp32 [rows]; per-row settings ``temperature``, ``top_p``, ``min_p`` fp32
@@ -73,7 +58,7 @@ class SamplingPlan:
         device, index, row, size = self.device, self._index, self._row, 4 * self.rows
         x = address(logits, self._logits, self.dtype, device, index, "logits")
         u = address(uniforms, row, torch.float32, device, index, "uniforms", 4)
-        inputs = [(x, x + 2 * self.rows * self.vocab), (u, u + size), *self._spans]
+        inputs = [(x, x + 2 * self.rows * self.vocab), (u, u + size)]
         settings = []
         for (name, dtype), value in zip(_SETTINGS, (temperature, top_k, top_p, min_p)):
             pointer = None
