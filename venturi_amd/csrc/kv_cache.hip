@@ -7,8 +7,8 @@
 // workgroup computes the r/2 cosines and sines once for all heads of its token. K and V units quantize by the q8_g32_fp16 rule:
 // four neighbouring lanes hold a group, two lane exchanges give its maximum.
 //
-// Bound by HBM, and by the launch where tokens are few. 8190 tokens, 24 heads and 2 KV heads of 256, fp16: the write 45 us
-// (235 MB, 5.2 TB/s; a large copy reaches 4.9), the read-back of K and V 11 us; one token 3.6 and 2.4 us.
+// Bound by HBM, and by the launch where tokens are few. 8190 tokens, 32 heads on 8 of 128, fp16: the write 45 us (202
+// MB, 4.5 TB/s; a large copy reaches 4.9), the read-back of K and V 11 us (51 MB, 4.6 TB/s); one token 3.6 and 2.4 us.
 #include "kv_cache.hpp"
 
 namespace vt {
