@@ -125,6 +125,28 @@ def test_masked_logits(backend, device, dtype):
         assert tokens[3] == tokens[4] == -1
 
 
+@pytest.mark.parametrize("dtype", [FP16, BF16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("vocab", [1000, 100001, 2**20])
+def test_signs(backend, device, dtype, vocab):
+    """The chosen class is looked for among the logits that may hold it: negative ones, zeros of either sign, NaN beside them."""
+    logits = random_logits(8, vocab, 2.0, dtype, 11)
+    logits[0] = -logits[0].abs() - 0.25
+    logits[1] = -logits[1].abs()
+    logits[1, ::3] = -0.0
+    logits[2, : vocab // 2] = -logits[2, : vocab // 2].abs() - 5
+    logits[2, vocab // 2:] = -logits[2, vocab // 2:].abs()
+    logits[3, ::2] = -math.nan
+    logits[3] = -logits[3].abs() - 1
+    logits[4, ::2] = math.nan
+    logits[5] = -0.0
+    logits[5, vocab - 1] = 0.0
+    logits[6, : vocab - 3] = -math.inf
+    logits[7] = -logits[7].abs()
+    logits[7, vocab - 2] = 1.0
+    for k in (0, 1, 40):
+        check(backend, device, logits, [0.999, 0.4, 0.8, 0.6, 0.9, 0.99, 0.5, 0.7], k=[k] * 8)
+
+
 def test_settings_that_are_no_number(backend, device):
     logits = random_logits(4, 300, 2.0, FP16, 9)
     nan = math.nan

@@ -13,11 +13,17 @@
 // Counters are 16 bits wide (128 KB of the CU's 160 KB): a row of more than 57344 logits is counted in segments, and
 // between two segments every class that has reached 16384 moves to a list (at most one entry per 16384 logits).
 //
-// A row takes about 43 us on its CU whatever their number up to 256 (151936 bf16 logits; 256 rows read 78 MB at 1.8 TB/s):
-// 3 to clear, 15 to count at what one CU loads, 9 to 13 to choose, 12 to find the occurrence. Counters in memory shared by
-// several workgroups of a row gain nothing (one row 46 us as here, 32 rows 150 us): the atomics and the 256 KB that one of
-// them reads at the end cost what the shorter count saves.
+// The token's place is found in a second pass over the row, of the chunks alone (512 logits) whose largest logit is not below
+// the class: noting those costs the count 0.8 us, passing the others by saves the search 5 (256 rows of 151936 logits: 42.2
+// -> 40.3 us).
+//
+// A row takes about 40 us on its CU whatever their number up to 256 (151936 bf16 logits; 256 rows read 78 MB at 1.9 TB/s):
+// 21 to clear and count, which the LDS atomics and the vector unit share, 8 to choose, 3 to find the occurrence. Counters in
+// memory shared by several workgroups of a row gain nothing (one row 46 us as here, 32 rows 150 us): the atomics and the 256 KB
+// that one of them reads at the end cost what the shorter count saves.
 #include "common.hpp"
+
+#include <climits>
 
 namespace vt {
 namespace {
@@ -28,6 +34,7 @@ constexpr int kMaxVocab = 1 << 20;
 constexpr std::uint32_t kHeavy = 16384;
 constexpr int kHeavyEntries = 2 * kMaxVocab / kHeavy;
 constexpr int kNone = -1;                  // no class
+constexpr int kChunks = kMaxVocab / 512;   // of 64 vectors, a wave's turn of a row
 // Vectors of 8 logits that a thread counts before the first sweep for heavy classes (57344 logits), and between two
 // sweeps (49152, on counters below 16384).
 constexpr int kFirst = 7, kNext = 6;
@@ -134,19 +141,23 @@ struct Shared {
     double turn_mass[kTurns];
     int turn_count[kTurns];
     std::uint32_t heavy_bits[kHeavyEntries], heavy_count[kHeavyEntries];
+    short largest[4 * kChunks];      // the largest signed_bits of 16 vectors
     double probability;
     int heavy, top, above_min, place, rank, count;
 };
 
-// A row's chosen class (kNone: nothing to take), and which of its `count` occurrences.
+// A row's chosen class (kNone: nothing to take), and which of its occurrences.
 struct Choice {
-    int place, rank, count;
+    int place, rank;
 };
+
+// A barrier of the workgroup's LDS accesses alone: __syncthreads() would also wait for the loads in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 __device__ __forceinline__ void clear(Shared& s) {
     for (int i = threadIdx.x; i < 32768 / 4; i += kThreads) reinterpret_cast<uint4*>(s.histogram)[i] = make_uint4(0, 0, 0, 0);
     if (threadIdx.x == 0) s.heavy = s.above_min = 0, s.top = 65536;
-    __syncthreads();
+    lds_barrier();
 }
 
 __device__ __forceinline__ void count_element(Shared& s, std::uint32_t bits) {
@@ -164,8 +175,41 @@ __device__ __forceinline__ void count_vector(Shared& s, const uint4& w) {
     }
 }
 
-// A barrier of the workgroup's LDS accesses alone: __syncthreads() would also wait for the loads in flight.
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// Logits in order as whole numbers: the magnitude's bits with the sign (both zeros are 0).
+__device__ __forceinline__ int signed_bits(std::uint32_t bits) {
+    const int magnitude = static_cast<int>(bits & 0x7fff);
+    return bits & 0x8000 ? -magnitude : magnitude;
+}
+
+template <int CONTROL>
+__device__ __forceinline__ int larger(int v) {
+    return max(v, __builtin_amdgcn_update_dpp(INT_MIN, v, CONTROL, 0xf, 0xf, false));
+}
+
+// The largest signed_bits (NaN by its bits) in the vectors of 16 lanes, in the last of them. Where a number has no sign it is
+// the largest signed half, else it is given by the smallest half: 0x8000 less that is the magnitude's negative, and what that
+// would make of one without a sign saturates below it.
+__device__ __forceinline__ short largest_of_16(const uint4& w) {
+    typedef short short2v __attribute__((ext_vector_type(2)));
+    typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
+    const std::uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    short2v high = __builtin_bit_cast(short2v, u[0]);
+    ushort2v low = __builtin_bit_cast(ushort2v, u[0]);
+#pragma unroll
+    for (int j = 1; j < 4; ++j) {
+        high = __builtin_elementwise_max(high, __builtin_bit_cast(short2v, u[j]));
+        low = __builtin_elementwise_min(low, __builtin_bit_cast(ushort2v, u[j]));
+    }
+    const short2v least = {SHRT_MIN, SHRT_MIN};
+    high = __builtin_elementwise_max(high, __builtin_elementwise_sub_sat(least, __builtin_bit_cast(short2v, low)));
+    high = __builtin_elementwise_max(high, __builtin_shufflevector(high, high, 1, 0));
+    int v = __builtin_bit_cast(int, high);  // ordered by its upper half
+    v = larger<0x111>(v);
+    v = larger<0x112>(v);
+    v = larger<0x114>(v);
+    v = larger<0x118>(v);
+    return static_cast<short>(v >> 16);
+}
 
 // Moves the classes that have reached kHeavy to the list.
 __device__ __forceinline__ void sweep(Shared& s) {
@@ -299,7 +343,7 @@ __device__ Choice choose(Shared& s, const Settings& set) {
     if (top >= 65536) {
         if (t == 0) s.probability = 0.0;
         __syncthreads();
-        return {kNone, 0, 0};
+        return {kNone, 0};
     }
     const bool greedy = !(set.temperature > 0.0f);
     // log2 e / T, from 4e-39 to 2e45.
@@ -331,13 +375,7 @@ __device__ Choice choose(Shared& s, const Settings& set) {
     if (wave == 0) {
         Lane<T> l;
         if (greedy) {
-            l.count(s, heavy, top >> 10);
-            if (lane == (top >> 4 & 63)) {
-                int n = 0;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) n = i == (top & 15) ? l.n[i] : n;
-                s.place = top, s.rank = 0, s.count = n, s.probability = 1.0;
-            }
+            if (lane == 0) s.place = top, s.rank = 0, s.probability = 1.0;
         } else {
             // What comes before turn `lane` in the whole order.
             const double turn_mass = s.turn_mass[lane], mass_scan = wave_scan(turn_mass), mass_all = lane_double(mass_scan, 63);
@@ -416,7 +454,6 @@ __device__ Choice choose(Shared& s, const Settings& set) {
                 if (place >= at && place < at + n) {
                     s.place = 1024 * turn + 16 * lane + i;
                     s.rank = place - at;
-                    s.count = n;
                     s.probability = w / kept;
                 }
                 at += n;
@@ -424,7 +461,7 @@ __device__ Choice choose(Shared& s, const Settings& set) {
         }
     }
     __syncthreads();
-    return {s.place, s.rank, s.count};
+    return {s.place, s.rank};
 }
 
 // A class's bits twice in a word, and the bits to compare (the class of 0 takes either sign).
@@ -492,30 +529,28 @@ struct Operands {
     }
 };
 
-// Visits the vectors begin + t, begin + t + kThreads, .. below end. The loads run a batch ahead of the visits, unconditional
-// (past the end they repeat the last vector): a load under a condition is waited for before the next one is issued.
-// `before` runs once, after the first loads are issued; `between`, for the whole workgroup, after every kFirst and then every
-// kNext vectors of a thread; it returns whether to go on.
+// Visits the vectors t, t + kThreads, .. below end. The loads run a batch ahead of the visits, unconditional (past the end they
+// repeat the last vector): a load under a condition is waited for before the next one is issued. `before` runs once, after the
+// first loads are issued; `between`, for the whole workgroup, after every kFirst and then every kNext vectors of a thread.
 template <class Before, class Visit, class Between>
-__device__ __forceinline__ void each_vector(const uint4* __restrict__ whole, int begin, int end, Before&& before, Visit&& visit,
-                                            Between&& between) {
-    if (begin >= end) {
+__device__ __forceinline__ void each_vector(const uint4* __restrict__ whole, int end, Before&& before, Visit&& visit, Between&& between) {
+    if (end <= 0) {
         before();
         return;
     }
-    const int at = begin + threadIdx.x;
+    const int at = threadIdx.x;
     const auto load = [&](int i) { return whole[min(at + i * kThreads, end - 1)]; };
     uint4 now[kFirst], next[kNext];
 #pragma unroll
     for (int j = 0; j < kFirst; ++j) now[j] = load(j);
     before();
-    for (int i = 0, count = kFirst; begin + i * kThreads < end; i += count, count = kNext) {
+    for (int i = 0, count = kFirst; i * kThreads < end; i += count, count = kNext) {
 #pragma unroll
         for (int j = 0; j < kNext; ++j) next[j] = load(i + count + j);
 #pragma unroll
         for (int j = 0; j < kFirst; ++j)
-            if (j < count && begin + (i + j) * kThreads < end) visit(now[j], i + j, at + (i + j) * kThreads < end);
-        if (begin + (i + count) * kThreads < end && !between(i + count)) break;
+            if (j < count && (i + j) * kThreads < end) visit(now[j], i + j, at + (i + j) * kThreads < end);
+        if ((i + count) * kThreads < end) between();
 #pragma unroll
         for (int j = 0; j < kNext; ++j) now[j] = next[j];
     }
@@ -532,43 +567,65 @@ struct Edge {
     __device__ __forceinline__ bool match(const Pattern& p) const { return live && ((bits ^ p.bits) & p.mask & 0xffff) == 0; }
 };
 
-// Occurrences among the vectors [begin, end), batch by batch until more than `rank` are found; every thread gets their
-// number, and `counts` holds them by chunk of 64 vectors. `found` is a word of LDS apart from them.
-__device__ __forceinline__ int count_matches(const Row& row, int begin, int end, const Pattern& p, int rank, int* counts, int* found) {
+// Lists the row's chunks that may hold the class, in order: those whose largest logit is not below it. One wave; their number.
+__device__ __forceinline__ int list_chunks(const Shared& s, const Row& row, const Pattern& p, int* list) {
+    const int lane = threadIdx.x & 63, chunks = (row.vectors + 63) / 64, least = signed_bits(p.bits & 0xffff);
+    int listed = 0;
+    for (int base = 0; base < chunks; base += 64) {
+        const int chunk = base + lane;
+        const short* largest = s.largest + 4 * min(chunk, kChunks - 1);
+        const bool may = chunk < chunks && max(max(largest[0], largest[1]), max(largest[2], largest[3])) >= least;
+        const unsigned long long all = __ballot(may);
+        if (may) list[listed + __popcll(all & ((1ull << lane) - 1))] = chunk;
+        listed += __popcll(all);
+    }
+    return listed;
+}
+
+// Occurrences in the listed chunks, batch by batch until more than `rank` are found; every thread gets their number, and
+// `counts` holds them by place in the list. `found` is a word of LDS apart from them, 0 at first.
+__device__ __forceinline__ int count_matches(const Row& row, const Pattern& p, int rank, const int* list, int listed, int* counts,
+                                             int* found) {
+    constexpr int kBatch = 6;  // loads of a wave in flight
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (threadIdx.x == 0) *found = 0;
-    __syncthreads();
-    each_vector(
-        row.whole(), begin, end, [] {},
-        [&](const uint4& w, int i, bool live) {
-            int n = live ? occurrences(w, p) : 0;
+    for (int base = 0; base < listed; base += kBatch * kWaves) {
+        uint4 w[kBatch];
+        int vector[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            vector[j] = list[min(base + j * kWaves + wave, listed - 1)] * 64 + lane;
+            w[j] = row.whole()[min(vector[j], row.vectors - 1)];
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int at = base + j * kWaves + wave;
+            if (at >= listed) break;
+            int n = vector[j] < row.vectors ? occurrences(w[j], p) : 0;
             n = __any(n) ? wave_sum(n) : 0;
             if (lane == 0) {
-                counts[i * kWaves + wave] = n;
+                counts[at] = n;
                 if (n) atomicAdd(found, n);
             }
-        },
-        [&](int) {
-            lds_barrier();
-            const bool enough = *found > rank;
-            lds_barrier();
-            return !enough;
-        });
-    __syncthreads();
+        }
+        __syncthreads();
+        const int now = *found;
+        __syncthreads();
+        if (now > rank) break;
+    }
     return *found;
 }
 
-// Writes the token of occurrence `rank` of the vectors [begin, end) from their counts. One wave.
-__device__ __forceinline__ void write_match(const Row& row, int begin, int end, const Pattern& p, int rank, const int* counts,
+// Writes the token of occurrence `rank` of the listed chunks from their counts. One wave.
+__device__ __forceinline__ void write_match(const Row& row, const Pattern& p, int rank, const int* list, int listed, const int* counts,
                                             std::int64_t* token) {
     const int lane = threadIdx.x & 63;
     int before;
-    const int chunk = find_chunk(counts, (end - begin + 63) / 64, rank, before);
-    const int vector = begin + chunk * 64 + lane;
-    const bool live = chunk >= 0 && vector < end;
+    const int at = find_chunk(counts, listed, rank, before);
+    const int vector = (at < 0 ? 0 : list[at]) * 64 + lane;
+    const bool live = at >= 0 && vector < row.vectors;
     const uint4 w = live ? row.whole()[vector] : make_uint4(~p.bits, ~p.bits, ~p.bits, ~p.bits);
-    const int at = find_element(w, p, before, rank);
-    if (at >= 0) *token = row.head + 8ll * vector + at;
+    const int element = find_element(w, p, before, rank);
+    if (element >= 0) *token = row.head + 8ll * vector + element;
 }
 
 // Occurrences in the row's head (tail: in its tail); the token, if rank is among them. One wave.
@@ -590,14 +647,13 @@ __global__ __launch_bounds__(kThreads) void sample(Operands o) {
     const Settings set = o.settings(index);
     const Edge edge(row);
     each_vector(
-        row.whole(), 0, row.vectors, [&] { clear(s); },
-        [&](const uint4& w, int, bool live) {
+        row.whole(), row.vectors, [&] { clear(s); },
+        [&](const uint4& w, int i, bool live) {
             if (live) count_vector(s, w);
+            const short largest = largest_of_16(w);  // past the end of the last vector again, which lists no chunk too few
+            if ((t & 15) == 15) s.largest[(i * kThreads + t) >> 4] = largest;
         },
-        [&](int) {
-            sweep(s);
-            return true;
-        });
+        [&] { sweep(s); });
     if (edge.live) count_element(s, edge.bits);
     __syncthreads();
     const Choice choice = choose<T>(s, set);
@@ -609,20 +665,21 @@ __global__ __launch_bounds__(kThreads) void sample(Operands o) {
     // The rank-th occurrence of the class: in the head, in the vectors or in the tail. (choose() has ended with a barrier:
     // the histogram's memory is free.)
     const Pattern pattern(choice.place);
-    int* counts = reinterpret_cast<int*>(s.histogram);
+    int *counts = reinterpret_cast<int*>(s.histogram), *list = counts + kChunks;
     if (wave == 0) {
         const int n = edge_match(row, edge, pattern, false, choice.rank, o.tokens + index);
-        if (t == 0) s.heavy = n;
+        const int listed = list_chunks(s, row, pattern, list);
+        if (t == 0) s.heavy = n, s.top = listed, s.count = 0;
     }
     __syncthreads();
-    const int first = s.heavy;
-    if (first > choice.rank) return;
-    const int found = count_matches(row, 0, row.vectors, pattern, choice.rank - first, counts, &s.count);
+    const int first = s.heavy, listed = s.top, rank = choice.rank - first;
+    if (rank < 0) return;
+    const int found = count_matches(row, pattern, rank, list, listed, counts, &s.count);
     if (wave != 0) return;
-    if (found > choice.rank - first)
-        write_match(row, 0, row.vectors, pattern, choice.rank - first, counts, o.tokens + index);
+    if (found > rank)
+        write_match(row, pattern, rank, list, listed, counts, o.tokens + index);
     else
-        edge_match(row, edge, pattern, true, choice.rank - first - found, o.tokens + index);
+        edge_match(row, edge, pattern, true, rank - found, o.tokens + index);
 }
 
 template <class T>
