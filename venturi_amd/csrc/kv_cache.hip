@@ -7,8 +7,9 @@
 // workgroup computes the r/2 cosines and sines once for all heads of its token. K and V units quantize by the q8_g32_fp16 rule:
 // four neighbouring lanes hold a group, two lane exchanges give its maximum.
 //
-// Bound by HBM, and by the launch where tokens are few. 8190 tokens, 32 heads on 8 of 128, fp16: the write 45 us (202
-// MB, 4.5 TB/s; a large copy reaches 4.9), the read-back of K and V 11 us (51 MB, 4.6 TB/s); one token 3.6 and 2.4 us.
+// Bound by HBM, and by the launch where tokens are few. 8190 tokens, 32 heads on 8 of 128, fp16: the write 39 us (202
+// MB, 5.2 TB/s; a large copy reaches 4.9; 45 us while each column chose its angle by
+// itself), the read-back of K and V 11 us (51 MB, 4.6 TB/s); one token 3.4 and 2.4 us.
 #include "kv_cache.hpp"
 
 namespace vt {
@@ -35,6 +36,14 @@ __device__ __forceinline__ float part_of_turn(double position, double rate, doub
     return static_cast<float>(part - rint(part));
 }
 
+__device__ __forceinline__ void floats8(const float* __restrict__ from, float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float4 v = reinterpret_cast<const float4*>(from)[i];
+        x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+    }
+}
+
 // Eight columns at `column` of a head, rotated. `head` is the head's first column.
 template <class T>
 __device__ __forceinline__ void rotated(const T* __restrict__ head, int column, int rotary, int interleaved,
@@ -53,23 +62,25 @@ __device__ __forceinline__ void rotated(const T* __restrict__ head, int column, 
         }
     } else {
         const int half = rotary >> 1;
-        float partner[8];
-        if ((half & 7) == 0) {
-            load8(head + (column < half ? column + half : column - half), partner);
+        if ((half & 7) == 0) {  // the unit lies on one side: eight pairs in order
+            const bool low = column < half;
+            const int pair = low ? column : column - half;
+            float partner[8], c[8], s[8];
+            load8(head + (low ? column + half : pair), partner);
+            floats8(cosines + pair, c);
+            floats8(sines + pair, s);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = x[i] * c[i] + partner[i] * (low ? -s[i] : s[i]);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int j = column + i;
-                partner[i] = j < rotary ? to_f32(head[j < half ? j + half : j - half]) : 0.0f;
+                const bool turns = j < rotary, low = j < half;
+                const int pair = turns ? (low ? j : j - half) : 0;
+                const float partner = turns ? to_f32(head[low ? j + half : j - half]) : 0.0f;
+                const float c = turns ? cosines[pair] : 1.0f, s = turns ? sines[pair] : 0.0f;
+                y[i] = x[i] * c + (low ? -partner : partner) * s;
             }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int j = column + i;
-            const bool turns = j < rotary, low = j < half;
-            const int pair = turns ? (low ? j : j - half) : 0;
-            const float c = turns ? cosines[pair] : 1.0f, s = turns ? sines[pair] : 0.0f;
-            y[i] = x[i] * c + (low ? -partner[i] : partner[i]) * s;
         }
     }
 #pragma unroll
@@ -108,7 +119,7 @@ __device__ __forceinline__ uint2 quantized(const float (&x)[8], __half& scale) {
 
 template <class T>
 __global__ __launch_bounds__(256) void kv_write(WriteArgs<T> a) {
-    __shared__ float cosines[128], sines[128];
+    __shared__ __align__(16) float cosines[128], sines[128];
     const std::int64_t token = blockIdx.x;
     if (a.rotary_dim) {
         const int pairs = a.rotary_dim >> 1;
