@@ -8,8 +8,8 @@
 // four neighbouring lanes hold a group, two lane exchanges give its maximum.
 //
 // Bound by HBM, and by the launch where tokens are few. 8190 tokens, 32 heads on 8 of 128, fp16: the write 39 us (202
-// MB, 5.2 TB/s; a large copy reaches 4.9; 45 us while each column chose its angle by
-// itself), the read-back of K and V 11 us (51 MB, 4.6 TB/s); one token 3.4 and 2.4 us.
+// MB, 5.2 TB/s; a large copy reaches 4.9; 45 us while each column chose its angle by itself), the read-back of K and V 11 us
+// (51 MB, 4.6 TB/s); one token 3.4 and 2.4 us.
 #include "kv_cache.hpp"
 
 namespace vt {
