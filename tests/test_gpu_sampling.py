@@ -188,3 +188,18 @@ def test_graph_and_side_stream(backend, device):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(tokens, want[0]) and torch.equal(chances, want[1])
+
+
+@pytest.mark.parametrize("dtype,value", [(FP16, 1.0), (FP16, 1.0009765625), (BF16, 1.0), (BF16, 1.0078125)],
+                         ids=["fp16-even", "fp16-odd", "bf16-even", "bf16-odd"])
+@pytest.mark.parametrize("vocab", [*range(106497, 106504), 106509, 106510, 155649])
+def test_a_class_that_fills_the_last_segment_and_the_ragged_ends(backend, device, dtype, value, vocab):
+    """Logits are counted 57344 and then 49152 at a time: a class one short of 16384 before the last segment that has all of
+    that, and the row's ends as well, in rows of every alignment."""
+    logits = torch.full((8, vocab), value).to(dtype)
+    for i in range(8):
+        head = -i * vocab % 8
+        logits[i, head: head + (vocab - head) // 8 * 8 - 49152 - 16383] = 0.0
+        logits[i, head + i] = value + 1  # the largest, once
+    check(backend, device, logits, [0.999, 0.3, 0.7, 0.0, 0.9, 0.5, 0.99, 0.1], k=[0, 0, 2, 50000, 65537, 66000, 0, 70000],
+          p=[1.0, 0.9, 1.0, 1.0, 1.0, 0.7, 0.99, 0.5])

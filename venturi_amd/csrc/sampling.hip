@@ -35,8 +35,8 @@ constexpr std::uint32_t kHeavy = 16384;
 constexpr int kHeavyEntries = 2 * kMaxVocab / kHeavy;
 constexpr int kNone = -1;                  // no class
 constexpr int kChunks = kMaxVocab / 512;   // of 64 vectors, a wave's turn of a row
-// Vectors of 8 logits that a thread counts before the first sweep for heavy classes (57344 logits), and between two
-// sweeps (49152, on counters below 16384).
+// Vectors of 8 logits that a thread counts before the first sweep for heavy classes (57344 logits, beside the up to 14 of the
+// row's ragged ends), and between two sweeps (49152, on counters below 16384: 65535 at most).
 constexpr int kFirst = 7, kNext = 6;
 
 template <class T> struct Bits;
@@ -647,14 +647,17 @@ __global__ __launch_bounds__(kThreads) void sample(Operands o) {
     const Settings set = o.settings(index);
     const Edge edge(row);
     each_vector(
-        row.whole(), row.vectors, [&] { clear(s); },
+        row.whole(), row.vectors,
+        [&] {
+            clear(s);
+            if (edge.live) count_element(s, edge.bits);
+        },
         [&](const uint4& w, int i, bool live) {
             if (live) count_vector(s, w);
             const short largest = largest_of_16(w);  // past the end of the last vector again, which lists no chunk too few
             if ((t & 15) == 15) s.largest[(i * kThreads + t) >> 4] = largest;
         },
         [&] { sweep(s); });
-    if (edge.live) count_element(s, edge.bits);
     __syncthreads();
     const Choice choice = choose<T>(s, set);
     if (t == 0 && o.probabilities) o.probabilities[index] = static_cast<float>(s.probability);
