@@ -187,8 +187,7 @@ __device__ __forceinline__ int larger(int v) {
 }
 
 // The largest signed_bits (NaN by its bits) in the vectors of 16 lanes, in the last of them. Where a number has no sign it is
-// the largest signed half, else it is given by the smallest half: 0x8000 less that is the magnitude's negative, and what that
-// would make of one without a sign saturates below it.
+// the largest signed half (and the smallest half less 0x8000 saturates to 0), else the negative of the smallest magnitude.
 __device__ __forceinline__ short largest_of_16(const uint4& w) {
     typedef short short2v __attribute__((ext_vector_type(2)));
     typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
@@ -200,8 +199,9 @@ __device__ __forceinline__ short largest_of_16(const uint4& w) {
         high = __builtin_elementwise_max(high, __builtin_bit_cast(short2v, u[j]));
         low = __builtin_elementwise_min(low, __builtin_bit_cast(ushort2v, u[j]));
     }
-    const short2v least = {SHRT_MIN, SHRT_MIN};
-    high = __builtin_elementwise_max(high, __builtin_elementwise_sub_sat(least, __builtin_bit_cast(short2v, low)));
+    const short2v none = {0, 0};
+    const ushort2v sign = {0x8000, 0x8000};
+    high = __builtin_elementwise_max(high, none) - __builtin_bit_cast(short2v, __builtin_elementwise_sub_sat(low, sign));
     high = __builtin_elementwise_max(high, __builtin_shufflevector(high, high, 1, 0));
     int v = __builtin_bit_cast(int, high);  // ordered by its upper half
     v = larger<0x111>(v);
