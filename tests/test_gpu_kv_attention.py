@@ -218,3 +218,45 @@ def test_same_bits_every_run_and_in_graphs(backend, device):
         assert torch.equal(out, want)
         assert torch.equal(want, first.view(torch.int16)) == (i % 2 == 0)
         out = out.view(BF16)
+
+
+def rewrite(cache, slots, k, v, device):
+    """Other rows [n, heads, d] in the cache's slots."""
+    rows = torch.cat([k.flatten(1), v.flatten(1)], 1).to(cache.dtype).to(device)
+    cache.prepare_write(tokens=len(slots), q_heads=0, rotary=None).run(rows, None, slots.to(device))
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("hq,hk,d,t", [(1, 1, 32, 1), (2, 2, 64, 1), (6, 2, 96, 2), (8, 2, 128, 1), (8, 1, 128, 3), (5, 1, 160, 5),
+                                       (7, 1, 224, 5), (12, 1, 256, 5), (2, 1, 256, 1)])
+@pytest.mark.parametrize("bits", [14, 18, 20, 24, 31, 38])
+def test_values_of_very_different_sizes(backend, device, dtype, hq, hk, d, t, bits):
+    """Columns 2^bits smaller than others of their head, and keys 2^bits larger than others whose weights are nothing: every
+    column's error goes by its own values. (A scale of 2^-24 has one bit; the cached values are what is compared with.)"""
+    n = 205
+    print(f"case kv values heads={hq}/{hk} d={d} {dtype} t={t} bits={bits}", flush=True)
+    gen = torch.Generator().manual_seed(bits + d)
+    top = 2.0**14  # the largest values' size: scales of 2^9
+    for keys in (False, True):
+        cache, q, table, sequences = make(backend, device, [n], hq, hk, d, dtype, 16, t, seed=bits)
+        k, v = torch.randn(n, hk, d, generator=gen), torch.randn(n, hk, d, generator=gen).clamp(-3.9, 3.9)  # within fp16
+        q[:] = q.abs() + 1
+        if keys:  # large values at the first, middle and last common keys, whose scores lie below -200
+            large = [0, 100, n - t]
+            v *= top * 2.0**-bits
+            v[large] *= 2.0**bits
+            k[large] = -300.0
+        else:  # columns by 16 and by 32: half a group of 32 is as small as the other half makes it
+            v *= top
+            for part in range(0, d, 32):
+                v[:, :, part: part + 32] *= 2.0 ** -(bits if part // 32 % 2 == 0 else bits // 2)
+            v[:, :, d - 16:] = torch.randn(n, hk, 16, generator=gen).clamp(-3.9, 3.9) * top
+            v[3::7] = 0  # scales of 0 beside them
+        rewrite(cache, sequences[0], k, v, device)
+        out = run(cache, q, table, [n], t, hq, device)
+        kc, vc = cached(cache, sequences[0])
+        want, mean, size = attend(q, kc, vc, [n - (t - 1 - i) for i in range(t)])
+        bound = attention_bound(want, mean, size, d, n, dtype, 2.0**-11, 2.0**-11)
+        error = (out.double() - want).abs()
+        assert (error <= bound).all(), (keys, float((error / bound).max()))

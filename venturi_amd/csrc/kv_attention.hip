@@ -15,12 +15,15 @@
 // Codes. A code c is stored as the byte u = c + 128, and a byte in the low half of a 16-bit word is the fp16 number
 // u 2^-24 (subnormal; the matrix cores keep it), so that one v_perm makes two operands.
 //   K: S = sum_groups scale_k * (sum u q - 128 sum q), the second term as the accumulator's start: exact products, fp32.
-//   V: a lane holds 8 keys of a few columns, a pair of keys is one v_perm of two keys' bytes, and v = fma(u 2^-24,
-//      scale_v 2^15 k, -scale_v k / 4) = v * k 2^-9, rounded once to fp16 (2^-11). k is a power of two that brings the
-//      largest scale so far to at most 1, so neither end of the scales' range overflows or underflows.
+//   V: a lane holds 8 keys of a few columns, a pair of keys is one v_perm of two keys' bytes, and v = ((u - 128) 2^-9)
+//      (scale_v k 2^14), the first factor exact, the product rounded once to fp16 (2^-11). k is a power of two that brings
+//      the largest scale so far to at most 1. Scales more than 2^18 below that one (other columns, or keys of any weight)
+//      would lose bits at fp16's lower end: steps that hold one multiply those scales apart, brought up by 2^19 or 2^38
+//      (32 sequences of 3000 keys, 32 heads on 8 of 128, bf16: 42 us; with such scales in every step 63).
 // Queries are scaled by a power of two per row into fp16's range: exact for fp16 and, but for numbers 2^28 below the
 // row's largest, for bf16. The weights are rounded to fp16 (2^-11); their sum is of the unrounded ones.
-// For bf16 rows, whose own rounding is eight times as coarse, that is that. For fp16 rows both factors of O = P V have a
+// For bf16 rows, whose own rounding is eight times as coarse, that is that (error against 64 bits 1.01 to 1.02 times that of the
+// one rounding at the end; with second terms 16 x 5 drafted tokens 45 -> 54 us). For fp16 rows both factors of O = P V have a
 // second term, what the first one's rounding left: the outputs' error against 64 bits at 1021 keys is that of the one
 // rounding at the end (2.1e-4 of their norm) where single terms leave 3.3e-4, for 2 to 5% of the time (64 sequences of 1 to
 // 8190 keys: 45.8 -> 48.1 us).
@@ -44,11 +47,13 @@ namespace {
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef float float4v __attribute__((ext_vector_type(4)));
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4, kBlock = 32;           // keys of a wave's step
 constexpr int kMinChunk = 128;
 constexpr int kTarget = 512;                     // workgroups: two to a CU
 constexpr float kLazy = 4.0f, kShift = 8.0f;     // weights are 2^(s - m + kShift), at most 2^12
+constexpr float kLeastScale = 0x1p-18f;          // of a value scale times k, below which code 1 times it loses bits in fp16
 
 struct Geometry {
     int sequences, query_tokens, q_heads, kv_heads, group, rows;  // rows = query_tokens * group, of one KV head
@@ -305,16 +310,92 @@ struct State {
     float bring;                 // k: 2^(-ceil(log2 of the largest value scale so far))
 };
 
-__device__ __forceinline__ float power_above(float v) {  // the smallest power of two >= v, for v > 0
+__device__ __forceinline__ int exponent_above(float v) {  // of the smallest power of two >= v, for v > 0
     int e;
-    const float f = frexpf(v, &e);
-    return ldexpf(1.0f, f == 0.5f ? e - 1 : e);
+    return frexpf(v, &e) == 0.5f ? e - 1 : e;
+}
+
+// The weights of a lane's query for its eight keys; FINE: and what their rounding to fp16 left.
+template <bool FINE>
+struct Weights {
+    half8v near;
+    half8v rest;  // of FINE alone
+    // Adds the products with the values ((u - 128) 2^-9) steep, the first factor exact, of the codes in byte `byte` of the words.
+    __device__ __forceinline__ void multiply(const std::uint32_t (&codes)[8], int byte, const half2v (&steep)[4], float4v& sum) const {
+        std::uint32_t v[4], left[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const std::uint32_t pair = permute(codes[2 * j + 1], codes[2 * j], 0x0c000c00u | byte | (4 + byte) << 16);
+            const half2v up = static_cast<_Float16>(32768.0f), down = static_cast<_Float16>(-0.25f);
+            const half2v code = __builtin_elementwise_fma(__builtin_bit_cast(half2v, pair), up, down);
+            const half2v value = code * steep[j];
+            v[j] = __builtin_bit_cast(std::uint32_t, value);
+            if constexpr (FINE) left[j] = __builtin_bit_cast(std::uint32_t, __builtin_elementwise_fma(code, steep[j], -value));
+        }
+        const half8v values = __builtin_bit_cast(half8v, make_uint4(v[0], v[1], v[2], v[3]));
+        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(values, near, sum, 0, 0, 0);
+        if constexpr (FINE) {
+            const half8v lefts = __builtin_bit_cast(half8v, make_uint4(left[0], left[1], left[2], left[3]));
+            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(values, rest, sum, 0, 0, 0);
+            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(lefts, near, sum, 0, 0, 0);
+        }
+    }
+};
+
+// The values of a step whose scales lie far below the largest so far (other columns', or those of keys of any weight), in windows
+// of 2^19 from kLeastScale down to 2^-40 (the least: 2^-24 beside 65504). The outputs go up with them and down again. Rare:
+// everything is read again, so that the usual step holds nothing for it.
+template <int D, bool FINE>
+__device__ __forceinline__ void far_below(const unsigned char* __restrict__ step, State<D>& a, const Weights<FINE>& weights, int first_key,
+                                          int length) {
+#pragma unroll 1
+    for (float up = 0x1p19f; up < 0x1p39f; up *= 0x1p19f) {
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane) : : "memory");  // no address of these reads is kept from one window or step to the next
+        const int m = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) a.out[d] *= 0x1p19f;
+#pragma unroll
+        for (int i = 0; i < Segments<D>::count; ++i) {
+            const int columns = Segments<D>::width(i) / 16, column = Segments<D>::offset(i) + columns * m;
+            half2v steep[4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const uint2 scale = *reinterpret_cast<const uint2*>(step + 4 * Step<D>::tile + (2 + t) * Step<D>::scales + 32 * (column >> 5) + 8 * g);
+                float x[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = half_at(scale, r) * (a.bring * up);
+                    if (!(x[r] >= kLeastScale && x[r] < 2.0f) || first_key + 16 * t + 4 * g + r >= length) x[r] = 0.0f;
+                }
+                steep[2 * t] = __builtin_bit_cast(half2v, pack(x[0] * 0x1p14f, x[1] * 0x1p14f));
+                steep[2 * t + 1] = __builtin_bit_cast(half2v, pack(x[2] * 0x1p14f, x[3] * 0x1p14f));
+            }
+#pragma unroll
+            for (int d = 0; d < columns; d += 4) {
+                std::uint32_t codes[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int row = 4 * g + (j & 3);
+                    const unsigned char* at = step + (2 + (j >> 2)) * Step<D>::tile + row * D + 16 * ((column >> 4) ^ Step<D>::swizzle(row)) + (column & 15) + d;
+                    if (columns == 2) codes[j] = *reinterpret_cast<const unsigned short*>(at);
+                    else codes[j] = *reinterpret_cast<const std::uint32_t*>(at);
+                }
+#pragma unroll
+                for (int byte = 0; byte < 4; ++byte)
+                    if (d + byte < columns) weights.multiply(codes, byte, steep, a.out[Segments<D>::tile(i) + d + byte]);
+            }
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) a.out[d] *= 0x1p-38f;
 }
 
 // One step of 32 keys for the wave's rows, from LDS. FULL: every row sees all of them. FINE: weights and values in two
-// fp16 terms.
+// fp16 terms. Returns whether values were left out for far_below().
 template <int D, bool FULL, bool FINE>
-__device__ __forceinline__ void compute(const unsigned char* __restrict__ step, State<D>& a, int first_key, int length) {
+__device__ __forceinline__ bool compute(const unsigned char* __restrict__ step, State<D>& a, int first_key, int length,
+                                        Weights<FINE>& weights) {
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const unsigned char* key_rows = step + m * D + 8 * (g & 1);
     const unsigned char* key_scales = step + 4 * Step<D>::tile + 8 * g;
@@ -378,23 +459,33 @@ __device__ __forceinline__ void compute(const unsigned char* __restrict__ step, 
             }
         }
     }
-    float value_scale[Segments<D>::count][8], top_scale = 0.0f;
+    // The largest finite scale and the least positive one, on fp16 bits: infinities and NaN wrap below the finite ones, 0 above
+    // all.
+    std::uint32_t value_scale[Segments<D>::count][4];
+    ushort2v top_bits = {0, 0}, least_bits = {0xffff, 0xffff};
+    const ushort2v finite = {0x8400, 0x8400}, one = {1, 1};
 #pragma unroll
     for (int i = 0; i < Segments<D>::count; ++i) {
         const int group = (Segments<D>::offset(i) + Segments<D>::width(i) / 16 * m) >> 5;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const uint2 scale = *reinterpret_cast<const uint2*>(step + 4 * Step<D>::tile + (2 + t) * Step<D>::scales + 32 * group + 8 * g);
+            value_scale[i][2 * t] = scale.x, value_scale[i][2 * t + 1] = scale.y;
+        }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float& v = value_scale[i][4 * t + r];
-                v = half_at(scale, r);
-                // Slots past the length hold anything: their weights are 0, and so has to be what they multiply.
-                if (!FULL && first_key + 16 * t + 4 * g + r >= length) v = 0.0f;
-                top_scale = fmaxf(top_scale, v <= 65504.0f ? v : 0.0f);
-            }
+        for (int j = 0; j < 4; ++j) {
+            std::uint32_t& w = value_scale[i][j];
+            // Slots past the length hold anything: their weights are 0, and so has to be what they multiply.
+            const int left = length - first_key - (16 * (j >> 1) + 4 * g + 2 * (j & 1));
+            if (!FULL && left < 2) w = left < 1 ? 0 : w & 0xffffu;
+            const ushort2v bits = __builtin_bit_cast(ushort2v, w);
+            top_bits = __builtin_elementwise_max(top_bits, bits + finite);
+            least_bits = __builtin_elementwise_min(least_bits, bits - one);
         }
     }
+    top_bits = __builtin_elementwise_sub_sat(top_bits, finite);
+    float top_scale = half_lo(max(top_bits.x, top_bits.y));
+    const float least_scale = half_lo((min(least_bits.x, least_bits.y) + 1) & 0xffff);  // 0: there is none
     bool raise = top_scale * a.bring > 1.99f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -407,9 +498,9 @@ __device__ __forceinline__ void compute(const unsigned char* __restrict__ step, 
         for (int step = 1; step < 64; step <<= 1) top_scale = fmaxf(top_scale, __shfl_xor(top_scale, step, 64));
         float shrink = 1.0f;
         if (top_scale * a.bring > 1.0f) {
-            const float bring = 1.0f / power_above(top_scale);
-            shrink = bring / a.bring;
-            a.bring = bring;
+            const int e = exponent_above(top_scale);
+            shrink = ldexpf(1.0f, -e - exponent_above(a.bring));
+            a.bring = ldexpf(1.0f, -e);
         }
         float top = a.reference;
 #pragma unroll
@@ -429,58 +520,45 @@ __device__ __forceinline__ void compute(const unsigned char* __restrict__ step, 
         p[j] = __builtin_amdgcn_exp2f(score[j] - base);
         a.sum += p[j];
     }
-    const half8v weights = __builtin_bit_cast(half8v, make_uint4(pack(p[0], p[1]), pack(p[2], p[3]), pack(p[4], p[5]), pack(p[6], p[7])));
-    half8v rests;
+    weights.near = __builtin_bit_cast(half8v, make_uint4(pack(p[0], p[1]), pack(p[2], p[3]), pack(p[4], p[5]), pack(p[6], p[7])));
     if constexpr (FINE) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) rests[j] = static_cast<_Float16>(p[j] - static_cast<float>(weights[j]));
+        for (int j = 0; j < 8; ++j) weights.rest[j] = static_cast<_Float16>(p[j] - static_cast<float>(weights.near[j]));
     }
+    const bool narrow = __any(least_scale > 0.0f && least_scale * a.bring < kLeastScale);
+    const float bring = a.bring * 0x1p14f;
 #pragma unroll
     for (int i = 0; i < Segments<D>::count; ++i) {
-        half2v steep[4], flat[4];
+        half2v steep[4];
         bool broken = false;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float x = value_scale[i][2 * j] * a.bring, y = value_scale[i][2 * j + 1] * a.bring;
-            // A row that does not see a key must not see its NaN: while rows differ, such scales are kept out of the
-            // product and marked below.
-            const bool mark = !FULL && !(x < 2.0f && y < 2.0f);
-            broken = broken || mark;
-            constexpr float kSteep = FINE ? 256.0f : 32768.0f;
-            steep[j] = __builtin_bit_cast(half2v, pack(!FULL && !(x < 2.0f) ? 0.0f : x * kSteep, !FULL && !(y < 2.0f) ? 0.0f : y * kSteep));
-            flat[j] = __builtin_bit_cast(half2v, pack(!FULL && !(x < 2.0f) ? 0.0f : x * -0.25f, !FULL && !(y < 2.0f) ? 0.0f : y * -0.25f));
+            float x[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                x[h] = (h ? half_hi(value_scale[i][j]) : half_lo(value_scale[i][j])) * bring;
+                // A row that does not see a key must not see its NaN: while rows differ, such scales are kept out of the
+                // product and marked below.
+                const bool mark = !FULL && !(x[h] < 0x1p15f);
+                broken = broken || mark;
+                if (mark || x[h] < 0x1p14f * kLeastScale) x[h] = 0.0f;
+            }
+            steep[j] = __builtin_bit_cast(half2v, pack(x[0], x[1]));
         }
         const int columns = Segments<D>::width(i) / 16, tile = Segments<D>::tile(i), word = Segments<D>::word(i);
 #pragma unroll
         for (int d = 0; d < columns; ++d) {
-            std::uint32_t v[4], left[4];
+            std::uint32_t codes[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const std::uint32_t pair = permute(value[2 * j + 1][word + d / 4], value[2 * j][word + d / 4], 0x0c000c00u | (d & 3) | (4 + (d & 3)) << 16);
-                const half2v x = __builtin_bit_cast(half2v, pair);
-                if constexpr (FINE) {
-                    const half2v up = static_cast<_Float16>(32768.0f), down = static_cast<_Float16>(-0.25f);
-                    const half2v code = __builtin_elementwise_fma(x, up, down);  // (u - 128) 2^-9, exact
-                    const half2v near = code * steep[j];
-                    v[j] = __builtin_bit_cast(std::uint32_t, near);
-                    left[j] = __builtin_bit_cast(std::uint32_t, __builtin_elementwise_fma(code, steep[j], -near));
-                } else {
-                    v[j] = __builtin_bit_cast(std::uint32_t, __builtin_elementwise_fma(x, steep[j], flat[j]));
-                }
-            }
-            const half8v values = __builtin_bit_cast(half8v, make_uint4(v[0], v[1], v[2], v[3]));
-            a.out[tile + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values, weights, a.out[tile + d], 0, 0, 0);
-            if constexpr (FINE) {
-                const half8v lefts = __builtin_bit_cast(half8v, make_uint4(left[0], left[1], left[2], left[3]));
-                a.out[tile + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values, rests, a.out[tile + d], 0, 0, 0);
-                a.out[tile + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lefts, weights, a.out[tile + d], 0, 0, 0);
-            }
+            for (int j = 0; j < 8; ++j) codes[j] = value[j][word + d / 4];
+            weights.multiply(codes, d & 3, steep, a.out[tile + d]);
         }
         if (!FULL && __any(broken)) {
             half8v marks, sees;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                marks[j] = value_scale[i][j] * a.bring < 2.0f ? static_cast<_Float16>(0.0f) : static_cast<_Float16>(1.0f);
+                const std::uint32_t w = value_scale[i][j / 2];
+                marks[j] = (j & 1 ? half_hi(w) : half_lo(w)) * bring < 0x1p15f ? static_cast<_Float16>(0.0f) : static_cast<_Float16>(1.0f);
                 sees[j] = first_key + 16 * (j >> 2) + 4 * g + (j & 3) < a.seen ? static_cast<_Float16>(1.0f) : static_cast<_Float16>(0.0f);
             }
             const float4v none = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -492,6 +570,7 @@ __device__ __forceinline__ void compute(const unsigned char* __restrict__ step, 
                     if (hits[r] > 0.0f) a.out[tile + d][r] = __builtin_nanf("");
         }
     }
+    return narrow;
 }
 
 // The wave's 16 query rows from row `first` of the KV head's on: the loads, and what becomes of them.
@@ -562,6 +641,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv_attention(const T* __restri
                                                             const std::int32_t* __restrict__ lengths, T* __restrict__ out,
                                                             float* __restrict__ partial, Geometry g) {
     using S = Shape<D, ROWS>;
+    constexpr bool kFine = std::is_same<T, __half>::value;
     extern __shared__ __align__(16) unsigned char memory[];
     __shared__ float references[kWaves][16], sums[kWaves][16];
     __shared__ int broken;
@@ -615,10 +695,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv_attention(const T* __restri
             next = places(i + S::ring);
         }
         const int key = key_of(i);
+        bool narrow = false;
+        Weights<kFine> weights;
         if (key + kBlock <= min(all_see, end))
-            compute<D, true, std::is_same<T, __half>::value>(memory + place_of(i), a, key, length);
+            narrow = compute<D, true, kFine>(memory + place_of(i), a, key, length, weights);
         else if (key < end)
-            compute<D, false, std::is_same<T, __half>::value>(memory + place_of(i), a, key, length);
+            narrow = compute<D, false, kFine>(memory + place_of(i), a, key, length, weights);
+        if (narrow) far_below<D, kFine>(memory + place_of(i), a, weights, key, length);
     }
     __syncthreads();
     if (bad && lane == 0) broken = 1;
@@ -633,9 +716,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv_attention(const T* __restri
     float top = references[row_wave][m];
 #pragma unroll
     for (int i = 1; i < S::keys; ++i) top = fmaxf(top, references[row_wave + i * ROWS][m]);
-    // 512 / bring (2 / bring with two terms) undoes the values' power of two.
+    // 2^-5 / bring undoes the values' power of two.
     const float keep = a.reference == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(a.reference - top);
-    const float undo = keep * ((std::is_same<T, __half>::value ? 2.0f : 512.0f) / a.bring);
+    const float undo = keep * (0x1p-5f / a.bring);
 #pragma unroll
     for (int i = 0; i < Segments<D>::count; ++i) {
         const int columns = Segments<D>::width(i) / 16;
