@@ -260,3 +260,33 @@ def test_values_of_very_different_sizes(backend, device, dtype, hq, hk, d, t, bi
         bound = attention_bound(want, mean, size, d, n, dtype, 2.0**-11, 2.0**-11)
         error = (out.double() - want).abs()
         assert (error <= bound).all(), (keys, float((error / bound).max()))
+
+
+@pytest.mark.parametrize("d", [64, 128, 160, 256])
+@pytest.mark.parametrize("dtype,spread,scale", [(BF16, 2.0**100, None), (BF16, 2.0**118, None), (BF16, 2.0**124, None), (BF16, 2.0**100, -1.0),
+                                                (BF16, 2.0**124, 2.0**30), (FP16, 100.0, 2.0**110), (FP16, 1.0, -2.0**127)])
+def test_scores_near_the_end_of_32_bits(backend, device, dtype, spread, scale, d):
+    """Queries, or scales, so large that the largest score takes all of a row's weight: its value is the row's output."""
+    n, t, hq = 70, 2, 3
+    print(f"case kv scores d={d} {dtype} spread={spread} scale={scale}", flush=True)
+    cache, q, table, sequences = make(backend, device, [n], hq, 1, d, dtype, 16, t, seed=d)
+    q = (q.float().clamp(-4, 4) * spread).to(dtype)  # below 2^127
+    q[1, 0] = 0  # equal weights
+    out = run(cache, q, table, [n], t, hq, device, scale)
+    kc, vc = cached(cache, sequences[0])
+    factor = d ** -0.5 if scale is None else scale
+    for i in range(t):
+        seen = n - (t - 1 - i)
+        for h in range(hq):
+            products = kc[:seen, 0] * q[i, h].double()
+            scores = products.sum(1) * factor
+            if (i, h) == (1, 0):
+                want, mean = vc[:seen, 0].mean(0), vc[:seen, 0].abs().mean(0)
+            else:
+                best, gap = int(scores.argmax()), scores.sort(descending=True)[0]
+                # What 32-bit sums may be off, and what leaves the second weight nothing.
+                assert gap[0] - gap[1] > 2 * (d + 6) * 2.0**-24 * float(products.abs().sum(1).max()) * abs(factor) + 100
+                want, mean = vc[best, 0], vc[best, 0].abs()
+            bound = attention_bound(want, mean, torch.zeros(()), d, n, dtype, 2.0**-11, 2.0**-11)
+            error = (out[i, h].double() - want).abs()
+            assert (error <= bound).all(), (i, h, float((error / bound).max()))

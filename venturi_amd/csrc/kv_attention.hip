@@ -622,7 +622,11 @@ struct Queries {
                 a.start[c] = float4v{total, total, total, total};
             }
         }
-        a.factor = ldexpf(g.scale * 1.44269504088896340736f, e + (kOffsetInStart<D> ? 24 : 9));
+        // Bounded, so that no score overflows (raw sums times scales are below 2^22, at large heads 2^37). Where the bound
+        // holds unequal scores, 2^-72 (2^-57) apart at least, are too far apart to share the weight with either factor.
+        constexpr float kMost = kOffsetInStart<D> ? 0x1p100f : 0x1p85f;
+        const float factor = ldexpf(g.scale * 1.44269504088896340736f, e + (kOffsetInStart<D> ? 24 : 9));
+        a.factor = fminf(fmaxf(factor, -kMost), kMost);
         a.reference = -__builtin_inff();
         a.sum = 0.0f;
 #pragma unroll
