@@ -290,3 +290,26 @@ def test_scores_near_the_end_of_32_bits(backend, device, dtype, spread, scale, d
             bound = attention_bound(want, mean, torch.zeros(()), d, n, dtype, 2.0**-11, 2.0**-11)
             error = (out[i, h].double() - want).abs()
             assert (error <= bound).all(), (i, h, float((error / bound).max()))
+
+
+@pytest.mark.parametrize("side", ["key", "value"])
+@pytest.mark.parametrize("d", [32, 64, 128, 192, 256])
+@pytest.mark.parametrize("t", [1, 3])
+def test_groups_whose_scale_overflows(backend, device, d, t, side):
+    """Such a group reads back as NaN: so it is for the rows that see it, whatever the signs of their queries, and for no other."""
+    n, hq = 75, 12
+    print(f"case kv overflow d={d} t={t} {side}", flush=True)
+    cache, q, table, sequences = make(backend, device, [n], hq, 1, d, BF16, 16, t, seed=d + t)
+    gen = torch.Generator().manual_seed(d)
+    k, v = torch.randn(n, 1, d, generator=gen), torch.randn(n, 1, d, generator=gen)
+    q *= 2.0 ** -torch.randint(0, 20, q.shape, generator=gen)  # their sums are not exact in 32 bits
+    last = n - 2 if t > 1 else 40  # not seen by the first of three new tokens
+    (k if side == "key" else v)[last, 0, d - 1] = -1e38
+    rewrite(cache, sequences[0], k, v, device)
+    out = run(cache, q, table, [n], t, hq, device)
+    for i in range(t):
+        sees = last < n - (t - 1 - i)
+        hit = out[i] if side == "key" else out[i, :, d - 32:]
+        assert hit.isnan().all() if sees else hit.isfinite().all()
+        if side == "value":
+            assert out[i, :, : d - 32].isfinite().all()

@@ -489,7 +489,8 @@ __device__ __forceinline__ bool compute(const unsigned char* __restrict__ step, 
     bool raise = top_scale * a.bring > 1.99f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        score[j] *= a.factor;
+        // An infinite scale stands beside codes of 0, whose products with the rounded start may not be: NaN either way.
+        score[j] = kOffsetInStart<D> ? fmaf(score[j], 0.0f, score[j] * a.factor) : score[j] * a.factor;
         if (!FULL && first_key + 16 * (j >> 2) + 4 * g + (j & 3) >= a.seen) score[j] = -__builtin_inff();
         raise = raise || score[j] > a.reference + kLazy;
     }
