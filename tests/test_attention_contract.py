@@ -187,6 +187,25 @@ def test_packed_attention_refusals(backend):
     assert len(backend.launches) == 1
 
 
+def test_packed_workspace_is_free_before_the_first_run_and_held_until_the_last(backend, monkeypatch):
+    """The plan's own memory, allocated on one stream and used on others: waited for once, recorded where it is used."""
+    waited, recorded, stream = [], [], [7]
+    fake = SimpleNamespace(synchronize=lambda: waited.append(stream[0]))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: fake)
+    monkeypatch.setattr("venturi_amd.attention.stream_of", lambda device: stream[0], raising=False)
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda tensor, on: recorded.append((tensor.data_ptr(), on)))
+    base = dict(q_heads=4, kv_heads=4, head_dim=64, dtype=FP16, device=CPU)
+    without = PackedAttentionPlan.create(backend, tokens=64, keys=64, sequences=1, **base)
+    assert not without.storage_tensors and not waited
+    plan = PackedAttentionPlan.create(backend, tokens=2, keys=1024, sequences=1, **base)
+    assert len(plan.storage_tensors) == 1 and waited == [7]
+    rows, keys = torch.zeros(2, 4, 64, dtype=FP16), torch.zeros(1024, 4, 64, dtype=FP16)
+    offsets = torch.zeros(2, dtype=torch.int32)
+    for stream[0] in (7, 8):
+        plan.run(rows, keys, keys, offsets, offsets, out=rows.clone())
+    assert recorded == [(plan.storage_tensors[0].data_ptr(), fake)] and waited == [7]
+
+
 def test_sampling_refusals(backend):
     for change in (dict(rows=0), dict(vocab=0), dict(vocab=2**20 + 1), dict(dtype=torch.float32)):
         with pytest.raises(ValueError):

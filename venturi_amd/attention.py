@@ -12,13 +12,14 @@ from dataclasses import dataclass, field
 import torch
 
 from .kv_cache import head_geometry, settle, softmax_scale
-from .operands import DTYPE_CODES, address, apart, device_index, extents, spans
+from .operands import DTYPE_CODES, address, apart, device_index, extents, spans, stream_of
 
 
 @dataclass(frozen=True)
 class PackedAttentionPlan:
     """``HipBackend.prepare_attention``. The plan owns its workspace (partial sums of calls with few rows, split over
-    their keys), so runs of one plan must be ordered: one stream at a time."""
+    their keys), so runs of one plan must be ordered: one stream at a time. Concurrent streams prepare a plan each, and a
+    captured graph needs its plan for as long as it is replayed."""
 
     _backend: object
     tokens: int
@@ -31,6 +32,7 @@ class PackedAttentionPlan:
     dtype: torch.dtype
     device: torch.device
     _workspace: object = field(repr=False)
+    _stream: object = field(repr=False)  # of the workspace's allocation
     workspace_bytes = 0  # nothing for the caller to provide
 
     def __post_init__(self):
@@ -57,11 +59,13 @@ class PackedAttentionPlan:
         nbytes = lib.venturi_packed_attention_bytes(tokens, keys, sequences, q_heads, kv_heads, head_dim)
         if nbytes == 0 and lib.venturi_blocks_error():
             raise ValueError(lib.error())
-        workspace = None
+        workspace = stream = None
         if nbytes:
             with torch.cuda.device(target):
-                workspace = torch.empty(nbytes, dtype=torch.uint8, device=target)
-        return cls(backend, tokens, keys, sequences, q_heads, kv_heads, head_dim, factor, dtype, target, workspace)
+                workspace, stream = torch.empty(nbytes, dtype=torch.uint8, device=target), stream_of(target)
+                # Earlier work of this stream may still use the memory; the plan may run on another.
+                torch.cuda.current_stream(target).synchronize()
+        return cls(backend, tokens, keys, sequences, q_heads, kv_heads, head_dim, factor, dtype, target, workspace, stream)
 
     def run(self, q, k, v, q_offsets, k_offsets, *, out):
         """``q`` and ``out`` [tokens, q_heads, head_dim], ``k`` and ``v`` [keys, kv_heads, head_dim], offsets int32
@@ -78,4 +82,7 @@ class PackedAttentionPlan:
         size, rows, starts = 2 * self.tokens * self.q_heads * self.head_dim, 2 * self.keys * self.kv_heads * self.head_dim, 4 * self._offsets[0]
         apart(y, size, (x, x + size), (a, a + rows), (b, b + rows), (m, m + starts), (n, n + starts), *self._spans)
         self._backend._call(self._entry, device, (x, a, b, m, n, y, *self._tail))
+        if self._workspace is not None and stream_of(device) != self._stream:
+            # A plan that is dropped now leaves its workspace to this run until it is done.
+            self._workspace.record_stream(torch.cuda.current_stream(device))
         return out
