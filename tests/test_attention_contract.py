@@ -131,6 +131,17 @@ def test_write_plan_refusals(backend):
     assert len(backend.launches) == 1
 
 
+def test_write_plans_of_one_embedding_share_its_upload(backend, monkeypatch):
+    """Preparing again, as a batch does whenever its token count changes, copies nothing and waits for nothing."""
+    c, rotary, waited = cache(backend), RotaryEmbedding(64), []
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: SimpleNamespace(synchronize=lambda: waited.append(device)))
+    plans = [c.prepare_write(tokens=n, q_heads=4, rotary=rotary) for n in (1, 3, 3)]
+    assert waited == [CPU] and all(p.storage_tensors[-1] is plans[0].storage_tensors[-1] for p in plans)
+    c.prepare_write(tokens=1, q_heads=4, rotary=None)
+    other = c.prepare_write(tokens=1, q_heads=4, rotary=RotaryEmbedding(64, base=1e6))
+    assert waited == [CPU, CPU] and not torch.equal(other.storage_tensors[-1], plans[0].storage_tensors[-1])
+
+
 def test_read_plan_refusals(backend):
     c = cache(backend)
     plan = c.prepare_read(tokens=5)

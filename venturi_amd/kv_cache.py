@@ -110,12 +110,7 @@ class Q8KVCache:
         width = (q_heads + 2 * self.kv_heads) * self.head_dim
         extents(width)
         self._backend.resolve_device(self.device)
-        rates = None
-        if rotary is not None:
-            with torch.cuda.device(self.device):
-                rates = rotary.rates.to(self.device)
-                torch.cuda.current_stream(self.device).synchronize()
-        return KVWritePlan(self, tokens, q_heads, rotary, rates)
+        return KVWritePlan(self, tokens, q_heads, rotary, None if rotary is None else rotary.rates_on(self.device))
 
     def prepare_read(self, *, tokens):
         """Plan of reading ``tokens`` slots back as rows of the cache's dtype."""

@@ -47,6 +47,7 @@ class RotaryEmbedding:
     frequencies: tuple = field(init=False, repr=False, compare=False)  # radians per position of each pair
     rates: torch.Tensor = field(init=False, repr=False, compare=False)  # turns per position, fp64 [2, r / 2]: words, rests
     factor: float = field(init=False, repr=False, compare=False)  # on cos and sin
+    _uploads: dict = field(init=False, repr=False, compare=False, default_factory=dict)  # rates by device
 
     def __post_init__(self):
         if type(self.head_dim) is not int or self.head_dim <= 0:
@@ -77,6 +78,16 @@ class RotaryEmbedding:
         object.__setattr__(self, "frequencies", tuple(frequencies))
         object.__setattr__(self, "rates", torch.tensor(rates, dtype=torch.float64))
         object.__setattr__(self, "factor", factor)
+
+    def rates_on(self, device):
+        """The rates on a device: uploaded once, and whole before any stream reads them."""
+        rates = self._uploads.get(device)
+        if rates is None:
+            with torch.cuda.device(device):
+                rates = self.rates.to(device)
+                torch.cuda.current_stream(device).synchronize()
+            rates = self._uploads.setdefault(device, rates)
+        return rates
 
 
 def _frequencies(dim, base, scaling):
