@@ -235,6 +235,23 @@ def test_sampling_refusals(backend):
     assert len(backend.launches) == 2
 
 
+@pytest.mark.parametrize("scale", [1e39, -1e39, 2e38, pytest.param(10**400, id="10^400"), math.inf, math.nan, True, "1"])
+def test_scales_out_of_range(backend, scale):
+    with pytest.raises(ValueError, match="scale"):
+        cache(backend).prepare_attention(sequences=2, q_heads=4, query_tokens=1, max_pages=4, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        PackedAttentionPlan.create(backend, tokens=6, keys=9, sequences=2, q_heads=4, kv_heads=2, head_dim=64, dtype=BF16, device=CPU,
+                                   scale=scale)
+    if type(scale) is float:  # 1e39 is an infinity by the time an entry point has it
+        for entry, good in (("venturi_kv_attention_run", ATTEND), ("venturi_packed_attention_run", PACKED)):
+            assert getattr(native.load(), entry)(*{**good, "scale": scale}.values()) == -1 and "scale" in native.load().error()
+
+
+@pytest.mark.parametrize("scale", [0, 2, -0.5, -(2.0**127)])
+def test_scales_in_range(backend, scale):
+    assert cache(backend).prepare_attention(sequences=2, q_heads=4, query_tokens=1, max_pages=4, scale=scale).scale == float(scale)
+
+
 def test_capabilities():
     caps = object.__new__(HipBackend).capabilities
     for operation in ("kv_cache", "attention", "sampling"):

@@ -71,6 +71,11 @@ def test_few_rows_over_many_keys(backend, device, dtype, hk, d):
     check(backend, device, [3, 1, 40], [1300, 0, 700], 3 * hk, hk, d, dtype, seed=d + 1)
 
 
+@pytest.mark.parametrize("scale", [2.0**127, -(2.0**127)])
+def test_largest_scales(backend, device, scale):
+    check(backend, device, [33, 2], [0, 300], 4, 2, 64, BF16, seed=5, scale=scale, spread=2.0**-130)
+
+
 def test_many_sequences(backend, device):
     queries = [(5 * i * i + i) % 23 for i in range(301)]
     check(backend, device, queries, [i % 4 for i in range(301)], 4, 2, 64, BF16, seed=4)

@@ -143,6 +143,12 @@ def test_scale(backend, device, scale):
     check(backend, device, [90], 4, 4, 64, FP16, 16, 2, seed=9, scale=scale)
 
 
+@pytest.mark.parametrize("scale", [2.0**127, -(2.0**127)])
+@pytest.mark.parametrize("d", [64, 256])
+def test_largest_scales(backend, device, scale, d):
+    check(backend, device, [90], 4, 4, d, BF16, 16, 2, seed=9, scale=scale, spread=2.0**-130)
+
+
 def test_bad_pages_and_lengths_mark_their_sequence(backend, device):
     lengths = [40, 40, 40, 40, 40]
     cache, q, table, _ = make(backend, device, lengths, 4, 2, 64, FP16, 16, 2, seed=10)

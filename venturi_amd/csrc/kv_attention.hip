@@ -39,6 +39,7 @@
 #include "kv_cache.hpp"
 
 #include <climits>
+#include <cmath>
 #include <type_traits>
 
 namespace vt {
@@ -946,6 +947,7 @@ VT_EXPORT int venturi_kv_attention_run(const void* q, const void* key_codes, con
                                              page_tokens);
         const auto g = vt::geometry(sequences, query_tokens, q_heads, kv_heads, head_dim, max_pages, page_tokens, scale);
         vt::require(q && page_table && lengths && out, "null cached attention operand");
+        vt::require(std::fabs(scale) <= 0x1p127f, "attention scale must be a number of at most 2^127");
         vt::require(vt::aligned(q, 16) && vt::aligned(out, 16), "cached attention rows must be 16-byte aligned");
         const std::uint64_t bytes = vt::partial_bytes(g);
         vt::require(!bytes || (workspace && available >= bytes && vt::aligned(workspace, 256)),

@@ -25,6 +25,7 @@
 #include "kv_cache.hpp"
 
 #include <climits>
+#include <cmath>
 
 namespace vt {
 namespace {
@@ -585,6 +586,7 @@ VT_EXPORT int venturi_packed_attention_run(const void* q, const void* k, const v
     return vt::guarded([&] {
         const auto g = vt::geometry(tokens, keys, sequences, q_heads, kv_heads, head_dim, scale);
         vt::require(q && k && v && q_offsets && k_offsets && out, "null packed attention operand");
+        vt::require(std::fabs(scale) <= 0x1p127f, "attention scale must be a number of at most 2^127");
         vt::require(vt::aligned(q, 16) && vt::aligned(k, 16) && vt::aligned(v, 16) && vt::aligned(out, 16),
                     "packed attention rows must be 16-byte aligned");
         const std::uint64_t bytes = vt::partial_bytes(g);

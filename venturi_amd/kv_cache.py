@@ -36,12 +36,12 @@ def head_geometry(q_heads, kv_heads, head_dim):
 
 
 def softmax_scale(scale, head_dim):
-    """The factor on q k^T: 1 / sqrt(head_dim) unless given."""
+    """The factor on q k^T: 1 / sqrt(head_dim) unless given. Up to 2^127, so that log2 e times it is an FP32 number."""
     if scale is None:
         return 1.0 / math.sqrt(head_dim)
-    if type(scale) in (int, float) and math.isfinite(scale):
+    if type(scale) in (int, float) and abs(scale) <= 2**127:
         return float(scale)
-    raise ValueError("attention scale must be a finite number")
+    raise ValueError("attention scale must be a number of at most 2^127")
 
 
 def settle(plan, **values):
