@@ -118,6 +118,27 @@ def test_slots_outside_the_cache(backend, device):
         assert changed.nonzero().tolist() == [[1, 15]]
 
 
+def test_rows_that_share_a_slot(backend, device):
+    """Codes and scales of any of the rows stay there, and nothing else is touched."""
+    d, hk, hq, tokens = 96, 2, 3, 300
+    x = rows(tokens, hq + 2 * hk, d, torch.float16, 30)
+    on = x.reshape(tokens, -1).to(device)
+    cache = backend.create_kv_cache(pages=2, page_tokens=16, kv_heads=hk, head_dim=d, dtype=torch.float16, device=device)
+    before = [t.clone() for t in cache.storage_tensors]
+    q, k = torch.empty(tokens, hq, d, dtype=torch.float16, device=device), torch.empty(tokens, hk, d, dtype=torch.float16, device=device)
+    slots = torch.full((tokens,), 21)
+    cache.prepare_write(tokens=tokens, q_heads=hq, rotary=None).run(on, None, slots.to(device), q=q, k=k)
+    torch.cuda.synchronize()
+    assert torch.equal(q.cpu(), x[:, :hq]) and torch.equal(k.cpu(), x[:, hq: hq + hk])
+    for (codes, scales), part in zip(planes(cache, slots[:1]), (x[:, hq: hq + hk], x[:, hq + hk:])):
+        want, steps = q8_rule(part)
+        assert (want.unflatten(2, (-1, 8)) == codes.unflatten(2, (-1, 8))).all(3).any(0).all()
+        assert (steps == scales).any(0).all()
+    for old, new in zip(before, cache.storage_tensors):
+        old, new = (t if t.dtype == torch.uint8 else t.transpose(2, 3) for t in (old, new))
+        assert (old != new).flatten(3).any(3).any(1).cpu().nonzero().tolist() == [[1, 5]]
+
+
 @pytest.mark.parametrize("dtype,large", [(torch.float16, 65504.0), (torch.bfloat16, 1e38)], ids=["fp16", "bf16"])
 def test_groups_that_hold_no_number(backend, device, dtype, large):
     d = 128

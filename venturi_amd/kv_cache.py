@@ -165,8 +165,9 @@ class KVWritePlan:
         keys to ``k`` [tokens, kv_heads, head_dim] where one is given.
 
         ``positions`` (int64 [tokens]; unused without rotary, may then be None) and ``slots`` (int64 [tokens]) stay on
-        the device. A row whose slot lies outside the cache (-1: padding) is not cached. Rows that share a slot leave
-        one of theirs there, unspecified which.
+        the device. A row whose slot lies outside the cache (-1: padding) is not cached. The slots inside it have to
+        differ: rows that share one leave codes and scales of any of them there, not one row's whole. Other slots and
+        ``q`` and ``k`` are not touched by that.
         """
         c, index, tokens = self.cache, self._index, self.tokens
         dtype, device = c.dtype, c.device
