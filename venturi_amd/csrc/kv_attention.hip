@@ -2,9 +2,9 @@
 //
 // Bound by HBM: every code and scale of K and V is read once (272 bytes a token and head at head_dim 128). A wave takes
 // 32 keys at a time out of LDS, into which the next ones' codes and scales are copied beside it without passing registers
-// (in registers they left one wave on a SIMD at head_dim 256: 16 x 5 drafted tokens 74 us, now 36), and keeps weights,
+// (in registers they left one wave on a SIMD at head_dim 256: 16 x 5 drafted tokens 74 us, now 40), and keeps weights,
 // outputs and statistics in registers until the waves of a workgroup join. 4 sequences of 90000 to 131000 keys, 48 heads
-// on 4 of 128: 92 to 99 us, 4.8 to 5.2 TB/s, where a large copy reaches 4.9.
+// on 4 of 128: 98 us a call, 94 of them this kernel's (503 MB read, 5.3 TB/s), where a large copy reaches 4.9.
 //
 // Rows. The query rows of one KV head (query_tokens x group) are the columns of 16-wide matrix tiles, so that a KV
 // head's codes are read once for all heads that share them: up to 16 rows the four waves of a workgroup take other keys, up
@@ -25,8 +25,9 @@
 // For bf16 rows, whose own rounding is eight times as coarse, that is that (error against 64 bits 1.01 to 1.02 times that of the
 // one rounding at the end; with second terms 16 x 5 drafted tokens 45 -> 54 us). For fp16 rows both factors of O = P V have a
 // second term, what the first one's rounding left: the outputs' error against 64 bits at 1021 keys is that of the one
-// rounding at the end (2.1e-4 of their norm) where single terms leave 3.3e-4, for 2 to 5% of the time (64 sequences of 1 to
-// 8190 keys: 45.8 -> 48.1 us).
+// rounding at the end (2.1e-4 of their norm) where single terms leave 3.3e-4, for 1 to 2% of the time (64 sequences of 1 to
+// 8190 keys: 46.4 -> 47.3 us). Weights reach down to 2^-33 of the row's largest (fp16's
+// least number beside 2^8): what a key with less weight adds is lost, at most 2^-33 of its value.
 //
 // Softmax. One pass: weights are 2^(s - m) for a reference m that follows the maximum only when a score passes it by
 // more than 4 (a factor of 16 fits fp16's range): the rescaling of the outputs is rare.
