@@ -1,0 +1,202 @@
+"""Verification of drafts against the definition in 64 bits: the tokens are equal."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def definition(p, q, drafted, count, u):
+    """(tokens, accepted) of one sequence: p [drafts + 1, vocab], q [drafts, vocab] or None."""
+    d, vocab = len(drafted), p.shape[1]
+    p = np.where((p > 0) & np.isfinite(p), p, 0.0).astype(np.float64)
+    tokens, at = [], 0
+    count = min(max(count, 0), d)
+    while at < count:
+        token = int(drafted[at])
+        if not 0 <= token < vocab:
+            break
+        chance = 1.0 if q is None else float(q[at, token])
+        if not float(u[at]) * chance < p[at, token]:
+            break
+        tokens.append(token)
+        at += 1
+    rest = p[at]
+    if at < count:
+        if q is None:
+            left = rest.copy()
+            if 0 <= int(drafted[at]) < vocab:
+                left[int(drafted[at])] = 0.0
+        else:
+            left = rest - q[at].astype(np.float64)
+            left = np.where(left > 0, left, 0.0)
+        if left.sum() > 0:
+            rest = left
+    some = np.flatnonzero(rest > 0)
+    if not len(some):
+        token = -1
+    else:
+        total = np.cumsum(rest)
+        past = np.flatnonzero((rest > 0) & (total > float(u[d]) * total[-1]))
+        token = int(past[0]) if len(past) else int(some[-1])
+    return tokens + [token] + [-1] * (d - at), at
+
+
+def check(backend, device, p, q, drafted, u, counts=None):
+    n, d = drafted.shape
+    vocab = p.shape[-1]
+    print(f"case verification {n} x {d} of {vocab}, {'certain' if q is None else 'drawn'}", flush=True)
+    plan = backend.prepare_verification(sequences=n, drafts=d, vocab=vocab, device=device)
+    tokens = torch.full((n * (d + 1) + 16,), -9, dtype=torch.int64, device=device)
+    accepted = torch.full((n + 16,), -9, dtype=torch.int32, device=device)
+    workspace = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=device)
+    plan.run(p.float().view(n * (d + 1), vocab).to(device), drafted.to(device), u.float().to(device),
+             proposal=None if q is None else q.float().view(n * d, vocab).to(device),
+             counts=None if counts is None else torch.as_tensor(counts, dtype=torch.int32).to(device),
+             tokens=tokens[8: 8 + n * (d + 1)].view(n, d + 1), accepted=accepted[8: 8 + n], workspace=workspace)
+    torch.cuda.synchronize()
+    for t, size in ((tokens, n * (d + 1)), (accepted, n)):
+        assert bool((t[:8] == -9).all()) and bool((t[8 + size:] == -9).all())
+    tokens, accepted = tokens[8: 8 + n * (d + 1)].view(n, d + 1).cpu().tolist(), accepted[8: 8 + n].cpu().tolist()
+    for i in range(n):
+        want, count = definition(p[i].float().numpy(), None if q is None else q[i].float().numpy(), drafted[i].numpy(),
+                                 d if counts is None else int(counts[i]), u[i].float().double().numpy())
+        assert (tokens[i], accepted[i]) == (want, count), i
+    return tokens, accepted
+
+
+def case(n, d, vocab, seed, noise=0.7, certain=False):
+    gen = torch.Generator().manual_seed(seed)
+    logits = 3 * torch.randn(n, d + 1, vocab, generator=gen)
+    other = logits[:, :d] + noise * torch.randn(n, d, vocab, generator=gen)
+    p = torch.softmax(logits, -1)
+    p = torch.where(p < 1e-3 * p.amax(-1, keepdim=True), 0.0, p)
+    p = p / p.sum(-1, keepdim=True)
+    u = torch.rand(n, d + 1, generator=gen)
+    if certain:
+        return p, None, other.argmax(-1), u
+    q = torch.softmax(other, -1)
+    drafted = torch.multinomial(q.view(n * d, vocab), 1, generator=gen).view(n, d)
+    return p, q, drafted, u
+
+
+@pytest.mark.parametrize("certain", [False, True], ids=["drawn", "certain"])
+@pytest.mark.parametrize("n,d,vocab", [(1, 1, 1), (3, 2, 2), (4, 3, 7), (9, 64, 5), (33, 7, 1000), (5, 4, 4095), (5, 4, 4097), (2, 3, 32003),
+                                       (70, 2, 9001), (1, 4, 248320), (2, 5, 151937), (300, 1, 2100), (2100, 1, 300), (1, 1, 2**20)])
+def test_random_drafts(backend, device, certain, n, d, vocab):
+    for noise in (0.3, 1.5):
+        p, q, drafted, u = case(n, d, vocab, n + vocab, noise, certain)
+        check(backend, device, p, q, drafted, u)
+    counts = torch.randint(-1, d + 2, (n,), generator=torch.Generator().manual_seed(1)).tolist()
+    check(backend, device, p, q, drafted, u, counts)
+
+
+def test_all_drafts_stand_and_none_does(backend, device):
+    p, q, drafted, u = case(8, 5, 5001, 3)
+    u[:, :5] = 0.0
+    positive = p[:, :5].gather(2, drafted[..., None])[..., 0] > 0
+    assert check(backend, device, p, q, drafted, u)[1] == positive.long().cumprod(1).sum(1).tolist()
+    u[:, :5] = 1e30
+    assert check(backend, device, p, q, drafted, u)[1] == [0] * 8
+    assert check(backend, device, p, q, drafted, u, [0] * 8)[1] == [0] * 8
+
+
+def test_borders_are_exact(backend, device):
+    """Probabilities in units of 2^-12, whose sums are exact: a draft stands below the border and not at it, and the drawn
+    token changes where the uniform is a running sum."""
+    vocab, d = 4096 + 512, 1
+    gen = torch.Generator().manual_seed(4)
+    p = torch.zeros(64, 2, vocab)
+    for i in range(64):
+        at = torch.randperm(vocab, generator=gen)[:8]
+        p[i, :, at] = torch.tensor([1024, 1024, 512, 512, 512, 256, 128, 128]) / 4096.0
+    drafted = p[:, 0].argmax(-1, keepdim=True)
+    q = torch.full((64, 1, vocab), 0.0)
+    q.scatter_(2, drafted[:, None], 0.5)
+    u = torch.zeros(64, 2)
+    u[:, 0] = torch.tensor([0.5, 0.5 - 2.0**-25] * 32)  # p / q is 0.5 exactly
+    u[:, 1] = torch.arange(64) / 64.0
+    _, accepted = check(backend, device, p, q, drafted, u)
+    assert accepted == [0, 1] * 32
+    check(backend, device, p, None, drafted, u / 2)
+
+
+def test_ends_of_the_uniforms(backend, device):
+    for vocab in (50, 9001):
+        p, q, drafted, u = case(6, 2, vocab, 5)
+        for last in (0.0, 2.0**-30, 1 - 2.0**-24, 1.0, 2.0, -1.0, math.nan, math.inf):
+            u[:, 2] = last
+            check(backend, device, p, q, drafted, u)
+        u[:, :2] = math.nan
+        assert check(backend, device, p, q, drafted, u)[1] == [0] * 6
+
+
+@pytest.mark.parametrize("vocab", [40, 9001])
+def test_rows_that_leave_nothing(backend, device, vocab):
+    """The drafter's row at or above the target's everywhere, empty rows, and values that are no probabilities."""
+    p, q, drafted, u = case(10, 2, vocab, 6)
+    u[:, :2] = 1e30
+    q[0] = p[0, :2]
+    q[1] = 1.0
+    p[2] = 0.0
+    p[3], p[4] = math.nan, -1.0
+    p[5, 0, : vocab // 2] = math.inf
+    q[6] = math.nan
+    p[7, 0] = 0.0
+    p[7, 0, 17] = 1e-45
+    drafted[8, 0], drafted[9, 0] = vocab, -3
+    check(backend, device, p, q, drafted, u)
+    check(backend, device, p, None, drafted, u)
+    p[:, 0] = 0.0
+    p.scatter_(2, drafted.clamp(0, vocab - 1)[..., None], 0.5)  # certain drafts hold the whole mass
+    check(backend, device, p, None, drafted, u)
+
+
+def test_emitted_tokens_are_distributed_as_the_target(backend, device):
+    """Drafts on a grid of the drafter's shares, uniforms on grids: the first token comes as often as its share says."""
+    vocab, steps = 5, 64
+    p = torch.tensor([0.4, 0.1, 0.25, 0.05, 0.2])
+    q = torch.tensor([0.125, 0.25, 0.25, 0.25, 0.125])
+    grid = (torch.arange(steps) + 0.5) / steps
+    drafts = torch.searchsorted(q.cumsum(0), grid)
+    n = steps**3
+    if n > 65535:
+        grid, drafts = grid[::2], drafts[::2]
+        n = len(grid) ** 3
+    d, a, b = (t.flatten() for t in torch.meshgrid(drafts.float(), grid, grid, indexing="ij"))
+    tokens, _ = check(backend, device, p.expand(n, 2, vocab), q.expand(n, 1, vocab), d[:, None].long(), torch.stack([a, b], 1))
+    first = torch.tensor([t[0] for t in tokens])
+    for i in range(vocab):  # a grid of 32 points a side is off by a point at each border
+        assert abs(float((first == i).double().mean()) - float(p[i])) <= 3 / len(grid)
+
+
+def test_graph_and_side_stream(backend, device):
+    for n, d, vocab in ((3, 4, 32003), (40, 2, 500)):
+        plan = backend.prepare_verification(sequences=n, drafts=d, vocab=vocab, device=device)
+        tensors = [t.to(device) for t in case(n, d, vocab, 1)]
+        p, q, drafted, u = tensors
+        p, q = p.view(n * (d + 1), vocab), q.view(n * d, vocab)
+        tokens, accepted = torch.empty(n, d + 1, dtype=torch.int64, device=device), torch.empty(n, dtype=torch.int32, device=device)
+        w = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=device)
+        arguments = dict(proposal=q, tokens=tokens, accepted=accepted, workspace=w)
+        side = torch.cuda.Stream(device)
+        side.wait_stream(torch.cuda.current_stream(device))
+        with torch.cuda.stream(side):
+            plan.run(p, drafted, u, **arguments)
+        torch.cuda.current_stream(device).wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            plan.run(p, drafted, u, **arguments)
+        for i in range(4):
+            for t, new in zip((p, q, drafted, u), case(n, d, vocab, 20 + i)):
+                t.copy_(new.view(t.shape))
+            plan.run(p, drafted, u, **arguments)
+            want = tokens.clone(), accepted.clone()
+            tokens.zero_(), accepted.zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(tokens, want[0]) and torch.equal(accepted, want[1])

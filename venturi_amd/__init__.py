@@ -33,6 +33,7 @@ __all__ = [
     "create_backend",
     "prepare_q8_dp4a",
     "prepare_q8_fused",
+    "prepare_residual_rms",
     "prepare_rms_q8",
     "quantize_q4_rtn",
     "decode_q4_fp16",
@@ -57,6 +58,10 @@ def __getattr__(name):
         from .q8_fused import prepare_q8_fused
 
         return prepare_q8_fused
+    if name == "prepare_residual_rms":
+        from .residual_norm import prepare_residual_rms
+
+        return prepare_residual_rms
     if name == "prepare_rms_q8":
         from .rms_quant import prepare_rms_q8
 

@@ -105,6 +105,10 @@ def _capabilities():
         OperatorSupport("kv_cache", devices, quant),
         OperatorSupport("attention", devices, quant),
         OperatorSupport("sampling", devices, quant),
+        OperatorSupport("residual_rmsnorm", devices, floating),
+        OperatorSupport("routing", devices, floating),
+        OperatorSupport("distribution", devices, quant),
+        OperatorSupport("verification", devices, frozenset((torch.float32,))),
     ]
     return BackendCapabilities("venturi-ops-gfx950", tuple(operators), reference=False, cuda_graphs=True)
 
@@ -346,6 +350,27 @@ class HipBackend(Backend):
         from .sampling import SamplingPlan
 
         return SamplingPlan.create(self, rows=rows, vocab=vocab, dtype=dtype, device=device)
+
+    def prepare_distribution(self, *, rows, vocab, dtype, device):
+        """Plan of the probabilities that sampling's settings leave of rows of logits (sampling.DistributionPlan)."""
+        from .sampling import DistributionPlan
+
+        return DistributionPlan.create(self, rows=rows, vocab=vocab, dtype=dtype, device=device)
+
+    def prepare_verification(self, *, sequences, drafts, vocab, device):
+        """Plan of accepting or refusing drafted tokens by such rows (verification.VerificationPlan)."""
+        from .verification import VerificationPlan
+
+        return VerificationPlan.create(self, sequences=sequences, drafts=drafts, vocab=vocab, device=device)
+
+    def prepare_routing(self, *, tokens, experts, top_k, dtype, device, score="softmax", groups=1, kept_groups=1, group_rank="pairs",
+                        renormalize=True, scale=1.0, score_dtype=torch.float16):
+        """Plan of choosing every token's experts and their weights from router logits (routing.RoutingPlan)."""
+        from .routing import RoutingPlan
+
+        return RoutingPlan.create(self, tokens=tokens, experts=experts, top_k=top_k, dtype=dtype, device=device, score=score,
+                                  groups=groups, kept_groups=kept_groups, group_rank=group_rank, renormalize=renormalize,
+                                  scale=scale, score_dtype=score_dtype)
 
 
 @dataclass(frozen=True)

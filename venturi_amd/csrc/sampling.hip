@@ -31,6 +31,7 @@ namespace {
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kTurns = 64;                 // of 1024 classes, 16 a lane
 constexpr int kMaxVocab = 1 << 20;
+constexpr int kMaxDistributionRows = 65535;  // a launch's second dimension
 constexpr std::uint32_t kHeavy = 16384;
 constexpr int kHeavyEntries = 2 * kMaxVocab / kHeavy;
 constexpr int kNone = -1;                  // no class
@@ -321,8 +322,14 @@ struct Lane {
     }
 };
 
-// Chooses from the workgroup's complete histogram.
-template <class T>
+// log2 e / T, from 4e-39 to 2e45; of a greedy row that of T = 1.
+__device__ __forceinline__ double heat_of(float temperature) {
+    return 1.44269504088896340736 / (temperature > 0.0f ? static_cast<double>(fminf(temperature, 3.402823466e38f)) : 1.0);
+}
+
+// Chooses from the workgroup's complete histogram: the token at the uniform's place, or with LAST the last kept one. The
+// probability that it leaves is the token's, or with LAST the kept mass in units of the largest weight.
+template <class T, bool LAST>
 __device__ Choice choose(Shared& s, const Settings& set) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, heavy = s.heavy;
     for (int turn = wave; turn < kTurns; turn += kWaves) {
@@ -346,9 +353,8 @@ __device__ Choice choose(Shared& s, const Settings& set) {
         return {kNone, 0};
     }
     const bool greedy = !(set.temperature > 0.0f);
-    // log2 e / T, from 4e-39 to 2e45.
     const double max_value = class_value<T>(top), least = set.min_p;
-    const double heat = 1.44269504088896340736 / (greedy ? 1.0 : static_cast<double>(fminf(set.temperature, 3.402823466e38f)));
+    const double heat = heat_of(set.temperature);
     const bool all_above = least <= 0.0;
     int above_min = 0;
     for (int turn = wave; turn < kTurns && !greedy; turn += kWaves) {
@@ -446,15 +452,20 @@ __device__ Choice choose(Shared& s, const Settings& set) {
             const double kept = prefix_mass(length);
             // A uniform of 1 or more stays below the end of the mass: the last token that adds to it.
             const double target = fmin(static_cast<double>(set.uniform) * kept, kept * (1.0 - 0x1p-52));
-            int place = target >= 0.0 && set.uniform >= 0.0f ? tokens_below(target, true) : 0;
-            place = max(min(place, length - 1), 0);
+            int place;
+            if constexpr (LAST) {
+                place = length - 1;
+            } else {
+                place = target >= 0.0 && set.uniform >= 0.0f ? tokens_below(target, true) : 0;
+                place = max(min(place, length - 1), 0);
+            }
             open(count_before <= place);
             int at = before;
             l.each([&](int i, int n, double w) {
                 if (place >= at && place < at + n) {
                     s.place = 1024 * turn + 16 * lane + i;
                     s.rank = place - at;
-                    s.probability = w / kept;
+                    s.probability = LAST ? kept : w / kept;
                 }
                 at += n;
             });
@@ -512,6 +523,14 @@ __device__ __forceinline__ int find_element(const uint4& w, const Pattern& p, in
     return at;
 }
 
+// What a row keeps: classes above `place`, and of its class the tokens up to `index`.
+struct Cut {
+    double max, heat;     // a token's weight is 2^((logit - max) heat)
+    std::int64_t index;
+    float inverse;        // of the kept mass
+    int place;            // kNone: the row keeps nothing
+};
+
 struct Operands {
     const void* logits;
     const float* uniforms;
@@ -521,10 +540,11 @@ struct Operands {
     const float* min_p;
     std::int64_t* tokens;
     float* probabilities;
+    Cut* cuts;  // of the distribution, in place of tokens and uniforms
     int rows, vocab;
 
     __device__ __forceinline__ Settings settings(int row) const {
-        return {temperature ? temperature[row] : 1.0f, top_p ? top_p[row] : 1.0f, min_p ? min_p[row] : 0.0f, uniforms[row],
+        return {temperature ? temperature[row] : 1.0f, top_p ? top_p[row] : 1.0f, min_p ? min_p[row] : 0.0f, uniforms ? uniforms[row] : 0.0f,
                 top_k ? top_k[row] : 0};
     }
 };
@@ -637,8 +657,8 @@ __device__ __forceinline__ int edge_match(const Row& row, const Edge& edge, cons
     return __popcll(all);
 }
 
-// A workgroup per row.
-template <class T>
+// A workgroup per row. CUT: what the row keeps, for distribution(), in place of a token.
+template <class T, bool CUT>
 __global__ __launch_bounds__(kThreads) void sample(Operands o) {
     extern __shared__ __align__(16) unsigned char memory[];
     Shared& s = *reinterpret_cast<Shared*>(memory);
@@ -659,18 +679,32 @@ __global__ __launch_bounds__(kThreads) void sample(Operands o) {
         },
         [&] { sweep(s); });
     __syncthreads();
-    const Choice choice = choose<T>(s, set);
-    if (t == 0 && o.probabilities) o.probabilities[index] = static_cast<float>(s.probability);
-    if (choice.place == kNone) {
-        if (t == 0) o.tokens[index] = -1;
-        return;
+    const Choice choice = choose<T, CUT>(s, set);
+    std::int64_t* token;
+    if constexpr (CUT) {
+        Cut& cut = o.cuts[index];
+        token = &cut.index;
+        if (t == 0) {
+            cut.place = choice.place;
+            cut.max = choice.place == kNone ? 0.0 : class_value<T>(s.top);
+            cut.heat = heat_of(set.temperature);
+            cut.inverse = static_cast<float>(1.0 / s.probability);
+        }
+        if (choice.place == kNone) return;
+    } else {
+        token = o.tokens + index;
+        if (t == 0 && o.probabilities) o.probabilities[index] = static_cast<float>(s.probability);
+        if (choice.place == kNone) {
+            if (t == 0) *token = -1;
+            return;
+        }
     }
     // The rank-th occurrence of the class: in the head, in the vectors or in the tail. (choose() has ended with a barrier:
     // the histogram's memory is free.)
     const Pattern pattern(choice.place);
     int *counts = reinterpret_cast<int*>(s.histogram), *list = counts + kChunks;
     if (wave == 0) {
-        const int n = edge_match(row, edge, pattern, false, choice.rank, o.tokens + index);
+        const int n = edge_match(row, edge, pattern, false, choice.rank, token);
         const int listed = list_chunks(s, row, pattern, list);
         if (t == 0) s.heavy = n, s.top = listed, s.count = 0;
     }
@@ -680,16 +714,69 @@ __global__ __launch_bounds__(kThreads) void sample(Operands o) {
     const int found = count_matches(row, pattern, rank, list, listed, counts, &s.count);
     if (wave != 0) return;
     if (found > rank)
-        write_match(row, pattern, rank, list, listed, counts, o.tokens + index);
+        write_match(row, pattern, rank, list, listed, counts, token);
     else
-        edge_match(row, edge, pattern, true, rank - found, o.tokens + index);
+        edge_match(row, edge, pattern, true, rank - found, token);
 }
 
+// Vectors of 8 logits of a workgroup of distribution().
+constexpr int kWriteThreads = 256, kWriteVectors = 4 * kWriteThreads;
+
+// The probability of a logit that is the row's token `index`.
 template <class T>
+__device__ __forceinline__ float probability(const Cut& cut, std::uint32_t last, std::uint32_t bits, int index) {
+    const float x = to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(bits)));
+    // Classes by value; the class of 0 holds both zeros.
+    const float border = to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(last)));
+    if (!(x > border || (x == border && index <= cut.index))) return 0.0f;  // NaN too
+    const double value = x;
+    if (value == cut.max) return cut.inverse;
+    // The exponent in two 32-bit parts, so that the weight errs by the exponential's own rounding alone.
+    const double exponent = (value - cut.max) * cut.heat;
+    const float high = static_cast<float>(exponent), low = static_cast<float>(exponent - static_cast<double>(high));
+    if (!(high > -150.0f)) return 0.0f;
+    const float w = __builtin_amdgcn_exp2f(high);
+    return fmaf(w, low * 0.693147181f, w) * cut.inverse;
+}
+
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// Writes a row's probabilities from its cut: a workgroup for kWriteVectors vectors, the row's ragged ends with the first.
+template <class T>
+__global__ __launch_bounds__(kWriteThreads) void distribution(Operands o) {
+    const int index = blockIdx.y;
+    const Row row(o.logits, index, o.vocab);
+    const Cut cut = o.cuts[index];
+    const bool some = cut.place != kNone;
+    const std::uint32_t last = place_bits(some ? cut.place : 0);
+    float* out = o.probabilities + static_cast<std::int64_t>(index) * o.vocab;
+    if (blockIdx.x == 0 && static_cast<int>(threadIdx.x) < row.head + row.tail) {
+        const int at = row.edge(threadIdx.x);
+        out[at] = some ? probability<T>(cut, last, row.start[at], at) : 0.0f;
+    }
+    for (int i = blockIdx.x * kWriteVectors + threadIdx.x; i < min(row.vectors, static_cast<int>(blockIdx.x + 1) * kWriteVectors);
+         i += kWriteThreads) {
+        const uint4 w = row.whole()[i];
+        const int first = row.head + 8 * i;
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = some ? probability<T>(cut, last, element(w, j), first + j) : 0.0f;
+        // Rows of odd vocabularies start at any multiple of 4 bytes.
+        *reinterpret_cast<float4u*>(out + first) = float4u{p[0], p[1], p[2], p[3]};
+        *reinterpret_cast<float4u*>(out + first + 4) = float4u{p[4], p[5], p[6], p[7]};
+    }
+}
+
+template <class T, bool CUT>
 void launch(const Operands& o, hipStream_t stream) {
     static LdsLimit limit;
-    limit.raise(sample<T>, sizeof(Shared));
-    sample<T><<<o.rows, kThreads, sizeof(Shared), stream>>>(o);
+    limit.raise(sample<T, CUT>, sizeof(Shared));
+    sample<T, CUT><<<o.rows, kThreads, sizeof(Shared), stream>>>(o);
+    if constexpr (CUT) {
+        check(hipGetLastError());
+        const unsigned parts = std::max((o.vocab / 8 + kWriteVectors - 1) / kWriteVectors, 1);
+        distribution<T><<<dim3(parts, o.rows), kWriteThreads, 0, stream>>>(o);
+    }
 }
 
 void require_geometry(int rows, int vocab) {
@@ -710,12 +797,44 @@ VT_EXPORT int venturi_sample_run(const void* logits, const float* uniforms, cons
         vt::require(logits && uniforms && tokens, "null sampling operand");
         vt::require(vt::aligned(logits, 16), "logits must be 16-byte aligned");
         const auto s = static_cast<hipStream_t>(stream);
-        const vt::Operands o{logits, uniforms, temperature, top_k, top_p, min_p, tokens, probabilities, rows, vocab};
+        const vt::Operands o{logits, uniforms, temperature, top_k, top_p, min_p, tokens, probabilities, nullptr, rows, vocab};
         if (dtype == vt::kF16)
-            vt::launch<__half>(o, s);
+            vt::launch<__half, false>(o, s);
         else if (dtype == vt::kBF16)
-            vt::launch<__hip_bfloat16>(o, s);
+            vt::launch<__hip_bfloat16, false>(o, s);
         else
             throw vt::Invalid("sampling takes fp16 or bf16 logits");
+    });
+}
+
+VT_EXPORT std::uint64_t venturi_distribution_bytes(int rows, int vocab) {
+    std::uint64_t bytes = 0;
+    vt::host_guarded([&] {
+        vt::require_geometry(rows, vocab);
+        vt::require(rows <= vt::kMaxDistributionRows, "a distribution takes at most 65535 rows");
+        bytes = sizeof(vt::Cut) * static_cast<std::uint64_t>(rows);
+    });
+    return bytes;
+}
+
+VT_EXPORT int venturi_distribution_run(const void* logits, const float* temperature, const std::int32_t* top_k, const float* top_p,
+                                       const float* min_p, float* probabilities, void* workspace, std::uint64_t available,
+                                       int rows, int vocab, int dtype, void* stream) {
+    return vt::guarded([&] {
+        vt::require_geometry(rows, vocab);
+        vt::require(rows <= vt::kMaxDistributionRows, "a distribution takes at most 65535 rows");
+        vt::require(logits && probabilities, "null distribution operand");
+        vt::require(vt::aligned(logits, 16) && vt::aligned(probabilities, 4), "logits must be 16-byte aligned");
+        vt::require(workspace && available >= sizeof(vt::Cut) * static_cast<std::uint64_t>(rows) && vt::aligned(workspace, 256),
+                    "a distribution needs its workspace, 256-byte aligned");
+        const auto s = static_cast<hipStream_t>(stream);
+        const vt::Operands o{logits, nullptr, temperature, top_k, top_p, min_p, nullptr, probabilities,
+                             static_cast<vt::Cut*>(workspace), rows, vocab};
+        if (dtype == vt::kF16)
+            vt::launch<__half, true>(o, s);
+        else if (dtype == vt::kBF16)
+            vt::launch<__hip_bfloat16, true>(o, s);
+        else
+            throw vt::Invalid("a distribution takes fp16 or bf16 logits");
     });
 }

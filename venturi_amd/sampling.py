@@ -1,4 +1,4 @@
-"""Sampling one token per row of logits from given random numbers.
+"""Sampling one token per row of logits from given random numbers, and the distributions that it samples from.
 
 A row's tokens are ordered by logit, largest first, equal logits by index. With weights w = exp((x - max) / temperature)
 the kept tokens are the longest prefix of that order in which every token
@@ -23,6 +23,7 @@ from .kv_cache import settle
 from .operands import DTYPE_CODES, address, apart, device_index, extents
 
 _MAX_VOCAB = 1 << 20
+_MAX_DISTRIBUTION_ROWS = 65535
 _SETTINGS = (("temperature", torch.float32), ("top_k", torch.int32), ("top_p", torch.float32), ("min_p", torch.float32))
 
 
@@ -73,3 +74,52 @@ class SamplingPlan:
             apart(p, size, (t, t + 2 * size), *inputs)
         self._backend._call(self._entry, device, (x, u, *settings, t, p, *self._tail))
         return tokens
+
+
+@dataclass(frozen=True)
+class DistributionPlan:
+    """``HipBackend.prepare_distribution``: the probabilities that sampling with the same settings draws from. The workspace is
+    the caller's: runs that share none may overlap."""
+
+    _backend: object
+    rows: int
+    vocab: int
+    dtype: torch.dtype
+    device: torch.device
+    workspace_bytes: int
+    storage_tensors = ()
+
+    def __post_init__(self):
+        settle(self, _entry=self._backend._native.venturi_distribution_run, _index=device_index(self.device),
+               _logits=(self.rows, self.vocab), _row=(self.rows,),
+               _tail=(self.workspace_bytes, self.rows, self.vocab, DTYPE_CODES[self.dtype]))
+
+    @classmethod
+    def create(cls, backend, *, rows, vocab, dtype, device):
+        extents(rows, vocab)
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("A distribution takes FP16/BF16 logits")
+        if vocab > _MAX_VOCAB or rows > _MAX_DISTRIBUTION_ROWS:
+            raise ValueError(f"A distribution takes at most {_MAX_DISTRIBUTION_ROWS} rows of a vocabulary of at most {_MAX_VOCAB}")
+        target = backend.validate_device(dtype, device)
+        return cls(backend, rows, vocab, dtype, target, int(backend._native.venturi_distribution_bytes(rows, vocab)))
+
+    def run(self, logits, temperature=None, top_k=None, top_p=None, min_p=None, *, probabilities, workspace):
+        """``logits`` [rows, vocab]; settings as ``SamplingPlan.run`` takes them. Writes ``probabilities`` fp32 [rows, vocab]:
+        the kept tokens' weights over their sum, 0 for the others, and for all of a row that has nothing to take."""
+        device, index, row, size = self.device, self._index, self._row, 4 * self.rows
+        x = address(logits, self._logits, self.dtype, device, index, "logits")
+        inputs = [(x, x + 2 * self.rows * self.vocab)]
+        settings = []
+        for (name, dtype), value in zip(_SETTINGS, (temperature, top_k, top_p, min_p)):
+            pointer = None
+            if value is not None:
+                pointer = address(value, row, dtype, device, index, name, 4)
+                inputs.append((pointer, pointer + size))
+            settings.append(pointer)
+        w = address(workspace, (self.workspace_bytes,), torch.uint8, device, index, "workspace", 256)
+        apart(w, self.workspace_bytes, *inputs)
+        p = address(probabilities, self._logits, torch.float32, device, index, "probabilities", 4)
+        apart(p, size * self.vocab, (w, w + self.workspace_bytes), *inputs)
+        self._backend._call(self._entry, device, (x, *settings, p, w, *self._tail))
+        return probabilities
