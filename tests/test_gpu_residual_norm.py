@@ -109,7 +109,7 @@ def test_bytes_of_the_int8_form(backend, device, passes, k):
 @pytest.mark.parametrize("dtype,tokens,k,shift,passes", [
     (FP16, 3, 5120, 1, 0), (FP16, 3, 5120, 4, 0), (FP16, 700, 2048, 2, 2), (BF16, 700, 4100, 4, 0), (FP32, 3, 1024, 1, 0),
     (FP16, 2, 30720, 0, 1), (FP16, 2, 30728, 0, 2), (BF16, 2, 65544, 0, 0), (FP32, 2, 15368, 0, 0), (FP32, 600, 4096, 0, 0),
-    (FP16, 66000, 40, 0, 1), (BF16, 70000, 520, 0, 0)])
+    (FP16, 66000, 40, 0, 1), (BF16, 70000, 520, 0, 0), (FP16, 2050, 512, 0, 2), (FP16, 2049, 1020, 0, 1), (BF16, 300, 2051, 8, 0)])
 def test_alignments_long_rows_and_many_rows(backend, device, dtype, tokens, k, shift, passes):
     print(f"case residual norm {dtype} {tokens} x {k} shift {shift} passes {passes}", flush=True)
     norm, _ = norm_of(backend, device, k, dtype)

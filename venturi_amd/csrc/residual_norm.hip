@@ -8,6 +8,7 @@
 #include "a8_group.hpp"
 
 #include <cmath>
+#include <type_traits>
 
 namespace vt {
 
@@ -16,6 +17,7 @@ std::uint64_t a8_bytes(int tokens, int k, int passes);
 namespace {
 
 constexpr int kChains = 256;
+constexpr int kStaged = 60 * 1024;  // bytes of a row in LDS
 
 // x, residual and total may be the same memory: a thread reads an element before it writes it.
 struct Operands {
@@ -83,9 +85,221 @@ __global__ __launch_bounds__(kChains) void residual_rms_any(Operands o) {
     for (int col = tid; col < k; col += kChains) out[col] = from_f32<T>((to_f32(total[col]) * inv) * o.gamma[col]);
 }
 
+// Four 16-bit values as f32.
+template <class T>
+__device__ __forceinline__ void unpack4(const uint2& w, float (&v)[4]) {
+    const unsigned short h[4] = {static_cast<unsigned short>(w.x), static_cast<unsigned short>(w.x >> 16),
+                                 static_cast<unsigned short>(w.y), static_cast<unsigned short>(w.y >> 16)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = to_f32(__builtin_bit_cast(T, h[i]));
+}
+template <class T>
+__device__ __forceinline__ uint2 pack4(const T (&v)[4]) {
+    uint2 w;
+    __builtin_memcpy(&w, v, sizeof(w));
+    return w;
+}
+
+// A wave per row of 16-bit values that stays in registers: P pieces of 256 columns, four neighbouring ones a lane, which are
+// chains 4 lane .. 4 lane + 3, so that no value leaves its lane before the tree.
+template <class T, int P>
+__global__ __launch_bounds__(256) void residual_rms_wave(Operands o) {
+    const int lane = threadIdx.x & 63, k = o.k;
+    const int token = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (token >= o.tokens) return;
+    const std::int64_t row = static_cast<std::int64_t>(token) * k;
+    const T* x = static_cast<const T*>(o.x) + row;
+    const T* residual = static_cast<const T*>(o.residual) + row;
+    T* total = static_cast<T*>(o.total) + row;
+    uint2 h[P], r[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        const int col = min(256 * j + 4 * lane, k - 4);
+        h[j] = *reinterpret_cast<const uint2*>(x + col);
+        r[j] = *reinterpret_cast<const uint2*>(residual + col);
+    }
+    float chain[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        const int col = 256 * j + 4 * lane;
+        float a[4], b[4];
+        unpack4<T>(h[j], a);
+        unpack4<T>(r[j], b);
+        T sum[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) sum[v] = from_f32<T>(__fadd_rn(a[v], b[v]));
+        h[j] = pack4(sum);
+        if (col >= k) h[j] = make_uint2(0, 0);  // adds nothing to a chain
+        else *reinterpret_cast<uint2*>(total + col) = h[j];
+        unpack4<T>(h[j], a);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) chain[v] = fmaf(a[v], a[v], chain[v]);
+    }
+    const float inv = inverse_rms(__shfl(canonical_sum(chain[0], chain[1], chain[2], chain[3]), 0, 64), k, o.epsilon);
+    T* out = o.out ? static_cast<T*>(o.out) + row : nullptr;
+    const std::int64_t count = static_cast<std::int64_t>(o.tokens) * o.groups;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        const int col = 256 * j + 4 * lane;
+        const float4 g = *reinterpret_cast<const float4*>(o.gamma + min(col, k - 4));
+        float a[4];
+        unpack4<T>(h[j], a);
+        const T y[4] = {from_f32<T>((a[0] * inv) * g.x), from_f32<T>((a[1] * inv) * g.y), from_f32<T>((a[2] * inv) * g.z),
+                        from_f32<T>((a[3] * inv) * g.w)};
+        if (out && col < k) *reinterpret_cast<uint2*>(out + col) = pack4(y);
+        if (o.passes) {
+            float q[4];
+            bool bad = false;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                q[v] = col < k ? to_f32(y[v]) : 0.0f;
+                bad |= !isfinite(q[v]);
+            }
+            const std::int64_t index = static_cast<std::int64_t>(token) * o.groups + (col >> 5);
+            if ((col >> 5) < o.groups)  // the 8 lanes of a group share it
+                quantize_group<4, 8>(q, bad, o.passes, o.codes + index * 32 + (col & 31), o.scales + index, count * 32, count,
+                                     (lane & 7) == 0);
+        }
+    }
+}
+
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// A workgroup per row that it stages in LDS: the row comes in one round of loads, and all threads share its columns but for
+// the chains. The tensors start at multiples of 16 bytes, and with ROUND so do the rows; else a row's first and last vector
+// are partial, and its LDS copy starts as far into a vector as the row does.
+template <class T, int THREADS, bool ROUND>
+__global__ __launch_bounds__(THREADS) void residual_rms_staged(Operands o) {
+    constexpr int V = 16 / sizeof(T);
+    extern __shared__ uint4 staged[];
+    __shared__ __align__(16) float chains[kChains];
+    const int tid = threadIdx.x, lane = tid & 63, k = o.k;
+    const std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * k;
+    const int shift = ROUND ? 0 : static_cast<int>(row % V), pieces = (k + shift + V - 1) / V;
+    auto* held = reinterpret_cast<T*>(staged) + shift;
+    const T* x = static_cast<const T*>(o.x) + row;
+    const T* residual = static_cast<const T*>(o.residual) + row;
+    T* total = static_cast<T*>(o.total) + row;
+    for (int p = tid; p < pieces; p += THREADS) {
+        const int first = V * p - shift;
+        if (ROUND || (first >= 0 && first + V <= k)) {
+            const uint4 a = *reinterpret_cast<const uint4*>(x + first), b = *reinterpret_cast<const uint4*>(residual + first);
+            T u[V], v[V];
+            __builtin_memcpy(u, &a, sizeof(a));
+            __builtin_memcpy(v, &b, sizeof(b));
+#pragma unroll
+            for (int i = 0; i < V; ++i) u[i] = from_f32<T>(__fadd_rn(to_f32(u[i]), to_f32(v[i])));
+            uint4 h;
+            __builtin_memcpy(&h, u, sizeof(h));
+            *reinterpret_cast<uint4*>(total + first) = h;
+            staged[p] = h;
+        } else {
+            for (int col = max(first, 0); col < min(first + V, k); ++col) {
+                const T h = from_f32<T>(__fadd_rn(to_f32(x[col]), to_f32(residual[col])));
+                total[col] = h;
+                held[col] = h;
+            }
+        }
+    }
+    __syncthreads();
+    if (THREADS == kChains || tid < kChains) {
+        float chain = 0.0f;
+#pragma unroll 8
+        for (int col = tid; col < k; col += kChains) chain = fmaf(to_f32(held[col]), to_f32(held[col]), chain);
+        chains[tid] = chain;
+    }
+    __syncthreads();
+    const float4 c = *reinterpret_cast<const float4*>(chains + 4 * lane);
+    const float inv = inverse_rms(__shfl(canonical_sum(c.x, c.y, c.z, c.w), 0, 64), k, o.epsilon);
+    T* out = o.out ? static_cast<T*>(o.out) + row : nullptr;
+    if constexpr (sizeof(T) == 2) {
+        if (o.passes) {
+            const std::int64_t count = static_cast<std::int64_t>(o.tokens) * o.groups;
+            for (int col = 4 * tid; col < 32 * o.groups; col += 4 * THREADS) {
+                float q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                bool bad = false;
+                if (ROUND && col < k) {
+                    const float4 g = *reinterpret_cast<const float4*>(o.gamma + col);
+                    unpack4<T>(*reinterpret_cast<const uint2*>(held + col), q);
+                    const T y[4] = {from_f32<T>((q[0] * inv) * g.x), from_f32<T>((q[1] * inv) * g.y), from_f32<T>((q[2] * inv) * g.z),
+                                    from_f32<T>((q[3] * inv) * g.w)};
+                    if (out) *reinterpret_cast<uint2*>(out + col) = pack4(y);
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) q[v] = to_f32(y[v]);
+                } else if (!ROUND) {
+#pragma unroll
+                    for (int v = 0; v < 4; ++v)
+                        if (col + v < k) {
+                            const T y = from_f32<T>((to_f32(held[col + v]) * inv) * o.gamma[col + v]);
+                            if (out) out[col + v] = y;
+                            q[v] = to_f32(y);
+                        }
+                }
+#pragma unroll
+                for (int v = 0; v < 4; ++v) bad |= !isfinite(q[v]);
+                const std::int64_t index = static_cast<std::int64_t>(blockIdx.x) * o.groups + (col >> 5);
+                quantize_group<4, 8>(q, bad, o.passes, o.codes + index * 32 + (col & 31), o.scales + index, count * 32, count,
+                                     (lane & 7) == 0);  // the 8 lanes of a group share it
+            }
+            return;
+        }
+    }
+    for (int p = tid; p < pieces; p += THREADS) {
+        const int first = V * p - shift;
+        if (ROUND || (first >= 0 && first + V <= k)) {
+            const uint4 h = staged[p];
+            T u[V];
+            __builtin_memcpy(u, &h, sizeof(h));
+#pragma unroll
+            for (int i = 0; i < V; i += 4) {
+                const float4u g = *reinterpret_cast<const float4u*>(o.gamma + first + i);
+                u[i] = from_f32<T>((to_f32(u[i]) * inv) * g[0]);
+                u[i + 1] = from_f32<T>((to_f32(u[i + 1]) * inv) * g[1]);
+                u[i + 2] = from_f32<T>((to_f32(u[i + 2]) * inv) * g[2]);
+                u[i + 3] = from_f32<T>((to_f32(u[i + 3]) * inv) * g[3]);
+            }
+            uint4 y;
+            __builtin_memcpy(&y, u, sizeof(y));
+            *reinterpret_cast<uint4*>(out + first) = y;
+        } else {
+            for (int col = max(first, 0); col < min(first + V, k); ++col) out[col] = from_f32<T>((to_f32(held[col]) * inv) * o.gamma[col]);
+        }
+    }
+}
+
 template <class T>
 void launch(const Operands& o, hipStream_t stream) {
-    residual_rms_any<T><<<o.tokens, kChains, 0, stream>>>(o);
+    if constexpr (sizeof(T) == 2) {
+        // Short rows leave most of a workgroup idle (us, wave against workgroup, fp16 without codes / with two passes: 512
+        // tokens of 256 2.6 / 3.5 against 2.9 / 3.6; 2048 of 1024 5.5 / 9.5 against 6.2 / 9.3; 60000 of 1024 88 / 123 against
+        // 96 / 142, of 512 46 / 66 against 67 / 93; but 512 of 1024 3.6 / 6.8 against 3.4 / 4.3).
+        const bool wave = o.k <= 256 || (o.k <= 1024 && o.tokens >= 2048);
+        if (wave && o.k % 4 == 0 && aligned(o.x, 8) && aligned(o.residual, 8) && aligned(o.total, 8) && aligned(o.out, 8) &&
+            aligned(o.gamma, 16)) {
+            const auto grid = static_cast<unsigned>((static_cast<std::int64_t>(o.tokens) + 3) / 4);
+            if (o.k <= 256) residual_rms_wave<T, 1><<<grid, 256, 0, stream>>>(o);
+            else if (o.k <= 512) residual_rms_wave<T, 2><<<grid, 256, 0, stream>>>(o);
+            else residual_rms_wave<T, 4><<<grid, 256, 0, stream>>>(o);
+            return;
+        }
+    }
+    // Few rows are as fast as a row's threads are many; many rows as the CU is full (us, 1024 / 512 / 256 threads, fp16 without
+    // codes: 61 tokens of 5120 3.9 / 4.1 / 4.8; 600 9.0 / 8.1 / 7.8; 2048 17.3 / 15.9 / 15.2; 8190 66 / 63 / 65; with two
+    // passes 61: 5.2 / 6.3 / 8.5; 600: 12.6 / 12.6 / 13.1; 8190: 101 / 90 / 91).
+    const std::int64_t bytes = static_cast<std::int64_t>(o.k) * sizeof(T);
+    if (bytes > kStaged || !(aligned(o.x, 16) && aligned(o.residual, 16) && aligned(o.total, 16) && aligned(o.out, 16) && aligned(o.gamma, 16))) {
+        residual_rms_any<T><<<o.tokens, kChains, 0, stream>>>(o);
+        return;
+    }
+    const auto staged = [&](auto round) {
+        constexpr bool R = decltype(round)::value;
+        const auto lds = static_cast<std::size_t>(bytes + 31) / 16 * 16;  // and what comes before the row in its first vector
+        if (o.k > 2048 && o.tokens <= 256) residual_rms_staged<T, 1024, R><<<o.tokens, 1024, lds, stream>>>(o);
+        else if (o.k > 2048) residual_rms_staged<T, 512, R><<<o.tokens, 512, lds, stream>>>(o);
+        else residual_rms_staged<T, kChains, R><<<o.tokens, kChains, lds, stream>>>(o);
+    };
+    if (bytes % 16 == 0) staged(std::true_type{});
+    else staged(std::false_type{});
 }
 
 bool meet(const void* a, std::uint64_t a_bytes, const void* b, std::uint64_t b_bytes) {
