@@ -1,5 +1,6 @@
 """Routing against the definition in 64 bits: experts equal and in order, weights to one rounding."""
 
+from itertools import combinations
 import math
 
 import pytest
@@ -14,8 +15,15 @@ FP16, BF16, FP32 = torch.float16, torch.bfloat16, torch.float32
 NAMES = {FP16: "fp16", BF16: "bf16", FP32: "fp32"}
 
 
-def definition(logits, bias, top_k, *, score="softmax", groups=1, kept_groups=1, group_rank="pairs", renormalize=True, scale=1.0):
+def definition(logits, bias, top_k, **settings):
     """(ids, weights) of one row, expert by expert."""
+    return next(definitions(logits, bias, top_k, **settings))
+
+
+def definitions(logits, bias, top_k, *, score="softmax", groups=1, kept_groups=1, group_rank="pairs", renormalize=True, scale=1.0):
+    """The definition's (ids, weights), and with a bias those of groups that come as near as 64 bits tell sums apart: a score
+    errs by 2^-53 of it for every expert in its sum, the exponentials, the division and the bias's addition, twice in a rank
+    of two."""
     x = [float(v) for v in logits.double()]
     broken = any(math.isnan(v) for v in x) or (score == "softmax" and math.inf in x)
     if not broken:
@@ -28,18 +36,24 @@ def definition(logits, bias, top_k, *, score="softmax", groups=1, kept_groups=1,
         c = [-math.inf if v == -math.inf else t + (0.0 if bias is None else float(bias[i])) for i, (v, t) in enumerate(zip(x, s))]
         broken = any(math.isnan(v) for v in c)
     if broken:
-        return [-1] * top_k, [math.nan] * top_k
+        yield [-1] * top_k, [math.nan] * top_k
+        return
     size = len(x) // groups
     ranks = []
     for g in range(groups):
         best = sorted(c[g * size: (g + 1) * size], reverse=True)
         ranks.append(best[0] + best[1] if group_rank == "pairs" and size > 1 else best[0])
-    kept = sorted(range(groups), key=lambda g: (-ranks[g], g))[:kept_groups]
-    order = sorted((e for e in range(len(x)) if e // size in kept), key=lambda e: (-c[e], e))[:top_k]
-    w = [s[e] for e in order]
-    if renormalize:
-        w = [v / sum(w) if sum(w) else 0.0 for v in w]
-    return order, [v * scale for v in w]
+    first = sorted(range(groups), key=lambda g: (-ranks[g], g))[:kept_groups]
+    others = combinations(range(groups), kept_groups) if bias is not None and 1 < groups <= 8 else ()
+    for kept in (first, *others):
+        out = [ranks[g] for g in range(groups) if g not in kept]
+        if out and min(ranks[g] for g in kept) < max(out) - (len(x) + 6) * 2.0**-52 * (1 + abs(max(out))):
+            continue
+        order = sorted((e for e in range(len(x)) if e // size in kept), key=lambda e: (-c[e], e))[:top_k]
+        w = [s[e] for e in order]
+        if renormalize:
+            w = [v / sum(w) if sum(w) else 0.0 for v in w]
+        yield order, [v * scale for v in w]
 
 
 def check(backend, device, logits, bias=None, top_k=1, score_dtype=FP16, **settings):
@@ -61,6 +75,9 @@ def check(backend, device, logits, bias=None, top_k=1, score_dtype=FP16, **setti
     least = {FP16: 2.0**-25, BF16: 2.0**-134, FP32: 2.0**-126}[score_dtype]
     for i in range(tokens):
         want, share = definition(logits[i], bias, top_k, **settings)
+        if got[i].tolist() != want:
+            near = (d for d in definitions(logits[i], bias, top_k, **settings) if d[0] == got[i].tolist())
+            want, share = next(near, (want, share))
         assert got[i].tolist() == want, (i, got[i].tolist(), want)
         for a, b in zip(weights[i].tolist(), share):
             assert (math.isnan(a) and math.isnan(b)) or abs(a - b) <= step * abs(b) * 1.01 + least, (i, a, b)

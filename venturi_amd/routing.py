@@ -7,7 +7,8 @@ chosen. Their weights are s without the bias, divided by their sum with ``renorm
 
 An expert whose logit is -inf is masked: it comes after all others, with weight 0, whatever its bias. Weights whose sum is 0
 stay 0. A token with a NaN among its logits or biased scores, or with +inf under softmax, gets ids -1 and NaN scores, which
-the experts' plan turns into a NaN row. Scores are computed in 64 bits, so that the order is the definition's.
+the experts' plan turns into a NaN row. Scores are computed in 64 bits, so that the order is the definition's: experts go by
+index where 64 bits do not tell them apart (without a bias, where their logits are equal).
 
 The reference's routed experts take ids and scores (flash_next_moe.py:139-161); this operator is an extension.
 """
