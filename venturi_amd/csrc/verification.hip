@@ -9,13 +9,19 @@
 // workgroup of a second launch finds the part and goes through it again.
 #include "common.hpp"
 
-#include <climits>
-
 namespace vt {
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kSumThreads = 256, kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kMaxDrafts = 64, kMaxParts = 64, kMaxVocab = 1 << 20, kMaxSequences = 65535;
+
+// What a sequence's drafts came to.
+struct Verdict {
+    int accepted;
+    int refused;  // the next token comes from what is left of the target's row
+    int without;  // a refused certain draft, or -1
+    int unused;
+};
 
 struct Operands {
     const float* target;          // [sequences][drafts + 1][vocab]
@@ -25,160 +31,211 @@ struct Operands {
     const float* uniforms;        // [sequences][drafts + 1]
     std::int64_t* tokens;         // [sequences][drafts + 1]
     std::int32_t* accepted;       // [sequences]
+    Verdict* verdicts;            // [sequences], where rows are summed in parts
     double2* sums;                // [sequences][parts]: of the remainder, and of the target's row
     int drafts, vocab, parts, slice;
 };
+
+// What is no positive finite number is 0.
+__device__ __forceinline__ float positive(float p) { return p > 0.0f && p <= 3.402823466e38f ? p : 0.0f; }
+
+// For a whole wave. What the drafts are looked up by comes in one round of loads, their probabilities in a second.
+__device__ __forceinline__ Verdict verdict_of(const Operands& o, int sequence) {
+    const int lane = threadIdx.x & 63, draft = min(lane, o.drafts - 1);
+    const std::int64_t first = static_cast<std::int64_t>(sequence) * o.drafts;  // of the sequence's drafts
+    const std::int32_t* counts = o.counts ? o.counts + sequence : nullptr;
+    const std::int64_t id = o.drafted[first + draft];
+    const double u = o.uniforms[first + sequence + draft];
+    const int count = counts ? min(max(*counts, 0), o.drafts) : o.drafts;
+    const bool there = id >= 0 && id < o.vocab;
+    const int token = there ? static_cast<int>(id) : -1;
+    const std::int64_t at = there ? id : 0;
+    const double p = positive(o.target[(first + sequence + draft) * o.vocab + at]);
+    const double q = o.proposal ? o.proposal[(first + draft) * o.vocab + at] : 1.0;
+    const unsigned long long bad = __ballot(lane < count && !(there && u * q < p));
+    const int accepted = bad ? __ffsll(bad) - 1 : count;
+    return {accepted, bad != 0, bad && !o.proposal ? __shfl(token, accepted, 64) : -1, 0};
+}
+
+// Rows start at any multiple of 4 bytes.
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 
 // The row that a sequence's last token comes from.
 struct Draw {
     const float* p;
     const float* q;  // null: nothing is taken off
-    int without;     // a refused certain draft, or -1
-    int accepted;
+    int without, vocab;
+
+    __device__ __forceinline__ Draw(const Operands& o, const Verdict& v, int sequence) : without(v.without), vocab(o.vocab) {
+        const std::int64_t first = static_cast<std::int64_t>(sequence) * o.drafts;
+        p = o.target + (first + sequence + v.accepted) * o.vocab;
+        q = v.refused && o.proposal ? o.proposal + (first + v.accepted) * o.vocab : nullptr;
+    }
+    // Where four tokens from `at` on are loaded from: the last four of the row may come in their place.
+    __device__ __forceinline__ int place(int at) const { return max(min(at, vocab - 4), 0); }
+    __device__ __forceinline__ float4u load(const float* row, int at) const {
+        if (vocab >= 4) return *reinterpret_cast<const float4u*>(row + at);
+        return float4u{row[0], row[min(1, vocab - 1)], row[min(2, vocab - 1)], 0.0f};
+    }
+    // Shares of the loaded tokens in the remainder (x) and in the target's row (y), of those from `at` up to `end`.
+    __device__ __forceinline__ double2 share(const float4u& pv, const float4u& qv, int j, int at, int end) const {
+        const int index = place(at) + j;
+        double2 s;
+        s.y = index >= at && index < end ? static_cast<double>(positive(pv[j])) : 0.0;
+        s.x = q ? fmax(s.y - static_cast<double>(qv[j]), 0.0) : index == without ? 0.0 : s.y;
+        if (!(s.y > 0.0)) s.x = 0.0;  // of a proposal below 0, too
+        return s;
+    }
 };
 
-// What is no positive finite number is 0.
-__device__ __forceinline__ double positive(float p) { return p > 0.0f && p <= 3.402823466e38f ? static_cast<double>(p) : 0.0; }
-
-// For a whole wave.
-__device__ __forceinline__ Draw draw_of(const Operands& o, int sequence) {
-    const int lane = threadIdx.x & 63;
-    const int count = o.counts ? min(max(o.counts[sequence], 0), o.drafts) : o.drafts;
-    const std::int64_t first = static_cast<std::int64_t>(sequence) * o.drafts;  // of the sequence's drafts
-    bool refused = false;
-    int token = -1;
-    if (lane < count) {
-        const std::int64_t id = o.drafted[first + lane];
-        refused = true;
-        if (id >= 0 && id < o.vocab) {
-            token = static_cast<int>(id);
-            const double p = positive(o.target[(first + sequence + lane) * o.vocab + id]);
-            const double q = o.proposal ? o.proposal[(first + lane) * o.vocab + id] : 1.0;
-            refused = !(o.uniforms[first + sequence + lane] * q < p);
-        }
-    }
-    const unsigned long long bad = __ballot(refused);
-    Draw d;
-    d.accepted = bad ? __ffsll(bad) - 1 : count;
-    d.p = o.target + (first + sequence + d.accepted) * o.vocab;
-    d.q = bad && o.proposal ? o.proposal + (first + d.accepted) * o.vocab : nullptr;
-    d.without = bad && !o.proposal ? __shfl(token, d.accepted, 64) : -1;
-    return d;
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ double moved(double v) {
+    const auto w = __builtin_bit_cast(std::uint64_t, v);
+    const auto lo = static_cast<std::uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(w), CONTROL, ROWS, 0xf, true));
+    const auto hi = static_cast<std::uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(w >> 32), CONTROL, ROWS, 0xf, true));
+    return __builtin_bit_cast(double, static_cast<std::uint64_t>(hi) << 32 | lo);
 }
-
-// A token's share of the remainder and of the target's row.
-__device__ __forceinline__ double2 share(const Draw& d, int index) {
-    double2 s;
-    s.y = positive(d.p[index]);
-    s.x = index == d.without ? 0.0 : s.y;
-    if (d.q) {
-        const double left = s.y - static_cast<double>(d.q[index]);
-        s.x = left > 0.0 ? left : 0.0;
-    }
-    return s;
-}
-
+// Sums over lanes 0..lane, by lane moves within rows of 16 and then across rows.
 __device__ __forceinline__ double wave_scan(double v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int step = 1; step < 64; step <<= 1) {
-        const double below = __shfl_up(v, step, 64);
-        if (lane >= step) v += below;
-    }
+    v += moved<0x111, 0xf>(v);
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);
+    v += moved<0x143, 0xc>(v);
     return v;
 }
-
-// Inclusive scan over the workgroup's threads, in order. `waves` is LDS of kWaves doubles.
-__device__ __forceinline__ double block_scan(double v, double* waves) {
-    const int wave = threadIdx.x >> 6;
-    v = wave_scan(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 63) waves[wave] = v;
-    __syncthreads();
-    double before = 0.0;
-    for (int i = 0; i < wave; ++i) before += waves[i];
-    return v + before;
+__device__ __forceinline__ double lane_value(double v, int lane) {
+    const auto w = __builtin_bit_cast(std::uint64_t, v);
+    const std::uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(w), lane);
+    const std::uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(w >> 32), lane);
+    return __builtin_bit_cast(double, static_cast<std::uint64_t>(hi) << 32 | lo);
 }
 
-// Sums of a part.
-__global__ __launch_bounds__(kThreads) void verify_sum(Operands o) {
-    __shared__ double waves[kWaves];
-    const int sequence = blockIdx.y, part = blockIdx.x;
-    const Draw d = draw_of(o, sequence);
-    const int begin = part * o.slice, end = min(begin + o.slice, o.vocab);
+// A thread's sum of the tokens begin + 4 thread .. + 3, and every 4 THREADS on, below end; loads run several ahead.
+template <int THREADS>
+__device__ __forceinline__ double2 sum_of(const Draw& d, int thread, int begin, int end) {
+    constexpr int kAhead = 4;
     double2 sum = {0.0, 0.0};
-    for (int i = begin + threadIdx.x; i < end; i += kThreads) {
-        const double2 s = share(d, i);
-        sum.x += s.x, sum.y += s.y;
+    for (int first = begin + 4 * thread; first < end; first += 4 * THREADS * kAhead) {
+        float4u p[kAhead], q[kAhead] = {};
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) p[u] = d.load(d.p, d.place(first + u * 4 * THREADS));
+        if (d.q) {
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) q[u] = d.load(d.q, d.place(first + u * 4 * THREADS));
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const double2 s = d.share(p[u], q[u], j, first + u * 4 * THREADS, end);
+                sum.x += s.x, sum.y += s.y;
+            }
     }
-    sum.x = block_scan(sum.x, waves);
-    sum.y = block_scan(sum.y, waves);
-    if (threadIdx.x == kThreads - 1) o.sums[static_cast<std::int64_t>(sequence) * o.parts + part] = sum;
+    return sum;
 }
 
-// The sequence's tokens. A workgroup per sequence; with one part it sums the row itself.
+// Sums of a part, and with the first one the verdict.
+__global__ __launch_bounds__(kSumThreads) void verify_sum(Operands o) {
+    constexpr int kSumWaves = kSumThreads / 64;
+    __shared__ double2 waves[kSumWaves];
+    const int sequence = blockIdx.y, part = blockIdx.x;
+    const Verdict v = verdict_of(o, sequence);
+    const Draw d(o, v, sequence);
+    const int begin = part * o.slice, end = min(begin + o.slice, o.vocab);
+    double2 sum = sum_of<kSumThreads>(d, threadIdx.x, begin, end);
+    sum = {wave_scan(sum.x), wave_scan(sum.y)};
+    if ((threadIdx.x & 63) == 63) waves[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < kSumWaves; ++i) waves[0].x += waves[i].x, waves[0].y += waves[i].y;
+        o.sums[static_cast<std::int64_t>(sequence) * o.parts + part] = waves[0];
+        if (part == 0) o.verdicts[sequence] = v;
+    }
+}
+
+// Which of up to 64 shares in order (a lane each) the target falls into: the first whose running sum passes it, or the last one
+// there is. `before` becomes what precedes it. For a whole wave.
+__device__ __forceinline__ int find(double share, double target, double& before) {
+    const double scan = before + wave_scan(share);
+    const unsigned long long some = __ballot(share > 0.0), past = __ballot(share > 0.0 && scan > target);
+    const int at = past ? __ffsll(past) - 1 : some ? 63 - __clzll(some) : 0;
+    if (at) before = lane_value(scan, at - 1);
+    return at;
+}
+
+// The sequence's tokens. A workgroup per sequence; with one part it sums the row itself. A wave takes a run of the part.
 __global__ __launch_bounds__(kThreads) void verify_take(Operands o) {
-    __shared__ double waves[kWaves];
-    __shared__ int found, last;
-    const int sequence = blockIdx.x, lane = threadIdx.x & 63;
-    const Draw d = draw_of(o, sequence);
+    __shared__ double2 waves[kWaves];
+    const int sequence = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Verdict v = o.parts > 1 ? o.verdicts[sequence] : verdict_of(o, sequence);
+    const Draw d(o, v, sequence);
     const std::int64_t row = static_cast<std::int64_t>(sequence) * (o.drafts + 1);
-    for (int i = threadIdx.x; i <= o.drafts; i += kThreads)
-        if (i != d.accepted) o.tokens[row + i] = i < d.accepted ? o.drafted[row - sequence + i] : -1;
-    if (threadIdx.x == 0) o.accepted[sequence] = d.accepted, found = INT_MAX, last = -1;
+    if (static_cast<int>(threadIdx.x) <= o.drafts && static_cast<int>(threadIdx.x) != v.accepted)
+        o.tokens[row + threadIdx.x] = static_cast<int>(threadIdx.x) < v.accepted ? o.drafted[row - sequence + threadIdx.x] : -1;
+    if (threadIdx.x == 0) o.accepted[sequence] = v.accepted;
     const double u = o.uniforms[row + o.drafts];
     int begin = 0, end = o.vocab;
     double before = 0.0, target = 0.0;
     bool rest = true;  // draw from the remainder
     if (o.parts > 1) {
-        // Every wave looks for the part on its own.
         const double2 none = {0.0, 0.0};
         const double2 own = lane < o.parts ? o.sums[static_cast<std::int64_t>(sequence) * o.parts + lane] : none;
-        const double2 scan = {wave_scan(own.x), wave_scan(own.y)};
-        rest = __shfl(scan.x, 63, 64) > 0.0;
-        const double mine = rest ? own.x : own.y, sum = rest ? scan.x : scan.y;
-        target = u * __shfl(sum, 63, 64);
-        const unsigned long long some = __ballot(mine > 0.0), past = __ballot(mine > 0.0 && sum > target);
-        const int part = past ? __ffsll(past) - 1 : some ? 63 - __clzll(some) : 0;
-        const double up = __shfl_up(sum, 1, 64);
-        before = __shfl(lane ? up : 0.0, part, 64);
-        begin = part * o.slice;
+        const double all = lane_value(wave_scan(own.x), 63);
+        rest = all > 0.0;
+        target = u * (rest ? all : lane_value(wave_scan(own.y), 63));
+        begin = find(rest ? own.x : own.y, target, before) * o.slice;
         end = min(begin + o.slice, o.vocab);
     }
-    // A thread's run of tokens.
-    const int run = (end - begin + kThreads - 1) / kThreads;
-    const int first = begin + static_cast<int>(threadIdx.x) * run, stop = min(first + run, end);
-    double2 sum = {0.0, 0.0};
-    for (int i = first; i < stop; ++i) {
-        const double2 s = share(d, i);
-        sum.x += s.x, sum.y += s.y;
-    }
-    const double scan_x = block_scan(sum.x, waves);
-    double all = 0.0;
-    for (int i = 0; i < kWaves; ++i) all += waves[i];
-    const double scan_y = block_scan(sum.y, waves);
-    if (o.parts == 1) {
-        double whole = 0.0;
-        for (int i = 0; i < kWaves; ++i) whole += waves[i];
-        rest = all > 0.0;
-        target = u * (rest ? all : whole);
-    }
-    double at = before + (rest ? scan_x - sum.x : scan_y - sum.y);
-    for (int i = first; i < stop; ++i) {
-        const double2 s = share(d, i);
-        const double w = rest ? s.x : s.y;
-        at += w;
-        if (w > 0.0) {
-            atomicMax(&last, i);
-            if (at > target) {
-                atomicMin(&found, i);
-                break;
-            }
-        }
-    }
+    const int run = ((end - begin + kWaves - 1) / kWaves + 3) / 4 * 4;
+    begin += wave * run;
+    end = min(begin + run, end);
+    double2 sum = sum_of<64>(d, lane, begin, end);
+    sum = {wave_scan(sum.x), wave_scan(sum.y)};
+    if (lane == 63) waves[wave] = sum;
     __syncthreads();
-    // Where no sum passes the target (a uniform of 1, or a last rounding) it is the last token with a share.
-    if (threadIdx.x == 0) o.tokens[row + d.accepted] = found != INT_MAX ? found : last;
+    const double2 own = lane < kWaves ? waves[lane] : double2{0.0, 0.0};
+    if (o.parts == 1) {
+        const double all = lane_value(wave_scan(own.x), 63);
+        rest = all > 0.0;
+        target = u * (rest ? all : lane_value(wave_scan(own.y), 63));
+    }
+    if (find(rest ? own.x : own.y, target, before) != wave) return;
+    // The wave that the token lies in goes through its run again.
+    int token = -1;
+    for (int first = begin; first < end; first += 256) {
+        const int at = first + 4 * lane;
+        const float4u p = d.load(d.p, d.place(at)), q = d.q ? d.load(d.q, d.place(at)) : float4u{};
+        double w[4], four = 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const double2 s = d.share(p, q, j, at, end);
+            w[j] = rest ? s.x : s.y;
+            four += w[j];
+        }
+        const double scan = before + wave_scan(four);
+        const unsigned long long some = __ballot(four > 0.0), past = __ballot(four > 0.0 && scan > target);
+        if (some) {
+            const int mine = past ? __ffsll(past) - 1 : 63 - __clzll(some);
+            // Of the lane's four the first that passes, or else the last with a share.
+            double running = mine ? lane_value(scan, mine - 1) : before;
+            int found = -1;
+            bool passed = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                running += lane_value(w[j], mine);
+                if (lane_value(w[j], mine) > 0.0 && !passed) {
+                    found = d.place(first + 4 * mine) + j;
+                    passed = running > target;
+                }
+            }
+            token = found;
+        }
+        if (past) break;
+        before = lane_value(scan, 63);
+    }
+    if (lane == 0) o.tokens[row + v.accepted] = token;
 }
 
 Operands geometry(int sequences, int drafts, int vocab) {
@@ -188,12 +245,12 @@ Operands geometry(int sequences, int drafts, int vocab) {
     // Parts of 2048 tokens and more, about 2048 workgroups in all.
     const int parts = std::max(std::min({kMaxParts, 2048 / sequences, vocab / 2048}), 1);
     Operands o{};
-    o.drafts = drafts, o.vocab = vocab, o.parts = parts, o.slice = (vocab + parts - 1) / parts;
+    o.drafts = drafts, o.vocab = vocab, o.parts = parts, o.slice = ((vocab + parts - 1) / parts + 3) / 4 * 4;
     return o;
 }
 
 std::uint64_t sum_bytes(const Operands& o, int sequences) {
-    return o.parts > 1 ? sizeof(double2) * static_cast<std::uint64_t>(o.parts) * sequences : 0;
+    return o.parts > 1 ? (sizeof(Verdict) + sizeof(double2) * o.parts) * static_cast<std::uint64_t>(sequences) : 0;
 }
 
 }  // namespace
@@ -220,10 +277,11 @@ VT_EXPORT int venturi_verify_run(const float* target, const float* proposal, con
         vt::require(!bytes || (workspace && available >= bytes && vt::aligned(workspace, 256)),
                     "verification needs its workspace, 256-byte aligned");
         o.target = target, o.proposal = proposal, o.drafted = drafted, o.counts = counts, o.uniforms = uniforms;
-        o.tokens = tokens, o.accepted = accepted, o.sums = static_cast<double2*>(workspace);
+        o.tokens = tokens, o.accepted = accepted, o.verdicts = static_cast<vt::Verdict*>(workspace);
+        o.sums = reinterpret_cast<double2*>(o.verdicts + sequences);
         const auto s = static_cast<hipStream_t>(stream);
         if (o.parts > 1) {
-            vt::verify_sum<<<dim3(o.parts, sequences), vt::kThreads, 0, s>>>(o);
+            vt::verify_sum<<<dim3(o.parts, sequences), vt::kSumThreads, 0, s>>>(o);
             vt::check(hipGetLastError());
         }
         vt::verify_take<<<sequences, vt::kThreads, 0, s>>>(o);
