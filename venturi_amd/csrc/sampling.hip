@@ -951,8 +951,7 @@ __global__ __launch_bounds__(kThreads) void sample(Operands o) {
         edge_match(row, edge, pattern, true, rank - found, token);
 }
 
-// Vectors of 8 logits of a workgroup of distribution().
-constexpr int kWriteThreads = 256, kWriteVectors = 4 * kWriteThreads;
+constexpr int kWriteThreads = 256;
 
 // The probability of a logit that is the row's token `index`.
 template <class T>
@@ -973,7 +972,8 @@ __device__ __forceinline__ float probability(const Cut& cut, std::uint32_t last,
 
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 
-// Writes a row's probabilities from its cut: a workgroup for kWriteVectors vectors, the row's ragged ends with the first.
+// Writes a row's probabilities from its cut: a vector of 8 a thread, the row's ragged ends with the first workgroup. (Four
+// vectors a thread: 5 rows of 248320 2 us more, 257 of 32003 1 us less.)
 template <class T>
 __global__ __launch_bounds__(kWriteThreads) void distribution(Operands o) {
     const int index = blockIdx.y;
@@ -986,17 +986,16 @@ __global__ __launch_bounds__(kWriteThreads) void distribution(Operands o) {
         const int at = row.edge(threadIdx.x);
         out[at] = some ? probability<T>(cut, last, row.start[at], at) : 0.0f;
     }
-    for (int i = blockIdx.x * kWriteVectors + threadIdx.x; i < min(row.vectors, static_cast<int>(blockIdx.x + 1) * kWriteVectors);
-         i += kWriteThreads) {
-        const uint4 w = row.whole()[i];
-        const int first = row.head + 8 * i;
-        float p[8];
+    const int i = blockIdx.x * kWriteThreads + threadIdx.x;
+    if (i >= row.vectors) return;
+    const uint4 w = row.whole()[i];
+    const int first = row.head + 8 * i;
+    float p[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = some ? probability<T>(cut, last, element(w, j), first + j) : 0.0f;
-        // Rows of odd vocabularies start at any multiple of 4 bytes.
-        *reinterpret_cast<float4u*>(out + first) = float4u{p[0], p[1], p[2], p[3]};
-        *reinterpret_cast<float4u*>(out + first + 4) = float4u{p[4], p[5], p[6], p[7]};
-    }
+    for (int j = 0; j < 8; ++j) p[j] = some ? probability<T>(cut, last, element(w, j), first + j) : 0.0f;
+    // Rows of odd vocabularies start at any multiple of 4 bytes.
+    *reinterpret_cast<float4u*>(out + first) = float4u{p[0], p[1], p[2], p[3]};
+    *reinterpret_cast<float4u*>(out + first + 4) = float4u{p[4], p[5], p[6], p[7]};
 }
 
 template <class T, bool CUT>
@@ -1006,7 +1005,7 @@ void launch(const Operands& o, hipStream_t stream) {
     sample<T, CUT><<<o.rows, kThreads, sizeof(Shared), stream>>>(o);
     if constexpr (CUT) {
         check(hipGetLastError());
-        const unsigned parts = std::max((o.vocab / 8 + kWriteVectors - 1) / kWriteVectors, 1);
+        const unsigned parts = std::max((o.vocab / 8 + kWriteThreads - 1) / kWriteThreads, 1);
         distribution<T><<<dim3(parts, o.rows), kWriteThreads, 0, stream>>>(o);
     }
 }
