@@ -42,7 +42,7 @@ def definitions(logits, bias, top_k, *, score="softmax", groups=1, kept_groups=1
     ranks = []
     for g in range(groups):
         best = sorted(c[g * size: (g + 1) * size], reverse=True)
-        ranks.append(best[0] + best[1] if group_rank == "pairs" and size > 1 else best[0])
+        ranks.append(best[0] + best[1] if group_rank == "pairs" and size > 1 and best[1] > -math.inf else best[0])
     first = sorted(range(groups), key=lambda g: (-ranks[g], g))[:kept_groups]
     others = combinations(range(groups), kept_groups) if bias is not None and 1 < groups <= 8 else ()
     for kept in (first, *others):
@@ -143,7 +143,13 @@ def test_scores_that_differ_in_their_last_bits(backend, device):
     steps = torch.randint(0, 6, (40, 64), generator=gen, dtype=torch.int32)
     logits = (torch.full((40, 64), 9.0).view(torch.int32) + steps).view(FP32)
     for score in ("softmax", "sigmoid"):
-        check(backend, device, logits, None, 8, score=score)
+        for top_k in (1, 8, 16):
+            check(backend, device, logits, None, top_k, score=score)
+            check(backend, device, logits, torch.zeros(64), top_k, score=score)
+    wide = (torch.full((5, 700), -3.0).view(torch.int32) + torch.randint(0, 2000, (5, 700), generator=gen, dtype=torch.int32)).view(FP32)
+    for top_k in (3, 16):
+        check(backend, device, wide, random_bias(700, 5) * 1e-6, top_k, score="sigmoid")
+        check(backend, device, wide, random_bias(700, 6) * 1e-7, top_k, score="softmax", renormalize=False)
     bias = (torch.full((64,), 0.001).view(torch.int32) + torch.randperm(64, generator=gen).int()).view(FP32)
     check(backend, device, torch.zeros(2, 64), bias, 8, score="sigmoid")
     check(backend, device, torch.zeros(2, 64), bias, 4, score="softmax", groups=8, kept_groups=2)

@@ -32,7 +32,7 @@ def definition(p, q, drafted, count, u):
                 left[int(drafted[at])] = 0.0
         else:
             left = rest - q[at].astype(np.float64)
-            left = np.where(left > 0, left, 0.0)
+            left = np.where((left > 0) & (rest > 0), left, 0.0)
         if left.sum() > 0:
             rest = left
     some = np.flatnonzero(rest > 0)
@@ -145,6 +145,7 @@ def test_rows_that_leave_nothing(backend, device, vocab):
     p[3], p[4] = math.nan, -1.0
     p[5, 0, : vocab // 2] = math.inf
     q[6] = math.nan
+    q[9] = -0.25
     p[7, 0] = 0.0
     p[7, 0, 17] = 1e-45
     drafted[8, 0], drafted[9, 0] = vocab, -3

@@ -264,6 +264,19 @@ def test_distribution_raises_its_lds_limit_on_every_device():
         assert len(launches) == 2 and limits[launches[0].kernel, launches[0].device] >= launches[0].shared > 65536
 
 
+def test_launches_keep_their_threads_within_32_bits():
+    """More rows than a launch takes go to several, which cover them all."""
+    for call, rows in ((rms(20_000_000, 4096, 0), 20_000_000), (rms(30_000_001, 512, 1), 30_000_001), (rms(5_000_000, 70000, 2), 5_000_000),
+                       (route(100_000_007, 64, 1, 0, 0, 1), 100_000_007), (route(50_000_000, 512, 64, 1, 1, 2), 50_000_000)):
+        entry, arguments = call
+        arguments = [(1 << 30) + (pointers(6).index(v) << 42) if v in pointers(6) else v for v in arguments]  # apart, whatever the size
+        launches = [e for e in record([(0, entry, arguments)])[0] if isinstance(e, Launch)]
+        assert len(launches) > 1 and all(e.blocks * e.threads < 2**32 for e in launches)
+        per_row = {"residual_rms_wave": 64, "route_logits": 16, "route_scores": 64}.get(launches[0].kernel.split("<")[0], launches[0].threads)
+        covered = sum(e.blocks * e.threads // per_row for e in launches)
+        assert rows <= covered < rows + 256 * len(launches)
+
+
 def test_verification_sums_rows_in_parts_where_they_are_long_and_few():
     counts = {(1, 4, 4000): 1, (1, 4, 4096): 2, (61, 7, 32003): 2, (2048, 1, 151936): 1}
     for (n, d, v), count in counts.items():

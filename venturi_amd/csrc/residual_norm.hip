@@ -29,6 +29,7 @@ struct Operands {
     std::int8_t* codes;
     float* scales;
     int tokens, k, groups, passes;
+    int first, count;  // the launch's rows
     float epsilon;
 };
 
@@ -42,7 +43,8 @@ template <class T>
 __global__ __launch_bounds__(kChains) void residual_rms_any(Operands o) {
     __shared__ __align__(16) float chains[kChains];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = o.k;
-    const std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * k;
+    const int token = o.first + blockIdx.x;
+    const std::int64_t row = static_cast<std::int64_t>(token) * k;
     const T* x = static_cast<const T*>(o.x) + row;
     const T* residual = static_cast<const T*>(o.residual) + row;
     T* total = static_cast<T*>(o.total) + row;
@@ -74,7 +76,7 @@ __global__ __launch_bounds__(kChains) void residual_rms_any(Operands o) {
                     }
                     bad |= !isfinite(r[v]);
                 }
-                const std::int64_t index = static_cast<std::int64_t>(blockIdx.x) * o.groups + g;
+                const std::int64_t index = static_cast<std::int64_t>(token) * o.groups + g;
                 if (g < o.groups)  // the 8 lanes of a group share g
                     quantize_group<4, 8>(r, bad, o.passes, o.codes + index * 32 + (col & 31), o.scales + index, count * 32, count,
                                          (lane & 7) == 0);
@@ -105,8 +107,8 @@ __device__ __forceinline__ uint2 pack4(const T (&v)[4]) {
 template <class T, int P>
 __global__ __launch_bounds__(256) void residual_rms_wave(Operands o) {
     const int lane = threadIdx.x & 63, k = o.k;
-    const int token = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (token >= o.tokens) return;
+    const int in_launch = blockIdx.x * 4 + (threadIdx.x >> 6), token = o.first + in_launch;
+    if (in_launch >= o.count) return;
     const std::int64_t row = static_cast<std::int64_t>(token) * k;
     const T* x = static_cast<const T*>(o.x) + row;
     const T* residual = static_cast<const T*>(o.residual) + row;
@@ -174,7 +176,8 @@ __global__ __launch_bounds__(THREADS) void residual_rms_staged(Operands o) {
     extern __shared__ uint4 staged[];
     __shared__ __align__(16) float chains[kChains];
     const int tid = threadIdx.x, lane = tid & 63, k = o.k;
-    const std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * k;
+    const int token = o.first + blockIdx.x;
+    const std::int64_t row = static_cast<std::int64_t>(token) * k;
     const int shift = ROUND ? 0 : static_cast<int>(row % V), pieces = (k + shift + V - 1) / V;
     auto* held = reinterpret_cast<T*>(staged) + shift;
     const T* x = static_cast<const T*>(o.x) + row;
@@ -237,7 +240,7 @@ __global__ __launch_bounds__(THREADS) void residual_rms_staged(Operands o) {
                 }
 #pragma unroll
                 for (int v = 0; v < 4; ++v) bad |= !isfinite(q[v]);
-                const std::int64_t index = static_cast<std::int64_t>(blockIdx.x) * o.groups + (col >> 5);
+                const std::int64_t index = static_cast<std::int64_t>(token) * o.groups + (col >> 5);
                 quantize_group<4, 8>(q, bad, o.passes, o.codes + index * 32 + (col & 31), o.scales + index, count * 32, count,
                                      (lane & 7) == 0);  // the 8 lanes of a group share it
             }
@@ -276,7 +279,7 @@ void launch(const Operands& o, hipStream_t stream) {
         const bool wave = o.k <= 256 || (o.k <= 1024 && o.tokens >= 2048);
         if (wave && o.k % 4 == 0 && aligned(o.x, 8) && aligned(o.residual, 8) && aligned(o.total, 8) && aligned(o.out, 8) &&
             aligned(o.gamma, 16)) {
-            const auto grid = static_cast<unsigned>((static_cast<std::int64_t>(o.tokens) + 3) / 4);
+            const auto grid = static_cast<unsigned>((o.count + 3) / 4);
             if (o.k <= 256) residual_rms_wave<T, 1><<<grid, 256, 0, stream>>>(o);
             else if (o.k <= 512) residual_rms_wave<T, 2><<<grid, 256, 0, stream>>>(o);
             else residual_rms_wave<T, 4><<<grid, 256, 0, stream>>>(o);
@@ -288,15 +291,15 @@ void launch(const Operands& o, hipStream_t stream) {
     // passes 61: 5.2 / 6.3 / 8.5; 600: 12.6 / 12.6 / 13.1; 8190: 101 / 90 / 91).
     const std::int64_t bytes = static_cast<std::int64_t>(o.k) * sizeof(T);
     if (bytes > kStaged || !(aligned(o.x, 16) && aligned(o.residual, 16) && aligned(o.total, 16) && aligned(o.out, 16) && aligned(o.gamma, 16))) {
-        residual_rms_any<T><<<o.tokens, kChains, 0, stream>>>(o);
+        residual_rms_any<T><<<o.count, kChains, 0, stream>>>(o);
         return;
     }
     const auto staged = [&](auto round) {
         constexpr bool R = decltype(round)::value;
         const auto lds = static_cast<std::size_t>(bytes + 31) / 16 * 16;  // and what comes before the row in its first vector
-        if (o.k > 2048 && o.tokens <= 256) residual_rms_staged<T, 1024, R><<<o.tokens, 1024, lds, stream>>>(o);
-        else if (o.k > 2048) residual_rms_staged<T, 512, R><<<o.tokens, 512, lds, stream>>>(o);
-        else residual_rms_staged<T, kChains, R><<<o.tokens, kChains, lds, stream>>>(o);
+        if (o.k > 2048 && o.tokens <= 256) residual_rms_staged<T, 1024, R><<<o.count, 1024, lds, stream>>>(o);
+        else if (o.k > 2048) residual_rms_staged<T, 512, R><<<o.count, 512, lds, stream>>>(o);
+        else residual_rms_staged<T, kChains, R><<<o.count, kChains, lds, stream>>>(o);
     };
     if (bytes % 16 == 0) staged(std::true_type{});
     else staged(std::false_type{});
@@ -341,13 +344,18 @@ VT_EXPORT int venturi_residual_rms_run(const void* x, const void* residual, cons
         const int groups = (k + 31) / 32;
         auto* codes = static_cast<std::int8_t*>(workspace);
         auto* scales = reinterpret_cast<float*>(codes + static_cast<std::int64_t>(tokens) * groups * 32 * passes);
-        const vt::Operands o{x, residual, gamma, total, out, codes, scales, tokens, k, groups, passes, epsilon};
         const auto s = static_cast<hipStream_t>(stream);
-        if (dtype == vt::kF16)
-            vt::launch<__half>(o, s);
-        else if (dtype == vt::kBF16)
-            vt::launch<__hip_bfloat16>(o, s);
-        else
-            vt::launch<float>(o, s);
+        // A launch takes 2^21 rows: its threads are counted in 32 bits.
+        for (std::int64_t first = 0; first < tokens; first += 1 << 21) {
+            const int count = static_cast<int>(std::min<std::int64_t>(tokens - first, 1 << 21));
+            const vt::Operands o{x, residual, gamma, total, out, codes, scales, tokens, k, groups, passes, static_cast<int>(first), count, epsilon};
+            if (dtype == vt::kF16)
+                vt::launch<__half>(o, s);
+            else if (dtype == vt::kBF16)
+                vt::launch<__hip_bfloat16>(o, s);
+            else
+                vt::launch<float>(o, s);
+            vt::check(hipGetLastError());
+        }
     });
 }

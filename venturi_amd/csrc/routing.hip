@@ -309,14 +309,11 @@ __global__ __launch_bounds__(kThreads) void route_logits(const T* __restrict__ l
     write<LANES>(g, indices, scores, token, place, expert, weight, bad);
 }
 
-// Below every score: a masked expert. It fits 32 bits.
-constexpr double kMasked = -3e38;
-
-// A score's key: its 32-bit number in order as a whole number above 0, without the low bits that say which of its lane's N
-// experts it is, the first the largest.
+// A score's key: its 32-bit number (infinities as the largest there is) in order as a whole number above 0, without the low
+// bits that say which of its lane's N experts it is, the first the largest.
 template <int N>
 __device__ __forceinline__ std::uint32_t key_of(double c, int i) {
-    const auto w = __builtin_bit_cast(std::uint32_t, static_cast<float>(c));
+    const auto w = __builtin_bit_cast(std::uint32_t, fminf(fmaxf(static_cast<float>(c), -3.402823466e38f), 3.402823466e38f));
     return ((w & 0x80000000u ? ~w : w | 0x80000000u) & ~(N - 1u)) | (N - 1 - i);
 }
 // Whether the first of two keys, the larger, may stand for no larger score: the 32-bit rounding and the low bits hide less than
@@ -366,10 +363,7 @@ __device__ __forceinline__ void keep_groups(const Geometry& g, const double (&c)
             }
         }
     }
-    // A masked expert counts as -inf.
-    if (best.most <= kMasked) best.most = none;
-    if (best.second <= kMasked) best.second = none;
-    const double rank = g.pairs && size > 1 ? best.most + best.second : best.most;
+    const double rank = g.pairs && best.second > none ? best.most + best.second : best.most;
     rank_of[place] = rank;
     wave_fence();
     int ahead = 0;
@@ -475,7 +469,7 @@ __global__ __launch_bounds__(kThreads) void route_scores(const T* __restrict__ l
     }
     const auto whole = [&](float logit, double s, float offset) {  // a score with its bias
         const double v = direct ? static_cast<double>(logit) : s + static_cast<double>(offset);
-        return logit == -kInf ? kMasked : fmax(v + 0.0, kMasked);  // one zero
+        return logit == -kInf ? -__builtin_inf() : fmax(v + 0.0, -__builtin_inf());  // one zero, and no NaN
     };
     std::uint32_t key[N];
 #pragma unroll
@@ -505,14 +499,14 @@ __global__ __launch_bounds__(kThreads) void route_scores(const T* __restrict__ l
         if (!sure) exact = whole(logit, weight, bias ? bias[chosen] : 0.0f);
     }
     if (!sure) {
-        const int ahead = rank_of_16(exact, chosen);
+        const int ahead = rank_of_16(exact, candidate ? chosen : kMaxExperts);
         rank = bad ? place : candidate ? ahead : kMaxTopK;
     }
     write<LANES>(g, indices, scores, token, rank, chosen, weight, bad);
 }
 
 template <class T, int LANES, int N>
-void launch_lanes(const T* logits, const float* bias, std::int64_t* indices, void* scores, const Geometry& g, hipStream_t stream) {
+void launch_some(const T* logits, const float* bias, std::int64_t* indices, void* scores, const Geometry& g, hipStream_t stream) {
     constexpr int tokens = kThreads / LANES;
     const auto grid = static_cast<unsigned>((static_cast<std::int64_t>(g.tokens) + tokens - 1) / tokens);
     const bool vector = g.experts % N == 0 && aligned(logits, 16) && aligned(bias, 16);
@@ -530,6 +524,20 @@ void launch_lanes(const T* logits, const float* bias, std::int64_t* indices, voi
     };
     if (g.sigmoid) run(std::true_type{});
     else run(std::false_type{});
+}
+
+// A launch takes 2^24 tokens (its threads are counted in 32 bits).
+template <class T, int LANES, int N>
+void launch_lanes(const T* logits, const float* bias, std::int64_t* indices, void* scores, const Geometry& g, hipStream_t stream) {
+    constexpr int kTokens = 1 << 24;
+    const std::int64_t size = g.score_type == kF32 ? 4 : 2;
+    for (std::int64_t first = 0; first < g.tokens; first += kTokens) {
+        Geometry part = g;
+        part.tokens = static_cast<int>(std::min<std::int64_t>(g.tokens - first, kTokens));
+        launch_some<T, LANES, N>(logits + first * g.experts, bias, indices + first * g.top_k,
+                                 static_cast<char*>(scores) + first * g.top_k * size, part, stream);
+        check(hipGetLastError());
+    }
 }
 
 // A token takes 16, 32 or 64 lanes of eight experts (four where they are few, 16 past 512), as many as groups and choices at

@@ -2,7 +2,8 @@
 
 Scores s = softmax(logits) or 1 / (1 + exp(-logits)) over all experts. Experts are ordered by c = s + bias, largest first,
 equal ones by index; with ``groups`` > 1 only those of the ``kept_groups`` best groups (consecutive experts of equal number),
-ordered by the sum of their two largest c ("pairs") or by their largest ("max"), equal ones by index. The first ``top_k`` are
+ordered by the sum of their two largest c ("pairs"; a lone one that is not masked by itself) or by their largest ("max"), equal
+ones by index. The first ``top_k`` are
 chosen. Their weights are s without the bias, divided by their sum with ``renormalize``, times ``scale``.
 
 An expert whose logit is -inf is masked: it comes after all others, with weight 0, whatever its bias. Weights whose sum is 0

@@ -6,8 +6,8 @@ max(p - q, 0) of that row (certain drafts: p without the draft), or from p where
 of the row behind the last. Tokens so emitted are distributed as the target's own samples. The drawn token is the first, by
 index, at which the running sum of the shares exceeds the uniform times their whole sum.
 
-Rows need not add to 1; probabilities that are no positive finite number count as 0, and a row of those alone gives token -1.
-A draft outside the vocabulary is refused. Sums are 64-bit, in a fixed order: the result depends on the inputs alone. The rows
+Rows need not add to 1; target probabilities that are no positive finite number count as 0 (such tokens are neither accepted
+nor drawn), and a row of those alone gives token -1. A draft outside the vocabulary is refused, and one whose proposal is NaN. Sums are 64-bit, in a fixed order: the result depends on the inputs alone. The rows
 come from ``HipBackend.prepare_distribution``. The reference decodes without drafts; this operator is an extension.
 """
 
