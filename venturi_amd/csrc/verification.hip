@@ -5,14 +5,16 @@
 // p without the draft), where that has a mass, else from p; after the last draft from p of the row behind it. It is the first
 // token, by index, at which the running sum passes u times the whole one; sums in 64 bits, in a fixed order.
 //
-// Bound by memory: one or two rows of 4-byte probabilities a sequence. A row is cut into parts that workgroups sum; one
-// workgroup of a second launch finds the part and goes through it again.
+// Bound by memory where sequences are many: one or two rows of 4-byte probabilities each (128 of 151936 tokens with a drafter's
+// rows 33.4 us, 4.7 TB/s), else by two launches and their chains of loads: the drafts, their probabilities, the row, and
+// in the second launch the sums, the part, and the run of it again (one sequence of 248320 tokens 8.6, 61 of 32003 11.4). A row
+// is cut into parts that workgroups sum; one workgroup of the second launch finds the part and the token in it. (The chosen
+// part token by token, a run a thread: 82.6, 20.2 and 16.6.)
 #include "common.hpp"
 
 namespace vt {
 namespace {
 
-constexpr int kSumThreads = 256, kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kMaxDrafts = 64, kMaxParts = 64, kMaxVocab = 1 << 20, kMaxSequences = 65535;
 
 // What a sequence's drafts came to.
@@ -112,10 +114,10 @@ __device__ __forceinline__ double lane_value(double v, int lane) {
     return __builtin_bit_cast(double, static_cast<std::uint64_t>(hi) << 32 | lo);
 }
 
-// A thread's sum of the tokens begin + 4 thread .. + 3, and every 4 THREADS on, below end; loads run several ahead.
+// A thread's sum of the tokens begin + 4 thread .. + 3, and every 4 THREADS on, below end, two loads of each row at once.
 template <int THREADS>
 __device__ __forceinline__ double2 sum_of(const Draw& d, int thread, int begin, int end) {
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 2;  // 4 or 8 load past the end of most runs: 128 sequences of 151936 tokens 33.4, 34.3, 46.9 us
     double2 sum = {0.0, 0.0};
     for (int first = begin + 4 * thread; first < end; first += 4 * THREADS * kAhead) {
         float4u p[kAhead], q[kAhead] = {};
@@ -137,19 +139,19 @@ __device__ __forceinline__ double2 sum_of(const Draw& d, int thread, int begin, 
 }
 
 // Sums of a part, and with the first one the verdict.
-__global__ __launch_bounds__(kSumThreads) void verify_sum(Operands o) {
-    constexpr int kSumWaves = kSumThreads / 64;
-    __shared__ double2 waves[kSumWaves];
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void verify_sum(Operands o) {
+    __shared__ double2 waves[THREADS / 64];
     const int sequence = blockIdx.y, part = blockIdx.x;
     const Verdict v = verdict_of(o, sequence);
     const Draw d(o, v, sequence);
     const int begin = part * o.slice, end = min(begin + o.slice, o.vocab);
-    double2 sum = sum_of<kSumThreads>(d, threadIdx.x, begin, end);
+    double2 sum = sum_of<THREADS>(d, threadIdx.x, begin, end);
     sum = {wave_scan(sum.x), wave_scan(sum.y)};
     if ((threadIdx.x & 63) == 63) waves[threadIdx.x >> 6] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int i = 1; i < kSumWaves; ++i) waves[0].x += waves[i].x, waves[0].y += waves[i].y;
+        for (int i = 1; i < THREADS / 64; ++i) waves[0].x += waves[i].x, waves[0].y += waves[i].y;
         o.sums[static_cast<std::int64_t>(sequence) * o.parts + part] = waves[0];
         if (part == 0) o.verdicts[sequence] = v;
     }
@@ -166,7 +168,9 @@ __device__ __forceinline__ int find(double share, double target, double& before)
 }
 
 // The sequence's tokens. A workgroup per sequence; with one part it sums the row itself. A wave takes a run of the part.
-__global__ __launch_bounds__(kThreads) void verify_take(Operands o) {
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void verify_take(Operands o) {
+    constexpr int kWaves = THREADS / 64;
     __shared__ double2 waves[kWaves];
     const int sequence = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Verdict v = o.parts > 1 ? o.verdicts[sequence] : verdict_of(o, sequence);
@@ -249,6 +253,31 @@ Operands geometry(int sequences, int drafts, int vocab) {
     return o;
 }
 
+template <int THREADS>
+void launch_sum(const Operands& o, int sequences, hipStream_t stream) {
+    verify_sum<THREADS><<<dim3(o.parts, sequences), THREADS, 0, stream>>>(o);
+}
+template <int THREADS>
+void launch_take(const Operands& o, int sequences, hipStream_t stream) {
+    verify_take<THREADS><<<sequences, THREADS, 0, stream>>>(o);
+}
+
+// Where the card is full, small workgroups, which repeat the verdict's loads in fewer waves (us, 128 threads against 256: 128
+// sequences of 151936 tokens 34.3 / 36.9, 64 19.8 / 22.1; one of 248320 11.5 / 9.3).
+void launch_sum(const Operands& o, int sequences, hipStream_t stream) {
+    if (o.parts * sequences > 256) launch_sum<128>(o, sequences, stream);
+    else launch_sum<256>(o, sequences, stream);
+}
+
+// As many threads as have a run of some length, fewer where sequences are many (they start sooner). Us, 256 / 512 / 1024
+// threads: one sequence of 1000 tokens 4.9 / 5.4 / 6.5, of 248320 (3880 in a part) 9.5 / 9.3 / 10.1; 128 of 151936 (9496) 42 /
+// 39 / 37; 512 of 32003 (8004) 31 / 28 / 31; 2100 of 9001 (one part) 34 / 42 / 49.
+void launch_take(const Operands& o, int sequences, hipStream_t stream) {
+    if (o.slice <= 1024 || sequences > 1024) launch_take<256>(o, sequences, stream);
+    else if (o.slice <= 6144 || sequences > 256) launch_take<512>(o, sequences, stream);
+    else launch_take<1024>(o, sequences, stream);
+}
+
 std::uint64_t sum_bytes(const Operands& o, int sequences) {
     return o.parts > 1 ? (sizeof(Verdict) + sizeof(double2) * o.parts) * static_cast<std::uint64_t>(sequences) : 0;
 }
@@ -281,9 +310,9 @@ VT_EXPORT int venturi_verify_run(const float* target, const float* proposal, con
         o.sums = reinterpret_cast<double2*>(o.verdicts + sequences);
         const auto s = static_cast<hipStream_t>(stream);
         if (o.parts > 1) {
-            vt::verify_sum<<<dim3(o.parts, sequences), vt::kSumThreads, 0, s>>>(o);
+            vt::launch_sum(o, sequences, s);
             vt::check(hipGetLastError());
         }
-        vt::verify_take<<<sequences, vt::kThreads, 0, s>>>(o);
+        vt::launch_take(o, sequences, s);
     });
 }
