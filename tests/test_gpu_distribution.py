@@ -111,6 +111,37 @@ def test_masked_logits(backend, device, dtype):
         assert not bool(out[3:5].any())
 
 
+@pytest.mark.parametrize("rows,vocab", [(3, 5003), (3, 70001), (40, 60001)])
+def test_temperatures_and_differences_beyond_32_bits(backend, device, rows, vocab):
+    """Inverse temperatures above 3e38, and rows whose largest and smallest logits differ by more."""
+    logits = random_logits(rows, vocab, 1.0, BF16, 11)
+    far, small = logits.float().mul(1e38).clamp(-3e38, 3e38).to(BF16), logits.float().mul(1e-38).to(BF16)
+    ties = logits.clamp(max=1.0)
+    for t in (3e38, 3.4e38, 1e30, 1e-30, 1e-38, 1e-40, 1e-45):
+        for x in (far, small, ties):
+            check(backend, device, x, t=[t] * rows)
+            check(backend, device, x, t=[t] * rows, p=[0.9, 1.0, 1.0] + [1.0] * (rows - 3), k=[0, 0, 9] + [0] * (rows - 3))
+
+
+@TYPES
+@pytest.mark.parametrize("rows", [2, 31, 32, 33])
+@pytest.mark.parametrize("vocab", [57344, 57345, 57352, 65536 + 8, 147456 + 3])
+def test_few_long_rows(backend, device, dtype, rows, vocab):
+    logits = random_logits(rows, vocab, 2.5, dtype, vocab)
+    check(backend, device, logits, k=[(0, 1, 50, 256, 257, 0)[i % 6] for i in range(rows)], p=[(1.0, 1.0, 0.9)[i % 3] for i in range(rows)])
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+def test_masked_logits_of_long_rows(backend, device, rows):
+    inf, nan, vocab = math.inf, math.nan, 70003
+    for dtype, fill in ((FP16, -inf), (BF16, nan), (BF16, -inf), (FP16, inf)):
+        for at in (0, 3, 8191, 8192, 70002):  # the only other logit
+            logits = torch.full((rows, vocab), fill, dtype=dtype)
+            logits[0, at] = -2.0
+            check(backend, device, logits, k=[1] + [0] * (rows - 1))
+            check(backend, device, logits)
+
+
 def test_the_distribution_is_what_sampling_draws_from(backend, device):
     """The sampled token's probability, row by row, for random settings."""
     rows, vocab = 64, 9001

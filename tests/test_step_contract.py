@@ -218,6 +218,8 @@ def test_entry_points_refuse_on_the_host(entry, good, changes):
 def test_workspace_sizes():
     lib = native.load()
     assert lib.venturi_distribution_bytes(96, 1000) == 96 * 32
+    # Of up to 32 long rows also parts of 8192 logits and chunks of 128.
+    assert [lib.venturi_distribution_bytes(*s) for s in ((5, 57344), (33, 81920), (32, 81920))] == [5 * 32, 33 * 32, 32 * (32 + 16 * 10 + 2 * 640)]
     for bad in ((0, 5), (65536, 5), (1, 0), (1, 2**20 + 1)):
         assert lib.venturi_distribution_bytes(*bad) == 0 and lib.error()
     for bad in ((0, 1, 5), (65536, 1, 5), (1, 0, 5), (1, 65, 5), (1, 1, 0), (1, 1, 2**20 + 1)):
@@ -262,6 +264,15 @@ def test_distribution_raises_its_lds_limit_on_every_device():
         launches = [e for e in events if isinstance(e, Launch)]
         limits.update({(e.kernel, e.device): e.bytes for e in events if isinstance(e, LdsLimit)})
         assert len(launches) == 2 and limits[launches[0].kernel, launches[0].device] >= launches[0].shared > 65536
+
+
+@pytest.mark.parametrize("rows,vocab,kernels", [(3, 80000, 3), (32, 57345, 3), (3, 57344, 2), (33, 80000, 2), (3, 7, 2)])
+def test_few_long_rows_are_looked_at_first(rows, vocab, kernels):
+    logits, p, w = pointers(3)
+    for dtype in (0, 1):
+        events = record([(0, "venturi_distribution_run", [logits, None, None, None, None, p, w, 1 << 40, rows, vocab, dtype, None])])[0]
+        launches = [e.kernel.split("<")[0] for e in events if isinstance(e, Launch)]
+        assert launches == ["distribution_scan", "distribution_cut", "distribution"][3 - kernels:]
 
 
 def test_launches_keep_their_threads_within_32_bits():

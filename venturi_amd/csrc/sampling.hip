@@ -21,6 +21,12 @@
 // 21 to clear and count, which the LDS atomics and the vector unit share, 8 to choose, 3 to find the occurrence. Counters in
 // memory shared by several workgroups of a row gain nothing (one row 46 us as here, 32 rows 150 us): the atomics and the 256 KB
 // that one of them reads at the end cost what the shorter count saves.
+//
+// Kept distributions are two or three launches: distribution_scan() looks at few long rows, distribution_cut() finds the last token
+// that a row keeps and the kept mass, and distribution() writes every token's probability. A row that limits leave at most 256 of,
+// and one without limits, need no histogram. The write is bound by memory (96 rows of 151936 bf16 logits: 15 us for 88 MB, 5.8
+// TB/s), the cut by its row's one CU (us, of the same 96 rows, all three together: 39 without limits, 31 with top_k 50, 55 with
+// top_p alone: 21 of them the count, 4 the largest class, 10 the turns' masses, 10 the choice, 8 the search).
 #include "common.hpp"
 
 #include <climits>
@@ -149,7 +155,7 @@ struct Shared {
     int heavy, top, above_min, place, rank, count;
     bool whole;                      // the chosen class has no occurrence after the chosen one
     // Of distribution rows: chunks of 16 vectors by the upper and then the lower byte of their largest logits, the chunks to
-    // look through, their candidates by order and index, and what waves have found.
+    // look through, and their candidates by order and index.
     int bins[2][256];
     int bin, above;
     unsigned short listed[kListed];
@@ -458,7 +464,7 @@ __device__ Choice choose(Shared& s, const Settings& set) {
             int length = all_above ? limit : min(limit, s.above_min);
             const double share = set.top_p;
             if (!(share >= 1.0)) {
-                const double border = share * prefix_mass(limit);
+                const double border = share * (prefix_mass(limit));
                 length = min(length, border > 0.0 ? tokens_below(border, false) : 0);
             }
             length = max(length, 1);
@@ -545,6 +551,13 @@ struct Cut {
     int place;            // kNone: the row keeps nothing
 };
 
+// A part of a row: its largest logit, and where the row's whole mass counts, the mass in units of that one's weight.
+struct Part {
+    double mass;
+    float top;
+    int unused;
+};
+
 struct Operands {
     const void* logits;
     const float* uniforms;
@@ -554,8 +567,11 @@ struct Operands {
     const float* min_p;
     std::int64_t* tokens;
     float* probabilities;
-    Cut* cuts;  // of the distribution, in place of tokens and uniforms
-    int rows, vocab;
+    // Of the distribution, in place of tokens and uniforms: a row's cut, its parts, and its chunks' largest logits.
+    Cut* cuts;
+    Part* parts;
+    short* largest;
+    int rows, vocab, part_count, chunk_count;
 
     __device__ __forceinline__ Settings settings(int row) const {
         return {temperature ? temperature[row] : 1.0f, top_p ? top_p[row] : 1.0f, min_p ? min_p[row] : 0.0f, uniforms ? uniforms[row] : 0.0f,
@@ -600,6 +616,24 @@ struct Edge {
     }
     __device__ __forceinline__ bool match(const Pattern& p) const { return live && ((bits ^ p.bits) & p.mask & 0xffff) == 0; }
 };
+
+// A row's complete histogram, and its chunks' largest logits.
+__device__ __forceinline__ void count_row(Shared& s, const Row& row, const Edge& edge) {
+    const int t = threadIdx.x;
+    each_vector(
+        row.whole(), row.vectors,
+        [&] {
+            clear(s);
+            if (edge.live) count_element(s, edge.bits);
+        },
+        [&](const uint4& w, int i, bool live) {
+            if (live) count_vector(s, w);
+            const short largest = largest_of_16(w);  // past the end of the last vector again, which lists no chunk too few
+            if ((t & 15) == 15) s.largest[(i * kThreads + t) >> 4] = largest;
+        },
+        [&] { sweep(s); });
+    __syncthreads();
+}
 
 // Lists the row's chunks that may hold the class, in order: those whose largest logit is not below it. One wave; their number.
 __device__ __forceinline__ int list_chunks(const Shared& s, const Row& row, const Pattern& p, int* list) {
@@ -671,37 +705,245 @@ __device__ __forceinline__ int edge_match(const Row& row, const Edge& edge, cons
     return __popcll(all);
 }
 
-// The last of up to `kept` largest logits that the other limits leave, found without the histogram; false if they are too many
-// for that. The `kept` largest of the chunks' largest logits bound the row's `kept` largest from below: the logits from that
-// bound on are all in those chunks, and few. They are put in order by counting who is ahead, a thread each, and the limits
-// go by running sums of 64 bits over them. (5 rows of 248320, top_k 50, top_p 0.95: 43.9 us through the histogram.)
-template <class T>
-__device__ __forceinline__ bool cut_largest(Shared& s, const Row& row, const Edge& edge, const Settings& set, int kept, Cut& cut) {
-    constexpr int kInf = static_cast<int>(Bits<T>::kInf), kOwn = 4 * kChunks / kThreads;
-    const int t = threadIdx.x, wave = t >> 6, lane = t & 63, chunks = (row.vectors + 15) / 16;
-    if (chunks < kept || kept > kCandidates) return false;
-    if (t < 512) (&s.bins[0][0])[t] = 0;
-    if (t == 0) s.count = s.rank = 0;
-    each_vector(
-        row.whole(), row.vectors, [] {},
-        [&](const uint4& w, int i, bool) {
-            const short largest = largest_of_16(w);
-            if ((t & 15) == 15) s.largest[(i * kThreads + t) >> 4] = largest;
-        },
-        [] {});
+// The token of the rank-th occurrence of the class: in the head, in the vectors or in the tail. (choose() has ended with a
+// barrier: the histogram's memory is free.)
+__device__ __forceinline__ void find_token(Shared& s, const Row& row, const Edge& edge, const Choice& choice, std::int64_t* token) {
+    const int t = threadIdx.x, wave = t >> 6;
+    const Pattern pattern(choice.place);
+    int *counts = reinterpret_cast<int*>(s.histogram), *list = counts + kChunks;
+    if (wave == 0) {
+        const int n = edge_match(row, edge, pattern, false, choice.rank, token);
+        const int listed = list_chunks(s, row, pattern, list);
+        if (t == 0) s.heavy = n, s.top = listed, s.count = 0;
+    }
     __syncthreads();
-    // The kept-th largest of the chunks' largest, by bytes of its distance from the lowest. Infinities and NaN below count as no
-    // chunk; a chunk with a NaN above infinity is looked through, but not counted on.
-    int own[kOwn];
+    const int first = s.heavy, listed = s.top, rank = choice.rank - first;
+    if (rank < 0) return;
+    const int found = count_matches(row, pattern, rank, list, listed, counts, &s.count);
+    if (wave != 0) return;
+    if (found > rank)
+        write_match(row, pattern, rank, list, listed, counts, token);
+    else
+        edge_match(row, edge, pattern, true, rank - found, token);
+}
+
+// What of a row decides its distribution.
+struct Limits {
+    bool open;  // without limits
+    int kept;   // at most so many tokens; 0: any number
+
+    __device__ __forceinline__ explicit Limits(const Settings& set) {
+        kept = set.temperature > 0.0f ? max(set.top_k, 0) : 1;
+        open = kept == 0 && set.top_p >= 1.0f && set.min_p <= 0.0f;
+    }
+    // Whether the largest logits of chunks of 16 vectors are a bound on what is kept.
+    __device__ __forceinline__ bool few(const Row& row) const { return kept > 0 && kept <= min((row.vectors + 15) / 16, kCandidates); }
+};
+
+template <class T>
+__device__ __forceinline__ float value_of(std::uint32_t bits) {
+    return to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(bits)));
+}
+
+// Sums of a row's weights 2^((x - top) heat) without a class for each: of 32 bits with the exponent's rest, added in eights and
+// then in 64 bits. Of 64 bits at temperatures whose inverse, or whose products with differences of any two logits, leave the
+// range of 32.
+template <class T>
+struct Weights {
+    double heat;
+    float top, high, low, least;
+    bool wide;
+
+    __device__ __forceinline__ Weights(float top, double heat)
+        : heat(heat), top(top), high(static_cast<float>(heat)), low(static_cast<float>(heat - static_cast<double>(high))), least(-160.0f / high),
+          wide(top == __builtin_inff() || !(heat >= 1e-30 && heat <= 1e30)) {}
+    __device__ __forceinline__ float near(std::uint32_t bits) const {
+        const float d = fmaxf(value_of<T>(bits) - top, least), e = d * high;  // NaN and -inf weigh 2^-160: nothing
+        const float rest = fmaf(d, low, fmaf(d, high, -e)), w = __builtin_amdgcn_exp2f(e);
+        return fmaf(w, rest * 0.693147181f, w);
+    }
+    __device__ __forceinline__ float far(std::uint32_t bits) const {
+        const float x = value_of<T>(bits);
+        return x == top ? 1.0f : static_cast<float>(falling_power((static_cast<double>(x) - static_cast<double>(top)) * heat));
+    }
+    __device__ __forceinline__ float operator()(std::uint32_t bits) const { return wide ? far(bits) : near(bits); }
+    __device__ __forceinline__ float sum(const uint4& v) const {
+        if (wide) {
+            float all = 0.0f;
+            for (int j = 0; j < 8; ++j) all += far(element(v, j));
+            return all;
+        }
+        float x[8];
 #pragma unroll
-    for (int j = 0; j < kOwn; ++j) own[j] = t + j * kThreads < chunks ? s.largest[t + j * kThreads] + 32768 : 0;
-    const auto counts = [&](int v) { return v > 32768 - kInf && v <= 32768 + kInf; };
+        for (int j = 0; j < 8; ++j) x[j] = near(element(v, j));
+        return ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+    }
+};
+
+template <class T>
+__device__ __forceinline__ float raised(float top, const uint4& w) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, value_of<T>(element(w, j)));
+    return top;
+}
+__device__ __forceinline__ float wave_top(float top) {
+#pragma unroll
+    for (int step = 32; step; step >>= 1) top = fmaxf(top, __shfl_xor(top, step, 64));
+    return top;
+}
+
+// Few and long rows are first looked at by the whole card: of a row without limits the largest logit and the mass of its parts, of
+// one that keeps few logits its chunks' largest ones. (Else a row's one CU sees and sums them. Us, with and without, for 5 rows
+// of 248320, 32 of 151936 and 96 of 151936: no limits 10.8 / 35.9, 17.9 / 29.1 and 30.5 / 38.5; top_k 50 15.3 / 19.7, 21.7 /
+// 22.3 and 32.1 / 30.7; in batches of 96 with mixed settings other rows take longest, 55. 16 rows of 32003, which a workgroup's registers hold:
+// 10.7 / 10.7 and 14.0 / 13.0.)
+constexpr int kScanThreads = 256, kScanWaves = kScanThreads / 64, kScanVectors = 4;  // vectors of a thread
+constexpr int kScanPart = kScanThreads * kScanVectors;
+constexpr int kScanRows = 32, kScanVocab = 8 * kFirst * kThreads;  // up to so many rows of more logits
+
+template <class T>
+__global__ __launch_bounds__(kScanThreads) void distribution_scan(Operands o) {
+    __shared__ float tops[kScanWaves];
+    __shared__ double masses[kScanWaves];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, index = blockIdx.y, begin = blockIdx.x * kScanPart;
+    const Row row(o.logits, index, o.vocab);
+    const Settings set = o.settings(index);
+    const Limits limits(set);
+    if (!limits.open && !limits.few(row)) return;
+    const bool edge = blockIdx.x == 0 && t < row.head + row.tail, some = begin < row.vectors;
+    const std::uint32_t edge_bits = edge ? row.start[row.edge(t)] : 0;
+    uint4 w[kScanVectors];
+    if (some) {
+#pragma unroll
+        for (int j = 0; j < kScanVectors; ++j) w[j] = row.whole()[min(begin + j * kScanThreads + t, row.vectors - 1)];
+    }
+    if (!limits.open) {
+        if (!some) return;
+#pragma unroll
+        for (int j = 0; j < kScanVectors; ++j) {
+            const short largest = largest_of_16(w[j]);  // past the end the last vector again
+            const int chunk = (begin + j * kScanThreads + t) >> 4;
+            if ((t & 15) == 15 && 16 * chunk < row.vectors) o.largest[static_cast<std::int64_t>(index) * o.chunk_count + chunk] = largest;
+        }
+        return;
+    }
+    const float none = -__builtin_inff();
+    float top = edge ? fmaxf(value_of<T>(edge_bits), none) : none;
+    if (some) {
+#pragma unroll
+        for (int j = 0; j < kScanVectors; ++j) top = raised<T>(top, w[j]);
+    }
+    top = wave_top(top);
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kScanWaves; ++i) top = fmaxf(top, tops[i]);
+    double mass = 0.0;
+    if (top > none) {
+        const Weights<T> weight(top, heat_of(set.temperature));
+        if (edge) mass = weight(edge_bits);
+        if (some) {
+#pragma unroll
+            for (int j = 0; j < kScanVectors; ++j) {
+                const float sum = weight.sum(w[j]);
+                if (begin + j * kScanThreads + t < row.vectors) mass += sum;
+            }
+        }
+    }
+    mass = wave_sum(mass);
+    if (lane == 0) masses[wave] = mass;
+    __syncthreads();
+    if (t != 0) return;
+    mass = 0.0;
+    for (int i = 0; i < kScanWaves; ++i) mass += masses[i];
+    o.parts[static_cast<std::int64_t>(index) * o.part_count + blockIdx.x] = {mass, top, 0};
+}
+
+// A row without limits, down to the lowest number; none at all if its largest logit is no class.
+template <class T>
+__device__ __forceinline__ Cut cut_of_all(float top, double heat, double mass) {
+    if (top == -__builtin_inff()) return {0.0, heat, INT_MAX, 0.0f, kNone};
+    return {top, heat, INT_MAX, static_cast<float>(1.0 / mass), 0x8000 + static_cast<int>(Bits<T>::kInf) - 1};
+}
+
+// The same from its parts, two a lane at most. One wave; its first lane's.
+template <class T>
+__device__ __forceinline__ Cut join_parts(const Part* parts, int count, double heat) {
+    const int lane = threadIdx.x & 63;
+    const bool there[2] = {lane < count, lane + 64 < count};
+    const Part part[2] = {parts[there[0] ? lane : 0], parts[there[1] ? lane + 64 : 0]};
+    const float top = wave_top(fmaxf(part[0].top, part[1].top));
+    double mass = 0.0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const double keep = part[i].top == top ? 1.0 : falling_power((static_cast<double>(part[i].top) - static_cast<double>(top)) * heat);
+        if (there[i]) mass += keep * part[i].mass;
+    }
+    return cut_of_all<T>(top, heat, wave_sum(mass));
+}
+
+// The same by the row's workgroup (257 rows of 32003: 33.5 us through the histogram, 26).
+template <class T>
+__device__ __forceinline__ Cut keep_all(Shared& s, const Row& row, const Edge& edge, double heat) {
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+    const float none = -__builtin_inff();
+    float top = edge.live ? fmaxf(value_of<T>(edge.bits), none) : none;
+    // Rows of up to 57344 logits stay in registers.
+    const bool held = row.vectors > 0 && row.vectors <= kFirst * kThreads;
+    uint4 first[kFirst];
+    if (held) {
+#pragma unroll
+        for (int j = 0; j < kFirst; ++j) first[j] = row.whole()[min(t + j * kThreads, row.vectors - 1)];
+#pragma unroll
+        for (int j = 0; j < kFirst; ++j) top = raised<T>(top, first[j]);
+    } else {
+        each_vector(row.whole(), row.vectors, [] {}, [&](const uint4& w, int, bool) { top = raised<T>(top, w); }, [] {});
+    }
+    top = wave_top(top);
+    if (lane == 0) s.wave_top[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) top = fmaxf(top, s.wave_top[i]);
+    const Weights<T> weight(top, heat);
+    double mass = edge.live ? weight(edge.bits) : 0.0;
+    if (held) {
+#pragma unroll
+        for (int j = 0; j < kFirst; ++j) {
+            if (j * kThreads >= row.vectors) break;
+            const float sum = weight.sum(first[j]);
+            if (t + j * kThreads < row.vectors) mass += sum;
+        }
+    } else {
+        each_vector(
+            row.whole(), row.vectors, [] {},
+            [&](const uint4& w, int, bool live) {
+                const float sum = weight.sum(w);
+                if (live) mass += sum;
+            },
+            [] {});
+    }
+    mass = wave_sum(mass);
+    if (lane == 0) s.wave_mass[wave] = mass;
+    __syncthreads();
+    mass = 0.0;
+    for (int i = 0; i < kWaves; ++i) mass += s.wave_mass[i];
+    return cut_of_all<T>(top, heat, mass);
+}
+
+// The `kept`-th largest of the chunks' largest logits in order (signed_bits + 32768, a thread's in `own`, 0: none), which
+// bounds the row's from below; -1 if there are fewer. Infinities below and NaN count as no chunk. By the upper and then the
+// lower byte; the bins are clear at first.
+template <class T, int OWN>
+__device__ __forceinline__ int bound_of(Shared& s, const int (&own)[OWN], int kept) {
+    constexpr int kInf = static_cast<int>(Bits<T>::kInf);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     int least = 0, left = kept;
 #pragma unroll
     for (int level = 0; level < 2; ++level) {
 #pragma unroll
-        for (int j = 0; j < kOwn; ++j)
-            if (counts(own[j]) && (level == 0 || own[j] >> 8 == least >> 8)) atomicAdd(&s.bins[level][level == 0 ? own[j] >> 8 : own[j] & 255], 1);
+        for (int j = 0; j < OWN; ++j)
+            if (own[j] > 32768 - kInf && own[j] <= 32768 + kInf && (level == 0 || own[j] >> 8 == least >> 8))
+                atomicAdd(&s.bins[level][level == 0 ? own[j] >> 8 : own[j] & 255], 1);
         __syncthreads();
         if (wave == 0) {  // bins from the highest down, four a lane
             const int high = 255 - 4 * lane;
@@ -718,14 +960,28 @@ __device__ __forceinline__ bool cut_largest(Shared& s, const Row& row, const Edg
         }
         __syncthreads();
         const int bin = s.bin;
-        if (bin < 0) return false;
+        if (bin < 0) return -1;
         left -= s.above;
         least |= bin << (level == 0 ? 8 : 0);
         __syncthreads();
     }
+    return least;
+}
+
+// The last of up to `kept` largest logits that the other limits leave, found without the histogram; false if they are too many
+// for that. The logits from `least` on are all in the chunks that reach it, and few. They are put in order by counting who is
+// ahead, a thread each, and the limits go by running sums of 64 bits over them. (5 rows of 248320, top_k 50, top_p 0.95: 43.9
+// us through the histogram.)
+template <class T, int OWN>
+__device__ __forceinline__ bool cut_largest(Shared& s, const Row& row, const Edge& edge, const Settings& set, int kept, const int (&own)[OWN],
+                                            int least, Cut& cut) {
+    constexpr int kInf = static_cast<int>(Bits<T>::kInf);
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+    if (t == 0) s.count = s.rank = 0;
+    __syncthreads();
     // List the chunks, and the candidates in them.
 #pragma unroll
-    for (int j = 0; j < kOwn; ++j) {
+    for (int j = 0; j < OWN; ++j) {
         const bool may = own[j] >= least;
         if (may) {
             const int at = atomicAdd(&s.count, 1);
@@ -737,7 +993,7 @@ __device__ __forceinline__ bool cut_largest(Shared& s, const Row& row, const Edg
     if (listed > kListed) return false;
     const auto candidate = [&](std::uint32_t bits, int index) {
         const int order = signed_bits(bits) + 32768;
-        if (order < least || !counts(order)) return;
+        if (order < least || order <= 32768 - kInf || order > 32768 + kInf) return;
         const int at = atomicAdd(&s.rank, 1);
         if (at < kCandidates) s.candidates[at] = static_cast<std::uint64_t>(order) << 32 | static_cast<std::uint32_t>(~index);
     };
@@ -764,20 +1020,19 @@ __device__ __forceinline__ bool cut_largest(Shared& s, const Row& row, const Edg
     }
     __syncthreads();
     if (wave != 0) return true;
-    const auto value_of = [](std::uint64_t c) {
+    const auto value = [](std::uint64_t c) {
         const int order = static_cast<int>(c >> 32) - 32768;
-        const std::uint32_t bits = order < 0 ? 0x8000 - order : order;
-        return to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(bits)));
+        return value_of<T>(order < 0 ? 0x8000 - order : order);
     };
     // Four candidates a lane, in order.
-    const float top = value_of(s.ordered[0]);
+    const float top = value(s.ordered[0]);
     const double heat = heat_of(set.temperature), least_weight = set.min_p, share = set.top_p;
     double w4[4], four = 0.0;
     int above_min = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int at = 4 * lane + i;
-        const float v = value_of(s.ordered[min(at, found - 1)]);
+        const float v = value(s.ordered[min(at, found - 1)]);
         const double weight = v == top ? 1.0 : falling_power((static_cast<double>(v) - static_cast<double>(top)) * heat);
         w4[i] = at < kept ? weight : 0.0;
         above_min += at < kept && weight >= least_weight;
@@ -812,143 +1067,80 @@ __device__ __forceinline__ bool cut_largest(Shared& s, const Row& row, const Edg
     return true;
 }
 
-// A row without limits keeps all: its largest logit and the sum of its weights, of 32 bits with the exponent's rest, added in
-// eights and then in 64 bits. 257 rows of 32003: 33.5 -> KERNEL us.
+// What a row keeps: a workgroup per row. Rows without limits are summed; up to 256 largest logits are put in order; else the
+// classes are counted and chosen from as sample() does.
 template <class T>
-__device__ __forceinline__ void keep_all(Shared& s, const Row& row, const Edge& edge, const Settings& set, Cut& cut) {
-    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
-    const float none = -__builtin_inff();
-    const auto value = [](std::uint32_t bits) { return to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(bits))); };
-    float top = edge.live ? fmaxf(value(edge.bits), none) : none;
-    const auto raise = [&](const uint4& w) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, value(element(w, j)));
-    };
-    // Rows of up to 57344 logits stay in registers.
-    const bool held = row.vectors > 0 && row.vectors <= kFirst * kThreads;
-    uint4 first[kFirst];
-    if (held) {
-#pragma unroll
-        for (int j = 0; j < kFirst; ++j) first[j] = row.whole()[min(t + j * kThreads, row.vectors - 1)];
-#pragma unroll
-        for (int j = 0; j < kFirst; ++j) raise(first[j]);
-    } else {
-        each_vector(row.whole(), row.vectors, [] {}, [&](const uint4& w, int, bool) { raise(w); }, [] {});
-    }
-#pragma unroll
-    for (int step = 32; step; step >>= 1) top = fmaxf(top, __shfl_xor(top, step, 64));
-    if (lane == 0) s.wave_top[wave] = top;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) top = fmaxf(top, s.wave_top[i]);
-    const double heat = heat_of(set.temperature);
-    const float high = static_cast<float>(heat), low = static_cast<float>(heat - static_cast<double>(high));
-    const auto weight = [&](std::uint32_t bits) {
-        const float d = fmaxf(value(bits) - top, none), e = d * high;  // NaN weighs nothing
-        const float rest = fmaf(d, low, fmaf(d, high, -e)), w = __builtin_amdgcn_exp2f(e);
-        return e > -150.0f ? fmaf(w, rest * 0.693147181f, w) : 0.0f;
-    };
-    const bool infinite = top == -none;
-    double mass = 0.0;
-    if (edge.live) mass = infinite ? value(edge.bits) == top : weight(edge.bits);
-    const auto add = [&](const uint4& w, bool live) {
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = infinite ? value(element(w, j)) == top : weight(element(w, j));
-        const float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-        if (live) mass += sum;
-    };
-    if (held) {
-#pragma unroll
-        for (int j = 0; j < kFirst; ++j)
-            if (j * kThreads < row.vectors) add(first[j], t + j * kThreads < row.vectors);
-    } else {
-        each_vector(row.whole(), row.vectors, [] {}, [&](const uint4& w, int, bool live) { add(w, live); }, [] {});
-    }
-    mass = wave_sum(mass);
-    if (lane == 0) s.wave_mass[wave] = mass;
-    __syncthreads();
-    if (t != 0) return;
-    mass = 0.0;
-    for (int i = 0; i < kWaves; ++i) mass += s.wave_mass[i];
-    cut.place = top == none ? kNone : 0x8000 + static_cast<int>(Bits<T>::kInf) - 1;  // the lowest number
-    cut.max = top;
-    cut.heat = heat;
-    cut.inverse = static_cast<float>(1.0 / mass);
-    cut.index = INT_MAX;
-}
-
-// A workgroup per row. CUT: what the row keeps, for distribution(), in place of a token.
-template <class T, bool CUT>
-__global__ __launch_bounds__(kThreads) void sample(Operands o) {
+__global__ __launch_bounds__(kThreads) void distribution_cut(Operands o) {
+    constexpr int kOwn = 4 * kChunks / kThreads;
     extern __shared__ __align__(16) unsigned char memory[];
     Shared& s = *reinterpret_cast<Shared*>(memory);
     const int t = threadIdx.x, wave = t >> 6, index = blockIdx.x;
     const Row row(o.logits, index, o.vocab);
     const Settings set = o.settings(index);
+    const Limits limits(set);
     const Edge edge(row);
-    if constexpr (CUT) {
-        const bool greedy = !(set.temperature > 0.0f);
-        if (!greedy && set.top_k <= 0 && set.top_p >= 1.0f && set.min_p <= 0.0f) {
-            keep_all<T>(s, row, edge, set, o.cuts[index]);
-            return;
+    const double heat = heat_of(set.temperature);
+    const bool scanned = o.part_count > 0;
+    Cut& cut = o.cuts[index];
+    if (limits.open) {
+        Cut all;
+        if (!scanned) all = keep_all<T>(s, row, edge, heat);
+        else if (wave == 0) all = join_parts<T>(o.parts + static_cast<std::int64_t>(index) * o.part_count, o.part_count, heat);
+        if (t == 0) cut = all;
+        return;
+    }
+    if (limits.few(row)) {
+        if (!scanned) {
+            each_vector(
+                row.whole(), row.vectors, [] {},
+                [&](const uint4& w, int i, bool) {
+                    const short largest = largest_of_16(w);
+                    if ((t & 15) == 15) s.largest[(i * kThreads + t) >> 4] = largest;
+                },
+                [] {});
         }
-        const int kept = greedy ? 1 : set.top_k;  // at most
-        if (kept > 0 && cut_largest<T>(s, row, edge, set, kept, o.cuts[index])) return;
+        if (t < 512) (&s.bins[0][0])[t] = 0;
+        __syncthreads();
+        const int chunks = (row.vectors + 15) / 16;
+        const short* known = scanned ? o.largest + static_cast<std::int64_t>(index) * o.chunk_count : s.largest;
+        int own[kOwn];
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) own[j] = t + j * kThreads < chunks ? known[t + j * kThreads] + 32768 : 0;
+        const int least = bound_of<T>(s, own, limits.kept);
+        if (least >= 0 && cut_largest<T>(s, row, edge, set, limits.kept, own, least, cut)) return;
         __syncthreads();
     }
-    each_vector(
-        row.whole(), row.vectors,
-        [&] {
-            clear(s);
-            if (edge.live) count_element(s, edge.bits);
-        },
-        [&](const uint4& w, int i, bool live) {
-            if (live) count_vector(s, w);
-            const short largest = largest_of_16(w);  // past the end of the last vector again, which lists no chunk too few
-            if ((t & 15) == 15) s.largest[(i * kThreads + t) >> 4] = largest;
-        },
-        [&] { sweep(s); });
-    __syncthreads();
-    const Choice choice = choose<T, CUT>(s, set);
-    std::int64_t* token;
-    if constexpr (CUT) {
-        Cut& cut = o.cuts[index];
-        token = &cut.index;
-        if (t == 0) {
-            cut.place = choice.place;
-            cut.max = choice.place == kNone ? 0.0 : class_value<T>(s.top);
-            cut.heat = heat_of(set.temperature);
-            cut.inverse = static_cast<float>(1.0 / s.probability);
-            cut.index = INT_MAX;
-        }
-        if (choice.place == kNone || s.whole) return;  // choose() has ended with a barrier
-    } else {
-        token = o.tokens + index;
-        if (t == 0 && o.probabilities) o.probabilities[index] = static_cast<float>(s.probability);
-        if (choice.place == kNone) {
-            if (t == 0) *token = -1;
-            return;
-        }
-    }
-    // The rank-th occurrence of the class: in the head, in the vectors or in the tail. (choose() has ended with a barrier:
-    // the histogram's memory is free.)
-    const Pattern pattern(choice.place);
-    int *counts = reinterpret_cast<int*>(s.histogram), *list = counts + kChunks;
-    if (wave == 0) {
-        const int n = edge_match(row, edge, pattern, false, choice.rank, token);
-        const int listed = list_chunks(s, row, pattern, list);
-        if (t == 0) s.heavy = n, s.top = listed, s.count = 0;
+    count_row(s, row, edge);
+    const Choice choice = choose<T, true>(s, set);
+    const bool ended = choice.place == kNone || s.whole;
+    if (t == 0) {
+        cut.max = choice.place == kNone ? 0.0 : class_value<T>(s.top);
+        cut.heat = heat;
+        cut.inverse = static_cast<float>(1.0 / s.probability);
+        cut.place = choice.place;
+        if (ended) cut.index = INT_MAX;
     }
     __syncthreads();
-    const int first = s.heavy, listed = s.top, rank = choice.rank - first;
-    if (rank < 0) return;
-    const int found = count_matches(row, pattern, rank, list, listed, counts, &s.count);
-    if (wave != 0) return;
-    if (found > rank)
-        write_match(row, pattern, rank, list, listed, counts, token);
-    else
-        edge_match(row, edge, pattern, true, rank - found, token);
+    if (!ended) find_token(s, row, edge, choice, &cut.index);
+}
+
+// A workgroup per row.
+template <class T>
+__global__ __launch_bounds__(kThreads) void sample(Operands o) {
+    extern __shared__ __align__(16) unsigned char memory[];
+    Shared& s = *reinterpret_cast<Shared*>(memory);
+    const int t = threadIdx.x, index = blockIdx.x;
+    const Row row(o.logits, index, o.vocab);
+    const Settings set = o.settings(index);
+    const Edge edge(row);
+    count_row(s, row, edge);
+    const Choice choice = choose<T, false>(s, set);
+    if (t == 0 && o.probabilities) o.probabilities[index] = static_cast<float>(s.probability);
+    if (choice.place == kNone) {
+        if (t == 0) o.tokens[index] = -1;
+        return;
+    }
+    find_token(s, row, edge, choice, o.tokens + index);
 }
 
 constexpr int kWriteThreads = 256;
@@ -998,16 +1190,35 @@ __global__ __launch_bounds__(kWriteThreads) void distribution(Operands o) {
     *reinterpret_cast<float4u*>(out + first + 4) = float4u{p[4], p[5], p[6], p[7]};
 }
 
-template <class T, bool CUT>
+template <class T>
 void launch(const Operands& o, hipStream_t stream) {
     static LdsLimit limit;
-    limit.raise(sample<T, CUT>, sizeof(Shared));
-    sample<T, CUT><<<o.rows, kThreads, sizeof(Shared), stream>>>(o);
-    if constexpr (CUT) {
+    limit.raise(sample<T>, sizeof(Shared));
+    sample<T><<<o.rows, kThreads, sizeof(Shared), stream>>>(o);
+}
+
+template <class T>
+void launch_distribution(const Operands& o, hipStream_t stream) {
+    static LdsLimit limit;
+    limit.raise(distribution_cut<T>, sizeof(Shared));
+    if (o.part_count > 0) {
+        distribution_scan<T><<<dim3(o.part_count, o.rows), kScanThreads, 0, stream>>>(o);
         check(hipGetLastError());
-        const unsigned parts = std::max((o.vocab / 8 + kWriteThreads - 1) / kWriteThreads, 1);
-        distribution<T><<<dim3(parts, o.rows), kWriteThreads, 0, stream>>>(o);
     }
+    distribution_cut<T><<<o.rows, kThreads, sizeof(Shared), stream>>>(o);
+    check(hipGetLastError());
+    const unsigned parts = std::max((o.vocab / 8 + kWriteThreads - 1) / kWriteThreads, 1);
+    distribution<T><<<dim3(parts, o.rows), kWriteThreads, 0, stream>>>(o);
+}
+
+// Of a row that is looked at first; 0: it is not.
+int part_count(int rows, int vocab) { return rows <= kScanRows && vocab > kScanVocab ? (vocab / 8 + kScanPart - 1) / kScanPart : 0; }
+int chunk_count(int vocab) { return (vocab / 8 + 15) / 16; }
+static_assert(kMaxVocab / 8 <= 128 * kScanPart, "two parts a lane");
+
+std::uint64_t distribution_bytes(int rows, int vocab) {
+    const int parts = part_count(rows, vocab);
+    return (sizeof(Cut) + sizeof(Part) * parts + (parts ? sizeof(short) * chunk_count(vocab) : 0)) * static_cast<std::uint64_t>(rows);
 }
 
 void require_geometry(int rows, int vocab) {
@@ -1028,11 +1239,11 @@ VT_EXPORT int venturi_sample_run(const void* logits, const float* uniforms, cons
         vt::require(logits && uniforms && tokens, "null sampling operand");
         vt::require(vt::aligned(logits, 16), "logits must be 16-byte aligned");
         const auto s = static_cast<hipStream_t>(stream);
-        const vt::Operands o{logits, uniforms, temperature, top_k, top_p, min_p, tokens, probabilities, nullptr, rows, vocab};
+        const vt::Operands o{logits, uniforms, temperature, top_k, top_p, min_p, tokens, probabilities, nullptr, nullptr, nullptr, rows, vocab, 0, 0};
         if (dtype == vt::kF16)
-            vt::launch<__half, false>(o, s);
+            vt::launch<__half>(o, s);
         else if (dtype == vt::kBF16)
-            vt::launch<__hip_bfloat16, false>(o, s);
+            vt::launch<__hip_bfloat16>(o, s);
         else
             throw vt::Invalid("sampling takes fp16 or bf16 logits");
     });
@@ -1043,7 +1254,7 @@ VT_EXPORT std::uint64_t venturi_distribution_bytes(int rows, int vocab) {
     vt::host_guarded([&] {
         vt::require_geometry(rows, vocab);
         vt::require(rows <= vt::kMaxDistributionRows, "a distribution takes at most 65535 rows");
-        bytes = sizeof(vt::Cut) * static_cast<std::uint64_t>(rows);
+        bytes = vt::distribution_bytes(rows, vocab);
     });
     return bytes;
 }
@@ -1056,15 +1267,19 @@ VT_EXPORT int venturi_distribution_run(const void* logits, const float* temperat
         vt::require(rows <= vt::kMaxDistributionRows, "a distribution takes at most 65535 rows");
         vt::require(logits && probabilities, "null distribution operand");
         vt::require(vt::aligned(logits, 16) && vt::aligned(probabilities, 4), "logits must be 16-byte aligned");
-        vt::require(workspace && available >= sizeof(vt::Cut) * static_cast<std::uint64_t>(rows) && vt::aligned(workspace, 256),
+        vt::require(workspace && available >= vt::distribution_bytes(rows, vocab) && vt::aligned(workspace, 256),
                     "a distribution needs its workspace, 256-byte aligned");
         const auto s = static_cast<hipStream_t>(stream);
-        const vt::Operands o{logits, nullptr, temperature, top_k, top_p, min_p, nullptr, probabilities,
-                             static_cast<vt::Cut*>(workspace), rows, vocab};
+        auto* cuts = static_cast<vt::Cut*>(workspace);
+        auto* parts = reinterpret_cast<vt::Part*>(cuts + rows);
+        const int part_count = vt::part_count(rows, vocab);
+        auto* largest = reinterpret_cast<short*>(parts + static_cast<std::int64_t>(rows) * part_count);
+        const vt::Operands o{logits, nullptr, temperature, top_k, top_p, min_p, nullptr, probabilities, cuts, parts, largest,
+                             rows, vocab, part_count, vt::chunk_count(vocab)};
         if (dtype == vt::kF16)
-            vt::launch<__half, true>(o, s);
+            vt::launch_distribution<__half>(o, s);
         else if (dtype == vt::kBF16)
-            vt::launch<__hip_bfloat16, true>(o, s);
+            vt::launch_distribution<__hip_bfloat16>(o, s);
         else
             throw vt::Invalid("a distribution takes fp16 or bf16 logits");
     });
