@@ -349,7 +349,7 @@ __device__ __forceinline__ double heat_of(float temperature) {
 // Chooses from the workgroup's complete histogram: the token at the uniform's place, or with LAST the last kept one. The
 // probability that it leaves is the token's, or with LAST the kept mass in units of the largest weight.
 template <class T, bool LAST>
-__device__ Choice choose(Shared& s, const Settings& set) {
+__device__ __forceinline__ Choice choose(Shared& s, const Settings& set) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, heavy = s.heavy;
     for (int turn = wave; turn < kTurns; turn += kWaves) {
         if (!__any(Lane<T>::occurs(s, heavy, turn))) continue;
@@ -770,7 +770,12 @@ struct Weights {
     __device__ __forceinline__ float sum(const uint4& v) const {
         if (wide) {
             float all = 0.0f;
-            for (int j = 0; j < 8; ++j) all += far(element(v, j));
+            uint4 u = v;
+#pragma unroll 1
+            for (int j = 0; j < 8; ++j) {
+                all += far(u.x & 0xffff);
+                u = make_uint4(u.x >> 16 | u.y << 16, u.y >> 16 | u.z << 16, u.z >> 16 | u.w << 16, u.w >> 16);
+            }
             return all;
         }
         float x[8];
