@@ -25,7 +25,7 @@
 // Kept distributions are two or three launches: distribution_scan() looks at few long rows, distribution_cut() finds the last token
 // that a row keeps and the kept mass, and distribution() writes every token's probability. A row that limits leave at most 256 of,
 // and one without limits, need no histogram. The write is bound by memory (96 rows of 151936 bf16 logits: 15 us for 88 MB, 5.8
-// TB/s), the cut by its row's one CU (us, of the same 96 rows, all three together: 39 without limits, 31 with top_k 50, 55 with
+// TB/s), the cut by its row's one CU (us, of the same 96 rows, all three together: 38 without limits, 29 with top_k 50, 52 with
 // top_p alone: 21 of them the count, 4 the largest class, 10 the turns' masses, 10 the choice, 8 the search).
 #include "common.hpp"
 
@@ -156,7 +156,7 @@ struct Shared {
     bool whole;                      // the chosen class has no occurrence after the chosen one
     // Of distribution rows: chunks of 16 vectors by the upper and then the lower byte of their largest logits, the chunks to
     // look through, and their candidates by order and index.
-    int bins[2][256];
+    std::uint32_t upper[256], bins[256];
     int bin, above;
     unsigned short listed[kListed];
     std::uint64_t candidates[kCandidates], ordered[kCandidates];
@@ -799,8 +799,8 @@ __device__ __forceinline__ float wave_top(float top) {
 
 // Few and long rows are first looked at by the whole card: of a row without limits the largest logit and the mass of its parts, of
 // one that keeps few logits its chunks' largest ones. (Else a row's one CU sees and sums them. Us, with and without, for 5 rows
-// of 248320, 32 of 151936 and 96 of 151936: no limits 10.8 / 35.9, 17.9 / 29.1 and 30.5 / 38.5; top_k 50 15.3 / 19.7, 21.7 /
-// 22.3 and 32.1 / 30.7; in batches of 96 with mixed settings other rows take longest, 55. 16 rows of 32003, which a workgroup's registers hold:
+// of 248320, 32 of 151936 and 96 of 151936: no limits 11.0 / 35.9, 17.9 / 29.1 and 30.5 / 38.5; top_k 50 14.4 / 19.7, 21.7 /
+// 22.3 and 32.1 / 30.7; in batches of 96 with mixed settings other rows take longest, 52. 16 rows of 32003, which a workgroup's registers hold:
 // 10.7 / 10.7 and 14.0 / 13.0.)
 constexpr int kScanThreads = 256, kScanWaves = kScanThreads / 64, kScanVectors = 4;  // vectors of a thread
 constexpr int kScanPart = kScanThreads * kScanVectors;
@@ -937,7 +937,8 @@ __device__ __forceinline__ Cut keep_all(Shared& s, const Row& row, const Edge& e
 
 // The `kept`-th largest of the chunks' largest logits in order (signed_bits + 32768, a thread's in `own`, 0: none), which
 // bounds the row's from below; -1 if there are fewer. Infinities below and NaN count as no chunk. By the upper and then the
-// lower byte; the bins are clear at first.
+// lower byte; the bins are clear at first, and so are 16 counters for each upper byte (most logits share a few) in the
+// histogram's place.
 template <class T, int OWN>
 __device__ __forceinline__ int bound_of(Shared& s, const int (&own)[OWN], int kept) {
     constexpr int kInf = static_cast<int>(Bits<T>::kInf);
@@ -948,13 +949,26 @@ __device__ __forceinline__ int bound_of(Shared& s, const int (&own)[OWN], int ke
 #pragma unroll
         for (int j = 0; j < OWN; ++j)
             if (own[j] > 32768 - kInf && own[j] <= 32768 + kInf && (level == 0 || own[j] >> 8 == least >> 8))
-                atomicAdd(&s.bins[level][level == 0 ? own[j] >> 8 : own[j] & 255], 1);
+                atomicAdd(level == 0 ? &s.histogram[(own[j] >> 8) * 16 + (lane & 15)] : &s.bins[own[j] & 255], 1u);
         __syncthreads();
+        if (level == 0) {
+            if (threadIdx.x < 256) {
+                std::uint32_t n = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint4 c = reinterpret_cast<const uint4*>(s.histogram)[4 * threadIdx.x + ((i + lane) & 3)];
+                    n += (c.x + c.y) + (c.z + c.w);
+                }
+                s.upper[threadIdx.x] = n;
+            }
+            __syncthreads();
+        }
+        const std::uint32_t* bins = level == 0 ? s.upper : s.bins;
         if (wave == 0) {  // bins from the highest down, four a lane
             const int high = 255 - 4 * lane;
             int n[4], four = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) n[i] = s.bins[level][high - i], four += n[i];
+            for (int i = 0; i < 4; ++i) n[i] = bins[high - i], four += n[i];
             int above = wave_scan(four) - four;
             if (lane == 63 && above + four < left) s.bin = -1;  // fewer than wanted
 #pragma unroll
@@ -975,7 +989,7 @@ __device__ __forceinline__ int bound_of(Shared& s, const int (&own)[OWN], int ke
 
 // The last of up to `kept` largest logits that the other limits leave, found without the histogram; false if they are too many
 // for that. The logits from `least` on are all in the chunks that reach it, and few. They are put in order by counting who is
-// ahead, a thread each, and the limits go by running sums of 64 bits over them. (5 rows of 248320, top_k 50, top_p 0.95: 43.9
+// ahead, 16 lanes for each, and the limits go by running sums of 64 bits over them. (5 rows of 248320, top_k 50, top_p 0.95: 43.9
 // us through the histogram.)
 template <class T, int OWN>
 __device__ __forceinline__ bool cut_largest(Shared& s, const Row& row, const Edge& edge, const Settings& set, int kept, const int (&own)[OWN],
@@ -1017,11 +1031,16 @@ __device__ __forceinline__ bool cut_largest(Shared& s, const Row& row, const Edg
     __syncthreads();
     const int found = s.rank;
     if (found > kCandidates) return false;
-    if (t < found) {
-        const std::uint64_t mine = s.candidates[t];
+    for (int base = 0; base < found; base += kThreads / 16) {
+        const int at = base + (t >> 4);
+        const std::uint64_t mine = s.candidates[min(at, found - 1)];
         int ahead = 0;
-        for (int i = 0; i < found; ++i) ahead += s.candidates[i] > mine;
-        s.ordered[ahead] = mine;
+        for (int i = t & 15; i < found; i += 16) ahead += s.candidates[i] > mine;
+        ahead += moved<0x111, 0xf>(ahead);  // sums over the 16 lanes
+        ahead += moved<0x112, 0xf>(ahead);
+        ahead += moved<0x114, 0xf>(ahead);
+        ahead += moved<0x118, 0xf>(ahead);
+        if ((t & 15) == 15 && at < found) s.ordered[ahead] = mine;
     }
     __syncthreads();
     if (wave != 0) return true;
@@ -1081,11 +1100,21 @@ __global__ __launch_bounds__(kThreads) void distribution_cut(Operands o) {
     Shared& s = *reinterpret_cast<Shared*>(memory);
     const int t = threadIdx.x, wave = t >> 6, index = blockIdx.x;
     const Row row(o.logits, index, o.vocab);
+    const int chunks = (row.vectors + 15) / 16;
+    const bool scanned = o.part_count > 0;
+    if (scanned) {  // used of a row that keeps few, and read beside the settings
+        const short* known = o.largest + static_cast<std::int64_t>(index) * o.chunk_count;
+        short largest[kOwn];
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) largest[j] = j * kThreads < chunks ? known[min(t + j * kThreads, chunks - 1)] : 0;
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j)
+            if (j * kThreads < chunks) s.largest[t + j * kThreads] = largest[j];
+    }
     const Settings set = o.settings(index);
     const Limits limits(set);
     const Edge edge(row);
     const double heat = heat_of(set.temperature);
-    const bool scanned = o.part_count > 0;
     Cut& cut = o.cuts[index];
     if (limits.open) {
         Cut all;
@@ -1095,6 +1124,8 @@ __global__ __launch_bounds__(kThreads) void distribution_cut(Operands o) {
         return;
     }
     if (limits.few(row)) {
+        reinterpret_cast<uint4*>(s.histogram)[t] = make_uint4(0, 0, 0, 0);
+        if (t < 256) s.bins[t] = 0;
         if (!scanned) {
             each_vector(
                 row.whole(), row.vectors, [] {},
@@ -1104,13 +1135,10 @@ __global__ __launch_bounds__(kThreads) void distribution_cut(Operands o) {
                 },
                 [] {});
         }
-        if (t < 512) (&s.bins[0][0])[t] = 0;
         __syncthreads();
-        const int chunks = (row.vectors + 15) / 16;
-        const short* known = scanned ? o.largest + static_cast<std::int64_t>(index) * o.chunk_count : s.largest;
         int own[kOwn];
 #pragma unroll
-        for (int j = 0; j < kOwn; ++j) own[j] = t + j * kThreads < chunks ? known[t + j * kThreads] + 32768 : 0;
+        for (int j = 0; j < kOwn; ++j) own[j] = t + j * kThreads < chunks ? s.largest[t + j * kThreads] + 32768 : 0;
         const int least = bound_of<T>(s, own, limits.kept);
         if (least >= 0 && cut_largest<T>(s, row, edge, set, limits.kept, own, least, cut)) return;
         __syncthreads();
