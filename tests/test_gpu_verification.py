@@ -156,6 +156,69 @@ def test_rows_that_leave_nothing(backend, device, vocab):
     check(backend, device, p, None, drafted, u)
 
 
+@pytest.mark.parametrize("n,d,vocab", [(2, 1, 16384), (3, 2, 16385), (2, 1, 32768), (2, 2, 32769), (5, 1, 40001), (256, 1, 17000), (257, 1, 17000),
+                                       (300, 1, 5000), (300, 1, 16001), (300, 1, 100001), (1030, 1, 9001), (683, 1, 40001), (1100, 1, 8001),
+                                       (256, 1, 270001)])
+@pytest.mark.parametrize("certain", [False, True], ids=["drawn", "certain"])
+def test_rows_in_one_part_and_in_several(backend, device, certain, n, d, vocab):
+    """Both sides of the borders between a workgroup's registers, its second reading, and parts; the last of a row, too."""
+    p, q, drafted, u = case(4, d, vocab, n + vocab, 0.7, certain)
+    times = -(-n // 4)
+    p, drafted, u = (t.repeat(times, *[1] * (t.dim() - 1))[:n].contiguous() for t in (p, drafted, u))
+    q = None if q is None else q.repeat(times, 1, 1)[:n].contiguous()
+    u[:, d] = torch.linspace(0, 1, n)
+    u[: n // 2, :d] = 1e30  # refused
+    check(backend, device, p, q, drafted, u)
+
+
+def test_long_rows_that_leave_nothing(backend, device):
+    """In parts: the drafter's row at or above the target's everywhere, or in all parts but one; empty rows."""
+    vocab = 50001
+    for certain in (False, True):
+        p, q, drafted, u = case(7, 1, vocab, 9, 0.7, certain)
+        u[:, 0] = 1e30
+        p[4], p[5] = 0.0, math.nan
+        if certain:
+            p[0, 0] = p[1, 0] = 0.0
+            p[0, 0, drafted[0, 0]] = 1.0
+            p[1, 0, drafted[1, 0]], p[1, 0, vocab - 1 if drafted[1, 0] < 100 else 0] = 0.5, 0.25
+        else:
+            q[0], q[2], q[3] = p[0, :1], 1.0, math.nan
+            q[1] = p[1, :1]
+            q[1, 0, 30000:30010] = 0.0
+            p[1, 0, 30005] = 0.125
+        for last in (0.0, 0.5, 1.0):
+            u[:, 1] = last
+            check(backend, device, p, q, drafted, u)
+
+
+def test_graph_of_rows_in_parts(backend, device):
+    n, d, vocab = 3, 2, 40003
+    plan = backend.prepare_verification(sequences=n, drafts=d, vocab=vocab, device=device)
+    p, q, drafted, u = (t.to(device) for t in case(n, d, vocab, 1))
+    p, q = p.view(n * (d + 1), vocab), q.view(n * d, vocab)
+    tokens, accepted = torch.empty(n, d + 1, dtype=torch.int64, device=device), torch.empty(n, dtype=torch.int32, device=device)
+    arguments = dict(proposal=q, tokens=tokens, accepted=accepted, workspace=torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=device))
+    side = torch.cuda.Stream(device)
+    side.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(side):
+        plan.run(p, drafted, u, **arguments)
+    torch.cuda.current_stream(device).wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.run(p, drafted, u, **arguments)
+    for i in range(4):
+        for t, new in zip((p, q, drafted, u), case(n, d, vocab, 20 + i)):
+            t.copy_(new.view(t.shape))
+        plan.run(p, drafted, u, **arguments)
+        want = tokens.clone(), accepted.clone()
+        tokens.zero_(), accepted.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(tokens, want[0]) and torch.equal(accepted, want[1])
+
+
 def test_emitted_tokens_are_distributed_as_the_target(backend, device):
     """Drafts on a grid of the drafter's shares, uniforms on grids: the first token comes as often as its share says."""
     vocab, steps = 5, 64

@@ -150,15 +150,15 @@ def test_distribution_refusals(backend):
 
 # -- verification ----------------------------------------------------------------
 def test_verification_refusals(backend):
-    base = dict(sequences=2, drafts=3, vocab=9000, device=CPU)
+    base = dict(sequences=2, drafts=3, vocab=40000, device=CPU)
     for change in (dict(sequences=0), dict(sequences=65536), dict(drafts=0), dict(drafts=65), dict(vocab=0), dict(vocab=2**20 + 1),
                    dict(drafts=True)):
         with pytest.raises(ValueError):
             VerificationPlan.create(backend, **{**base, **change})
     plan = VerificationPlan.create(backend, **base)
     assert plan.workspace_bytes and not VerificationPlan.create(backend, **{**base, "vocab": 4000}).workspace_bytes
-    good = dict(target=torch.zeros(8, 9000), drafted=torch.zeros(2, 3, dtype=torch.int64), uniforms=torch.zeros(2, 4),
-                proposal=torch.zeros(6, 9000), counts=torch.zeros(2, dtype=torch.int32), tokens=torch.zeros(2, 4, dtype=torch.int64),
+    good = dict(target=torch.zeros(8, 40000), drafted=torch.zeros(2, 3, dtype=torch.int64), uniforms=torch.zeros(2, 4),
+                proposal=torch.zeros(6, 40000), counts=torch.zeros(2, dtype=torch.int32), tokens=torch.zeros(2, 4, dtype=torch.int64),
                 accepted=torch.zeros(2, dtype=torch.int32), workspace=aligned(plan.workspace_bytes, torch.uint8))
     plan.run(**good)
     plan.run(**{**good, "proposal": None, "counts": None})
@@ -289,6 +289,18 @@ def test_launches_keep_their_threads_within_32_bits():
 
 
 def test_verification_sums_rows_in_parts_where_they_are_long_and_few():
-    counts = {(1, 4, 4000): 1, (1, 4, 4096): 2, (61, 7, 32003): 2, (2048, 1, 151936): 1}
+    counts = {(1, 4, 4000): 1, (1, 4, 32768): 1, (1, 4, 32769): 2, (256, 7, 32003): 1, (257, 7, 32003): 2, (300, 1, 16384): 1, (682, 1, 151936): 2,
+              (683, 1, 151936): 1, (2048, 1, 151936): 1}
     for (n, d, v), count in counts.items():
-        assert len(kernels([(0, "venturi_verify_run", [*VERIFY.values()][:9] + [n, d, v, None])])[0]) == count
+        assert len(kernels([(0, "venturi_verify_run", verify(n, d, v)[1])])[0]) == count
+
+
+def verify(n, d, vocab):
+    return "venturi_verify_run", [*VERIFY.values()][:9] + [n, d, vocab, None]
+
+
+def test_verification_tests_reach_every_instance():
+    sizes = [(1, 1, 1), (1100, 1, 8001), (1030, 1, 9001), (300, 1, 5000), (300, 1, 16001), (300, 1, 100001), (2, 1, 16384), (2, 1, 32768),
+             (256, 1, 270001), (5, 1, 40001)]
+    names = built("verify_sum") | built("verify_take")
+    assert names and names == reached([verify(*size) for size in sizes])

@@ -800,8 +800,8 @@ __device__ __forceinline__ float wave_top(float top) {
 // Few and long rows are first looked at by the whole card: of a row without limits the largest logit and the mass of its parts, of
 // one that keeps few logits its chunks' largest ones. (Else a row's one CU sees and sums them. Us, with and without, for 5 rows
 // of 248320, 32 of 151936 and 96 of 151936: no limits 11.0 / 35.9, 17.9 / 29.1 and 30.5 / 38.5; top_k 50 14.4 / 19.7, 21.7 /
-// 22.3 and 32.1 / 30.7; in batches of 96 with mixed settings other rows take longest, 52. 16 rows of 32003, which a workgroup's registers hold:
-// 10.7 / 10.7 and 14.0 / 13.0.)
+// 22.3 and 32.1 / 30.7; in batches of 96 with mixed settings other rows take longest, 52. 16 rows of 32003, which a workgroup's
+// registers hold: 10.7 / 10.7 and 14.0 / 13.0.)
 constexpr int kScanThreads = 256, kScanWaves = kScanThreads / 64, kScanVectors = 4;  // vectors of a thread
 constexpr int kScanPart = kScanThreads * kScanVectors;
 constexpr int kScanRows = 32, kScanVocab = 8 * kFirst * kThreads;  // up to so many rows of more logits

@@ -6,10 +6,9 @@
 // token, by index, at which the running sum passes u times the whole one; sums in 64 bits, in a fixed order.
 //
 // Bound by memory where sequences are many: one or two rows of 4-byte probabilities each (128 of 151936 tokens with a drafter's
-// rows 33.4 us, 4.7 TB/s), else by two launches and their chains of loads: the drafts, their probabilities, the row, and
-// in the second launch the sums, the part, and the run of it again (one sequence of 248320 tokens 8.6, 61 of 32003 11.4). A row
-// is cut into parts that workgroups sum; one workgroup of the second launch finds the part and the token in it. (The chosen
-// part token by token, a run a thread: 82.6, 20.2 and 16.6.)
+// rows 30.4 us, 5.1 TB/s), else by launches and their chains of loads: the drafts, their probabilities, the row. A long row is cut
+// into parts that workgroups sum, and in a second launch one workgroup finds the part and the token in it (one sequence of 248320
+// tokens 8.0 us); a short one is summed and searched in one launch from registers (61 of 32003 10.0).
 #include "common.hpp"
 
 namespace vt {
@@ -34,7 +33,7 @@ struct Operands {
     std::int64_t* tokens;         // [sequences][drafts + 1]
     std::int32_t* accepted;       // [sequences]
     Verdict* verdicts;            // [sequences], where rows are summed in parts
-    double2* sums;                // [sequences][parts]: of the remainder, and of the target's row
+    double* sums;                 // [sequences][parts]
     int drafts, vocab, parts, slice;
 };
 
@@ -79,14 +78,28 @@ struct Draw {
         if (vocab >= 4) return *reinterpret_cast<const float4u*>(row + at);
         return float4u{row[0], row[min(1, vocab - 1)], row[min(2, vocab - 1)], 0.0f};
     }
-    // Shares of the loaded tokens in the remainder (x) and in the target's row (y), of those from `at` up to `end`.
-    __device__ __forceinline__ double2 share(const float4u& pv, const float4u& qv, int j, int at, int end) const {
-        const int index = place(at) + j;
-        double2 s;
-        s.y = index >= at && index < end ? static_cast<double>(positive(pv[j])) : 0.0;
-        s.x = q ? fmax(s.y - static_cast<double>(qv[j]), 0.0) : index == without ? 0.0 : s.y;
-        if (!(s.y > 0.0)) s.x = 0.0;  // of a proposal below 0, too
-        return s;
+    // Shares of the tokens at .. at + 3 that lie below `end`, loaded from their place, where the wave's first is `first`. A step
+    // of a wave that ends before `end` and does not hold the refused draft needs no look at indices: 4 operations a token, 8
+    // with a proposal.
+    __device__ __forceinline__ void shares(const float4u& pv, const float4u& qv, int first, int at, int end, double (&w)[4]) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = share(pv[j], qv[j]);
+        if (first + 256 > end || (without >= first && without < first + 256)) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int index = place(at) + j;
+                w[j] = index >= at && index < end && index != without ? w[j] : 0.0;
+            }
+        }
+    }
+
+private:
+    __device__ __forceinline__ double share(float pj, float qj) const {
+        constexpr int kPositive = 0x180;  // normal and subnormal numbers above 0
+        const bool some = __builtin_amdgcn_classf(pj, kPositive);
+        if (!q) return static_cast<double>(some ? pj : 0.0f);
+        const double rest = fmax(static_cast<double>(pj) - static_cast<double>(qj), 0.0);
+        return some ? rest : 0.0;
     }
 };
 
@@ -116,43 +129,46 @@ __device__ __forceinline__ double lane_value(double v, int lane) {
 
 // A thread's sum of the tokens begin + 4 thread .. + 3, and every 4 THREADS on, below end, two loads of each row at once.
 template <int THREADS>
-__device__ __forceinline__ double2 sum_of(const Draw& d, int thread, int begin, int end) {
-    constexpr int kAhead = 2;  // 4 or 8 load past the end of most runs: 128 sequences of 151936 tokens 33.4, 34.3, 46.9 us
-    double2 sum = {0.0, 0.0};
-    for (int first = begin + 4 * thread; first < end; first += 4 * THREADS * kAhead) {
+__device__ __forceinline__ double sum_of(const Draw& d, int thread, int begin, int end) {
+    constexpr int kAhead = 2;  // 1 and 4: 300 sequences of 151936 tokens 74 us, 87, 80
+    const int lane = thread & 63;
+    double sum = 0.0;
+    for (int first = begin + 4 * (thread - lane); first < end; first += 4 * THREADS * kAhead) {
         float4u p[kAhead], q[kAhead] = {};
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) p[u] = d.load(d.p, d.place(first + u * 4 * THREADS));
+        for (int u = 0; u < kAhead; ++u) p[u] = d.load(d.p, d.place(first + 4 * lane + u * 4 * THREADS));
         if (d.q) {
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) q[u] = d.load(d.q, d.place(first + u * 4 * THREADS));
+            for (int u = 0; u < kAhead; ++u) q[u] = d.load(d.q, d.place(first + 4 * lane + u * 4 * THREADS));
         }
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const double2 s = d.share(p[u], q[u], j, first + u * 4 * THREADS, end);
-                sum.x += s.x, sum.y += s.y;
-            }
+        for (int u = 0; u < kAhead; ++u) {
+            double w[4];
+            d.shares(p[u], q[u], first + u * 4 * THREADS, first + 4 * lane + u * 4 * THREADS, end, w);
+            sum += (w[0] + w[1]) + (w[2] + w[3]);
+        }
     }
     return sum;
 }
 
+// Tokens of a wave's run, where `waves` of them share a part: whole vectors.
+__host__ __device__ constexpr int run_of(int tokens, int waves) { return ((tokens + waves - 1) / waves + 3) / 4 * 4; }
+
 // Sums of a part, and with the first one the verdict.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void verify_sum(Operands o) {
-    __shared__ double2 waves[THREADS / 64];
+    __shared__ double waves[THREADS / 64];
     const int sequence = blockIdx.y, part = blockIdx.x;
     const Verdict v = verdict_of(o, sequence);
     const Draw d(o, v, sequence);
     const int begin = part * o.slice, end = min(begin + o.slice, o.vocab);
-    double2 sum = sum_of<THREADS>(d, threadIdx.x, begin, end);
-    sum = {wave_scan(sum.x), wave_scan(sum.y)};
+    const double sum = wave_scan(sum_of<THREADS>(d, threadIdx.x, begin, end));
     if ((threadIdx.x & 63) == 63) waves[threadIdx.x >> 6] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int i = 1; i < THREADS / 64; ++i) waves[0].x += waves[i].x, waves[0].y += waves[i].y;
-        o.sums[static_cast<std::int64_t>(sequence) * o.parts + part] = waves[0];
+        double all = waves[0];
+        for (int i = 1; i < THREADS / 64; ++i) all += waves[i];
+        o.sums[static_cast<std::int64_t>(sequence) * o.parts + part] = all;
         if (part == 0) o.verdicts[sequence] = v;
     }
 }
@@ -167,87 +183,135 @@ __device__ __forceinline__ int find(double share, double target, double& before)
     return at;
 }
 
-// The sequence's tokens. A workgroup per sequence; with one part it sums the row itself. A wave takes a run of the part.
-template <int THREADS>
+// Goes through a run of the row from `before` on: the first token at which the running sum passes the target, or the last one
+// with a share; -1 if there is none. For a whole wave, 256 tokens at a step.
+struct Search {
+    double before, target;
+    int token;
+    bool past;
+
+    __device__ __forceinline__ void step(const Draw& d, const float4u& p, const float4u& q, int first, int end) {
+        double w[4];
+        d.shares(p, q, first, first + 4 * static_cast<int>(threadIdx.x & 63), end, w);
+        const double four = (w[0] + w[1]) + (w[2] + w[3]), scan = before + wave_scan(four);
+        const unsigned long long some = __ballot(four > 0.0), beyond = __ballot(four > 0.0 && scan > target);
+        if (some) {
+            const int mine = beyond ? __ffsll(beyond) - 1 : 63 - __clzll(some);
+            // Of the lane's four the first that passes, or else the last with a share.
+            double running = mine ? lane_value(scan, mine - 1) : before;
+            bool passed = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                running += lane_value(w[j], mine);
+                if (lane_value(w[j], mine) > 0.0 && !passed) {
+                    token = d.place(first + 4 * mine) + j;
+                    passed = running > target;
+                }
+            }
+        }
+        past = beyond != 0;
+        before = lane_value(scan, 63);
+    }
+};
+
+// The sequence's tokens. A workgroup per sequence; with one part it sums the row itself. A wave takes a run of the part: one of
+// up to 256 HELD tokens stays in its registers, else the wave that the token lies in reads its run again. Where nothing is left
+// of the target's row without the proposal, the workgroup starts again with the whole of it.
+template <int THREADS, int HELD>
 __global__ __launch_bounds__(THREADS) void verify_take(Operands o) {
     constexpr int kWaves = THREADS / 64;
-    __shared__ double2 waves[kWaves];
+    __shared__ double waves[kWaves];
     const int sequence = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Verdict v = o.parts > 1 ? o.verdicts[sequence] : verdict_of(o, sequence);
-    const Draw d(o, v, sequence);
+    Draw d(o, v, sequence);
     const std::int64_t row = static_cast<std::int64_t>(sequence) * (o.drafts + 1);
     if (static_cast<int>(threadIdx.x) <= o.drafts && static_cast<int>(threadIdx.x) != v.accepted)
         o.tokens[row + threadIdx.x] = static_cast<int>(threadIdx.x) < v.accepted ? o.drafted[row - sequence + threadIdx.x] : -1;
     if (threadIdx.x == 0) o.accepted[sequence] = v.accepted;
     const double u = o.uniforms[row + o.drafts];
     int begin = 0, end = o.vocab;
-    double before = 0.0, target = 0.0;
-    bool rest = true;  // draw from the remainder
+    double before = 0.0, target = 0.0, own = 0.0;
+    bool narrow = o.parts == 1;  // to one part
     if (o.parts > 1) {
-        const double2 none = {0.0, 0.0};
-        const double2 own = lane < o.parts ? o.sums[static_cast<std::int64_t>(sequence) * o.parts + lane] : none;
-        const double all = lane_value(wave_scan(own.x), 63);
-        rest = all > 0.0;
-        target = u * (rest ? all : lane_value(wave_scan(own.y), 63));
-        begin = find(rest ? own.x : own.y, target, before) * o.slice;
-        end = min(begin + o.slice, o.vocab);
+        const double share = lane < o.parts ? o.sums[static_cast<std::int64_t>(sequence) * o.parts + lane] : 0.0;
+        const double all = lane_value(wave_scan(share), 63);
+        narrow = all > 0.0;
+        target = u * all;
+        if (narrow) begin = find(share, target, before) * o.slice, end = min(begin + o.slice, o.vocab);
     }
-    const int run = ((end - begin + kWaves - 1) / kWaves + 3) / 4 * 4;
-    begin += wave * run;
-    end = min(begin + run, end);
-    double2 sum = sum_of<64>(d, lane, begin, end);
-    sum = {wave_scan(sum.x), wave_scan(sum.y)};
-    if (lane == 63) waves[wave] = sum;
-    __syncthreads();
-    const double2 own = lane < kWaves ? waves[lane] : double2{0.0, 0.0};
-    if (o.parts == 1) {
-        const double all = lane_value(wave_scan(own.x), 63);
-        rest = all > 0.0;
-        target = u * (rest ? all : lane_value(wave_scan(own.y), 63));
-    }
-    if (find(rest ? own.x : own.y, target, before) != wave) return;
-    // The wave that the token lies in goes through its run again.
-    int token = -1;
-    for (int first = begin; first < end; first += 256) {
-        const int at = first + 4 * lane;
-        const float4u p = d.load(d.p, d.place(at)), q = d.q ? d.load(d.q, d.place(at)) : float4u{};
-        double w[4], four = 0.0;
+    float4u p[HELD ? HELD : 1], q[HELD ? HELD : 1];
+    const auto split = [&] {  // the wave's run
+        const int run = run_of(end - begin, kWaves);
+        begin += wave * run;
+        end = min(begin + run, end);
+    };
+    const auto join = [&](double sum) {
+        sum = wave_scan(sum);
+        if (lane == 63) waves[wave] = sum;
+        __syncthreads();
+        own = lane < kWaves ? waves[lane] : 0.0;
+    };
+    if (narrow) {
+        split();
+        double sum = 0.0;
+        if constexpr (HELD) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const double2 s = d.share(p, q, j, at, end);
-            w[j] = rest ? s.x : s.y;
-            four += w[j];
-        }
-        const double scan = before + wave_scan(four);
-        const unsigned long long some = __ballot(four > 0.0), past = __ballot(four > 0.0 && scan > target);
-        if (some) {
-            const int mine = past ? __ffsll(past) - 1 : 63 - __clzll(some);
-            // Of the lane's four the first that passes, or else the last with a share.
-            double running = mine ? lane_value(scan, mine - 1) : before;
-            int found = -1;
-            bool passed = false;
+            for (int i = 0; i < HELD; ++i) p[i] = d.load(d.p, d.place(begin + 256 * i + 4 * lane));
+            if (d.q) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                running += lane_value(w[j], mine);
-                if (lane_value(w[j], mine) > 0.0 && !passed) {
-                    found = d.place(first + 4 * mine) + j;
-                    passed = running > target;
-                }
+                for (int i = 0; i < HELD; ++i) q[i] = d.load(d.q, d.place(begin + 256 * i + 4 * lane));
             }
-            token = found;
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+                if (begin + 256 * i >= end) break;
+                double w[4];
+                d.shares(p[i], q[i], begin + 256 * i, begin + 256 * i + 4 * lane, end, w);
+                sum += (w[0] + w[1]) + (w[2] + w[3]);
+            }
+        } else {
+            sum = sum_of<64>(d, lane, begin, end);
         }
-        if (past) break;
-        before = lane_value(scan, 63);
+        join(sum);
+        if (o.parts == 1) {
+            const double all = lane_value(wave_scan(own), 63);
+            narrow = all > 0.0;
+            target = u * all;
+        }
     }
-    if (lane == 0) o.tokens[row + v.accepted] = token;
+    const bool held = HELD && narrow;
+    if (!narrow) {
+        d.q = nullptr, d.without = -1;
+        begin = 0, end = o.vocab;
+        split();
+        __syncthreads();
+        join(sum_of<64>(d, lane, begin, end));
+        target = u * lane_value(wave_scan(own), 63);
+    }
+    if (find(own, target, before) != wave) return;
+    Search search{before, target, -1, false};
+    if (held) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (!search.past && begin + 256 * i < end) search.step(d, p[i], q[i], begin + 256 * i, end);
+    } else {
+        for (int first = begin; first < end && !search.past; first += 256) {
+            const int at = d.place(first + 4 * lane);
+            search.step(d, d.load(d.p, at), d.q ? d.load(d.q, at) : float4u{}, first, end);
+        }
+    }
+    if (lane == 0) o.tokens[row + v.accepted] = search.token;
 }
 
 Operands geometry(int sequences, int drafts, int vocab) {
     require(sequences > 0 && sequences <= kMaxSequences, "verification takes 1 to 65535 sequences");
     require(drafts > 0 && drafts <= kMaxDrafts, "verification takes 1 to 64 drafts of a sequence");
     require(vocab > 0 && vocab <= kMaxVocab, "verification takes a vocabulary of at most 1048576");
-    // Parts of 2048 tokens and more, about 2048 workgroups in all.
-    const int parts = std::max(std::min({kMaxParts, 2048 / sequences, vocab / 2048}), 1);
+    // Parts of 2048 tokens and more, about 2048 workgroups in all; one part, and one launch, where a workgroup's registers hold
+    // the row and each has a CU, where the row is short, or where two parts would be all. (Us in a chain of calls, parts against
+    // one: one sequence of 32003 tokens 11.9 / 9.1, 61 11.8 / 11.3, 256 14.6 / 14.0, 257 15.8 / 19.7; 300 of 16001 13.1 / 12.7, of
+    // 32003 19.4 / 23.7; 512 of 151936 98 / 125, 700 170 / 157. A call with one launch takes the host 8, with two 11.)
+    int parts = std::max(std::min({kMaxParts, 2048 / sequences, vocab / 2048}), 1);
+    if (parts < 3 || vocab <= (sequences <= 256 ? 32768 : 16384)) parts = 1;
     Operands o{};
     o.drafts = drafts, o.vocab = vocab, o.parts = parts, o.slice = ((vocab + parts - 1) / parts + 3) / 4 * 4;
     return o;
@@ -259,19 +323,22 @@ void launch_sum(const Operands& o, int sequences, hipStream_t stream) {
 }
 template <int THREADS>
 void launch_take(const Operands& o, int sequences, hipStream_t stream) {
-    verify_take<THREADS><<<sequences, THREADS, 0, stream>>>(o);
+    const int run = run_of(std::min(o.slice, o.vocab), THREADS / 64);
+    if (run <= 1024) verify_take<THREADS, 4><<<sequences, THREADS, 0, stream>>>(o);
+    else if (run <= 2048) verify_take<THREADS, 8><<<sequences, THREADS, 0, stream>>>(o);
+    else verify_take<THREADS, 0><<<sequences, THREADS, 0, stream>>>(o);
 }
 
 // Where the card is full, small workgroups, which repeat the verdict's loads in fewer waves (us, 128 threads against 256: 128
-// sequences of 151936 tokens 34.3 / 36.9, 64 19.8 / 22.1; one of 248320 11.5 / 9.3).
+// sequences of 151936 tokens 28.0 / 28.5, 64 17.1 / 18.5; one of 248320 9.0 / 8.2).
 void launch_sum(const Operands& o, int sequences, hipStream_t stream) {
     if (o.parts * sequences > 256) launch_sum<128>(o, sequences, stream);
     else launch_sum<256>(o, sequences, stream);
 }
 
 // As many threads as have a run of some length, fewer where sequences are many (they start sooner). Us, 256 / 512 / 1024
-// threads: one sequence of 1000 tokens 4.9 / 5.4 / 6.5, of 248320 (3880 in a part) 9.5 / 9.3 / 10.1; 128 of 151936 (9496) 42 /
-// 39 / 37; 512 of 32003 (8004) 31 / 28 / 31; 2100 of 9001 (one part) 34 / 42 / 49.
+// threads: 300 sequences of 1000 tokens 4.5 / 5.2 / 7.7, of 9001 12.5 / 9.1 / 10.3; one of 5001 5.6 / 4.4 / 4.6, of 16001 9.9 /
+// 6.5 / 6.0, of 248320 (3880 in a part) 7.7 / 7.5 / 8.0; 128 of 151936 (9496) 29.5 / 25.6 / 24.7; 2100 of 9001 28 / 31 / 40.
 void launch_take(const Operands& o, int sequences, hipStream_t stream) {
     if (o.slice <= 1024 || sequences > 1024) launch_take<256>(o, sequences, stream);
     else if (o.slice <= 6144 || sequences > 256) launch_take<512>(o, sequences, stream);
@@ -279,7 +346,7 @@ void launch_take(const Operands& o, int sequences, hipStream_t stream) {
 }
 
 std::uint64_t sum_bytes(const Operands& o, int sequences) {
-    return o.parts > 1 ? (sizeof(Verdict) + sizeof(double2) * o.parts) * static_cast<std::uint64_t>(sequences) : 0;
+    return o.parts > 1 ? (sizeof(Verdict) + sizeof(double) * o.parts) * static_cast<std::uint64_t>(sequences) : 0;
 }
 
 }  // namespace
@@ -307,7 +374,7 @@ VT_EXPORT int venturi_verify_run(const float* target, const float* proposal, con
                     "verification needs its workspace, 256-byte aligned");
         o.target = target, o.proposal = proposal, o.drafted = drafted, o.counts = counts, o.uniforms = uniforms;
         o.tokens = tokens, o.accepted = accepted, o.verdicts = static_cast<vt::Verdict*>(workspace);
-        o.sums = reinterpret_cast<double2*>(o.verdicts + sequences);
+        o.sums = reinterpret_cast<double*>(o.verdicts + sequences);
         const auto s = static_cast<hipStream_t>(stream);
         if (o.parts > 1) {
             vt::launch_sum(o, sequences, s);
