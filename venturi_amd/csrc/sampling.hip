@@ -887,38 +887,39 @@ __device__ __forceinline__ Cut join_parts(const Part* parts, int count, double h
     return cut_of_all<T>(top, heat, wave_sum(mass));
 }
 
-// The same by the row's workgroup (257 rows of 32003: 33.5 us through the histogram, 26).
+// The same by the row's workgroup (257 rows of 32003: 33.5 us through the histogram, 25).
 template <class T>
 __device__ __forceinline__ Cut keep_all(Shared& s, const Row& row, const Edge& edge, double heat) {
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const float none = -__builtin_inff();
-    float top = edge.live ? fmaxf(value_of<T>(edge.bits), none) : none;
-    // Rows of up to 57344 logits stay in registers.
-    const bool held = row.vectors > 0 && row.vectors <= kFirst * kThreads;
-    uint4 first[kFirst];
-    if (held) {
+    const auto join_top = [&](float top) {
+        top = wave_top(edge.live ? fmaxf(value_of<T>(edge.bits), top) : top);
+        if (lane == 0) s.wave_top[wave] = top;
+        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < kFirst; ++j) first[j] = row.whole()[min(t + j * kThreads, row.vectors - 1)];
+        for (int i = 0; i < kWaves; ++i) top = fmaxf(top, s.wave_top[i]);
+        return top;
+    };
+    float top = none;
+    double mass = 0.0;
+    if (row.vectors > 0 && row.vectors <= kFirst * kThreads) {  // rows of up to 57344 logits stay in registers
+        uint4 all[kFirst];
 #pragma unroll
-        for (int j = 0; j < kFirst; ++j) top = raised<T>(top, first[j]);
-    } else {
-        each_vector(row.whole(), row.vectors, [] {}, [&](const uint4& w, int, bool) { top = raised<T>(top, w); }, [] {});
-    }
-    top = wave_top(top);
-    if (lane == 0) s.wave_top[wave] = top;
-    __syncthreads();
+        for (int j = 0; j < kFirst; ++j) all[j] = row.whole()[min(t + j * kThreads, row.vectors - 1)];
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) top = fmaxf(top, s.wave_top[i]);
-    const Weights<T> weight(top, heat);
-    double mass = edge.live ? weight(edge.bits) : 0.0;
-    if (held) {
+        for (int j = 0; j < kFirst; ++j) top = raised<T>(top, all[j]);
+        top = join_top(top);
+        const Weights<T> weight(top, heat);
 #pragma unroll
         for (int j = 0; j < kFirst; ++j) {
             if (j * kThreads >= row.vectors) break;
-            const float sum = weight.sum(first[j]);
+            const float sum = weight.sum(all[j]);
             if (t + j * kThreads < row.vectors) mass += sum;
         }
     } else {
+        each_vector(row.whole(), row.vectors, [] {}, [&](const uint4& w, int, bool) { top = raised<T>(top, w); }, [] {});
+        top = join_top(top);
+        const Weights<T> weight(top, heat);
         each_vector(
             row.whole(), row.vectors, [] {},
             [&](const uint4& w, int, bool live) {
@@ -927,6 +928,7 @@ __device__ __forceinline__ Cut keep_all(Shared& s, const Row& row, const Edge& e
             },
             [] {});
     }
+    if (edge.live) mass += Weights<T>(top, heat)(edge.bits);
     mass = wave_sum(mass);
     if (lane == 0) s.wave_mass[wave] = mass;
     __syncthreads();
