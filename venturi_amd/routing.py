@@ -3,8 +3,8 @@
 Scores s = softmax(logits) or 1 / (1 + exp(-logits)) over all experts. Experts are ordered by c = s + bias, largest first,
 equal ones by index; with ``groups`` > 1 only those of the ``kept_groups`` best groups (consecutive experts of equal number),
 ordered by the sum of their two largest c ("pairs"; a lone one that is not masked by itself) or by their largest ("max"), equal
-ones by index. The first ``top_k`` are
-chosen. Their weights are s without the bias, divided by their sum with ``renormalize``, times ``scale``.
+ones by index. The first ``top_k`` are chosen. Their weights are s without the bias, divided by their sum with
+``renormalize``, times ``scale``.
 
 An expert whose logit is -inf is masked: it comes after all others, with weight 0, whatever its bias. Weights whose sum is 0
 stay 0. A token with a NaN among its logits or biased scores, or with +inf under softmax, gets ids -1 and NaN scores, which

@@ -7,8 +7,9 @@ of the row behind the last. Tokens so emitted are distributed as the target's ow
 index, at which the running sum of the shares exceeds the uniform times their whole sum.
 
 Rows need not add to 1; target probabilities that are no positive finite number count as 0 (such tokens are neither accepted
-nor drawn), and a row of those alone gives token -1. A draft outside the vocabulary is refused, and one whose proposal is NaN. Sums are 64-bit, in a fixed order: the result depends on the inputs alone. The rows
-come from ``HipBackend.prepare_distribution``. The reference decodes without drafts; this operator is an extension.
+nor drawn), and a row of those alone gives token -1. A draft outside the vocabulary is refused, and one whose proposal is NaN.
+Sums are 64-bit, in a fixed order: the result depends on the inputs alone. The rows come from
+``HipBackend.prepare_distribution``. The reference decodes without drafts; this operator is an extension.
 """
 
 from dataclasses import dataclass
