@@ -156,6 +156,34 @@ def test_scores_that_differ_in_their_last_bits(backend, device):
     check(backend, device, logits, bias, 8, score="softmax")
 
 
+@pytest.mark.parametrize("experts", [64, 128, 252, 256, 512, 1008])
+def test_near_scores_and_groups_of_a_bias(backend, device, experts):
+    """What 32-bit scores cannot tell apart, sigmoid scores with biases on both sides of 4, and masked groups."""
+    gen = torch.Generator().manual_seed(experts)
+    steps = torch.randperm(experts, generator=gen).float()
+    settings = dict(score="sigmoid", groups=4, kept_groups=2)
+    for spacing in (2.0**-25, 2.0**-22, 2.0**-19):
+        for rank in ("pairs", "max"):
+            check(backend, device, torch.zeros(3, experts), 0.25 + spacing * steps, 8, group_rank=rank, **settings)
+        check(backend, device, torch.zeros(3, experts), 0.25 + spacing * steps, 8, score="sigmoid")
+    logits = torch.randn(9, experts, generator=gen)
+    for scale in (1e-6, 0.1, 1.0, 3.0, 1e4):
+        bias = scale * torch.randn(experts, generator=gen)
+        check(backend, device, logits, bias, 8, **settings)
+        check(backend, device, 30 * logits, bias, 8, **settings)
+    bias[::3], bias[1::3] = 4.0, -4.0
+    check(backend, device, logits, bias, 8, **settings)
+    bias[3] = 4.0 + 2.0**-21
+    check(backend, device, logits, bias, 8, **settings)
+    logits[:, : 3 * experts // 4] = -math.inf  # fewer groups than are kept
+    logits[4:, experts // 2:] = -math.inf
+    logits[2, 5] = 1.0
+    for bias in (0.1 * torch.randn(experts, generator=gen), 9.0 * torch.randn(experts, generator=gen)):
+        for rank in ("pairs", "max"):
+            check(backend, device, logits, bias, 8, group_rank=rank, **settings)
+            check(backend, device, logits.half(), bias, 8, group_rank=rank, **settings)
+
+
 @pytest.mark.parametrize("dtype", [FP16, BF16, FP32], ids=NAMES.values())
 @pytest.mark.parametrize("experts", [16, 64, 160])
 def test_masks_and_values_that_are_no_numbers(backend, device, dtype, experts):

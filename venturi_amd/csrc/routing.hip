@@ -10,7 +10,7 @@
 // Bound by the vector unit, and for few tokens by the length of its chain: a score's exponential and division are 24 steps of 64
 // bits, a choice ten of moves and maxima between the lanes of a token. So a lane sorts its own few experts once (19 exchanges
 // of eight), and a choice then is the largest of the lists' heads: 16384 tokens of 128 experts, 16-bit logits 6.0 us (49 with a
-// wave per token and one 64-bit maximum over it for each choice), 32-bit ones 8.0; 4099 tokens of 256 in 8 groups, a bias, 9.9
+// wave per token and one 64-bit maximum over it for each choice), 32-bit ones 7.8; 4099 tokens of 256 in 8 groups, a bias, 8.2
 // (22); one token 3.5 to 6.0, of which a launch is 2.3. Memory would take 16384 x 128 of 16 bits 1.1 us.
 #include "common.hpp"
 
@@ -312,36 +312,51 @@ __global__ __launch_bounds__(kThreads) void route_logits(const T* __restrict__ l
 // A score's key: its 32-bit number (infinities as the largest there is) in order as a whole number above 0, without the low
 // bits that say which of its lane's N experts it is, the first the largest.
 template <int N>
-__device__ __forceinline__ std::uint32_t key_of(double c, int i) {
-    const auto w = __builtin_bit_cast(std::uint32_t, fminf(fmaxf(static_cast<float>(c), -3.402823466e38f), 3.402823466e38f));
+__device__ __forceinline__ std::uint32_t key_of(float c, int i) {
+    const auto w = __builtin_bit_cast(std::uint32_t, fminf(fmaxf(c, -3.402823466e38f), 3.402823466e38f));
     return ((w & 0x80000000u ? ~w : w | 0x80000000u) & ~(N - 1u)) | (N - 1 - i);
 }
 // Whether the first of two keys, the larger, may stand for no larger score: the 32-bit rounding and the low bits hide less than
-// 2^-18 of either, and of numbers below 2^-126 all.
-__device__ __forceinline__ bool near_keys(std::uint32_t a, std::uint32_t b) {
+// 2^-18 of either, and of numbers below 2^-126 all. `slack`: 2^-120, or 2^-20 for keys of quick scores.
+constexpr float kExactSlack = 0x1p-120f;
+__device__ __forceinline__ bool near_keys(std::uint32_t a, std::uint32_t b, float slack) {
     const auto value = [](std::uint32_t k) { return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k); };
     const float most = value(a), difference = most - value(b);
-    return b != 0 && !(difference > fmaf(fabsf(most), 0x1p-17f, 0x1p-120f));
+    return b != 0 && !(difference > fmaf(fabsf(most), 0x1p-17f, slack));
+}
+
+// 1 / (1 + exp(-x)) to 2^-22: the product's rounding weighs |x| s (1 - s) 2^-24, the exponential's last bit s (1 - s) 2^-23, and
+// the sum and its inverse s (2^-24 + 2^-23).
+// With a bias of up to 4, whose sum is rounded by 5 x 2^-24 at most, it errs by less than 2^-21: two by less than 2^-20, and
+// sums of two with their own rounding by less than 2^-19 each.
+constexpr float kQuickBias = 4.0f, kQuickSlack = 0x1p-20f;
+__device__ __forceinline__ float quick_sigmoid(float x) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504f));
 }
 
 // The two largest.
+template <class V>
 struct Best {
-    double most, second;
-    __device__ __forceinline__ void add(double v, double w) {  // v >= w
-        second = fmax(fmax(second, w), fmin(most, v));
-        most = fmax(most, v);
+    V most, second;
+    __device__ __forceinline__ void add(V v, V w) {  // v >= w
+        second = max_of(max_of(second, w), min_of(most, v));
+        most = max_of(most, v);
     }
+    static __device__ __forceinline__ double max_of(double a, double b) { return fmax(a, b); }
+    static __device__ __forceinline__ double min_of(double a, double b) { return fmin(a, b); }
+    static __device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
+    static __device__ __forceinline__ float min_of(float a, float b) { return fminf(a, b); }
 };
 
 // Takes the experts of groups that are not kept out of `key` (0: not there, or in no kept group). A lane ranks a group, from
 // LDS of its own token: from what the lanes of a group have found in their own experts, or where groups end inside a lane's,
-// from all scores.
-template <int N>
-__device__ __forceinline__ void keep_groups(const Geometry& g, const double (&c)[N], std::uint32_t (&key)[N], double* mine, double* rank_of,
-                                            int place) {
-    const double none = -__builtin_inf();
+// from all scores. False in a lane whose group quick scores neither keep nor drop for sure.
+template <class V, int N>
+__device__ __forceinline__ bool keep_groups(const Geometry& g, const V (&c)[N], std::uint32_t (&key)[N], V* mine, V* rank_of, int place) {
+    constexpr V none = -static_cast<V>(__builtin_inff());
     const int first = place * N, size = g.experts / g.groups;
-    Best best = {none, none};
+    Best<V> best = {none, none};
+    wave_fence();
     if (size % N == 0) {
 #pragma unroll
         for (int i = 0; i < N; ++i) best.add(c[i], none);
@@ -363,22 +378,29 @@ __device__ __forceinline__ void keep_groups(const Geometry& g, const double (&c)
             }
         }
     }
-    const double rank = g.pairs && best.second > none ? best.most + best.second : best.most;
+    const V rank = g.pairs && best.second > none ? best.most + best.second : best.most;
     rank_of[place] = rank;
     wave_fence();
-    int ahead = 0;
+    int ahead = 0, may_be_ahead = 0;
 #pragma unroll 4
     for (int i = 0; i < g.groups; ++i) {
-        const double other = rank_of[i];
-        ahead += other > rank || (other == rank && i < place);
+        const V other = rank_of[i];
+        if constexpr (sizeof(V) == 8) {
+            ahead += other > rank || (other == rank && i < place);
+        } else {
+            ahead += other > rank + 4 * kQuickSlack;
+            may_be_ahead += other >= rank - 4 * kQuickSlack && i != place;
+        }
     }
-    const unsigned long long kept = __ballot(place < g.groups && ahead < g.kept) >> ((threadIdx.x & 63) - place);
+    const bool keep = place < g.groups && ahead < g.kept;
+    const unsigned long long kept = __ballot(keep) >> ((threadIdx.x & 63) - place);
     int group = first / size, in_group = first - group * size;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         if (!(kept >> min(group, 63) & 1)) key[i] = 0;
         if (++in_group == size) in_group = 0, ++group;
     }
+    return sizeof(V) == 8 || !keep || may_be_ahead < g.kept;
 }
 
 // The token's choices in order, choice k in lane k, by scores and indices.
@@ -428,7 +450,9 @@ __device__ __forceinline__ int rank_of_16(double c, std::uint32_t expert) {
 
 // Any logits, a bias, groups. Scores have 64 bits; the choice goes by 32-bit keys, past top_k as long as the next key is near
 // the last, and where keys that follow each other are near, the scores of the up to 16 candidates, a lane each, decide. More
-// candidates than that (many equal scores, or masked experts) are picked score by score.
+// candidates than that (many equal scores, or masked experts) are picked score by score. Keys and groups' ranks of sigmoid scores
+// are first made of quick 32-bit ones; where those do not decide on the groups, the wave starts again with 64 bits (4099 tokens
+// of 256 in 8 groups 9.7 -> 8.2 us, 16384 21.1 -> 17.1).
 template <class T, int LANES, int N, bool SIGMOID, bool VECTOR>
 __global__ __launch_bounds__(kThreads) void route_scores(const T* __restrict__ logits, const float* __restrict__ bias,
                                                          std::int64_t* __restrict__ indices, void* __restrict__ scores, Geometry g) {
@@ -464,30 +488,54 @@ __global__ __launch_bounds__(kThreads) void route_scores(const T* __restrict__ l
             sum = join_sum<LANES>(sum);
             row.inverse = sum > 0.0 ? 1.0 / sum : 0.0;
         }
-    } else if (!direct) {
-        terms_of<true>(x, 0.0, c);
     }
     const auto whole = [&](float logit, double s, float offset) {  // a score with its bias
         const double v = direct ? static_cast<double>(logit) : s + static_cast<double>(offset);
         return logit == -kInf ? -__builtin_inf() : fmax(v + 0.0, -__builtin_inf());  // one zero, and no NaN
     };
-    std::uint32_t key[N];
+    const auto exactly = [&] {
+        if constexpr (SIGMOID) {
+            if (!direct) terms_of<true>(x, 0.0, c);
+        }
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        c[i] = whole(x[i], direct ? 0.0 : c[i] * row.inverse, b[i]);
-        key[i] = first + i < g.experts ? key_of<N>(c[i], i) : 0;
+        for (int i = 0; i < N; ++i) c[i] = whole(x[i], direct ? 0.0 : c[i] * row.inverse, b[i]);
+    };
+    std::uint32_t key[N];
+    const auto keys_of = [&](auto& v) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) key[i] = first + i < g.experts ? key_of<N>(static_cast<float>(v[i]), i) : 0;
+        using V = std::remove_reference_t<decltype(v[0])>;
+        return g.groups == 1 || keep_groups<V, N>(g, v, key, reinterpret_cast<V*>(all + (threadIdx.x - place) * N),
+                                                  reinterpret_cast<V*>(ranks + (threadIdx.x - place)), place);
+    };
+    bool quick = false;
+    if constexpr (SIGMOID) {
+        if (!direct) {
+            float f[N];
+            bool far = false;
+#pragma unroll
+            for (int i = 0; i < N; ++i) far = far || fabsf(b[i]) > kQuickBias;
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = x[i] == -kInf ? -kInf : fmaxf(quick_sigmoid(x[i]) + b[i], -kInf) + 0.0f;
+            quick = !__any(far) && __all(keys_of(f) || bad);
+        }
     }
-    if (g.groups > 1) keep_groups<N>(g, c, key, all + (threadIdx.x - place) * N, ranks + (threadIdx.x - place), place);
+    if (!quick) {
+        exactly();
+        keys_of(c);
+    }
+    const float slack = quick ? kQuickSlack : kExactSlack;
     std::uint32_t open = 0, own;
 #pragma unroll
     for (int i = 0; i < N; ++i) open |= key[i] ? 1u << i : 0;
     int chosen, rank = place;
     const bool whole_list = pick<LANES, N>(g.top_k, key, place, own, chosen,
                                      [](int owner, std::uint32_t w) { return owner * N + N - 1 - static_cast<int>(w & (N - 1)); },
-                                     [](std::uint32_t w, std::uint32_t last) { return near_keys(last, w); });
+                                     [&](std::uint32_t w, std::uint32_t last) { return near_keys(last, w, slack); });
     const std::uint32_t after = moved<0x101>(own);  // of the next lane; 0 in the last of 16
-    bool sure = !__any(place < 15 && own && near_keys(own, after));
+    bool sure = !__any(place < 15 && own && near_keys(own, after, slack));
     if (!whole_list) {
+        if (quick) exactly();
         chosen = pick_exactly<LANES, N>(g.top_k, c, open, place);
         own = 1, sure = true;
     }
@@ -541,7 +589,7 @@ void launch_lanes(const T* logits, const float* bias, std::int64_t* indices, voi
 }
 
 // A token takes 16, 32 or 64 lanes of eight experts (four where they are few, 16 past 512), as many as groups and choices at
-// least. 16 experts a lane take half the lanes: 16384 tokens of 256 with a bias 17.1 us for 17.6, but 512 tokens 7.7 for 6.0.
+// least. 16 experts a lane take half the lanes: 16384 tokens of 256 with a bias 14.0 us for 14.0, 512 tokens 6.9 for 5.6.
 template <class T>
 void launch(const void* logits, const float* bias, std::int64_t* indices, void* scores, const Geometry& g, hipStream_t stream) {
     const auto* x = static_cast<const T*>(logits);
