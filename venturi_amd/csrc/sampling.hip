@@ -25,8 +25,8 @@
 // Kept distributions are two or three launches: distribution_scan() looks at few long rows, distribution_cut() finds the last token
 // that a row keeps and the kept mass, and distribution() writes every token's probability. A row that limits leave at most 256 of,
 // and one without limits, need no histogram. The write is bound by memory (96 rows of 151936 bf16 logits: 15 us for 88 MB, 5.8
-// TB/s), the cut by its row's one CU (us, of the same 96 rows, all three together: 38 without limits, 29 with top_k 50, 52 with
-// top_p alone: 21 of them the count, 4 the largest class, 10 the turns' masses, 10 the choice, 8 the search).
+// TB/s), the cut by its row's one CU (the same rows, all in all: 38 us without limits, 29 with top_k 50, 52 with top_p alone: 20
+// of those the count, 2 the largest class, 4 the turns' masses, 4 the choice, 7 the search).
 #include "common.hpp"
 
 #include <climits>
