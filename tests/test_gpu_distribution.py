@@ -182,3 +182,22 @@ def test_graph_and_side_stream(backend, device):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(p, want)
+
+
+def test_runs_that_share_no_workspace_overlap(backend, device):
+    for rows, vocab in ((4, 70001), (64, 30001)):
+        plan = backend.prepare_distribution(rows=rows, vocab=vocab, dtype=BF16, device=device)
+        k = torch.tensor([0, 50, 400, 1] * (rows // 4), dtype=torch.int32, device=device)
+        inputs = [random_logits(rows, vocab, 2.5, BF16, i).to(device) for i in range(2)]
+        outs = [torch.empty(rows, vocab, device=device) for _ in range(2)]
+        work = [torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=device) for _ in range(2)]
+        want = [plan.run(x, None, k, probabilities=torch.empty_like(outs[0]), workspace=work[0]).clone() for x in inputs]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream(device) for _ in range(2)]
+        for _ in range(10):
+            for i, stream in enumerate(streams):
+                with torch.cuda.stream(stream):
+                    plan.run(inputs[i], None, k, probabilities=outs[i], workspace=work[i])
+        torch.cuda.synchronize()
+        for got, wanted in zip(outs, want):
+            assert torch.equal(got, wanted)

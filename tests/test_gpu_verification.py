@@ -264,3 +264,26 @@ def test_graph_and_side_stream(backend, device):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(tokens, want[0]) and torch.equal(accepted, want[1])
+
+
+def test_runs_that_share_no_workspace_overlap(backend, device):
+    n, d, vocab = 5, 3, 60001
+    plan = backend.prepare_verification(sequences=n, drafts=d, vocab=vocab, device=device)
+    calls, want = [], []
+    for i in range(2):
+        p, q, drafted, u = (t.to(device) for t in case(n, d, vocab, 40 + i))
+        out = torch.empty(n, d + 1, dtype=torch.int64, device=device), torch.empty(n, dtype=torch.int32, device=device)
+        work = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=device)
+        calls.append(((p.view(n * (d + 1), vocab), drafted, u),
+                      dict(proposal=q.view(n * d, vocab), tokens=out[0], accepted=out[1], workspace=work)))
+        plan.run(*calls[i][0], **calls[i][1])
+        want.append([t.clone() for t in out])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(device) for _ in range(2)]
+    for _ in range(20):
+        for (inputs, outputs), stream in zip(calls, streams):
+            with torch.cuda.stream(stream):
+                plan.run(*inputs, **outputs)
+    torch.cuda.synchronize()
+    for (_, outputs), (tokens, accepted) in zip(calls, want):
+        assert torch.equal(outputs["tokens"], tokens) and torch.equal(outputs["accepted"], accepted)
