@@ -545,10 +545,16 @@ __device__ __forceinline__ int find_element(const uint4& w, const Pattern& p, in
 
 // What a row keeps: classes above `place`, and of its class the tokens up to `index`.
 struct Cut {
-    double max, heat;     // a token's weight is 2^((logit - max) heat)
-    std::int64_t index;
-    float inverse;        // of the kept mass
-    int place;            // kNone: the row keeps nothing
+    double max, heat;    // a token's weight is 2^((logit - max) heat)
+    float inverse, rest; // of the kept mass, in two parts
+    int place, index;    // place kNone: the row keeps nothing
+
+    __device__ __forceinline__ void set(double top, double heat_, double mass, int place_) {
+        const double whole = 1.0 / mass;
+        max = top, heat = heat_, place = place_;
+        inverse = static_cast<float>(whole);
+        rest = static_cast<float>(whole - static_cast<double>(inverse));
+    }
 };
 
 // A part of a row: its largest logit, and where the row's whole mass counts, the mass in units of that one's weight.
@@ -684,8 +690,9 @@ __device__ __forceinline__ int count_matches(const Row& row, const Pattern& p, i
 }
 
 // Writes the token of occurrence `rank` of the listed chunks from their counts. One wave.
+template <class Index>
 __device__ __forceinline__ void write_match(const Row& row, const Pattern& p, int rank, const int* list, int listed, const int* counts,
-                                            std::int64_t* token) {
+                                            Index* token) {
     const int lane = threadIdx.x & 63;
     int before;
     const int at = find_chunk(counts, listed, rank, before);
@@ -693,11 +700,12 @@ __device__ __forceinline__ void write_match(const Row& row, const Pattern& p, in
     const bool live = at >= 0 && vector < row.vectors;
     const uint4 w = live ? row.whole()[vector] : make_uint4(~p.bits, ~p.bits, ~p.bits, ~p.bits);
     const int element = find_element(w, p, before, rank);
-    if (element >= 0) *token = row.head + 8ll * vector + element;
+    if (element >= 0) *token = row.head + 8 * vector + element;
 }
 
 // Occurrences in the row's head (tail: in its tail); the token, if rank is among them. One wave.
-__device__ __forceinline__ int edge_match(const Row& row, const Edge& edge, const Pattern& p, bool tail, int rank, std::int64_t* token) {
+template <class Index>
+__device__ __forceinline__ int edge_match(const Row& row, const Edge& edge, const Pattern& p, bool tail, int rank, Index* token) {
     const int lane = threadIdx.x & 63;
     const bool match = edge.match(p) && (lane < row.head) != tail;
     const unsigned long long all = __ballot(match);
@@ -707,7 +715,8 @@ __device__ __forceinline__ int edge_match(const Row& row, const Edge& edge, cons
 
 // The token of the rank-th occurrence of the class: in the head, in the vectors or in the tail. (choose() has ended with a
 // barrier: the histogram's memory is free.)
-__device__ __forceinline__ void find_token(Shared& s, const Row& row, const Edge& edge, const Choice& choice, std::int64_t* token) {
+template <class Index>
+__device__ __forceinline__ void find_token(Shared& s, const Row& row, const Edge& edge, const Choice& choice, Index* token) {
     const int t = threadIdx.x, wave = t >> 6;
     const Pattern pattern(choice.place);
     int *counts = reinterpret_cast<int*>(s.histogram), *list = counts + kChunks;
@@ -867,8 +876,11 @@ __global__ __launch_bounds__(kScanThreads) void distribution_scan(Operands o) {
 // A row without limits, down to the lowest number; none at all if its largest logit is no class.
 template <class T>
 __device__ __forceinline__ Cut cut_of_all(float top, double heat, double mass) {
-    if (top == -__builtin_inff()) return {0.0, heat, INT_MAX, 0.0f, kNone};
-    return {top, heat, INT_MAX, static_cast<float>(1.0 / mass), 0x8000 + static_cast<int>(Bits<T>::kInf) - 1};
+    Cut cut;
+    cut.index = INT_MAX;
+    if (top == -__builtin_inff()) cut.set(0.0, heat, 1.0, kNone);
+    else cut.set(top, heat, mass, 0x8000 + static_cast<int>(Bits<T>::kInf) - 1);
+    return cut;
 }
 
 // The same from its parts, two a lane at most. One wave; its first lane's.
@@ -1085,11 +1097,8 @@ __device__ __forceinline__ bool cut_largest(Shared& s, const Row& row, const Edg
     if (lane != 0) return true;
     const std::uint64_t last = s.ordered[length - 1];
     const int order = static_cast<int>(last >> 32) - 32768;
-    cut.place = order < 0 ? 0x8000 - order : 32767 - order;
-    cut.max = top;
-    cut.heat = heat;
-    cut.inverse = static_cast<float>(1.0 / mass);
-    cut.index = static_cast<std::int64_t>(~static_cast<std::uint32_t>(last));
+    cut.set(top, heat, mass, order < 0 ? 0x8000 - order : 32767 - order);
+    cut.index = static_cast<int>(~static_cast<std::uint32_t>(last));
     return true;
 }
 
@@ -1149,10 +1158,8 @@ __global__ __launch_bounds__(kThreads) void distribution_cut(Operands o) {
     const Choice choice = choose<T, true>(s, set);
     const bool ended = choice.place == kNone || s.whole;
     if (t == 0) {
-        cut.max = choice.place == kNone ? 0.0 : class_value<T>(s.top);
-        cut.heat = heat;
-        cut.inverse = static_cast<float>(1.0 / s.probability);
-        cut.place = choice.place;
+        if (choice.place == kNone) cut.set(0.0, heat, 1.0, kNone);
+        else cut.set(class_value<T>(s.top), heat, s.probability, choice.place);
         if (ended) cut.index = INT_MAX;
     }
     __syncthreads();
@@ -1193,8 +1200,9 @@ __device__ __forceinline__ float probability(const Cut& cut, std::uint32_t last,
     const double exponent = (value - cut.max) * cut.heat;
     const float high = static_cast<float>(exponent), low = static_cast<float>(exponent - static_cast<double>(high));
     if (!(high > -150.0f)) return 0.0f;
+    // The rests of exponent and inverse together: the exponential's own error and one rounding are left.
     const float w = __builtin_amdgcn_exp2f(high);
-    return fmaf(w, low * 0.693147181f, w) * cut.inverse;
+    return fmaf(w, cut.inverse, w * fmaf(low * 0.693147181f, cut.inverse, cut.rest));
 }
 
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
