@@ -201,3 +201,16 @@ def test_runs_that_share_no_workspace_overlap(backend, device):
         torch.cuda.synchronize()
         for got, wanted in zip(outs, want):
             assert torch.equal(got, wanted)
+
+
+@pytest.mark.parametrize("rows,vocab,exponent,apart", [(2, 151936, 7, 8192), (33, 57001, 8, 57001), (33, 70003, 9, 70003)])
+def test_a_tail_that_holds_the_mass_and_is_no_multiple_of_the_largest_logits_last_bit(backend, device, rows, vocab, exponent, apart):
+    """A difference of two logits that 32 bits do not hold: rounding it would move every weight of the tail, and so the mass, by
+    6 to 9 x 2^-24. Else a weight errs by the exponential's step (2 x 2^-24) and its argument's rounding (0.2 x 2^-24), the mass by
+    as much (the tail's sums are exact), and a probability by both and its own rounding: 5.4 x 2^-24, within check()'s 6."""
+    far, near = 8.0625, 1.984375 * 2.0**-22
+    for top, tail in ((far, near), (near, -far), (far, -near)):
+        logits = torch.full((rows, vocab), tail, dtype=BF16)
+        for i in range(rows):
+            logits[i, 17 * i:: apart] = top
+        check(backend, device, logits, t=[far / exponent] * rows)

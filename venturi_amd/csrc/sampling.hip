@@ -754,42 +754,35 @@ __device__ __forceinline__ float value_of(std::uint32_t bits) {
     return to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(bits)));
 }
 
-// Sums of a row's weights 2^((x - top) heat) without a class for each: of 32 bits with the exponent's rest, added in eights and
-// then in 64 bits. Of 64 bits at temperatures whose inverse, or whose products with differences of any two logits, leave the
-// range of 32.
+// Sums of a row's weights 2^((x - top) heat) without a class for each: exponents of 64 bits, whose fraction (half a step of 2^-25)
+// goes through an exponential of 32 (a step of 2^-23), added in eights and then in 64 bits. (A difference of logits is no number of
+// 32 bits where one is 2^14 times the other: rounded to one, it weighed a whole tail by up to 2^-20 too much. 257 rows of 32003
+// 24.2 -> 25.0 us.)
 template <class T>
 struct Weights {
-    double heat;
-    float top, high, low, least;
-    bool wide;
+    double top, heat, least;
+    bool infinite;
 
     __device__ __forceinline__ Weights(float top, double heat)
-        : heat(heat), top(top), high(static_cast<float>(heat)), low(static_cast<float>(heat - static_cast<double>(high))), least(-160.0f / high),
-          wide(top == __builtin_inff() || !(heat >= 1e-30 && heat <= 1e30)) {}
-    __device__ __forceinline__ float near(std::uint32_t bits) const {
-        const float d = fmaxf(value_of<T>(bits) - top, least), e = d * high;  // NaN and -inf weigh 2^-160: nothing
-        const float rest = fmaf(d, low, fmaf(d, high, -e)), w = __builtin_amdgcn_exp2f(e);
-        return fmaf(w, rest * 0.693147181f, w);
+        : top(top), heat(heat), least(-1000.0 / heat), infinite(top == __builtin_inff()) {}
+    __device__ __forceinline__ float of_finite(std::uint32_t bits) const {
+        constexpr double kWhole = 0x1.8p52;  // what is added to it is rounded to a whole number, which its low word holds
+        const double d = fmax(static_cast<double>(value_of<T>(bits)) - top, least);  // of NaN and -inf too: they weigh nothing
+        const double sum = fma(d, heat, kWhole), rest = fma(d, heat, kWhole - sum);
+        const int whole = static_cast<int>(__builtin_bit_cast(std::uint64_t, sum));
+        return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(static_cast<float>(rest)), whole);
     }
-    __device__ __forceinline__ float far(std::uint32_t bits) const {
-        const float x = value_of<T>(bits);
-        return x == top ? 1.0f : static_cast<float>(falling_power((static_cast<double>(x) - static_cast<double>(top)) * heat));
-    }
-    __device__ __forceinline__ float operator()(std::uint32_t bits) const { return wide ? far(bits) : near(bits); }
+    __device__ __forceinline__ float of_infinite(std::uint32_t bits) const { return value_of<T>(bits) == top ? 1.0f : 0.0f; }
+    __device__ __forceinline__ float operator()(std::uint32_t bits) const { return infinite ? of_infinite(bits) : of_finite(bits); }
     __device__ __forceinline__ float sum(const uint4& v) const {
-        if (wide) {
-            float all = 0.0f;
-            uint4 u = v;
-#pragma unroll 1
-            for (int j = 0; j < 8; ++j) {
-                all += far(u.x & 0xffff);
-                u = make_uint4(u.x >> 16 | u.y << 16, u.y >> 16 | u.z << 16, u.z >> 16 | u.w << 16, u.w >> 16);
-            }
-            return all;
-        }
         float x[8];
+        if (infinite) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = near(element(v, j));
+            for (int j = 0; j < 8; ++j) x[j] = of_infinite(element(v, j));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = of_finite(element(v, j));
+        }
         return ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
     }
 };
