@@ -274,3 +274,39 @@ def test_routed_tokens_go_through_the_experts(backend, device):
     assert bool(outs[0][4].isnan().all()) and torch.equal(outs[0].isnan(), outs[1].isnan())
     fine = [i for i in range(tokens) if i != 4]
     assert torch.equal(outs[0][fine], outs[1][fine])
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16, FP32], ids=NAMES.values())
+@pytest.mark.parametrize("experts", [16, 64, 160, 1024])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_masked_experts_come_after_those_with_a_bias_of_minus_infinity(backend, device, dtype, experts, score):
+    """Experts and groups by (masked, c, index); a group of masked experts alone comes after all others."""
+    inf, top_k = math.inf, 6
+    logits = random_logits(5, experts, dtype, 21)
+    logits[:, ::2] = -inf
+    logits[1, : experts // 4] = -inf
+    logits[2, 3:] = -inf
+    logits[3, : experts - 3] = -inf
+    logits[4] = -inf
+    bias = torch.full((experts,), -inf)
+    bias[5], bias[experts // 2 + 1], bias[0] = 0.25, inf, inf
+    for groups, kept, rank in ((1, 1, "max"), (4, 2, "pairs"), (4, 2, "max"), (8, 6, "pairs")):
+        size = experts // groups
+        plan = backend.prepare_routing(tokens=5, experts=experts, top_k=top_k, dtype=dtype, device=device, score=score, groups=groups,
+                                       kept_groups=kept, group_rank=rank, score_dtype=FP32, renormalize=False)
+        ids = torch.empty(5, top_k, dtype=torch.int64, device=device)
+        weights = torch.empty(5, top_k, device=device)
+        plan.run(logits.to(device), bias.to(device), indices=ids, scores=weights)
+        for x, got, shares in zip(logits.double(), ids.tolist(), weights.double().cpu()):
+            s = torch.sigmoid(x) if score == "sigmoid" else torch.softmax(x, -1).nan_to_num(0.0)
+            masked, c = (x == -inf).tolist(), (s + bias.double()).tolist()
+
+            def group(g):
+                there = sorted((c[e] for e in range(g * size, (g + 1) * size) if not masked[e]), reverse=True)[: 2 if rank == "pairs" else 1]
+                return not there, -(inf if inf in there else sum(there)), g
+
+            order = [g for g in sorted(range(groups), key=group)][:kept]
+            order = sorted((e for e in range(experts) if e // size in order), key=lambda e: (masked[e], 0.0 if masked[e] else -c[e], e))
+            assert got == order[:top_k], (groups, rank)
+            want = torch.where(x == -inf, 0.0, s)[got]
+            assert bool(((shares - want).abs() <= 2.0**-23 * want + 2.0**-126).all())

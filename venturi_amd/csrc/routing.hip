@@ -159,6 +159,7 @@ __device__ __forceinline__ void reciprocal(double (&x)[B]) {
 }
 
 constexpr double kLog2e = 1.44269504088896340736;
+constexpr double kLeast = -1.7976931348623157e308;  // of biases of -inf: a masked expert's -inf lies below, whatever its index
 
 // exp(x - top), or 1 / (1 + exp(-x)); below 2^-1000 they are 0, of NaN too.
 template <bool SIGMOID, int B>
@@ -378,7 +379,8 @@ __device__ __forceinline__ bool keep_groups(const Geometry& g, const V (&c)[N], 
             }
         }
     }
-    const V rank = g.pairs && best.second > none ? best.most + best.second : best.most;
+    V rank = g.pairs && best.second > none ? best.most + best.second : best.most;
+    if constexpr (sizeof(V) == 8) rank = best.most > none ? fmax(rank, kLeast) : none;
     rank_of[place] = rank;
     wave_fence();
     int ahead = 0, may_be_ahead = 0;
@@ -491,7 +493,7 @@ __global__ __launch_bounds__(kThreads) void route_scores(const T* __restrict__ l
     }
     const auto whole = [&](float logit, double s, float offset) {  // a score with its bias
         const double v = direct ? static_cast<double>(logit) : s + static_cast<double>(offset);
-        return logit == -kInf ? -__builtin_inf() : fmax(v + 0.0, -__builtin_inf());  // one zero, and no NaN
+        return logit == -kInf ? -__builtin_inf() : fmax(v + 0.0, kLeast);  // one zero, and no NaN
     };
     const auto exactly = [&] {
         if constexpr (SIGMOID) {
