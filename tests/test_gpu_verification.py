@@ -287,3 +287,24 @@ def test_runs_that_share_no_workspace_overlap(backend, device):
     torch.cuda.synchronize()
     for (_, outputs), (tokens, accepted) in zip(calls, want):
         assert torch.equal(outputs["tokens"], tokens) and torch.equal(outputs["accepted"], accepted)
+
+
+@pytest.mark.parametrize("vocab", [40, 50001])
+def test_a_draft_without_a_probability_is_refused_whatever_its_proposal_and_uniform(backend, device, vocab):
+    """Proposals and uniforms below 0 do not let a token of probability 0, or of none, stand, nor is it drawn."""
+    n, inf, nan = 6, math.inf, math.nan
+    p, q = torch.full((n, 2, vocab), 0.5 / vocab), torch.full((n, 1, vocab), 0.25 / vocab)
+    drafted = torch.full((n, 1), 7)
+    u = torch.full((n, 2), 0.5)
+    p[:, 0, 7] = torch.tensor([0.0, -1.0, nan, inf, 0.0, 0.125])
+    q[:, 0, 7] = torch.tensor([-0.25, -2.0, -0.25, -inf, 0.25, -0.25])
+    u[4, 0] = -1.0
+    plan = backend.prepare_verification(sequences=n, drafts=1, vocab=vocab, device=device)
+    for proposal in (q, None):
+        tokens, accepted = torch.empty(n, 2, dtype=torch.int64, device=device), torch.empty(n, dtype=torch.int32, device=device)
+        uniforms = u if proposal is not None else torch.tensor([[-0.5, 0.5]] * n)
+        plan.run(p.view(2 * n, vocab).to(device), drafted.to(device), uniforms.to(device),
+                 proposal=None if proposal is None else q.view(n, vocab).to(device), tokens=tokens, accepted=accepted,
+                 workspace=torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=device))
+        assert accepted.tolist() == [0, 0, 0, 0, 0, 1]
+        assert all(token != 7 and 0 <= token < vocab and end == -1 for token, end in tokens[:5].tolist()) and tokens[5, 0] == 7

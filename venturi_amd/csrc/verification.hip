@@ -1,7 +1,7 @@
 // Verification of drafted tokens against the target's probabilities, from given random numbers.
 //
-// Draft i of a sequence stands while u_i q_i(d_i) < p_i(d_i) (q = 1 for certain drafts): both sides are products of 32-bit
-// numbers, exact in 64 bits. After the first refusal the next token comes from max(p - q, 0) of that row (of certain drafts:
+// Draft i of a sequence stands while u_i q_i(d_i) < p_i(d_i) and p_i(d_i) > 0 (q = 1 for certain drafts): both sides are products
+// of 32-bit numbers, exact in 64 bits. After the first refusal the next token comes from max(p - q, 0) of that row (of certain drafts:
 // p without the draft), where that has a mass, else from p; after the last draft from p of the row behind it. It is the first
 // token, by index, at which the running sum passes u times the whole one; sums in 64 bits, in a fixed order.
 //
@@ -53,7 +53,7 @@ __device__ __forceinline__ Verdict verdict_of(const Operands& o, int sequence) {
     const std::int64_t at = there ? id : 0;
     const double p = positive(o.target[(first + sequence + draft) * o.vocab + at]);
     const double q = o.proposal ? o.proposal[(first + draft) * o.vocab + at] : 1.0;
-    const unsigned long long bad = __ballot(lane < count && !(there && u * q < p));
+    const unsigned long long bad = __ballot(lane < count && !(there && p > 0.0 && u * q < p));
     const int accepted = bad ? __ffsll(bad) - 1 : count;
     return {accepted, bad != 0, bad && !o.proposal ? __shfl(token, accepted, 64) : -1, 0};
 }
