@@ -308,3 +308,22 @@ def test_a_draft_without_a_probability_is_refused_whatever_its_proposal_and_unif
                  workspace=torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=device))
         assert accepted.tolist() == [0, 0, 0, 0, 0, 1]
         assert all(token != 7 and 0 <= token < vocab and end == -1 for token, end in tokens[:5].tolist()) and tokens[5, 0] == 7
+
+
+@pytest.mark.parametrize("certain", [False, True], ids=["drawn", "certain"])
+@pytest.mark.parametrize("vocab", [500, 40001])
+def test_what_lies_behind_the_last_token_has_no_effect(backend, device, certain, vocab):
+    """Drafts past a sequence's count and rows past the drawn token's, of any bits."""
+    n, d = 12, 5
+    p, q, drafted, u = case(n, d, vocab, 31, 0.3, certain)
+    counts = [i % (d + 1) for i in range(n)]
+    tokens, accepted = check(backend, device, p, q, drafted, u, counts)
+    assert any(a == c < d for a, c in zip(accepted, counts)) and any(a < c for a, c in zip(accepted, counts))
+    for value, token in ((math.nan, 2**62), (math.inf, -2**63), (-1.0, vocab - 1)):
+        for i in range(n):
+            p[i, accepted[i] + 1:] = value
+            u[i, counts[i]: d] = value
+            drafted[i, counts[i]:] = token
+            if q is not None:
+                q[i, accepted[i] + 1:], q[i, counts[i]:] = value, value
+        assert check(backend, device, p, q, drafted, u, counts) == (tokens, accepted)

@@ -53,7 +53,8 @@ class VerificationPlan:
         ``uniforms`` fp32 [sequences, drafts + 1], the last of a sequence for its drawn token; ``proposal`` fp32
         [sequences * drafts, vocab], None for certain drafts; ``counts`` int32 [sequences], the drafts that a sequence has,
         None for all. Writes ``accepted`` int32 [sequences] and ``tokens`` int64 [sequences, drafts + 1]: the drafts that
-        stand, the drawn token, and -1. Rows behind the drawn token's are not read."""
+        stand, the drawn token, and -1. Nothing behind a sequence's count, and no row behind the drawn token's, has an effect;
+        the probabilities of the drafts there may be loaded all the same."""
         device, index, n, v = self.device, self._index, self.sequences, self.vocab
         d = self.drafts
         x = address(target, self._target, torch.float32, device, index, "target", 4)
