@@ -465,7 +465,8 @@ int venturi_sample_run(const void* logits, const float* uniforms, const float* t
                        const float* top_p, const float* min_p, int64_t* tokens, float* probabilities,
                        int rows, int vocab, int dtype, void* stream);
 /* The probabilities fp32 [rows][vocab] that sampling with these settings draws from: the kept tokens' weights over their
- * sum, else 0. rows: at most 65535. workspace: venturi_distribution_bytes, 256-byte aligned. */
+ * sum, else 0. rows: at most 65535. workspace: venturi_distribution_bytes, 256-byte aligned. Outputs share no byte with other
+ * operands. */
 uint64_t venturi_distribution_bytes(int rows, int vocab);
 int venturi_distribution_run(const void* logits, const float* temperature, const int32_t* top_k, const float* top_p,
                              const float* min_p, float* probabilities, void* workspace, uint64_t available, int rows,
@@ -474,7 +475,8 @@ int venturi_distribution_run(const void* logits, const float* temperature, const
  * stands while uniforms[i] * proposal_i < target_i at its token; the next token is drawn with uniforms[drafts] from what
  * target - proposal leaves of the first refused row, or from the row behind the last draft. proposal fp32
  * [sequences * drafts][vocab], NULL for certain drafts (probability 1); counts [sequences], NULL for all drafts. tokens
- * int64 [sequences][drafts + 1] ends in -1. workspace: venturi_verify_bytes (may be 0), 256-byte aligned. */
+ * int64 [sequences][drafts + 1] ends in -1. workspace: venturi_verify_bytes (may be 0), 256-byte aligned. Outputs share no byte
+ * with other operands. */
 uint64_t venturi_verify_bytes(int sequences, int drafts, int vocab);
 int venturi_verify_run(const float* target, const float* proposal, const int64_t* drafted, const int32_t* counts,
                        const float* uniforms, int64_t* tokens, int32_t* accepted, void* workspace, uint64_t available,
@@ -485,7 +487,7 @@ int venturi_verify_run(const float* target, const float* proposal, const int64_t
  * experts), ordered by s + bias (fp32 [experts] or NULL), ties by index, within the kept_groups best of `groups` groups of
  * equal size (ranked by their largest, or with pairs != 0 the sum of their two largest). indices int64 and scores
  * (score_dtype) [tokens][top_k], top_k <= 16: s, with renormalize != 0 over its sum, times scale. A token with a NaN (or
- * +inf under softmax) gets -1 and NaN. */
+ * +inf under softmax) gets -1 and NaN. Outputs share no byte with other operands. */
 int venturi_route_run(const void* logits, const float* bias, int64_t* indices, void* scores, int tokens, int experts,
                       int top_k, int groups, int kept_groups, int sigmoid, int pairs, int renormalize, float scale,
                       int dtype, int score_dtype, void* stream);

@@ -304,3 +304,31 @@ def test_verification_tests_reach_every_instance():
              (256, 1, 270001), (5, 1, 40001)]
     names = built("verify_sum") | built("verify_take")
     assert names and names == reached([verify(*size) for size in sizes])
+
+
+@pytest.mark.parametrize("entry,good,changes", [
+    ("venturi_route_run", ROUTED, [
+        dict(indices=A), dict(indices=A + 120), dict(indices=B + 248), dict(scores=A + 126), dict(scores=B), dict(scores=C + 24),
+        dict(indices=D - 24), dict(indices=A + 248, dtype=2), dict(scores=C - 8, score_dtype=2)]),
+    ("venturi_distribution_run", {**KEPT, "t": D, "k": D + 64, "p": E, "m": F}, [
+        dict(out=A), dict(out=A + 16), dict(out=A - 36), dict(out=D - 36), dict(out=D + 64), dict(out=E), dict(out=F), dict(workspace=A),
+        dict(workspace=D), dict(workspace=E), dict(workspace=F), dict(workspace=B), dict(out=C + 28)]),
+    ("venturi_verify_run", VERIFY, [
+        dict(tokens=A + 8 * 36000 - 8), dict(tokens=B), dict(tokens=C + 40), dict(tokens=D + 24), dict(accepted=A), dict(accepted=B + 215996),
+        dict(accepted=C), dict(accepted=D + 28), dict(accepted=E + 60), dict(accepted=E - 4), dict(counts=E), dict(counts=F + 4)]),
+    ("venturi_verify_run", {**VERIFY, "vocab": 40000}, [
+        dict(workspace=A), dict(workspace=B), dict(workspace=C), dict(workspace=D), dict(workspace=E), dict(workspace=F), dict(tokens=F + 4096),
+        dict(counts=F + 4096)])])
+def test_entry_points_refuse_outputs_that_overlap(entry, good, changes):
+    lib = native.load()
+    for change in changes:
+        assert getattr(lib, entry)(*{**good, **change}.values()) == -1, change
+        assert "overlap" in lib.error(), (change, lib.error())
+
+
+def test_operands_side_by_side_do_not_overlap():
+    calls = [("venturi_route_run", {**ROUTED, "scores": A + 128, "indices": B + 256}),
+             ("venturi_distribution_run", {**KEPT, "out": A + 20, "workspace": A + 256}),
+             ("venturi_verify_run", {**VERIFY, "tokens": D + 32, "accepted": D + 96, "workspace": D + 96})]  # empty
+    for entry, good in calls:
+        assert record([(0, entry, list(good.values()))])[0]

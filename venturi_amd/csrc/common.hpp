@@ -39,6 +39,12 @@ inline bool aligned(const void* p, std::uintptr_t bytes) {
     return (reinterpret_cast<std::uintptr_t>(p) % bytes) == 0;
 }
 
+// Whether two operands share a byte; null and empty ones do not.
+inline bool meet(const void* a, std::uint64_t a_bytes, const void* b, std::uint64_t b_bytes) {
+    const auto first = reinterpret_cast<std::uintptr_t>(a), second = reinterpret_cast<std::uintptr_t>(b);
+    return a && b && a_bytes && b_bytes && first < second + b_bytes && second < first + a_bytes;
+}
+
 inline std::int64_t padded_k(std::int64_t k) { return (k + 127) / 128 * 128; }
 
 // Runs `body`, mapping exceptions to the -1 / message convention.

@@ -305,11 +305,6 @@ void launch(const Operands& o, hipStream_t stream) {
     else staged(std::false_type{});
 }
 
-bool meet(const void* a, std::uint64_t a_bytes, const void* b, std::uint64_t b_bytes) {
-    const auto first = reinterpret_cast<std::uintptr_t>(a), second = reinterpret_cast<std::uintptr_t>(b);
-    return a && b && first < second + b_bytes && second < first + a_bytes;
-}
-
 }  // namespace
 }  // namespace vt
 

@@ -622,6 +622,12 @@ VT_EXPORT int venturi_route_run(const void* logits, const float* bias, std::int6
         vt::require(vt::aligned(logits, dtype == vt::kF32 ? 4 : 2) && vt::aligned(bias, 4) && vt::aligned(indices, 8) &&
                         vt::aligned(scores, score_dtype == vt::kF32 ? 4 : 2),
                     "routing operands must be aligned to their elements");
+        const std::uint64_t logit_bytes = (dtype == vt::kF32 ? 4ull : 2ull) * tokens * experts, bias_bytes = 4ull * experts;
+        const std::uint64_t index_bytes = 8ull * tokens * top_k, score_bytes = (score_dtype == vt::kF32 ? 4ull : 2ull) * tokens * top_k;
+        vt::require(!vt::meet(indices, index_bytes, logits, logit_bytes) && !vt::meet(indices, index_bytes, bias, bias_bytes) &&
+                        !vt::meet(scores, score_bytes, logits, logit_bytes) && !vt::meet(scores, score_bytes, bias, bias_bytes) &&
+                        !vt::meet(scores, score_bytes, indices, index_bytes),
+                    "routing outputs must not overlap other operands");
         const vt::Geometry g{tokens, experts, top_k, groups, kept_groups, sigmoid != 0, pairs != 0, renormalize != 0, scale, score_dtype};
         const auto s = static_cast<hipStream_t>(stream);
         if (dtype == vt::kF16)

@@ -1305,6 +1305,15 @@ VT_EXPORT int venturi_distribution_run(const void* logits, const float* temperat
         vt::require(vt::aligned(logits, 16) && vt::aligned(probabilities, 4), "logits must be 16-byte aligned");
         vt::require(workspace && available >= vt::distribution_bytes(rows, vocab) && vt::aligned(workspace, 256),
                     "a distribution needs its workspace, 256-byte aligned");
+        const std::uint64_t settings_bytes = 4ull * rows, logit_bytes = 2ull * rows * vocab, needed = vt::distribution_bytes(rows, vocab);
+        const auto meets_an_input = [&](const void* out, std::uint64_t bytes) {
+            return vt::meet(out, bytes, logits, logit_bytes) || vt::meet(out, bytes, temperature, settings_bytes) ||
+                   vt::meet(out, bytes, top_k, settings_bytes) || vt::meet(out, bytes, top_p, settings_bytes) ||
+                   vt::meet(out, bytes, min_p, settings_bytes);
+        };
+        vt::require(!meets_an_input(probabilities, 2 * logit_bytes) && !meets_an_input(workspace, needed) &&
+                        !vt::meet(probabilities, 2 * logit_bytes, workspace, needed),
+                    "a distribution's outputs must not overlap other operands");
         const auto s = static_cast<hipStream_t>(stream);
         auto* cuts = static_cast<vt::Cut*>(workspace);
         auto* parts = reinterpret_cast<vt::Part*>(cuts + rows);

@@ -372,6 +372,16 @@ VT_EXPORT int venturi_verify_run(const float* target, const float* proposal, con
         const std::uint64_t bytes = vt::sum_bytes(o, sequences);
         vt::require(!bytes || (workspace && available >= bytes && vt::aligned(workspace, 256)),
                     "verification needs its workspace, 256-byte aligned");
+        const std::uint64_t n = sequences, d = drafts, token_bytes = 8 * n * (d + 1), accepted_bytes = 4 * n;
+        const auto meets_an_input = [&](const void* out, std::uint64_t size) {
+            return vt::meet(out, size, target, 4 * n * (d + 1) * vocab) || vt::meet(out, size, proposal, 4 * n * d * vocab) ||
+                   vt::meet(out, size, drafted, 8 * n * d) || vt::meet(out, size, counts, 4 * n) ||
+                   vt::meet(out, size, uniforms, 4 * n * (d + 1));
+        };
+        vt::require(!meets_an_input(tokens, token_bytes) && !meets_an_input(accepted, accepted_bytes) &&
+                        !meets_an_input(workspace, bytes) && !vt::meet(tokens, token_bytes, accepted, accepted_bytes) &&
+                        !vt::meet(workspace, bytes, tokens, token_bytes) && !vt::meet(workspace, bytes, accepted, accepted_bytes),
+                    "verification outputs must not overlap other operands");
         o.target = target, o.proposal = proposal, o.drafted = drafted, o.counts = counts, o.uniforms = uniforms;
         o.tokens = tokens, o.accepted = accepted, o.verdicts = static_cast<vt::Verdict*>(workspace);
         o.sums = reinterpret_cast<double*>(o.verdicts + sequences);
