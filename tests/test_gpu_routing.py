@@ -310,3 +310,21 @@ def test_masked_experts_come_after_those_with_a_bias_of_minus_infinity(backend, 
             assert got == order[:top_k], (groups, rank)
             want = torch.where(x == -inf, 0.0, s)[got]
             assert bool(((shares - want).abs() <= 2.0**-23 * want + 2.0**-126).all())
+
+
+@pytest.mark.parametrize("bias", [None, 0.0], ids=["none", "zeros"])
+def test_scores_below_2_to_the_minus_1000_count_as_0(backend, device, bias):
+    """Shares of sigmoids down to logits of -693, and weights of 0 below; experts in order either way."""
+    logits = -692.0 - torch.arange(16.0).flip(0) / 16  # the largest last, all above -693.1
+    logits = torch.stack([logits, logits - 2, logits.clamp(min=-692.5)])
+    logits[2, 9] = -1000.0
+    offsets = None if bias is None else torch.full((16,), bias, device=device)
+    plan = backend.prepare_routing(tokens=3, experts=16, top_k=8, dtype=FP32, device=device, score="sigmoid", score_dtype=FP32)
+    ids, weights = torch.empty(3, 8, dtype=torch.int64, device=device), torch.empty(3, 8, device=device)
+    plan.run(logits.to(device), offsets, indices=ids, scores=weights)
+    weights = weights.double().cpu()
+    for row in (0, 2):
+        want = torch.softmax(logits[row].double()[ids[row].cpu()], 0)  # 1 / (1 + exp(-x)) is exp(x) here
+        assert bool(((weights[row] - want).abs() <= 2.0**-23 * want).all())
+    assert ids[0].tolist() == list(range(15, 7, -1)) and not bool(weights[1].any())
+    assert ids[1].tolist() == (list(range(15, 7, -1)) if bias is None else list(range(8)))

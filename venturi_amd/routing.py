@@ -7,8 +7,9 @@ ones by index. The first ``top_k`` are chosen. Their weights are s without the b
 ``renormalize``, times ``scale``.
 
 An expert whose logit is -inf is masked: it comes after all others, those with a bias of -inf among them, with weight 0,
-whatever its bias, and so does a group of masked experts alone. A sum of +inf and -inf counts as +inf. Weights whose sum is 0
-stay 0. A token with a NaN among its logits or biased scores, or with +inf under softmax, gets ids -1 and NaN scores, which
+whatever its bias, and so does a group of masked experts alone. A sum of +inf and -inf counts as +inf. Scores below 2^-1000
+(sigmoids of logits under -693.1, and softmax scores that far under the largest) count as 0, and weights whose sum is 0 stay 0.
+A token with a NaN among its logits or biased scores, or with +inf under softmax, gets ids -1 and NaN scores, which
 the experts' plan turns into a NaN row. Scores are computed in 64 bits, so that the order is the definition's: experts go by
 index where 64 bits do not tell them apart (without a bias, where their logits are equal).
 
