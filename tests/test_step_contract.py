@@ -332,3 +332,12 @@ def test_operands_side_by_side_do_not_overlap():
              ("venturi_verify_run", {**VERIFY, "tokens": D + 32, "accepted": D + 96, "workspace": D + 96})]  # empty
     for entry, good in calls:
         assert record([(0, entry, list(good.values()))])[0]
+
+
+def test_columns_whose_count_a_step_on_leaves_32_bits_are_refused():
+    wide = {**RMS, "workspace": None, "passes": 0}
+    for dtype in (0, 1, 2):
+        for k in (2**31 - 1, 2**31 - 1024):
+            assert native.load().venturi_residual_rms_run(*{**wide, "dtype": dtype, "k": k}.values()) == -1
+            assert "columns" in native.load().error()
+        assert kernels([(0, "venturi_residual_rms_run", list({**wide, "dtype": dtype, "k": 2**31 - 1025}.values()))])[0]

@@ -315,6 +315,7 @@ VT_EXPORT int venturi_residual_rms_run(const void* x, const void* residual, cons
                                        float epsilon, void* stream) {
     return vt::guarded([&] {
         vt::require(tokens > 0 && k > 0, "the residual norm needs tokens and columns");
+        vt::require(k <= INT32_MAX - 1024, "the residual norm counts columns, a workgroup's step past the last, in 32 bits");
         vt::require(x && residual && gamma && total, "null residual norm operand");
         vt::require(epsilon > 0.0f && std::isfinite(epsilon), "invalid RMSNorm epsilon");
         vt::require(dtype == vt::kF16 || dtype == vt::kBF16 || dtype == vt::kF32, "unsupported scalar type");

@@ -63,7 +63,7 @@ class ResidualRMSPlan:
 
 def prepare_residual_rms(norm, *, tokens, a8_passes=0):
     """Plan of total = x + residual and its RMSNorm for ``tokens`` rows of a ResidentRMSNorm's dtype. ``a8_passes`` 1 or 2
-    (with the second pass for the first one's residuals) adds the int8 form, of fp16 rows."""
+    (with the second pass for the first one's residuals) adds the int8 form, of fp16 rows. A run takes up to 2^31 - 1025 features."""
     if not isinstance(norm, ResidentRMSNorm):
         raise ValueError("The residual norm requires a resident RMSNorm")
     if type(a8_passes) is not int or not 0 <= a8_passes <= 2:
