@@ -38,7 +38,8 @@ __device__ __forceinline__ float inverse_rms(float sum, int k, float epsilon) {
 }
 
 // A workgroup per row, any width and alignment: thread c runs chain c on the elements that it adds and stores, and the norm
-// reads them back.
+// reads them back. One element at a time: 8190 rows of 5120 off 16 bytes 111 us where staged ones take 62, 2048 of 16384 fp32
+// columns 147 (a copy's rate: 106), 61 of 32768 bf16 columns 68 where the add and the norm apart take 29.
 template <class T>
 __global__ __launch_bounds__(kChains) void residual_rms_any(Operands o) {
     __shared__ __align__(16) float chains[kChains];

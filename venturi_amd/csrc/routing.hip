@@ -328,7 +328,7 @@ __device__ __forceinline__ bool near_keys(std::uint32_t a, std::uint32_t b, floa
 
 // 1 / (1 + exp(-x)) to 2^-22: the product's rounding weighs |x| s (1 - s) 2^-24, the exponential's last bit s (1 - s) 2^-23, and
 // the sum and its inverse s (2^-24 + 2^-23).
-// With a bias of up to 4, whose sum is rounded by 5 x 2^-24 at most, it errs by less than 2^-21: two by less than 2^-20, and
+// With a bias of up to 4, whose sum is rounded by 4 x 2^-24 at most, it errs by less than 2^-21: two by less than 2^-20, and
 // sums of two with their own rounding by less than 2^-19 each.
 constexpr float kQuickBias = 4.0f, kQuickSlack = 0x1p-20f;
 __device__ __forceinline__ float quick_sigmoid(float x) {
@@ -454,7 +454,8 @@ __device__ __forceinline__ int rank_of_16(double c, std::uint32_t expert) {
 // the last, and where keys that follow each other are near, the scores of the up to 16 candidates, a lane each, decide. More
 // candidates than that (many equal scores, or masked experts) are picked score by score. Keys and groups' ranks of sigmoid scores
 // are first made of quick 32-bit ones; where those do not decide on the groups, the wave starts again with 64 bits (4099 tokens
-// of 256 in 8 groups 9.7 -> 8.2 us, 16384 21.1 -> 17.1).
+// of 256 in 8 groups 9.7 -> 8.2 us, 16384 21.1 -> 17.6). Softmax scores take 64 bits at once (16384 tokens of 128 with a bias 9.7,
+// of 256 16.9).
 template <class T, int LANES, int N, bool SIGMOID, bool VECTOR>
 __global__ __launch_bounds__(kThreads) void route_scores(const T* __restrict__ logits, const float* __restrict__ bias,
                                                          std::int64_t* __restrict__ indices, void* __restrict__ scores, Geometry g) {
@@ -591,7 +592,9 @@ void launch_lanes(const T* logits, const float* bias, std::int64_t* indices, voi
 }
 
 // A token takes 16, 32 or 64 lanes of eight experts (four where they are few, 16 past 512), as many as groups and choices at
-// least. 16 experts a lane take half the lanes: 16384 tokens of 256 with a bias 14.0 us for 14.0, 512 tokens 6.9 for 5.6.
+// least. (Us in captured chains, 4 / 8 / 16 experts a lane, sigmoid scores of 256 with a bias: 512 tokens 4.8 / 5.6 / 7.3, 4099 7.1
+// / 6.5 / 7.7, 16384 16.7 / 14.2 / 14.4; in 8 groups 6.1 / 6.3 / 8.2, 8.8 / 8.2 / 9.8 and 21.8 / 17.7 / 17.9; 16-bit logits alone
+// 3.8 / 3.9 / 4.9, 5.7 / 4.9 / 5.4 and 12.7 / 9.1 / 8.3.)
 template <class T>
 void launch(const void* logits, const float* bias, std::int64_t* indices, void* scores, const Geometry& g, hipStream_t stream) {
     const auto* x = static_cast<const T*>(logits);

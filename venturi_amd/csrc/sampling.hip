@@ -23,10 +23,11 @@
 // that one of them reads at the end cost what the shorter count saves.
 //
 // Kept distributions are two or three launches: distribution_scan() looks at few long rows, distribution_cut() finds the last token
-// that a row keeps and the kept mass, and distribution() writes every token's probability. A row that limits leave at most 256 of,
-// and one without limits, need no histogram. The write is bound by memory (96 rows of 151936 bf16 logits: 15 us for 88 MB, 5.8
-// TB/s), the cut by its row's one CU (the same rows, all in all: 38 us without limits, 29 with top_k 50, 52 with top_p alone: 20
-// of those the count, 2 the largest class, 4 the turns' masses, 4 the choice, 7 the search).
+// that a row keeps and the kept mass, and distribution() writes every token's probability. A row without limits needs no histogram,
+// nor does one whose top_k is at most 256 and the number of its chunks of 128 logits (any other top_k, that of the whole row too,
+// and top_p or min_p alone do). The write is bound by memory (96 rows of 151936 bf16 logits: 15 us for 88 MB, 5.8 TB/s), the cut by
+// its row's one CU (the same rows, all in all: 39 us without limits, 29 with top_k 50, 41 with min_p alone, 52 with top_p alone:
+// 20 of those the count, 2 the largest class, 4 the turns' masses, 4 the choice, 7 the search).
 #include "common.hpp"
 
 #include <climits>
@@ -800,10 +801,12 @@ __device__ __forceinline__ float wave_top(float top) {
 }
 
 // Few and long rows are first looked at by the whole card: of a row without limits the largest logit and the mass of its parts, of
-// one that keeps few logits its chunks' largest ones. (Else a row's one CU sees and sums them. Us, with and without, for 5 rows
-// of 248320, 32 of 151936 and 96 of 151936: no limits 11.0 / 35.9, 17.9 / 29.1 and 30.5 / 38.5; top_k 50 14.4 / 19.7, 21.7 /
-// 22.3 and 32.1 / 30.7; in batches of 96 with mixed settings other rows take longest, 52. 16 rows of 32003, which a workgroup's
-// registers hold: 10.7 / 10.7 and 14.0 / 13.0.)
+// one that keeps few logits its chunks' largest ones. (Else a row's one CU sees and sums them. Us in captured chains, with and
+// without, for 5 rows of 248320 and 32, 48 and 96 of 151936: no limits 11.0 / 35.5, 18.6 / 30.0, 21.5 / 32.0 and 32.1 / 39.1;
+// top_k 50 14.0 / 18.5, 20.5 / 20.5, 23.0 / 22.4 and 30.5 / 29.0. But every batch pays for the launch, rows that use nothing of it
+// too: top_p alone 59 / 57, 47 / 45, 49 / 47 and 55 / 52, and of 96 rows with mixed settings, the slowest of which count classes,
+// 58 / 51. So it stops at 32 rows, where it gains little for most settings. 16 rows of 32003, which a workgroup's registers hold:
+// 10.7 / 10.7 and 14.0 / 13.0.)
 constexpr int kScanThreads = 256, kScanWaves = kScanThreads / 64, kScanVectors = 4;  // vectors of a thread
 constexpr int kScanPart = kScanThreads * kScanVectors;
 constexpr int kScanRows = 32, kScanVocab = 8 * kFirst * kThreads;  // up to so many rows of more logits

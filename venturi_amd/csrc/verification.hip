@@ -6,9 +6,10 @@
 // token, by index, at which the running sum passes u times the whole one; sums in 64 bits, in a fixed order.
 //
 // Bound by memory where sequences are many: one or two rows of 4-byte probabilities each (128 of 151936 tokens with a drafter's
-// rows 30.4 us, 5.1 TB/s), else by launches and their chains of loads: the drafts, their probabilities, the row. A long row is cut
+// rows 30.2 us, 5.1 TB/s), else by launches and their chains of loads: the drafts, their probabilities, the row. A long row is cut
 // into parts that workgroups sum, and in a second launch one workgroup finds the part and the token in it (one sequence of 248320
-// tokens 8.0 us); a short one is summed and searched in one launch from registers (61 of 32003 10.0).
+// tokens 8.2 us); a short one is summed and searched in one launch from registers (61 of 32003 10.1). Times are a call's in a
+// captured chain; a call from the host takes 8 with one launch and 11 with two.
 #include "common.hpp"
 
 namespace vt {

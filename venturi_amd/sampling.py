@@ -12,7 +12,8 @@ falls, in that order; its probability is its share. A temperature of 0 (below, o
 probability 1. Logits of -inf and NaN are never taken; a row with no others gives token -1 with probability 0. The
 reference samples on the host apart from its greedy kernel (ops_api.h:46-47); this operator is an extension.
 
-The result depends on the inputs alone: counts are whole numbers, masses 64-bit sums in a fixed order.
+The result depends on the inputs alone: counts are whole numbers, masses 64-bit sums in a fixed order. (A distribution of rows
+without limits adds eight 32-bit weights at a time before that; probabilities below 2^-126 may be 0.)
 """
 
 from dataclasses import dataclass
